@@ -36,7 +36,7 @@
 extern "C" {
 #endif
 
-#define OMNIKV_ABI_VERSION 5
+#define OMNIKV_ABI_VERSION 6
 
 typedef enum {
   OMNIKV_OK = 0,
@@ -516,6 +516,135 @@ typedef struct {
 
 int omnikv_decode_chain(const omnikv_chain_params* p, void* stream);
 int omnikv_decode_chain_supported(int dtype, int hidden, int inter, int H);
+
+/* ------------------------------------------------------------------------------------------
+ * A KV cache held in 8 bits (no counterpart in the reference, whose caches keep the model's 16-bit type,
+ * modeling/spec_cache.py:308-369): one fp32 scale per block of `block` consecutive rows and head,
+ *
+ *     row r of head h reads as  code[r] * scale[r / block]          (K and V each with scales of their own)
+ *
+ * Codes are int8 (top = 127) or e4m3 (top = 448).  For a block whose rows hold the 16-bit values x, with a = max |x|:
+ *     scale = a / top,   code = round(top * x / a)  to the nearest code, ties to even;     a = 0: all codes 0.
+ * A block that holds an infinity or a NaN gets that scale and codes 0: all of it reads as NaN.  The e4m3 NaN codes
+ * (0x7f, 0xff) are never written; attention reads them as +-480.
+ *
+ * k, v: one byte per element, rows of head_dim contiguous codes; strides in elements, multiples of 16, bases 16-byte
+ * aligned; [0, rows) is readable memory for every (sequence, head), at most 2^31 - 1 rows.  k_scale, v_scale:
+ * [B, KVH, ceil(rows / block)], the last dimension contiguous, equal strides for both.  block: a power of two, 1..256.
+ * ------------------------------------------------------------------------------------------ */
+typedef enum { OMNIKV_KV8_INT8 = 0, OMNIKV_KV8_E4M3 = 1 } omnikv_kv8_format;
+
+typedef struct {
+  int32_t format; /* omnikv_kv8_format */
+  int32_t block;
+  int32_t B, KVH, head_dim;
+  int32_t rows;
+  void* k;
+  void* v;
+  int64_t stride_b, stride_h, stride_row;
+  float* k_scale;
+  float* v_scale;
+  int64_t scale_stride_b, scale_stride_h;
+} omnikv_kv8_cache;
+
+/* Rows [start, start + n) of every (sequence, head) from 16-bit k, v [B, KVH, n, d] (element strides, multiples of 8,
+ * bases 16-byte aligned): a prompt, or the next chunk of one.  start: a multiple of block.  lens (device [B] or NULL):
+ * sequence b has min(lens[b], n) rows; what lies behind them is neither read nor written, their absence counts as
+ * nothing in a block's maximum, and a block without rows keeps its scale. */
+int omnikv_kv8_store(const omnikv_kv8_cache* c, int dtype, const void* k, int64_t k_stride_b, int64_t k_stride_h,
+                     int64_t k_stride_row, const void* v, int64_t v_stride_b, int64_t v_stride_h, int64_t v_stride_row,
+                     int start, int n, const int32_t* lens, void* stream);
+
+/* One row per sequence, k_new, v_new [B, KVH, d] 16-bit, at row pos[b] (device; negative or >= rows: sequence skipped).
+ * The row's block keeps its scale s0 when the row fits (max |x| / top < s0).  Else the scale becomes max |x| / top and
+ * the rows of the block before pos are re-coded, code = round(code * (s0 / scale)).  The first row of a block starts it
+ * afresh (s0 = 0).  The rows of the block behind pos are left as they are.  Appending the same row again changes nothing. */
+int omnikv_kv8_append(const omnikv_kv8_cache* c, int dtype, const void* k_new, const void* v_new, int64_t new_stride_b,
+                      int64_t new_stride_h, const int32_t* pos, void* stream);
+
+/* Rows back in 16 bits (code * scale in fp32, rounded once): rows [start, start + n) when idx is NULL, else rows
+ * idx[b][0..n) (device, in any order, repeated or not); a row outside [0, rows) reads as zeros.  k_out, v_out
+ * [B, KVH, n, d] with element strides (multiples of 8, equal for both, bases 16-byte aligned). */
+int omnikv_kv8_load(const omnikv_kv8_cache* c, int dtype, int start, int n, const int32_t* idx, int64_t idx_stride,
+                    void* k_out, void* v_out, int64_t out_stride_b, int64_t out_stride_h, int64_t out_stride_row,
+                    void* stream);
+
+/* Decode attention over such a cache: omnikv_decode_attn's definition with K and V as the rows read.
+ *   rows of sequence b: idx == NULL: positions [0, len[b]); else positions idx[b][0..len[b]); then the tail positions
+ *   [tail_start[b], tail_start[b] + tail_len[b]) when tail_len is given.
+ * len is taken into [0, rows] (with idx: [0, idx_cap]), the tail into the cache; an index outside [0, rows) counts as no
+ * row.  No rows at all: the output is zero.  score_out (idx == NULL, no tail): as in omnikv_decode_attn.
+ * q, out [B, H, d] 16-bit; H / KVH at most 16.
+ * The workspace (omnikv_kv8_attn_workspace_bytes) starts with 16 KiB of counters that are ZERO before its first use and
+ * are left zero; calls that share it must not overlap. */
+typedef struct {
+  omnikv_kv8_cache cache;
+  int32_t dtype; /* OMNIKV_BF16 or OMNIKV_F16: q, out */
+  int32_t H;
+  float scale;
+  const void* q;
+  int64_t q_stride_b, q_stride_h;
+  void* out; /* same strides as q */
+  const int32_t* idx;
+  int64_t idx_stride;
+  int32_t idx_cap;
+  const int32_t* len;
+  const int32_t* tail_start;
+  const int32_t* tail_len;
+  float* score_out; /* [KVH, B, score_stride] or NULL */
+  int64_t score_stride;
+  const int32_t* score_len;
+  int32_t n_splits; /* 1..512 */
+  void* workspace;
+  size_t workspace_bytes;
+  int32_t* status; /* optional device word: set to 5 if a bounded wait for a KV copy ran out */
+} omnikv_kv8_attn_params;
+
+size_t omnikv_kv8_attn_workspace_bytes(int B, int H, int n_splits);
+int omnikv_kv8_decode_attn(const omnikv_kv8_attn_params* p, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Matrix product in 8-bit integers with one scale per token and per output channel (the reference offers 8-bit weights
+ * through a third-party package, infer.py:192-287):
+ *
+ *   omnikv_quant_rows:   for every row of x (16-bit, [n, K]): a = max |x|, scale = a / 127, code = round(127 x / a)
+ *                        (ties to even; a = 0: codes 0; a row with an infinity or a NaN: codes 0 and that scale)
+ *   omnikv_linear_w8a8:  out[t][c] = (sum_k x[t][k] * w[c][k]) * x_scale[t] * w_scale[c] (+ residual[t][c])
+ *
+ * The sum is exact (32-bit integers, K <= 32768); the scales are applied in fp32 and the result is rounded once.  x, w:
+ * int8, rows of K contiguous codes, K a multiple of 16, row strides (elements) multiples of 16, bases 16-byte aligned.
+ * out: OMNIKV_F32 or a 16-bit type, residual of the same type (may alias out).  omnikv_quant_rows serves the activations
+ * of a call and, once, a weight matrix [channels, K].
+ * The workspace of omnikv_linear_w8a8 (omnikv_linear_w8a8_workspace_bytes, may be 0 bytes) starts with counters that are
+ * ZERO before its first use and are left zero; calls that share it must not overlap.
+ * ------------------------------------------------------------------------------------------ */
+int omnikv_quant_rows(int dtype, const void* x, int64_t x_stride_row, int n, int K, int8_t* codes, int64_t code_stride_row,
+                      float* scale, void* stream);
+
+typedef struct {
+  int32_t n_tokens, channels, K;
+  const int8_t* x;
+  int64_t x_stride_row;
+  const float* x_scale; /* [n_tokens] */
+  const int8_t* w;
+  int64_t w_stride_row;
+  const float* w_scale; /* [channels] */
+  int32_t out_dtype;
+  const void* residual; /* or NULL */
+  int64_t residual_stride_row;
+  void* out;
+  int64_t out_stride_row;
+  void* workspace;
+  size_t workspace_bytes;
+  int32_t* status; /* optional device word: set to 7 if a bounded wait ran out */
+} omnikv_linear_w8a8_params;
+
+size_t omnikv_linear_w8a8_workspace_bytes(int n_tokens, int channels, int K);
+int omnikv_linear_w8a8(const omnikv_linear_w8a8_params* p, void* stream);
+
+/* Identity of the graph capture that `stream` records into, 0 when it records none (callers keep one workspace per
+ * captured graph: two graphs may be replayed at the same time). */
+unsigned long long omnikv_capture_id(void* stream);
 
 #ifdef __cplusplus
 }

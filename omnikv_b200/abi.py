@@ -12,7 +12,7 @@ from pathlib import Path
 _LIB_PATH = Path(os.environ.get("OMNIKV_B200_LIB") or Path(__file__).resolve().parent / "_lib" / "libomnikv_b200.so")
 _lib = None
 
-ABI_VERSION = 5
+ABI_VERSION = 6
 F32, BF16, F16 = 0, 1, 2
 SEL_SOFTMAX_LAST, SEL_UNIFORM, SEL_EXP = 0, 1, 2
 NO_ALLOC_SCRATCH_BYTES = 4 * 1024 * 1024
@@ -111,6 +111,46 @@ class ChainParams(C.Structure):
     ]
 
 
+KV8_INT8, KV8_E4M3 = 0, 1
+
+
+class Kv8Cache(C.Structure):
+    """Mirror of ``omnikv_kv8_cache``."""
+
+    _fields_ = [
+        ("format", C.c_int32), ("block", C.c_int32), ("B", C.c_int32), ("KVH", C.c_int32), ("head_dim", C.c_int32),
+        ("rows", C.c_int32), ("k", C.c_void_p), ("v", C.c_void_p),
+        ("stride_b", C.c_int64), ("stride_h", C.c_int64), ("stride_row", C.c_int64),
+        ("k_scale", C.c_void_p), ("v_scale", C.c_void_p), ("scale_stride_b", C.c_int64), ("scale_stride_h", C.c_int64),
+    ]
+
+
+class Kv8AttnParams(C.Structure):
+    """Mirror of ``omnikv_kv8_attn_params``."""
+
+    _fields_ = [
+        ("cache", Kv8Cache), ("dtype", C.c_int32), ("H", C.c_int32), ("scale", C.c_float),
+        ("q", C.c_void_p), ("q_stride_b", C.c_int64), ("q_stride_h", C.c_int64), ("out", C.c_void_p),
+        ("idx", C.c_void_p), ("idx_stride", C.c_int64), ("idx_cap", C.c_int32), ("len", C.c_void_p),
+        ("tail_start", C.c_void_p), ("tail_len", C.c_void_p),
+        ("score_out", C.c_void_p), ("score_stride", C.c_int64), ("score_len", C.c_void_p),
+        ("n_splits", C.c_int32), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t), ("status", C.c_void_p),
+    ]
+
+
+class LinearW8A8Params(C.Structure):
+    """Mirror of ``omnikv_linear_w8a8_params``."""
+
+    _fields_ = [
+        ("n_tokens", C.c_int32), ("channels", C.c_int32), ("K", C.c_int32),
+        ("x", C.c_void_p), ("x_stride_row", C.c_int64), ("x_scale", C.c_void_p),
+        ("w", C.c_void_p), ("w_stride_row", C.c_int64), ("w_scale", C.c_void_p),
+        ("out_dtype", C.c_int32), ("residual", C.c_void_p), ("residual_stride_row", C.c_int64),
+        ("out", C.c_void_p), ("out_stride_row", C.c_int64), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+        ("status", C.c_void_p),
+    ]
+
+
 # name -> (restype, argtypes); every symbol the header declares
 SIGNATURES = {
     "omnikv_abi_version": (C.c_int, []),
@@ -158,6 +198,19 @@ SIGNATURES = {
     "omnikv_rope_window": (C.c_int, [C.c_int, C.c_void_p, C.c_int64, C.c_int64, C.c_int, C.c_int, C.c_int, C.c_int,
                                      C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
     "omnikv_silu_mul": (C.c_int, [C.c_int, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_int, C.c_int, C.c_void_p]),
+    "omnikv_kv8_store": (C.c_int, [C.POINTER(Kv8Cache), C.c_int, C.c_void_p, C.c_int64, C.c_int64, C.c_int64, C.c_void_p,
+                                   C.c_int64, C.c_int64, C.c_int64, C.c_int, C.c_int, C.c_void_p, C.c_void_p]),
+    "omnikv_kv8_append": (C.c_int, [C.POINTER(Kv8Cache), C.c_int, C.c_void_p, C.c_void_p, C.c_int64, C.c_int64,
+                                    C.c_void_p, C.c_void_p]),
+    "omnikv_kv8_load": (C.c_int, [C.POINTER(Kv8Cache), C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_int64, C.c_void_p,
+                                  C.c_void_p, C.c_int64, C.c_int64, C.c_int64, C.c_void_p]),
+    "omnikv_kv8_attn_workspace_bytes": (C.c_size_t, [C.c_int, C.c_int, C.c_int]),
+    "omnikv_kv8_decode_attn": (C.c_int, [C.POINTER(Kv8AttnParams), C.c_void_p]),
+    "omnikv_quant_rows": (C.c_int, [C.c_int, C.c_void_p, C.c_int64, C.c_int, C.c_int, C.c_void_p, C.c_int64, C.c_void_p,
+                                    C.c_void_p]),
+    "omnikv_linear_w8a8_workspace_bytes": (C.c_size_t, [C.c_int, C.c_int, C.c_int]),
+    "omnikv_linear_w8a8": (C.c_int, [C.POINTER(LinearW8A8Params), C.c_void_p]),
+    "omnikv_capture_id": (C.c_ulonglong, [C.c_void_p]),
     "omnikv_kv_append": (C.c_int, [C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int,
                                    C.c_int, C.c_int64, C.c_int64, C.c_int64, C.c_int64, C.c_int64, C.c_void_p,
                                    C.c_void_p]),
