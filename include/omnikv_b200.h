@@ -594,13 +594,13 @@ typedef struct {
   float* score_out; /* [KVH, B, score_stride] or NULL */
   int64_t score_stride;
   const int32_t* score_len;
-  int32_t n_splits; /* 1..512 */
+  int32_t n_ctas; /* the work of all sequences is cut into at most this many equal pieces; 1..65536 */
   void* workspace;
   size_t workspace_bytes;
   int32_t* status; /* optional device word: set to 5 if a bounded wait for a KV copy ran out */
 } omnikv_kv8_attn_params;
 
-size_t omnikv_kv8_attn_workspace_bytes(int B, int H, int n_splits);
+size_t omnikv_kv8_attn_workspace_bytes(int B, int H, int KVH, int n_ctas);
 int omnikv_kv8_decode_attn(const omnikv_kv8_attn_params* p, void* stream);
 
 /* ------------------------------------------------------------------------------------------

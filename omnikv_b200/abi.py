@@ -134,7 +134,7 @@ class Kv8AttnParams(C.Structure):
         ("idx", C.c_void_p), ("idx_stride", C.c_int64), ("idx_cap", C.c_int32), ("len", C.c_void_p),
         ("tail_start", C.c_void_p), ("tail_len", C.c_void_p),
         ("score_out", C.c_void_p), ("score_stride", C.c_int64), ("score_len", C.c_void_p),
-        ("n_splits", C.c_int32), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t), ("status", C.c_void_p),
+        ("n_ctas", C.c_int32), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t), ("status", C.c_void_p),
     ]
 
 
@@ -204,7 +204,7 @@ SIGNATURES = {
                                     C.c_void_p, C.c_void_p]),
     "omnikv_kv8_load": (C.c_int, [C.POINTER(Kv8Cache), C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_int64, C.c_void_p,
                                   C.c_void_p, C.c_int64, C.c_int64, C.c_int64, C.c_void_p]),
-    "omnikv_kv8_attn_workspace_bytes": (C.c_size_t, [C.c_int, C.c_int, C.c_int]),
+    "omnikv_kv8_attn_workspace_bytes": (C.c_size_t, [C.c_int, C.c_int, C.c_int, C.c_int]),
     "omnikv_kv8_decode_attn": (C.c_int, [C.POINTER(Kv8AttnParams), C.c_void_p]),
     "omnikv_quant_rows": (C.c_int, [C.c_int, C.c_void_p, C.c_int64, C.c_int, C.c_int, C.c_void_p, C.c_int64, C.c_void_p,
                                     C.c_void_p]),

@@ -1,14 +1,41 @@
 // Decode attention over a KV cache held in 8 bits.
 //
-// Grid (n_splits, KVH, B): a CTA owns a contiguous share of its sequence's row list, writes one un-normalised partial
-// (o, m, l) per query head, and the CTA that finishes last for a (sequence, KV head) merges them, so a call is one launch.
+// Mathematics.  With K = ck * sk, V = cv * sv (codes and per-block scales) a row j contributes, to one query head,
+//     x_j = (q . ck_j) * sk_j * scale * log2(e)          l = sum_j 2^(x_j - m)
+//     y_j = x_j + log2(sv_j)                              o = sum_j 2^(y_j - M + 15) cv_j
+//     out = o / l * 2^(M - m - 15)
+// m and M are running maxima of x and y.  The V scale rides in the exponent, so the weights that meet the codes lie in
+// [0, 2^15] whatever the scales: they round to fp16 (11 bits, three more than the bf16 weights of a 16-bit cache) and one
+// that is 2^-39 of the largest still counts.  The codes are fp16 numbers exactly (int8: 1024 + 128 + code by a byte
+// permutation, minus 1152; e4m3: exponent field moved, the factor 2^8 goes into the scale), the queries too after a power
+// of two per head.  Sums are fp32, in the MMA and outside.
+//
+// Layout.  A warp works alone: its own ring of 32-row tiles, its own mbarriers, no CTA barrier until the end of a segment.
+// Rows are the M side of both products (S^T = K q^T and O^T = V^T P^T with m16n8k16), the query heads of a KV head the N
+// side, so up to 8 heads cost one MMA column block, and a K row's 16-byte pieces are A fragments as they lie in shared
+// memory: the order of the 128 dimensions inside a product is free as long as q follows it.  V rows are interleaved in
+// pairs (byte permutations), P^T comes from S^T by movmatrix.
+//
+// Work.  The 32-row tiles of all (sequence, KV head) segments form one list that is cut into equal pieces, one per CTA
+// (two CTAs per SM, at least four tiles each), whatever the lengths: a CTA may end one segment and begin the next.  Every
+// CTA leaves one partial (o, M, m, l) per segment that it touches, and the one that arrives last at a segment merges.
+//
+// Bound: HBM, 256 bytes of codes and 8 / block bytes of scales per (row, KV head).
 #include "kv8.cuh"
+
+#include <atomic>
 
 namespace omnikv {
 namespace {
 
 constexpr int MAX_G = 16;
 constexpr int NW = 4, NT = NW * 32;
+constexpr int TILE = 32;                     // rows per tile: one lane per row when rows are fetched one by one
+constexpr int STAGES = 3;
+constexpr int BOX = TILE * kHeadDim;         // bytes of a K or V tile
+constexpr int PITCH = 2 * kHeadDim + 16;     // row pitch of a tile fetched row by row (K | V | pad): conflict-free
+constexpr int ROWS_STAGE = TILE * PITCH, TMA_STAGE = 2 * BOX;
+constexpr int OS_PITCH = kHeadDim + 4;       // floats per head in the CTA's merge buffer
 
 struct A8Args {
   const unsigned char *k, *v;
@@ -26,15 +53,19 @@ struct A8Args {
   float* score_out;
   int64_t score_stride;
   const int* score_len;
-  float *ws_o, *ws_ml;
-  unsigned* ws_cnt;
-  int B, H, KVH, G, S;
+  float* ws_o;      // [slot][G][128]
+  float4* ws_ml;    // [slot][G] {M, m, l, -}
+  unsigned* ws_cnt; // [B * KVH] arrivals, zero between launches
+  int* status;
+  int B, H, KVH, G, pair;
   float scale;
 };
 
 // The rows of a sequence: nA listed ones, then the tail [t0, t0 + nB).
 struct RowList {
   int nA, nB, t0;
+  __device__ __forceinline__ int n() const { return nA + nB; }
+  __device__ __forceinline__ int tiles() const { return max(1, ceil_div(nA + nB, TILE)); }  // an empty one is written too
 };
 __device__ __forceinline__ RowList row_list(const A8Args& a, int b) {
   RowList r;
@@ -48,94 +79,582 @@ __device__ __forceinline__ RowList row_list(const A8Args& a, int b) {
   return r;
 }
 
-template <typename T, int FMT>
-__global__ void __launch_bounds__(NT) decode_attn_kv8_kernel(const A8Args a) {
-  __shared__ float o_s[NW][MAX_G][kHeadDim];
-  __shared__ float ml_s[NW][MAX_G][2];
-  __shared__ int last_flag;
-  pdl_wait();
-  const int split = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int G = a.G;
-  const RowList list = row_list(a, b);
-  const int n = list.nA + list.nB;
-  const int chunk = ceil_div(n, a.S), r0 = min(n, split * chunk), r1 = min(n, r0 + chunk);
-  const unsigned char* k = a.k + (size_t)b * a.sb + (size_t)kvh * a.sh;
-  const unsigned char* v = a.v + (size_t)b * a.sb + (size_t)kvh * a.sh;
-  const float* ks = a.ks + (size_t)b * a.ssb + (size_t)kvh * a.ssh;
-  const float* vs = a.vs + (size_t)b * a.ssb + (size_t)kvh * a.ssh;
-  const int score_lim = a.score_out ? min(a.score_len[b], list.nA) : 0;
-  float* score_row = a.score_out ? a.score_out + ((size_t)kvh * a.B + b) * a.score_stride : nullptr;
-  const T* q = static_cast<const T*>(a.q) + (size_t)b * a.q_sb + (size_t)kvh * G * a.q_sh;
-  for (int g = 0; g < G; ++g) {
-    float qv[4];
-    for (int e = 0; e < 4; ++e) qv[e] = to_float(q[(size_t)g * a.q_sh + lane * 4 + e]) * a.scale;
-    float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int r = r0 + warp; r < r1; r += NW) {
-      const int64_t row = r < list.nA ? (a.idx ? a.idx[(size_t)b * a.idx_stride + r] : r) : list.t0 + (r - list.nA);
-      if (row < 0 || row >= a.rows) continue;
-      const unsigned kw = *reinterpret_cast<const unsigned*>(k + row * a.sr + lane * 4);
-      const unsigned vw = *reinterpret_cast<const unsigned*>(v + row * a.sr + lane * 4);
-      float s = 0.f;
-      for (int e = 0; e < 4; ++e) s = fmaf(qv[e], code_value<FMT>((kw >> (8 * e)) & 0xffu), s);
-      for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-      s *= ks[row >> a.shift];
-      if (lane == 0 && r < score_lim) score_row[r] = g == 0 ? s : fmaxf(score_row[r], s);
-      const float mn = fmaxf(m, s), c = m == -INFINITY ? 0.f : expf(m - mn), p = expf(s - mn);
-      const float pv = p * vs[row >> a.shift];
-      l = l * c + p;
-      for (int e = 0; e < 4; ++e) o[e] = o[e] * c + pv * code_value<FMT>((vw >> (8 * e)) & 0xffu);
-      m = mn;
-    }
-    for (int e = 0; e < 4; ++e) o_s[warp][g][lane * 4 + e] = o[e];
-    if (lane == 0) {
-      ml_s[warp][g][0] = m;
-      ml_s[warp][g][1] = l;
+// A place in the list of tiles.
+struct Cursor {
+  int b, kvh, tile, nt;
+  RowList list;
+  __device__ __forceinline__ void load(const A8Args& a) {
+    list = row_list(a, b);
+    nt = list.tiles();
+  }
+  __device__ __forceinline__ void forward(const A8Args& a, int by) {
+    tile += by;
+    while (tile >= nt) {
+      tile -= nt;
+      if (++kvh == a.KVH) {
+        kvh = 0;
+        if (++b >= a.B) return;
+        load(a);
+      }
     }
   }
-  __syncthreads();
-  for (int g = 0; g < G; ++g) {
-    float M = -INFINITY, L = 0.f, acc = 0.f;
-    for (int w = 0; w < NW; ++w) M = fmaxf(M, ml_s[w][g][0]);
-    for (int w = 0; w < NW; ++w) {
-      const float c = ml_s[w][g][0] == -INFINITY ? 0.f : expf(ml_s[w][g][0] - M);
-      L += ml_s[w][g][1] * c;
-      acc += o_s[w][g][tid] * c;
-    }
-    const size_t base = (size_t)(b * a.H + kvh * G + g) * a.S + split;
-    a.ws_o[base * kHeadDim + tid] = acc;
-    if (tid == 0) {
-      a.ws_ml[base * 2] = M;
-      a.ws_ml[base * 2 + 1] = L;
-    }
-  }
-  __threadfence();
-  __syncthreads();
-  if (tid == 0) last_flag = atomicAdd(a.ws_cnt + b * a.KVH + kvh, 1u) == (unsigned)(a.S - 1);
-  __syncthreads();
-  if (!last_flag) return;
-  __threadfence();
-  for (int g = 0; g < G; ++g) {
-    const size_t base = (size_t)(b * a.H + kvh * G + g) * a.S;
-    float M = -INFINITY, L = 0.f, acc = 0.f;
-    for (int s = 0; s < a.S; ++s) M = fmaxf(M, __ldcg(a.ws_ml + (base + s) * 2));
-    for (int s = 0; s < a.S; ++s) {
-      const float ms = __ldcg(a.ws_ml + (base + s) * 2), c = ms == -INFINITY ? 0.f : expf(ms - M);
-      L += __ldcg(a.ws_ml + (base + s) * 2 + 1) * c;
-      acc += __ldcg(a.ws_o + (base + s) * kHeadDim + tid) * c;
-    }
-    static_cast<T*>(a.out)[(size_t)b * a.q_sb + (size_t)(kvh * G + g) * a.q_sh + tid] = from_float<T>(L == 0.f ? 0.f : acc / L);
-  }
-  if (tid == 0) a.ws_cnt[b * a.KVH + kvh] = 0u;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
 }
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;\n" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+__device__ __forceinline__ unsigned movmatrix_trans(unsigned x) {
+  unsigned y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ unsigned sub_h2(unsigned a, unsigned b) {
+  unsigned y;
+  asm("sub.f16x2 %0, %1, %2;\n" : "=r"(y) : "r"(a), "r"(b));
+  return y;
+}
+
+// Bytes 0, 1 (hi = false) or 2, 3 of w as two fp16 numbers.  int8: the code.  e4m3: the value times 2^-8 (sign kept,
+// exponent and mantissa moved to fp16's fields; subnormals come out right, the NaN codes as 480 * 2^-8).
+template <int FMT>
+__device__ __forceinline__ unsigned prepare_word(unsigned w) {
+  return FMT == kInt8 ? w ^ 0x80808080u : w;
+}
+template <int FMT, bool HI>
+__device__ __forceinline__ unsigned half2_of(unsigned w) {
+  if constexpr (FMT == kInt8) {
+    return sub_h2(__byte_perm(w, 0x64646464u, HI ? 0x4342 : 0x4140), 0x64806480u);
+  } else {
+    const unsigned x = __byte_perm(w, 0, HI ? 0x3424 : 0x1404);
+    return ((x >> 1) & 0x3f803f80u) | (x & 0x80008000u);
+  }
+}
+template <int FMT>
+__host__ __device__ constexpr float half2_unit() {  // what the conversion leaves to be multiplied
+  return FMT == kInt8 ? 1.f : 256.f;
+}
+
+__device__ __forceinline__ void cp_async4(void* smem_dst, const void* gmem_src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;\n" ::"r"(smem_u32(smem_dst)), "l"(gmem_src) : "memory");
+}
+
+struct Shared {
+  uint64_t full[NW][STAGES];
+  float scale[NW][STAGES][2][TILE];  // K and V scale of each row of a tile
+  unsigned valid[NW][STAGES];        // rows of the tile that exist
+  float ml[NW][MAX_G][3];            // M, m, l of the warps
+  int last;
+};
+
+// COLS: n8 column blocks of query heads (1: up to 8 heads per KV head, 2: up to 16).  TMA: tiles as boxes of a tensor map
+// (rows that follow one another), else rows fetched one by one.
+template <typename T, int FMT, int COLS, bool TMA>
+__global__ void __launch_bounds__(NT, 2)
+decode_attn_kv8_kernel(const A8Args a, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
+  extern __shared__ __align__(128) unsigned char smem_raw[];
+  __shared__ Shared sh;
+  constexpr int STAGE_BYTES = TMA ? TMA_STAGE : ROWS_STAGE;
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  unsigned char* ring = smem + warp * STAGES * STAGE_BYTES;
+  float* o_s = reinterpret_cast<float*>(smem + NW * STAGES * STAGE_BYTES);
+  const int G = a.G;
+
+  if (lane < STAGES) mbar_init(&sh.full[warp][lane], 1);
+  asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+  __syncwarp();
+  pdl_wait();
+
+  // ---- this CTA's piece of the list: tiles [w0, w1) of W ----
+  int per_head = 0;  // tiles of all sequences, per KV head
+  for (int b0 = 0; b0 < a.B; b0 += 32) {
+    const int mine = b0 + lane < a.B ? row_list(a, b0 + lane).tiles() : 0;
+    per_head += __reduce_add_sync(0xffffffffu, mine);
+  }
+  const long long W = (long long)per_head * a.KVH;
+  const long long C = max(1ll, min((long long)gridDim.x, W / NW));
+  const int c = blockIdx.x;
+  if (c >= C) return;
+  const long long w0 = W * c / C, w1 = W * (c + 1) / C;
+  const auto owner = [&](long long tile) { return (int)(((tile + 1) * C - 1) / W); };  // the CTA that has this tile
+  Cursor seg;  // the segment being worked on; tile = 0
+  long long seg_lo;
+  {
+    long long before = 0;  // tiles of the sequences in front
+    int b0 = 0, found = -1, in_front = 0;
+    for (; found < 0; b0 += 32) {
+      const int mine = b0 + lane < a.B ? row_list(a, b0 + lane).tiles() : 0;
+      int sum = mine;
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, sum, off);
+        if (lane >= off) sum += x;
+      }
+      const unsigned hit = __ballot_sync(0xffffffffu, (before + sum) * a.KVH > w0);
+      if (hit) {
+        found = b0 + __ffs(hit) - 1;
+        in_front = __shfl_sync(0xffffffffu, sum - mine, __ffs(hit) - 1);
+      } else {
+        before += __shfl_sync(0xffffffffu, sum, 31);
+      }
+    }
+    seg.b = found;
+    seg.load(a);
+    const long long first = (before + in_front) * a.KVH;
+    seg.kvh = (int)((w0 - first) / seg.nt);
+    seg.tile = 0;
+    seg_lo = first + (long long)seg.kvh * seg.nt;
+  }
+
+  // ---- the warp's stream of tiles: every NW-th of the piece ----
+  Cursor ahead = seg;  // the next tile to ask for
+  long long ahead_w = w0 + warp;
+  int asked = 0, pos = -1;
+  const auto find_row = [&]() {  // the cache position of this lane's row in the tile to ask for, -1: none
+    pos = -1;
+    if (ahead_w < w1) {
+      const int r = ahead.tile * TILE + lane;
+      if (r < ahead.list.nA) pos = a.idx ? __ldg(a.idx + (size_t)ahead.b * a.idx_stride + r) : r;
+      else if (r < ahead.list.n()) pos = ahead.list.t0 + (r - ahead.list.nA);
+    }
+  };
+  const auto ask = [&]() {  // copies of one tile, and of its rows' scales
+    if (ahead_w < w1) {
+      const int s = asked % STAGES;
+      unsigned char* dst = ring + s * STAGE_BYTES;
+      const bool ok = pos >= 0 && pos < a.rows;
+      if constexpr (TMA) {
+        if (lane == 0) {
+          mbar_expect_tx(&sh.full[warp][s], TMA_STAGE);
+          tma_load_4d(dst, &tm_k, 0, ahead.tile * TILE, ahead.kvh, ahead.b, &sh.full[warp][s]);
+          tma_load_4d(dst + BOX, &tm_v, 0, ahead.tile * TILE, ahead.kvh, ahead.b, &sh.full[warp][s]);
+        }
+      }
+      const unsigned valid = __ballot_sync(0xffffffffu, ok);
+      if (lane == 0) {
+        sh.valid[warp][s] = valid;
+        if constexpr (!TMA) mbar_expect_tx(&sh.full[warp][s], __popc(valid) * 2 * kHeadDim);
+      }
+      __syncwarp();
+      if (ok) {
+        if constexpr (!TMA) {
+          const int64_t at = (int64_t)ahead.b * a.sb + (int64_t)ahead.kvh * a.sh + (int64_t)pos * a.sr;
+          if (a.pair) {
+            tma_bulk_g2s(dst + lane * PITCH, a.k + at, 2 * kHeadDim, &sh.full[warp][s]);
+          } else {
+            tma_bulk_g2s(dst + lane * PITCH, a.k + at, kHeadDim, &sh.full[warp][s]);
+            tma_bulk_g2s(dst + lane * PITCH + kHeadDim, a.v + at, kHeadDim, &sh.full[warp][s]);
+          }
+        }
+        const int64_t sat = (int64_t)ahead.b * a.ssb + (int64_t)ahead.kvh * a.ssh + (pos >> a.shift);
+        cp_async4(&sh.scale[warp][s][0][lane], a.ks + sat);
+        cp_async4(&sh.scale[warp][s][1][lane], a.vs + sat);
+      }
+      ++asked;
+      ahead_w += NW;
+      if (ahead_w < w1) ahead.forward(a, NW);
+    }
+    cp_async_commit();
+    find_row();
+  };
+  ahead.tile = (int)(w0 - seg_lo);
+  if (ahead_w < w1) ahead.forward(a, warp);
+  find_row();
+#pragma unroll
+  for (int s = 0; s < STAGES - 1; ++s) ask();
+
+  int used = 0;
+  bool dead = false;
+  long long next_w = w0 + warp;  // the warp's next tile
+  for (long long lo = w0; lo < w1;) {
+    const long long seg_hi = seg_lo + seg.nt, hi = min(w1, seg_hi);  // this CTA's tiles of the segment: [lo, hi)
+    const int b = seg.b, kvh = seg.kvh;
+
+    // ---- queries: fragments of q * 2^e (largest element in [2^13, 2^14)), e folded into the head's factor ----
+    unsigned qf[COLS][8][2];
+    float qs[COLS][2];
+#pragma unroll
+    for (int cb = 0; cb < COLS; ++cb) {
+      const int h = cb * 8 + g;
+      uint2 raw[8];
+      unsigned top = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        raw[j] = make_uint2(0, 0);
+        if (h < G)
+          raw[j] = *reinterpret_cast<const uint2*>(static_cast<const T*>(a.q) + (size_t)b * a.q_sb + (size_t)(kvh * G + h) * a.q_sh +
+                                                   16 * (2 * t + (j >> 2)) + 4 * (j & 3));
+        const float2 x = unpack16<T>(raw[j].x), y = unpack16<T>(raw[j].y);
+        top = max(top, max(max(abs_bits(x.x), abs_bits(x.y)), max(abs_bits(y.x), abs_bits(y.y))));
+      }
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const int e = min(13 - ((int)(top >> 23) - 127), 126);
+      const float up = __uint_as_float((unsigned)(e + 127) << 23), down = exp2f((float)-e);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float2 x = unpack16<T>(raw[j].x), y = unpack16<T>(raw[j].y);
+        qf[cb][j][0] = pack2<__half>(x.x * up, x.y * up);
+        qf[cb][j][1] = pack2<__half>(y.x * up, y.y * up);
+      }
+      const float f = down * a.scale * half2_unit<FMT>();
+      qs[cb][0] = __shfl_sync(0xffffffffu, f, 8 * t);
+      qs[cb][1] = __shfl_sync(0xffffffffu, f, 8 * t + 4);
+    }
+    const int score_lim = a.score_out ? min(a.score_len[b], seg.list.nA) : 0;
+    float* score_row = a.score_out ? a.score_out + ((size_t)kvh * a.B + b) * a.score_stride : nullptr;
+
+    float m[COLS][2], M[COLS][2], l[COLS][2], o[COLS][8][4];
+#pragma unroll
+    for (int cb = 0; cb < COLS; ++cb) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) m[cb][e] = M[cb][e] = -INFINITY, l[cb][e] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o[cb][i][0] = o[cb][i][1] = o[cb][i][2] = o[cb][i][3] = 0.f;
+    }
+
+    for (; next_w < hi; next_w += NW) {
+      const int s = used % STAGES;
+      __syncwarp();  // all lanes are done with the tile whose stage is refilled now
+      ask();
+      cp_async_wait<STAGES - 1>();
+      if (!dead && !mbar_wait(&sh.full[warp][s], (used / STAGES) & 1)) {
+        dead = true;
+        if (a.status) atomicExch(a.status, 5);
+      }
+      __syncwarp();
+      const unsigned char* tile = ring + s * STAGE_BYTES;
+      // the 16-byte piece c of row r of the tile's K or V rows
+      const auto piece = [&](int v, int r, int cc) {
+        if constexpr (TMA) return *reinterpret_cast<const uint4*>(tile + v * BOX + r * kHeadDim + ((cc ^ (r & 7)) << 4));
+        else return *reinterpret_cast<const uint4*>(tile + r * PITCH + v * kHeadDim + (cc << 4));
+      };
+      const unsigned valid = sh.valid[warp][s];
+      const float my_ks = sh.scale[warp][s][0][lane], my_lv = log2f(sh.scale[warp][s][1][lane]);
+
+      // ---- S^T = K q^T ----
+      float x[2][COLS][4];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int cb = 0; cb < COLS; ++cb) x[i][cb][0] = x[i][cb][1] = x[i][cb][2] = x[i][cb][3] = 0.f;
+        uint4 r0[2], r1[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          r0[u] = piece(0, 16 * i + g, 2 * t + u);
+          r1[u] = piece(0, 16 * i + 8 + g, 2 * t + u);
+        }
+        const unsigned* p0 = reinterpret_cast<const unsigned*>(r0);
+        const unsigned* p1 = reinterpret_cast<const unsigned*>(r1);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const unsigned u0 = prepare_word<FMT>(p0[j]), u1 = prepare_word<FMT>(p1[j]);
+          const unsigned af[4] = {half2_of<FMT, false>(u0), half2_of<FMT, false>(u1), half2_of<FMT, true>(u0), half2_of<FMT, true>(u1)};
+#pragma unroll
+          for (int cb = 0; cb < COLS; ++cb) mma_16816<__half>(x[i][cb], af, qf[cb][j][0], qf[cb][j][1]);
+        }
+      }
+      // ---- scales, mask, scores ----
+      const int row0 = (int)(next_w - seg_lo) * TILE;
+      float lv[2][2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {  // rows 16 i + 8 u + g
+          const int r = 16 * i + 8 * u + g;
+          const float ks = __shfl_sync(0xffffffffu, my_ks, r);
+          lv[i][u] = __shfl_sync(0xffffffffu, my_lv, r);
+          const bool ok = (valid >> r) & 1u;
+          float best = -INFINITY;
+#pragma unroll
+          for (int cb = 0; cb < COLS; ++cb)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const float z = x[i][cb][2 * u + e] * ks * qs[cb][e];
+              if (cb * 8 + 2 * t + e < G) best = max_nan(best, z);
+              x[i][cb][2 * u + e] = ok ? z * kLog2e : -INFINITY;
+            }
+          if (a.score_out) {
+            best = max_nan(best, __shfl_xor_sync(0xffffffffu, best, 1));
+            best = max_nan(best, __shfl_xor_sync(0xffffffffu, best, 2));
+            if (t == 0 && row0 + r < score_lim) score_row[row0 + r] = best;
+          }
+          if (!ok) lv[i][u] = 0.f;  // a scale that was not read
+        }
+      // ---- weights ----
+      unsigned pb[2][COLS][2];
+#pragma unroll
+      for (int cb = 0; cb < COLS; ++cb) {
+        float corr[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float mx = m[cb][e], My = M[cb][e];
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              mx = fmaxf(mx, x[i][cb][2 * u + e]);
+              My = fmaxf(My, x[i][cb][2 * u + e] + lv[i][u]);
+            }
+#pragma unroll
+          for (int off = 4; off < 32; off <<= 1) {
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+            My = fmaxf(My, __shfl_xor_sync(0xffffffffu, My, off));
+          }
+          const float mu = mx == -INFINITY ? 0.f : mx, Mu = My == -INFINITY ? 0.f : My;
+          float sum = 0.f;
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              float& z = x[i][cb][2 * u + e];
+              sum += ex2(z - mu);
+              z = ex2(z + lv[i][u] - Mu + 15.f);
+            }
+          l[cb][e] = fmaf(l[cb][e], ex2(m[cb][e] - mu), sum);
+          corr[e] = ex2(M[cb][e] - Mu);
+          m[cb][e] = mx;
+          M[cb][e] = My;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          o[cb][i][0] *= corr[0];
+          o[cb][i][1] *= corr[1];
+          o[cb][i][2] *= corr[0];
+          o[cb][i][3] *= corr[1];
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          pb[i][cb][0] = movmatrix_trans(pack2<__half>(x[i][cb][0], x[i][cb][1]));
+          pb[i][cb][1] = movmatrix_trans(pack2<__half>(x[i][cb][2], x[i][cb][3]));
+        }
+      }
+      // ---- O^T += V^T P^T: thread (g, t) holds dimensions 16 g .. 16 g + 15 of four rows ----
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint4 v0 = piece(1, 16 * i + 2 * t, g), v1 = piece(1, 16 * i + 2 * t + 1, g);
+        const uint4 v2 = piece(1, 16 * i + 8 + 2 * t, g), v3 = piece(1, 16 * i + 9 + 2 * t, g);
+        const unsigned* w0p = reinterpret_cast<const unsigned*>(&v0);
+        const unsigned* w1p = reinterpret_cast<const unsigned*>(&v1);
+        const unsigned* w2p = reinterpret_cast<const unsigned*>(&v2);
+        const unsigned* w3p = reinterpret_cast<const unsigned*>(&v3);
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const unsigned sel = half ? 0x7362 : 0x5140;  // bytes 2 half, 2 half + 1 of two rows, interleaved
+            const unsigned ab = prepare_word<FMT>(__byte_perm(w0p[w], w1p[w], sel));
+            const unsigned cd = prepare_word<FMT>(__byte_perm(w2p[w], w3p[w], sel));
+            const unsigned af[4] = {half2_of<FMT, false>(ab), half2_of<FMT, true>(ab), half2_of<FMT, false>(cd), half2_of<FMT, true>(cd)};
+#pragma unroll
+            for (int cb = 0; cb < COLS; ++cb) mma_16816<__half>(o[cb][2 * w + half], af, pb[i][cb][0], pb[i][cb][1]);
+          }
+      }
+      ++used;
+    }
+
+    // ---- the CTA's partial of the segment: the warps add up in turn, in warp order ----
+    if (hi == w1) pdl_trigger();
+#pragma unroll
+    for (int cb = 0; cb < COLS; ++cb)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) l[cb][e] += __shfl_xor_sync(0xffffffffu, l[cb][e], off);
+        const int h = cb * 8 + 2 * t + e;
+        if (g == 0) {
+          sh.ml[warp][h][0] = M[cb][e];
+          sh.ml[warp][h][1] = m[cb][e];
+          sh.ml[warp][h][2] = l[cb][e];
+        }
+      }
+    __syncthreads();
+#pragma unroll 1
+    for (int turn = 0; turn < NW; ++turn) {
+      if (warp == turn) {
+#pragma unroll
+        for (int cb = 0; cb < COLS; ++cb)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int h = cb * 8 + 2 * t + e;
+            if (h >= G) continue;
+            float Ms = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < NW; ++w) Ms = fmaxf(Ms, sh.ml[w][h][0]);
+            const float f = M[cb][e] == -INFINITY && Ms == -INFINITY ? 1.f : ex2(M[cb][e] - Ms);
+            float4* dst = reinterpret_cast<float4*>(o_s + h * OS_PITCH + 16 * g);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              float4 y = make_float4(o[cb][2 * i][e] * f, o[cb][2 * i][2 + e] * f, o[cb][2 * i + 1][e] * f, o[cb][2 * i + 1][2 + e] * f);
+              if (turn) {
+                const float4 old = dst[i];
+                y.x += old.x, y.y += old.y, y.z += old.z, y.w += old.w;
+              }
+              dst[i] = y;
+            }
+          }
+      }
+      __syncthreads();
+    }
+    const int seg_no = b * a.KVH + kvh;
+    const int c_lo = owner(seg_lo), parts = owner(seg_hi - 1) - c_lo + 1;
+    const auto finish = [](float acc, float Ms, float ms, float L) {  // a head without rows: zero
+      return L == 0.f ? 0.f : acc / L * exp2f(Ms - ms - 15.f);
+    };
+    for (int h = 0; h < G; ++h) {
+      float Ms = -INFINITY, ms = -INFINITY, L = 0.f;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        Ms = fmaxf(Ms, sh.ml[w][h][0]);
+        ms = fmaxf(ms, sh.ml[w][h][1]);
+      }
+#pragma unroll
+      for (int w = 0; w < NW; ++w)
+        if (sh.ml[w][h][2] != 0.f) L = fmaf(sh.ml[w][h][2], ex2(sh.ml[w][h][1] - ms), L);
+      const float acc = o_s[h * OS_PITCH + tid];
+      if (parts == 1) {
+        static_cast<T*>(a.out)[(size_t)b * a.q_sb + (size_t)(kvh * G + h) * a.q_sh + tid] = from_float<T>(finish(acc, Ms, ms, L) * half2_unit<FMT>());
+      } else {
+        const size_t slot = (size_t)(c + seg_no) * G + h;  // (CTA, segment) pairs walk a staircase: their sum is unique
+        a.ws_o[slot * kHeadDim + tid] = acc;
+        if (tid == 0) a.ws_ml[slot] = make_float4(Ms, ms, L, 0.f);
+      }
+    }
+    if (parts > 1) {
+      __threadfence();
+      __syncthreads();
+      if (tid == 0) sh.last = atomicAdd(a.ws_cnt + seg_no, 1u) == (unsigned)(parts - 1);
+      __syncthreads();
+      if (sh.last) {
+        __threadfence();
+        // one warp per head, four dimensions per lane
+        for (int h = warp; h < G; h += NW) {
+          const size_t base = (size_t)(c_lo + seg_no) * G + h;
+          const float4* op = reinterpret_cast<const float4*>(a.ws_o + base * kHeadDim) + lane;
+          const float4* mp = a.ws_ml + base;
+          const int o_step = G * (kHeadDim / 4);
+          constexpr int PRE = 16;
+          float4 first_o[PRE];  // asked for together with the maxima
+#pragma unroll
+          for (int p = 0; p < PRE; ++p) first_o[p] = p < parts ? __ldcg(op + (size_t)p * o_step) : make_float4(0.f, 0.f, 0.f, 0.f);
+          float Ms = -INFINITY, ms = -INFINITY;
+          for (int p = lane; p < parts; p += 32) {
+            const float4 v = __ldcg(mp + (size_t)p * G);
+            Ms = fmaxf(Ms, v.x);
+            ms = fmaxf(ms, v.y);
+          }
+#pragma unroll
+          for (int off = 16; off > 0; off >>= 1) {
+            Ms = fmaxf(Ms, __shfl_xor_sync(0xffffffffu, Ms, off));
+            ms = fmaxf(ms, __shfl_xor_sync(0xffffffffu, ms, off));
+          }
+          float L = 0.f;
+          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+          const auto add = [&](const float4& v, float f) {
+            acc.x = fmaf(v.x, f, acc.x), acc.y = fmaf(v.y, f, acc.y), acc.z = fmaf(v.z, f, acc.z), acc.w = fmaf(v.w, f, acc.w);
+          };
+          for (int p0 = 0; p0 < parts; p0 += 32) {
+            float f = 0.f;
+            if (p0 + lane < parts) {
+              const float4 v = __ldcg(mp + (size_t)(p0 + lane) * G);
+              f = v.x == -INFINITY && Ms == -INFINITY ? 1.f : ex2(v.x - Ms);
+              if (v.z != 0.f) L = fmaf(v.z, ex2(v.y - ms), L);
+            }
+            const int n = min(32, parts - p0);
+            if (p0 == 0) {
+#pragma unroll
+              for (int p = 0; p < PRE; ++p) add(first_o[p], __shfl_sync(0xffffffffu, f, p));
+#pragma unroll 16
+              for (int p = PRE; p < n; ++p) add(__ldcg(op + (size_t)p * o_step), __shfl_sync(0xffffffffu, f, p));
+            } else {
+#pragma unroll 16
+              for (int p = 0; p < n; ++p) add(__ldcg(op + (size_t)(p0 + p) * o_step), __shfl_sync(0xffffffffu, f, p));
+            }
+          }
+#pragma unroll
+          for (int off = 16; off > 0; off >>= 1) L += __shfl_xor_sync(0xffffffffu, L, off);
+          T* dst = static_cast<T*>(a.out) + (size_t)b * a.q_sb + (size_t)(kvh * G + h) * a.q_sh + lane * 4;
+          dst[0] = from_float<T>(finish(acc.x, Ms, ms, L) * half2_unit<FMT>());
+          dst[1] = from_float<T>(finish(acc.y, Ms, ms, L) * half2_unit<FMT>());
+          dst[2] = from_float<T>(finish(acc.z, Ms, ms, L) * half2_unit<FMT>());
+          dst[3] = from_float<T>(finish(acc.w, Ms, ms, L) * half2_unit<FMT>());
+        }
+        if (tid == 0) a.ws_cnt[seg_no] = 0u;
+      }
+    }
+    // ---- the next segment ----
+    lo = hi;
+    if (lo < w1) {
+      __syncthreads();  // the merge buffers are free again
+      seg_lo = seg_hi;
+      seg.tile = seg.nt;
+      seg.forward(a, 0);
+    }
+  }
+  cp_async_wait<0>();
+  if (dead)  // let every copy that was asked for land (bounded) before the shared memory is given up
+    for (int i = used; i < asked; ++i) mbar_wait(&sh.full[warp][i % STAGES], (i / STAGES) & 1);
+}
+
+constexpr int smem_bytes(bool tma, int G) {
+  return NW * STAGES * (tma ? TMA_STAGE : ROWS_STAGE) + G * OS_PITCH * 4 + 1024;
+}
+
+// cudaFuncSetAttribute once per kernel and device.
+template <typename Kern>
+int allow_smem(Kern kern, int bytes, std::atomic<unsigned long long>& done) {
+  int dev = 0;
+  OMNIKV_CUDA_OK(cudaGetDevice(&dev));
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (done.load(std::memory_order_acquire) & bit) return OMNIKV_OK;
+  OMNIKV_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  done.fetch_or(bit, std::memory_order_release);
+  return OMNIKV_OK;
+}
+
+template <typename T, int FMT, int COLS, bool TMA>
+int launch(const A8Args& a, int ctas, const CUtensorMap& tm_k, const CUtensorMap& tm_v, cudaStream_t st) {
+  static std::atomic<unsigned long long> done{0};
+  auto kern = decode_attn_kv8_kernel<T, FMT, COLS, TMA>;
+  if (const int rc = allow_smem(kern, smem_bytes(TMA, 8 * COLS), done)) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(NT);
+  cfg.dynamicSmemBytes = smem_bytes(TMA, a.G);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  OMNIKV_CUDA_OK(cudaLaunchKernelEx(&cfg, kern, a, tm_k, tm_v));
+  return OMNIKV_OK;
+}
+
+template <typename T, int FMT>
+int launch_any(const A8Args& a, int ctas, bool tma, const CUtensorMap& tm_k, const CUtensorMap& tm_v, cudaStream_t st) {
+  if (a.G <= 8) return tma ? launch<T, FMT, 1, true>(a, ctas, tm_k, tm_v, st) : launch<T, FMT, 1, false>(a, ctas, tm_k, tm_v, st);
+  return tma ? launch<T, FMT, 2, true>(a, ctas, tm_k, tm_v, st) : launch<T, FMT, 2, false>(a, ctas, tm_k, tm_v, st);
+}
+
+constexpr long long kMaxCtas = 65536;
+
+inline long long slots_of(int B, int KVH, int ctas) { return (long long)ctas + (long long)B * KVH; }
 
 }  // namespace
 }  // namespace omnikv
 
-extern "C" size_t omnikv_kv8_attn_workspace_bytes(int B, int H, int n_splits) {
-  if (B <= 0 || H <= 0 || n_splits <= 0) return 0;
-  return omnikv::kAttnCntBytes +
-         (omnikv::attn_ws_o_floats(B, H, n_splits) + omnikv::attn_ws_ml_floats(B, H, n_splits)) * sizeof(float);
+extern "C" size_t omnikv_kv8_attn_workspace_bytes(int B, int H, int KVH, int n_ctas) {
+  using namespace omnikv;
+  if (B <= 0 || H <= 0 || KVH <= 0 || H % KVH || n_ctas <= 0) return 0;
+  return kAttnCntBytes + (size_t)slots_of(B, KVH, n_ctas) * (H / KVH) * (kHeadDim * sizeof(float) + sizeof(float4));
 }
 
 extern "C" int omnikv_kv8_decode_attn(const omnikv_kv8_attn_params* p, void* stream) {
@@ -144,14 +663,14 @@ extern "C" int omnikv_kv8_decode_attn(const omnikv_kv8_attn_params* p, void* str
   const omnikv_kv8_cache& c = p->cache;
   if (const int rc = check_kv8_cache(&c)) return rc;
   const auto bad16 = [](const void* q) { return !q || (reinterpret_cast<uintptr_t>(q) & 15); };
-  if (bad16(p->q) || bad16(p->out) || !p->len || p->H <= 0 || p->H % c.KVH || p->n_splits <= 0) return OMNIKV_E_BADARG;
+  if (bad16(p->q) || bad16(p->out) || !p->len || p->H <= 0 || p->H % c.KVH || p->n_ctas <= 0) return OMNIKV_E_BADARG;
   if (p->q_stride_b % 8 || p->q_stride_h % 8) return OMNIKV_E_BADARG;
   if (p->idx && (p->idx_cap <= 0 || p->idx_stride < 0)) return OMNIKV_E_BADARG;
   if (p->tail_len && !p->tail_start) return OMNIKV_E_BADARG;
   if (p->score_out && (p->idx || p->tail_len || !p->score_len || p->score_stride <= 0)) return OMNIKV_E_BADARG;
   if (!is_16bit(p->dtype) || p->H / c.KVH > MAX_G) return OMNIKV_E_UNSUPPORTED;
-  if (p->n_splits > 512 || (size_t)c.B * c.KVH * 4 > kAttnCntBytes) return OMNIKV_E_UNSUPPORTED;
-  if (!p->workspace || p->workspace_bytes < omnikv_kv8_attn_workspace_bytes(c.B, p->H, p->n_splits)) return OMNIKV_E_WORKSPACE;
+  if (p->n_ctas > kMaxCtas || (size_t)c.B * c.KVH * 4 > kAttnCntBytes) return OMNIKV_E_UNSUPPORTED;
+  if (!p->workspace || p->workspace_bytes < omnikv_kv8_attn_workspace_bytes(c.B, p->H, c.KVH, p->n_ctas)) return OMNIKV_E_WORKSPACE;
   if (bad16(p->workspace)) return OMNIKV_E_BADARG;
   A8Args a;
   a.k = static_cast<const unsigned char*>(c.k); a.v = static_cast<const unsigned char*>(c.v);
@@ -162,17 +681,21 @@ extern "C" int omnikv_kv8_decode_attn(const omnikv_kv8_attn_params* p, void* str
   a.idx = p->idx; a.idx_stride = p->idx_stride; a.idx_cap = p->idx_cap;
   a.len = p->len; a.tail_start = p->tail_start; a.tail_len = p->tail_len;
   a.score_out = p->score_out; a.score_stride = p->score_stride; a.score_len = p->score_len;
+  a.B = c.B; a.H = p->H; a.KVH = c.KVH; a.G = p->H / c.KVH;
   a.ws_cnt = static_cast<unsigned*>(p->workspace);
-  a.ws_o = reinterpret_cast<float*>(static_cast<unsigned char*>(p->workspace) + kAttnCntBytes);
-  a.ws_ml = a.ws_o + attn_ws_o_floats(c.B, p->H, p->n_splits);
-  a.B = c.B; a.H = p->H; a.KVH = c.KVH; a.G = p->H / c.KVH; a.S = p->n_splits;
+  a.ws_ml = reinterpret_cast<float4*>(static_cast<unsigned char*>(p->workspace) + kAttnCntBytes);
+  a.ws_o = reinterpret_cast<float*>(a.ws_ml + (size_t)slots_of(c.B, c.KVH, p->n_ctas) * a.G);
+  a.status = p->status;
   a.scale = p->scale;
+  a.pair = a.v == a.k + kHeadDim;  // V rows right behind their K rows: one copy brings both
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const dim3 grid(a.S, a.KVH, a.B);
+  // rows that follow one another come as boxes of a tensor map (where the layout can be described as one)
+  CUtensorMap tm_k = {}, tm_v = {};
+  const bool tma = !p->idx && !p->tail_len &&
+                   make_kv8_tensor_map(&tm_k, c.k, c.rows, c.KVH, c.B, c.stride_row, c.stride_h, c.stride_b, TILE) &&
+                   make_kv8_tensor_map(&tm_v, c.v, c.rows, c.KVH, c.B, c.stride_row, c.stride_h, c.stride_b, TILE);
   const bool i8 = c.format == kInt8;
-  auto kern = p->dtype == OMNIKV_BF16
-                  ? (i8 ? decode_attn_kv8_kernel<__nv_bfloat16, kInt8> : decode_attn_kv8_kernel<__nv_bfloat16, kE4m3>)
-                  : (i8 ? decode_attn_kv8_kernel<__half, kInt8> : decode_attn_kv8_kernel<__half, kE4m3>);
-  OMNIKV_CUDA_OK(launch_pdl(kern, grid, dim3(NT), 0, st, a));
-  return OMNIKV_OK;
+  if (p->dtype == OMNIKV_BF16)
+    return i8 ? launch_any<__nv_bfloat16, kInt8>(a, p->n_ctas, tma, tm_k, tm_v, st) : launch_any<__nv_bfloat16, kE4m3>(a, p->n_ctas, tma, tm_k, tm_v, st);
+  return i8 ? launch_any<__half, kInt8>(a, p->n_ctas, tma, tm_k, tm_v, st) : launch_any<__half, kE4m3>(a, p->n_ctas, tma, tm_k, tm_v, st);
 }

@@ -78,6 +78,10 @@ inline int check_kv8_cache(const omnikv_kv8_cache* c) {
   if (c->B > 65535 || c->KVH > 32767) return OMNIKV_E_UNSUPPORTED;  // grid dimensions
   return OMNIKV_OK;
 }
+// Tensor map over the codes of an 8-bit cache (false: the layout cannot be described as one).
+bool make_kv8_tensor_map(CUtensorMap* map, const void* base, int64_t rows, int KVH, int B, int64_t sr, int64_t sh,
+                         int64_t sb, int box_rows);
+
 inline bool is_16bit(int dtype) { return dtype == OMNIKV_BF16 || dtype == OMNIKV_F16; }
 
 }  // namespace omnikv

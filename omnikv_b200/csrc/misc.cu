@@ -62,6 +62,24 @@ bool make_matrix_tensor_map(CUtensorMap* map, bool is_bf16, const void* base, in
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// 4-D map [B, KVH, rows, d] of bytes over the codes of an 8-bit cache; box 128 x box_rows rows, 128-byte swizzle.
+bool make_kv8_tensor_map(CUtensorMap* map, const void* base, int64_t rows, int KVH, int B, int64_t sr, int64_t sh,
+                         int64_t sb, int box_rows) {
+  PFN_encodeTiled enc = encode_tiled_fn();
+  if (!enc) return false;
+  // a dimension of extent 1 still needs a legal stride
+  if (KVH == 1 && (sh <= 0 || sh % 16)) sh = sr * rows;
+  if (B == 1 && (sb <= 0 || sb % 16)) sb = sh * KVH;
+  if (sr <= 0 || sh <= 0 || sb <= 0) return false;
+  const cuuint64_t dims[4] = {(cuuint64_t)kHeadDim, (cuuint64_t)rows, (cuuint64_t)KVH, (cuuint64_t)B};
+  const cuuint64_t strides[3] = {(cuuint64_t)sr, (cuuint64_t)sh, (cuuint64_t)sb};
+  const cuuint32_t box[4] = {(cuuint32_t)kHeadDim, (cuuint32_t)box_rows, 1, 1};
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(base), dims, strides, box, estr,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 static thread_local char g_last_error[256] = "";
 
 int record_cuda_error(cudaError_t e, const char* where) {

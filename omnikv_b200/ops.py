@@ -655,7 +655,8 @@ def kv8_decode_attn(q: torch.Tensor, k8, v8, k_scale, v_scale, len_a: torch.Tens
     """``omnikv_kv8_decode_attn``: ``decode_attn`` over an 8-bit cache.  q 16-bit ``[B,H,128]``; the rows of a sequence
     are positions ``[0, len_a[b])``, or ``idx[b][0..len_a[b])`` (int32 ``[B, cap]``) followed by the ``tail_len[b]``
     positions from ``tail_start[b]`` of the same cache.  ``score_out`` ``[KVH,B,stride]`` fp32 (without ``idx`` and tail):
-    selector-``last`` scores of positions ``< score_len[b]``.  ``max_rows`` (default: all) only sizes the splits."""
+    selector-``last`` scores of positions ``< score_len[b]``.  ``n_splits``: CTAs per (sequence, KV head) on average
+    (default: as many as the GPU holds); ``max_rows`` (default: all) is only a hint for that number."""
     dev = _on(q, k8, v8, k_scale, v_scale, len_a, idx, tail_start, tail_len, out, score_out, score_len, ws)
     p = abi.Kv8AttnParams()
     p.cache = c = _kv8_cache(k8, v8, k_scale, v_scale, block)
@@ -690,8 +691,9 @@ def kv8_decode_attn(q: torch.Tensor, k8, v8, k_scale, v_scale, len_a: torch.Tens
                 or not score_out.is_contiguous() or score_out.shape[2] == 0:
             raise abi.OmniKVError("kv8_decode_attn: score_out must be contiguous fp32 [KVH, B, stride]")
         p.score_out, p.score_stride, p.score_len = score_out.data_ptr(), score_out.shape[2], score_len.data_ptr()
-    p.n_splits = int(n_splits or default_splits(B, KVH, max_rows or cap, dev))
-    need = abi.lib().omnikv_kv8_attn_workspace_bytes(B, H, p.n_splits)
+    # two CTAs per SM, each with at least four tiles of 32 rows (the kernel cuts the rows that there are into equal pieces)
+    p.n_ctas = n_splits * B * KVH if n_splits else min(2 * sm_count(dev), max(1, (max_rows or cap) // 128 + 1) * B * KVH)
+    need = abi.lib().omnikv_kv8_attn_workspace_bytes(B, H, KVH, p.n_ctas)
     if ws is None:
         ws = _own_workspace(dev, need, "kv8_attn")
     p.workspace, p.workspace_bytes = ws.data_ptr(), ws.numel() * ws.element_size()

@@ -47,17 +47,17 @@ def test_attention_arguments_are_checked():
         p = abi.Kv8AttnParams()
         p.cache, p.dtype, p.H, p.scale = _cache(abi), abi.BF16, 32, 0.1
         p.q = p.out = p.len = p.workspace = 256
-        p.q_stride_b, p.q_stride_h, p.n_splits = 4096, 128, 4
-        p.workspace_bytes = lib.omnikv_kv8_attn_workspace_bytes(1, 32, 4)
+        p.q_stride_b, p.q_stride_h, p.n_ctas = 4096, 128, 4
+        p.workspace_bytes = lib.omnikv_kv8_attn_workspace_bytes(1, 32, 8, 4)
         for name, v in change.items():
             setattr(p, name, v)
         return lib.omnikv_kv8_decode_attn(ctypes.byref(p), None)
 
-    for change in (dict(q=None), dict(q=8), dict(len=None), dict(H=30), dict(n_splits=0), dict(q_stride_h=4), dict(idx=256),
+    for change in (dict(q=None), dict(q=8), dict(len=None), dict(H=30), dict(n_ctas=0), dict(q_stride_h=4), dict(idx=256),
                    dict(tail_len=256), dict(score_out=256), dict(score_out=256, score_len=256, score_stride=8, idx=256, idx_cap=4),
                    dict(workspace=264)):
         assert call(**change) == -1, change
-    for change in (dict(dtype=abi.F32), dict(H=136), dict(n_splits=513)):
+    for change in (dict(dtype=abi.F32), dict(H=136), dict(n_ctas=65537)):
         assert call(**change) == -2, change
     assert call(workspace_bytes=16384) == -3 and call(workspace=None) == -3
     assert lib.omnikv_kv8_decode_attn(None, None) == -1

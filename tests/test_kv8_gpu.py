@@ -483,7 +483,7 @@ def test_refusals():
         lambda: o.kv8_decode_attn(q, *cache, n, block=16, tail_len=n),
         lambda: o.kv8_decode_attn(q, *cache, n, block=16, score_out=torch.zeros(2, 2, 64, device="cuda")),
         lambda: o.kv8_decode_attn(q, *cache, n, block=16, out=torch.empty(2, 4, D, device="cuda")),
-        lambda: o.kv8_decode_attn(q, *cache, n, block=16, n_splits=513),
+        lambda: o.kv8_decode_attn(q, *cache, n, block=16, n_splits=20000),
         lambda: o.kv8_decode_attn(q, *cache, n, block=16, ws=torch.zeros(64, dtype=torch.uint8, device="cuda")),
         lambda: o.kv8_decode_attn(torch.zeros(2, 34, D, dtype=torch.bfloat16, device="cuda"), *cache, n, block=16),
         lambda: o.kv8_alloc(1, 1, 16, block=16, dtype=torch.uint8, device="cuda"),
