@@ -615,8 +615,8 @@ int omnikv_kv8_decode_attn(const omnikv_kv8_attn_params* p, void* stream);
  * int8, rows of K contiguous codes, K a multiple of 16, row strides (elements) multiples of 16, bases 16-byte aligned.
  * out: OMNIKV_F32 or a 16-bit type, residual of the same type (may alias out).  omnikv_quant_rows serves the activations
  * of a call and, once, a weight matrix [channels, K].
- * The workspace of omnikv_linear_w8a8 (omnikv_linear_w8a8_workspace_bytes, may be 0 bytes) starts with counters that are
- * ZERO before its first use and are left zero; calls that share it must not overlap.
+ * The workspace of omnikv_linear_w8a8 (omnikv_linear_w8a8_workspace_bytes, may be 0 bytes) starts with 1 KiB of counters
+ * that are ZERO before its first use and are left zero; calls that share it must not overlap.
  * ------------------------------------------------------------------------------------------ */
 int omnikv_quant_rows(int dtype, const void* x, int64_t x_stride_row, int n, int K, int8_t* codes, int64_t code_stride_row,
                       float* scale, void* stream);

@@ -221,7 +221,7 @@ decode_attn_kv8_kernel(const A8Args a, const __grid_constant__ CUtensorMap tm_k,
     pos = -1;
     if (ahead_w < w1) {
       const int r = ahead.tile * TILE + lane;
-      if (r < ahead.list.nA) pos = a.idx ? __ldg(a.idx + (size_t)ahead.b * a.idx_stride + r) : r;
+      if (r < ahead.list.nA) pos = a.idx ? a.idx[(size_t)ahead.b * a.idx_stride + r] : r;
       else if (r < ahead.list.n()) pos = ahead.list.t0 + (r - ahead.list.nA);
     }
   };
@@ -605,18 +605,6 @@ decode_attn_kv8_kernel(const A8Args a, const __grid_constant__ CUtensorMap tm_k,
 
 constexpr int smem_bytes(bool tma, int G) {
   return NW * STAGES * (tma ? TMA_STAGE : ROWS_STAGE) + G * OS_PITCH * 4 + 1024;
-}
-
-// cudaFuncSetAttribute once per kernel and device.
-template <typename Kern>
-int allow_smem(Kern kern, int bytes, std::atomic<unsigned long long>& done) {
-  int dev = 0;
-  OMNIKV_CUDA_OK(cudaGetDevice(&dev));
-  const unsigned long long bit = 1ull << (dev & 63);
-  if (done.load(std::memory_order_acquire) & bit) return OMNIKV_OK;
-  OMNIKV_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-  done.fetch_or(bit, std::memory_order_release);
-  return OMNIKV_OK;
 }
 
 template <typename T, int FMT, int COLS, bool TMA>

@@ -53,7 +53,7 @@ __global__ void __launch_bounds__(ST_THREADS) kv8_store_kernel(const StoreArgs a
   for (int p = 0; p < PASSES; ++p) {
     const int r = r0 + p * ST_ROWS + row16;
     x[p] = make_uint4(0, 0, 0, 0);
-    if (r < n) x[p] = __ldg(reinterpret_cast<const uint4*>(src + (size_t)r * s_sr) + lane16);
+    if (r < n) x[p] = reinterpret_cast<const uint4*>(src + (size_t)r * s_sr)[lane16];
   }
   __syncthreads();
 #pragma unroll

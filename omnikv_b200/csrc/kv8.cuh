@@ -3,6 +3,8 @@
 
 #include <cuda_fp8.h>
 
+#include <atomic>
+
 #include "common.cuh"
 
 namespace omnikv {
@@ -81,6 +83,21 @@ inline int check_kv8_cache(const omnikv_kv8_cache* c) {
 // Tensor map over the codes of an 8-bit cache (false: the layout cannot be described as one).
 bool make_kv8_tensor_map(CUtensorMap* map, const void* base, int64_t rows, int KVH, int B, int64_t sr, int64_t sh,
                          int64_t sb, int box_rows);
+
+// Tensor map over a row-major matrix of bytes: box 128 bytes x box_rows rows, 128-byte swizzle, zeros past its edges.
+bool make_bytes_tensor_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t ld, int box_rows);
+
+// cudaFuncSetAttribute once per kernel and device.
+template <typename Kern>
+int allow_smem(Kern kern, int bytes, std::atomic<unsigned long long>& done) {
+  int dev = 0;
+  OMNIKV_CUDA_OK(cudaGetDevice(&dev));
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (done.load(std::memory_order_acquire) & bit) return OMNIKV_OK;
+  OMNIKV_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  done.fetch_or(bit, std::memory_order_release);
+  return OMNIKV_OK;
+}
 
 inline bool is_16bit(int dtype) { return dtype == OMNIKV_BF16 || dtype == OMNIKV_F16; }
 

@@ -1,5 +1,16 @@
 // Matrix products in 8-bit integers, one scale per token and per output channel, and the row quantiser in front.
+//
+//     out[t][c] = (sum_k x[t][k] w[c][k]) * x_scale[t] * w_scale[c] (+ residual[t][c])
+//
+// The sum is an integer (|sum| <= 128 * 128 * 32768 = 2^29), so it is exact and independent of the order in which slices
+// of K are added.  Up to 16 tokens the call is a stream of the weights (HBM bound: K * channels bytes) and runs on
+// mma.sync; more tokens run on tcgen05 (kind::i8) with the channels on the M side, which leaves the N side to a token
+// count of any size.
+#include <atomic>
+#include <type_traits>
+
 #include "kv8.cuh"
+#include "tc05.cuh"
 
 namespace omnikv {
 namespace {
@@ -14,6 +25,7 @@ __global__ void __launch_bounds__(THREADS) quant_rows_kernel(const T* x, int64_t
                                                              float* scale) {
   __shared__ unsigned top[THREADS / 32];
   pdl_wait();
+  pdl_trigger();  // the product behind it may set itself up; it waits for this grid before it reads anything
   const int row = blockIdx.x, tid = threadIdx.x, nvec = K / 8;
   const uint4* src = reinterpret_cast<const uint4*>(x + (size_t)row * x_sr);
   uint4 v[QR_VEC];
@@ -54,7 +66,6 @@ __global__ void __launch_bounds__(THREADS) quant_rows_kernel(const T* x, int64_t
   }
 }
 
-// ---- the product: one thread per output -----------------------------------------------------------------------------
 struct LinArgs {
   const int8_t* x;
   int64_t x_sr;
@@ -67,26 +78,379 @@ struct LinArgs {
   void* out;
   int64_t out_sr;
   int n, N, K;
+  int* counters;  // tile kernel with slices of K: [tiles] arrivals, zero between launches
+  int* part;      // [tiles][slices][tokens of a tile][128]
+  int* status;
+  int S, token_tiles, chunks;
 };
 
-template <typename T>
-__global__ void __launch_bounds__(256) linear_w8a8_kernel(const LinArgs a) {
+// ---- up to 16 tokens: a stream of the weights -------------------------------------------------------------------------
+// A CTA owns 16 channels, its eight warps take 64-byte chunks of K in turn.  The fragments of m16n8k32 come straight from
+// global memory with 16-byte loads: inside a chunk of 64 the order of k is free as long as both operands agree, so thread
+// (g, t) takes bytes 16 t .. 16 t + 15 of rows g and g + 8 (weights) and of token g, and their words 0..3 are two MMAs.
+// Four chunks are asked for while the four before them are multiplied.  The eight integer sums meet in shared memory.
+constexpr int SK_THREADS = 256, SK_WARPS = SK_THREADS / 32, SK_ROWS = 16, SK_DEPTH = 4;
+
+__device__ __forceinline__ void mma_i8(int (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint4 ld_stream(const int8_t* p) {  // weights: read once
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+  return v;
+}
+
+// NB: blocks of eight tokens
+template <typename T, int NB>
+__global__ void __launch_bounds__(SK_THREADS, 2) linear_stream_kernel(const LinArgs a) {
+  __shared__ int sums[SK_WARPS][NB * 8][SK_ROWS + 1];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int c0 = blockIdx.x * SK_ROWS;
+  // While the kernel before finishes, this CTA's weights start on their way into L2.  Nothing is read: weights that the
+  // kernel before wrote would be wrong in registers, in L2 they are not.
+  if (tid < SK_ROWS && c0 + tid < a.N)
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;\n" ::"l"(a.w + (size_t)(c0 + tid) * a.w_sr), "r"(a.K) : "memory");
   pdl_wait();
-  const int c = blockIdx.x * 32 + (threadIdx.x >> 3), t = blockIdx.y * 8 + (threadIdx.x & 7);
-  if (c >= a.N || t >= a.n) return;
-  const int4* w = reinterpret_cast<const int4*>(a.w + (size_t)c * a.w_sr);
-  const int4* x = reinterpret_cast<const int4*>(a.x + (size_t)t * a.x_sr);
-  int acc = 0;
-  for (int i = 0; i < a.K / 16; ++i) {
-    const int4 p = w[i], q = x[i];
-    acc = __dp4a(p.x, q.x, __dp4a(p.y, q.y, __dp4a(p.z, q.z, __dp4a(p.w, q.w, acc))));
+  pdl_trigger();
+  const int8_t* w0 = a.w + (size_t)min(c0 + g, a.N - 1) * a.w_sr + 16 * t;  // rows past the end: read again, dropped below
+  const int8_t* w1 = a.w + (size_t)min(c0 + g + 8, a.N - 1) * a.w_sr + 16 * t;
+  const int8_t* xp[NB];
+#pragma unroll
+  for (int b = 0; b < NB; ++b) xp[b] = a.x + (size_t)min(b * 8 + g, a.n - 1) * a.x_sr + 16 * t;
+  const int chunks = (a.K + 63) >> 6;
+  int acc[NB][4];
+#pragma unroll
+  for (int b = 0; b < NB; ++b) acc[b][0] = acc[b][1] = acc[b][2] = acc[b][3] = 0;
+  uint4 wa[2][SK_DEPTH][2], xb[2][SK_DEPTH][NB];
+  const auto fetch = [&](int buf, int first) {
+#pragma unroll
+    for (int u = 0; u < SK_DEPTH; ++u) {
+      const int k = (first + u * SK_WARPS) * 64;
+      const bool in = k + 16 * t < a.K;
+      wa[buf][u][0] = in ? ld_stream(w0 + k) : make_uint4(0, 0, 0, 0);
+      wa[buf][u][1] = in ? ld_stream(w1 + k) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int b = 0; b < NB; ++b) xb[buf][u][b] = in ? *reinterpret_cast<const uint4*>(xp[b] + k) : make_uint4(0, 0, 0, 0);
+    }
+  };
+  const auto multiply = [&](int buf) {
+#pragma unroll
+    for (int u = 0; u < SK_DEPTH; ++u) {
+      const uint4 p = wa[buf][u][0], q = wa[buf][u][1];
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        mma_i8(acc[b], p.x, q.x, p.y, q.y, xb[buf][u][b].x, xb[buf][u][b].y);
+        mma_i8(acc[b], p.z, q.z, p.w, q.w, xb[buf][u][b].z, xb[buf][u][b].w);
+      }
+    }
+  };
+  constexpr int STEP = SK_DEPTH * SK_WARPS;
+  fetch(0, warp);
+  for (int c = warp; c < chunks; c += 2 * STEP) {
+    fetch(1, c + STEP);
+    multiply(0);
+    if (c + STEP >= chunks) break;
+    fetch(0, c + 2 * STEP);
+    multiply(1);
   }
-  float y = (float)acc * a.x_scale[t] * a.w_scale[c];
-  if (a.res) y += to_float(static_cast<const T*>(a.res)[(size_t)t * a.res_sr + c]);
-  static_cast<T*>(a.out)[(size_t)t * a.out_sr + c] = from_float<T>(y);
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sums[warp][b * 8 + 2 * t + (e & 1)][g + 8 * (e >> 1)] = acc[b][e];
+  __syncthreads();
+  const int tok = tid / SK_ROWS, c = c0 + tid % SK_ROWS;
+  if (tok >= NB * 8 || tok >= a.n || c >= a.N) return;
+  int sum = 0;
+#pragma unroll
+  for (int w = 0; w < SK_WARPS; ++w) sum += sums[w][tok][tid % SK_ROWS];
+  float y = (float)sum * a.x_scale[tok] * a.w_scale[c];
+  if (a.res) y += to_float(static_cast<const T*>(a.res)[(size_t)tok * a.res_sr + c]);
+  static_cast<T*>(a.out)[(size_t)tok * a.out_sr + c] = from_float<T>(y);
+}
+
+// ---- more tokens: tiles of 128 channels x BN tokens on tcgen05 -----------------------------------------------------------
+// Warp 4 fetches 128-byte wide boxes of weights and tokens (TMA, 128-byte swizzle), warp 5 issues the MMAs (K = 32 bytes
+// each), int32 accumulators in tensor memory, two of them so that the epilogue of a tile runs under the next tile's MMAs.
+// Warps 0-3 read a tile back: thread = channel (TMEM lane), columns = tokens, so a warp's store is 32 neighbouring channels
+// of a token whatever the alignment of the output.  When there are too few tiles for the GPU, K is cut into slices: their
+// integer sums go to the workspace and the CTA that arrives last at a tile adds them up.
+constexpr int TK_M = 128, TK_KB = 128, TK_THREADS = 192, TK_CTAS = 148;
+
+template <int BN>
+struct TkShape {
+  static constexpr int STAGE = (TK_M + BN) * TK_KB;
+  static constexpr int STAGES = BN >= 256 ? 4 : (BN >= 128 ? 6 : 8);
+  static constexpr int SMEM = STAGES * STAGE + 1024;
+};
+
+__device__ __forceinline__ void tc_mma_i8(unsigned d_tmem, uint64_t a_desc, uint64_t b_desc, unsigned idesc, unsigned accumulate) {
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      "setp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n"
+      "}\n" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Instruction descriptor (kind::i8): s32 accumulator, signed 8-bit A and B, both K-major.
+__host__ __device__ constexpr unsigned i8_instr_desc(int M, int N) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | ((unsigned)(N >> 3) << 17) | ((unsigned)(M >> 4) << 24);
+}
+// 16 consecutive 32-bit columns of this thread's TMEM lane
+__device__ __forceinline__ void tmem_ld16i(unsigned taddr, int (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void epilogue_bar() { asm volatile("bar.sync 1, 128;\n" ::: "memory"); }
+__device__ __forceinline__ bool epilogue_any(bool pred) {  // OR over the 128 epilogue threads
+  unsigned r;
+  asm volatile(
+      "{\n"
+      ".reg .pred p, q;\n"
+      "setp.ne.b32 p, %1, 0;\n"
+      "barrier.cta.red.or.pred q, 1, 128, p;\n"
+      "selp.u32 %0, 1, 0, q;\n"
+      "}\n"
+      : "=r"(r)
+      : "r"((unsigned)pred)
+      : "memory");
+  return r != 0;
+}
+
+struct TkShared {
+  uint64_t full[8], empty[8], acc_full[2], acc_empty[2];
+  unsigned tmem_base;
+  int fail, issued, last;
+};
+
+template <typename T, int BN>
+__global__ void __launch_bounds__(TK_THREADS, 1)
+linear_tile_kernel(const LinArgs a, const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x) {
+  extern __shared__ __align__(128) unsigned char smem_raw[];
+  __shared__ TkShared sh;
+  constexpr int STAGES = TkShape<BN>::STAGES, STAGE = TkShape<BN>::STAGE;
+  constexpr unsigned TMEM_COLS = 2 * BN;
+  unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int S = a.S, units = ceil_div(a.N, TK_M) * a.token_tiles * S;
+
+  if (tid == 0) {
+    sh.fail = 0;
+    sh.issued = 0;
+    for (int i = 0; i < STAGES; ++i) {
+      mbar_init(&sh.full[i], 1);
+      mbar_init(&sh.empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sh.acc_full[i], 1);
+      mbar_init(&sh.acc_empty[i], 128);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+  }
+  __syncwarp();
+  if (warp == 0) {
+    tmem_alloc(&sh.tmem_base, TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const unsigned tmem = sh.tmem_base;
+  pdl_wait();
+  pdl_trigger();
+  // unit u: slice u % S of tile u / S; the tiles of a block of channels follow one another
+  const auto slice_lo = [&](int s) { return (int)((long long)s * a.chunks / S); };
+
+  if (warp == 4) {
+    if (lane == 0) {
+      int it = 0;
+      for (int u = blockIdx.x; u < units && !sh.fail; u += gridDim.x) {
+        const int s = u % S, tile = u / S, tt = tile % a.token_tiles, ct = tile / a.token_tiles;
+        const int k1 = slice_lo(s + 1);
+        for (int k = slice_lo(s); k < k1; ++k, ++it) {
+          const int st = it % STAGES;
+          if (!mbar_wait(&sh.empty[st], ((it / STAGES) & 1) ^ 1, &sh.fail)) {
+            if (!sh.fail && a.status) atomicExch(a.status, 7);
+            sh.fail = 1;
+            break;
+          }
+          unsigned char* dst = ring + (size_t)st * STAGE;
+          mbar_expect_tx(&sh.full[st], STAGE);
+          tma_load_2d(dst, &tm_w, k * TK_KB, ct * TK_M, &sh.full[st]);
+          tma_load_2d(dst + TK_M * TK_KB, &tm_x, k * TK_KB, tt * BN, &sh.full[st]);
+          sh.issued = it + 1;
+        }
+      }
+    }
+  } else if (warp == 5) {
+    if (lane == 0) {
+      constexpr unsigned idesc = i8_instr_desc(TK_M, BN);
+      bool ok = true;
+      int it = 0, n = 0;
+      for (int u = blockIdx.x; ok && u < units; u += gridDim.x, ++n) {
+        const int buf = n & 1, s = u % S, k0 = slice_lo(s), k1 = slice_lo(s + 1);
+        if (!mbar_wait(&sh.acc_empty[buf], ((n >> 1) & 1) ^ 1, &sh.fail)) { ok = false; break; }
+        tc_fence_after();
+        const unsigned d_tmem = tmem + (unsigned)buf * BN;
+        for (int k = k0; k < k1; ++k, ++it) {
+          const int st = it % STAGES;
+          if (!mbar_wait(&sh.full[st], (it / STAGES) & 1, &sh.fail)) { ok = false; break; }
+          tc_fence_after();
+          const unsigned w_base = smem_u32(ring + (size_t)st * STAGE), x_base = w_base + TK_M * TK_KB;
+#pragma unroll
+          for (int j = 0; j < TK_KB / 32; ++j)
+            tc_mma_i8(d_tmem, smem_desc_sw128(w_base + j * 32), smem_desc_sw128(x_base + j * 32), idesc, (k > k0 || j) ? 1u : 0u);
+          tc_commit(&sh.empty[st]);
+        }
+        if (ok) tc_commit(&sh.acc_full[buf]);
+      }
+      if (!ok) {
+        if (!sh.fail && a.status) atomicExch(a.status, 7);
+        sh.fail = 1;
+      }
+    }
+  } else {
+    int n = 0;
+    for (int u = blockIdx.x; u < units; u += gridDim.x, ++n) {
+      const int buf = n & 1, s = u % S, tile = u / S, t0 = (tile % a.token_tiles) * BN, c = (tile / a.token_tiles) * TK_M + tid;
+      const bool got = mbar_wait(&sh.acc_full[buf], (n >> 1) & 1, &sh.fail);
+      if (epilogue_any(!got)) {  // the 128 threads leave together
+        if (!sh.fail && a.status) atomicExch(a.status, 7);
+        sh.fail = 1;
+        break;
+      }
+      tc_fence_after();
+      const unsigned src = tmem + ((unsigned)(warp * 32) << 16) + (unsigned)buf * BN;
+      const int tokens = min(BN, a.n - t0);
+      const float ws = c < a.N ? a.w_scale[c] : 0.f;
+      const T* res = static_cast<const T*>(a.res);
+      T* out = static_cast<T*>(a.out);
+      const auto finish = [&](int j0, const int (&v)[16]) {  // 16 tokens of this thread's channel
+        float r[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          r[j] = res && c < a.N && j0 + j < tokens ? to_float(res[(size_t)(t0 + j0 + j) * a.res_sr + c]) : 0.f;
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          if (c < a.N && j0 + j < tokens) {
+            const float y = (float)v[j] * a.x_scale[t0 + j0 + j] * ws;
+            out[(size_t)(t0 + j0 + j) * a.out_sr + c] = from_float<T>(y + r[j]);
+          }
+      };
+      int* part = a.part + ((size_t)tile * S + s) * BN * TK_M + tid;
+#pragma unroll 1
+      for (int j0 = 0; j0 < tokens; j0 += 16) {
+        int v[16];
+        tmem_ld16i(src + j0, v);
+        tmem_ld_wait();
+        if (S == 1) {
+          finish(j0, v);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) __stcg(part + (j0 + j) * TK_M, v[j]);
+        }
+      }
+      tc_fence_before();
+      mbar_arrive(&sh.acc_empty[buf]);
+      if (S == 1) continue;
+      __threadfence();
+      epilogue_bar();
+      if (tid == 0) {
+        sh.last = atomicAdd(a.counters + tile, 1) == S - 1;
+        if (sh.last) a.counters[tile] = 0;  // nobody else touches it any more in this call
+      }
+      epilogue_bar();
+      if (sh.last) {
+        __threadfence();
+        const int* all = a.part + (size_t)tile * S * BN * TK_M + tid;
+#pragma unroll 1
+        for (int j0 = 0; j0 < tokens; j0 += 16) {
+          int v[16];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) v[j] = 0;
+          for (int q = 0; q < S; ++q)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] += __ldcg(all + ((size_t)q * BN + j0 + j) * TK_M);
+          finish(j0, v);
+        }
+      }
+      epilogue_bar();  // sh.last is used again
+    }
+  }
+
+  // ---- teardown ----
+  tc_fence_before();
+  __syncthreads();
+  if (sh.fail) {
+    if (tid == 128) {  // wait (bounded) for the last requested tile of every stage before the memory is given up
+      for (int st = 0; st < STAGES; ++st) {
+        const int last = sh.issued - 1 - ((sh.issued - 1 - st) % STAGES + STAGES) % STAGES;
+        if (sh.issued > st && last >= 0) mbar_wait(&sh.full[st], (last / STAGES) & 1);
+      }
+    }
+    __syncthreads();
+  }
+  if (warp == 0) {
+    tc_fence_after();
+    tmem_dealloc(tmem, TMEM_COLS);
+  }
+}
+
+// ---- which kernel, and how K is cut -------------------------------------------------------------------------------------
+constexpr int kStreamTokens = 16;
+
+struct TilePlan {
+  int BN, token_tiles, tiles, S, chunks;
+};
+inline TilePlan tile_plan(int n, int N, int K) {
+  TilePlan p;
+  p.BN = n <= 32 ? 32 : n <= 64 ? 64 : n <= 128 ? 128 : 256;
+  p.token_tiles = ceil_div(n, p.BN);
+  p.tiles = p.token_tiles * ceil_div(N, TK_M);
+  p.chunks = ceil_div(K, TK_KB);
+  // slices: as many as keep all SMs busy, of four chunks at least
+  p.S = p.tiles >= TK_CTAS ? 1 : max(1, min(TK_CTAS / p.tiles, p.chunks / 4));
+  return p;
+}
+inline size_t tile_workspace(const TilePlan& p) {
+  return p.S == 1 ? 0 : 1024 + (size_t)p.tiles * p.S * p.BN * TK_M * sizeof(int);  // counters: tiles < 148
 }
 
 inline bool bad16(const void* p) { return !p || (reinterpret_cast<uintptr_t>(p) & 15); }
+
+template <typename T, int BN>
+int launch_tile(const LinArgs& a, const TilePlan& pl, cudaStream_t st) {
+  static std::atomic<unsigned long long> done{0};
+  auto kern = linear_tile_kernel<T, BN>;
+  if (const int rc = allow_smem(kern, TkShape<BN>::SMEM, done)) return rc;
+  CUtensorMap tm_w, tm_x;
+  if (!make_bytes_tensor_map(&tm_w, a.w, a.N, a.K, a.w_sr, TK_M) || !make_bytes_tensor_map(&tm_x, a.x, a.n, a.K, a.x_sr, BN))
+    return OMNIKV_E_UNSUPPORTED;
+  OMNIKV_CUDA_OK(launch_pdl_smem_args(kern, dim3(min(TK_CTAS, pl.tiles * pl.S)), dim3(TK_THREADS), TkShape<BN>::SMEM, st, a, tm_w, tm_x));
+  return OMNIKV_OK;
+}
+
+template <typename T>
+int launch_linear(const LinArgs& a, const TilePlan& pl, cudaStream_t st) {
+  if (a.n <= kStreamTokens) {
+    auto kern = a.n <= 8 ? linear_stream_kernel<T, 1> : linear_stream_kernel<T, 2>;
+    OMNIKV_CUDA_OK(launch_pdl(kern, dim3(ceil_div(a.N, SK_ROWS)), dim3(SK_THREADS), 0, st, a));
+    return OMNIKV_OK;
+  }
+  switch (pl.BN) {
+    case 32: return launch_tile<T, 32>(a, pl, st);
+    case 64: return launch_tile<T, 64>(a, pl, st);
+    case 128: return launch_tile<T, 128>(a, pl, st);
+    default: return launch_tile<T, 256>(a, pl, st);
+  }
+}
 
 }  // namespace
 }  // namespace omnikv
@@ -113,7 +477,11 @@ extern "C" int omnikv_quant_rows(int dtype, const void* x, int64_t x_stride_row,
   return small ? go(__half(), Small()) : go(__half(), Large());
 }
 
-extern "C" size_t omnikv_linear_w8a8_workspace_bytes(int, int, int) { return 0; }
+extern "C" size_t omnikv_linear_w8a8_workspace_bytes(int n_tokens, int channels, int K) {
+  using namespace omnikv;
+  if (n_tokens <= kStreamTokens || channels <= 0 || K <= 0) return 0;
+  return tile_workspace(tile_plan(n_tokens, channels, K));
+}
 
 extern "C" int omnikv_linear_w8a8(const omnikv_linear_w8a8_params* p, void* stream) {
   using namespace omnikv;
@@ -124,10 +492,20 @@ extern "C" int omnikv_linear_w8a8(const omnikv_linear_w8a8_params* p, void* stre
   if (p->K > 32768 || (p->out_dtype != OMNIKV_F32 && !is_16bit(p->out_dtype))) return OMNIKV_E_UNSUPPORTED;
   LinArgs a{p->x, p->x_stride_row, p->x_scale, p->w, p->w_stride_row, p->w_scale, p->residual, p->residual_stride_row,
             p->out, p->out_stride_row, p->n_tokens, p->channels, p->K};
+  const TilePlan pl = tile_plan(a.n, a.N, a.K);
+  const size_t need = a.n <= kStreamTokens ? 0 : tile_workspace(pl);
+  if (need && (!p->workspace || p->workspace_bytes < need)) return OMNIKV_E_WORKSPACE;
+  if (need && bad16(p->workspace)) return OMNIKV_E_BADARG;
+  a.counters = static_cast<int*>(p->workspace);
+  a.part = a.counters + 256;
+  a.status = p->status;
+  a.S = pl.S;
+  a.token_tiles = pl.token_tiles;
+  a.chunks = pl.chunks;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const dim3 grid(ceil_div(a.N, 32), ceil_div(a.n, 8));
-  auto kern = p->out_dtype == OMNIKV_F32 ? linear_w8a8_kernel<float>
-              : p->out_dtype == OMNIKV_BF16 ? linear_w8a8_kernel<__nv_bfloat16> : linear_w8a8_kernel<__half>;
-  OMNIKV_CUDA_OK(launch_pdl(kern, grid, dim3(256), 0, st, a));
-  return OMNIKV_OK;
+  switch (p->out_dtype) {
+    case OMNIKV_F32: return launch_linear<float>(a, pl, st);
+    case OMNIKV_BF16: return launch_linear<__nv_bfloat16>(a, pl, st);
+    default: return launch_linear<__half>(a, pl, st);
+  }
 }
