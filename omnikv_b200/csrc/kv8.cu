@@ -59,12 +59,10 @@ __global__ void __launch_bounds__(ST_THREADS) kv8_store_kernel(const StoreArgs a
 #pragma unroll
   for (int p = 0; p < PASSES; ++p) {
     const unsigned* w = reinterpret_cast<const unsigned*>(&x[p]);
-    unsigned m = 0;
+    unsigned m2 = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = unpack16<T>(w[i]);
-      m = max(m, max(abs_bits(f.x), abs_bits(f.y)));
-    }
+    for (int i = 0; i < 4; ++i) m2 = max_abs2(m2, w[i]);
+    unsigned m = abs_bits_of<T>(m2);
 #pragma unroll
     for (int off = 8; off > 0; off >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, off));
     if (lane16 == 0 && m) atomicMax(&top[(p * ST_ROWS + row16) >> shift], m);
@@ -78,14 +76,9 @@ __global__ void __launch_bounds__(ST_THREADS) kv8_store_kernel(const StoreArgs a
     if (r >= n) continue;
     const CodeRule rule = code_rule<FMT>(top[lr >> shift]);
     const unsigned* w = reinterpret_cast<const unsigned*>(&x[p]);
-    unsigned out[2] = {0, 0};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = unpack16<T>(w[i]);
-      out[i >> 1] |= (code_with<FMT>(rule, f.x) | code_with<FMT>(rule, f.y) << 8) << (16 * (i & 1));
-    }
     const int64_t at = (int64_t)a.start + r;
-    *reinterpret_cast<uint2*>(dst + at * a.c.sr + lane16 * 8) = make_uint2(out[0], out[1]);
+    *reinterpret_cast<uint2*>(dst + at * a.c.sr + lane16 * 8) =
+        make_uint2(code4<FMT>(rule, unpack16<T>(w[0]), unpack16<T>(w[1])), code4<FMT>(rule, unpack16<T>(w[2]), unpack16<T>(w[3])));
     if (lane16 == 0 && (r & (a.c.block - 1)) == 0) scale[at >> shift] = rule.scale;
   }
 }

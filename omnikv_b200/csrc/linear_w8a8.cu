@@ -34,16 +34,13 @@ __global__ void __launch_bounds__(THREADS) quant_rows_kernel(const T* x, int64_t
     v[u] = make_uint4(0, 0, 0, 0);
     if (tid + u * THREADS < nvec) v[u] = src[tid + u * THREADS];
   }
-  unsigned m = 0;
+  unsigned m2 = 0;
 #pragma unroll
   for (int u = 0; u < QR_VEC; ++u) {
-    const unsigned* w = reinterpret_cast<const unsigned*>(&v[u]);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = unpack16<T>(w[i]);
-      m = max(m, max(abs_bits(f.x), abs_bits(f.y)));
-    }
+    m2 = max_abs2(max_abs2(m2, v[u].x), v[u].y);
+    m2 = max_abs2(max_abs2(m2, v[u].z), v[u].w);
   }
+  unsigned m = abs_bits_of<T>(m2);
   m = __reduce_max_sync(0xffffffffu, m);
   if ((tid & 31) == 0) top[tid >> 5] = m;
   __syncthreads();
@@ -55,14 +52,8 @@ __global__ void __launch_bounds__(THREADS) quant_rows_kernel(const T* x, int64_t
 #pragma unroll
   for (int u = 0; u < QR_VEC; ++u) {
     if (tid + u * THREADS >= nvec) continue;
-    const unsigned* w = reinterpret_cast<const unsigned*>(&v[u]);
-    unsigned o[2] = {0, 0};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = unpack16<T>(w[i]);
-      o[i >> 1] |= (code_with<kInt8>(rule, f.x) | code_with<kInt8>(rule, f.y) << 8) << (16 * (i & 1));
-    }
-    dst[tid + u * THREADS] = make_uint2(o[0], o[1]);
+    dst[tid + u * THREADS] = make_uint2(code4<kInt8>(rule, unpack16<T>(v[u].x), unpack16<T>(v[u].y)),
+                                        code4<kInt8>(rule, unpack16<T>(v[u].z), unpack16<T>(v[u].w)));
   }
 }
 
@@ -225,6 +216,7 @@ __device__ __forceinline__ bool epilogue_any(bool pred) {  // OR over the 128 ep
 }
 
 struct TkShared {
+  float x_scale[256];
   uint64_t full[8], empty[8], acc_full[2], acc_empty[2];
   unsigned tmem_base;
   int fail, issued, last;
@@ -320,6 +312,31 @@ linear_tile_kernel(const LinArgs a, const __grid_constant__ CUtensorMap tm_w, co
     int n = 0;
     for (int u = blockIdx.x; u < units; u += gridDim.x, ++n) {
       const int buf = n & 1, s = u % S, tile = u / S, t0 = (tile % a.token_tiles) * BN, c = (tile / a.token_tiles) * TK_M + tid;
+      const int tokens = min(BN, a.n - t0);
+      const float ws = c < a.N ? a.w_scale[c] : 0.f;
+      for (int j = tid; j < tokens; j += 128) sh.x_scale[j] = a.x_scale[t0 + j];  // the unit before ended with a barrier
+      const T* res = c < a.N ? static_cast<const T*>(a.res) : nullptr;
+      // 16 tokens of this thread's channel; what they need from memory is asked for one step ahead
+      T r[16];
+      const auto ask = [&](int j0) {
+        if (res)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) r[j] = res[(size_t)(t0 + min(j0 + j, tokens - 1)) * a.res_sr + c];
+      };
+      const auto finish = [&](int j0, const int (&v)[16]) {
+        float y[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          y[j] = (float)v[j] * sh.x_scale[j0 + j] * ws;
+          if (res) y[j] += to_float(r[j]);
+        }
+        if (j0 + 16 < tokens) ask(j0 + 16);
+        T* out = static_cast<T*>(a.out) + (size_t)(t0 + j0) * a.out_sr + c;
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          if (c < a.N && j0 + j < tokens) out[(size_t)j * a.out_sr] = from_float<T>(y[j]);
+      };
+      if (S == 1) ask(0);
       const bool got = mbar_wait(&sh.acc_full[buf], (n >> 1) & 1, &sh.fail);
       if (epilogue_any(!got)) {  // the 128 threads leave together
         if (!sh.fail && a.status) atomicExch(a.status, 7);
@@ -328,22 +345,6 @@ linear_tile_kernel(const LinArgs a, const __grid_constant__ CUtensorMap tm_w, co
       }
       tc_fence_after();
       const unsigned src = tmem + ((unsigned)(warp * 32) << 16) + (unsigned)buf * BN;
-      const int tokens = min(BN, a.n - t0);
-      const float ws = c < a.N ? a.w_scale[c] : 0.f;
-      const T* res = static_cast<const T*>(a.res);
-      T* out = static_cast<T*>(a.out);
-      const auto finish = [&](int j0, const int (&v)[16]) {  // 16 tokens of this thread's channel
-        float r[16];
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-          r[j] = res && c < a.N && j0 + j < tokens ? to_float(res[(size_t)(t0 + j0 + j) * a.res_sr + c]) : 0.f;
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-          if (c < a.N && j0 + j < tokens) {
-            const float y = (float)v[j] * a.x_scale[t0 + j0 + j] * ws;
-            out[(size_t)(t0 + j0 + j) * a.out_sr + c] = from_float<T>(y + r[j]);
-          }
-      };
       int* part = a.part + ((size_t)tile * S + s) * BN * TK_M + tid;
 #pragma unroll 1
       for (int j0 = 0; j0 < tokens; j0 += 16) {
@@ -359,29 +360,32 @@ linear_tile_kernel(const LinArgs a, const __grid_constant__ CUtensorMap tm_w, co
       }
       tc_fence_before();
       mbar_arrive(&sh.acc_empty[buf]);
-      if (S == 1) continue;
-      __threadfence();
-      epilogue_bar();
-      if (tid == 0) {
-        sh.last = atomicAdd(a.counters + tile, 1) == S - 1;
-        if (sh.last) a.counters[tile] = 0;  // nobody else touches it any more in this call
-      }
-      epilogue_bar();
-      if (sh.last) {
+      if (S > 1) {
         __threadfence();
-        const int* all = a.part + (size_t)tile * S * BN * TK_M + tid;
+        epilogue_bar();
+        if (tid == 0) {
+          sh.last = atomicAdd(a.counters + tile, 1) == S - 1;
+          if (sh.last) a.counters[tile] = 0;  // nobody else touches it any more in this call
+        }
+        epilogue_bar();
+        if (sh.last) {
+          __threadfence();
+          const int* all = a.part + (size_t)tile * S * BN * TK_M + tid;
+          ask(0);
 #pragma unroll 1
-        for (int j0 = 0; j0 < tokens; j0 += 16) {
-          int v[16];
+          for (int j0 = 0; j0 < tokens; j0 += 16) {
+            int v[16];
 #pragma unroll
-          for (int j = 0; j < 16; ++j) v[j] = 0;
-          for (int q = 0; q < S; ++q)
+            for (int j = 0; j < 16; ++j) v[j] = 0;
+#pragma unroll 4
+            for (int q = 0; q < S; ++q)
 #pragma unroll
-            for (int j = 0; j < 16; ++j) v[j] += __ldcg(all + ((size_t)q * BN + j0 + j) * TK_M);
-          finish(j0, v);
+              for (int j = 0; j < 16; ++j) v[j] += __ldcg(all + ((size_t)q * BN + j0 + j) * TK_M);
+            finish(j0, v);
+          }
         }
       }
-      epilogue_bar();  // sh.last is used again
+      epilogue_bar();  // sh.x_scale and sh.last are used again
     }
   }
 
