@@ -511,66 +511,86 @@ def host_device_pointer(t: torch.Tensor) -> int:
 # ------------------------------------------------------------------------------------------------
 # KV cache held in 8 bits
 # ------------------------------------------------------------------------------------------------
+# A call of this section costs the host a few microseconds, of the order of its kernel for a single token, so what a
+# check needs is read from a tensor once and the C structs are filled by position.
 _KV8 = {torch.int8: abi.KV8_INT8, torch.float8_e4m3fn: abi.KV8_E4M3}
+_DT16 = {torch.bfloat16: abi.BF16, torch.float16: abi.F16}
+_own_workspaces = {}
 
 
-def _on(*ts):
-    """The one device of the given tensors (None entries allowed); raises for CPU tensors or several devices."""
-    _need_cuda(*ts)
-    devs = {t.device for t in ts if t is not None}
-    if len(devs) != 1:
-        raise abi.OmniKVError(f"all tensors of a call must be on one device, got {sorted(map(str, devs))}")
-    return devs.pop()
+def _on(first: torch.Tensor, *others) -> int:
+    """The ordinal of the device that all given tensors (None entries allowed) are on; raises for CPU tensors or several devices."""
+    dev = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != dev:
+            raise abi.OmniKVError("all tensors of a call must be on one CUDA device")
+    if dev < 0:
+        raise abi.OmniKVError("omnikv_b200 kernels need CUDA tensors; there is no CPU path")
+    return dev
 
 
-def _launch(device, fn, what: str, n: int = 1) -> None:
-    """``fn(stream)`` on the current stream of ``device``, which is made the current device for the call."""
-    if device.index == torch.cuda.current_device():
-        rc = fn(torch.cuda.current_stream(device).cuda_stream)
+def _launch(dev: int, what: str, *args) -> None:
+    """Calls the C entry point ``what`` on the current stream of device ``dev``, with that device current."""
+    fn = getattr(abi.lib(), what)
+    if dev == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
     else:
-        with torch.cuda.device(device):
-            rc = fn(torch.cuda.current_stream(device).cuda_stream)
-    abi.check(rc, what)
-    _count(n)
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    if rc:
+        abi.check(rc, what)
+    _count(1)
 
 
-def _own_workspace(device, nbytes: int, tag: str) -> torch.Tensor:
+def _own_workspace(dev: int, nbytes: int, tag: str) -> torch.Tensor:
     """A zero-filled workspace for calls that follow one another: one per stream, and one per captured graph (two
-    graphs, or a graph and eager calls, may run at the same time)."""
-    stream = torch.cuda.current_stream(device).cuda_stream
-    capture = abi.lib().omnikv_capture_id(stream) if torch.cuda.is_current_stream_capturing() else 0
-    return workspace(device, nbytes, f"{tag}:{stream}:{capture}")
+    graphs, or a graph and eager calls, may run at the same time).  One that was outgrown is kept: a captured graph
+    may still use it."""
+    stream = torch._C._cuda_getCurrentRawStream(dev)
+    key = (dev, tag, stream, abi.lib().omnikv_capture_id(stream))
+    kept = _own_workspaces.get(key)
+    if kept is None or kept[-1].numel() < nbytes:
+        kept = _own_workspaces.setdefault(key, [])
+        kept.append(torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=f"cuda:{dev}"))
+    return kept[-1]
 
 
-def _need_i32(B: int, **named) -> None:
-    for name, t in named.items():
-        if t is not None and (t.dtype != torch.int32 or t.dim() != 1 or t.numel() != B or not t.is_contiguous()):
-            raise abi.OmniKVError(f"{name} must be contiguous int32 [{B}]")
+def _status_ptr(dev: int) -> int:
+    word = _status.get(dev)
+    return (status_word(dev) if word is None else word).data_ptr()
+
+
+def _need_i32(what: str, B: int, t: Optional[torch.Tensor]) -> Optional[int]:
+    """Address of a contiguous int32 ``[B]`` tensor (None stays None)."""
+    if t is None:
+        return None
+    if t.dtype is not torch.int32 or t.shape != (B,) or not t.is_contiguous():
+        raise abi.OmniKVError(f"{what} must be contiguous int32 [{B}]")
+    return t.data_ptr()
 
 
 def _kv8_cache(k8, v8, k_scale, v_scale, block: int) -> abi.Kv8Cache:
     """The C description of a cache: codes ``[B,KVH,rows,128]`` (int8 or float8_e4m3fn) and fp32 scales ``[B,KVH,>=ceil(rows/block)]``."""
-    if k8.dtype not in _KV8 or v8.dtype != k8.dtype or k8.dim() != 4 or k8.shape != v8.shape or k8.shape[3] != 128:
-        raise abi.OmniKVError("kv8: k8 and v8 must be int8 or float8_e4m3fn tensors [B, KVH, rows, 128] of one shape")
-    if _kv_strides(k8) != _kv_strides(v8):
-        raise abi.OmniKVError("kv8: k8 and v8 must share strides")
-    B, KVH, rows, d = k8.shape
+    fmt, shape, strides = _KV8.get(k8.dtype), k8.shape, k8.stride()
+    if fmt is None or v8.dtype is not k8.dtype or len(shape) != 4 or v8.shape != shape or shape[3] != 128 \
+            or strides[3] != 1 or v8.stride() != strides:
+        raise abi.OmniKVError("kv8: k8 and v8 must be int8 or float8_e4m3fn [B, KVH, rows, 128] of one layout, rows contiguous")
     if block < 1 or block > 256 or block & (block - 1):
         raise abi.OmniKVError(f"kv8: block must be a power of two between 1 and 256, got {block}")
-    for s in (k_scale, v_scale):
-        if s.dtype != torch.float32 or s.dim() != 3 or s.shape[0] != B or s.shape[1] != KVH or s.shape[2] * block < rows or s.stride(2) != 1:
-            raise abi.OmniKVError(f"kv8: scales must be fp32 [{B}, {KVH}, >= {-(-rows // block)}], last dimension contiguous")
-    if k_scale.stride() != v_scale.stride():
-        raise abi.OmniKVError("kv8: k_scale and v_scale must share strides")
-    return abi.Kv8Cache(_KV8[k8.dtype], block, B, KVH, d, rows, k8.data_ptr(), v8.data_ptr(), *_kv_strides(k8),
-                        k_scale.data_ptr(), v_scale.data_ptr(), k_scale.stride(0), k_scale.stride(1))
+    B, KVH, rows, d = shape
+    scales, steps = k_scale.shape, k_scale.stride()
+    if k_scale.dtype is not torch.float32 or v_scale.dtype is not torch.float32 or len(scales) != 3 or scales[0] != B \
+            or scales[1] != KVH or scales[2] * block < rows or steps[2] != 1 or v_scale.shape != scales or v_scale.stride() != steps:
+        raise abi.OmniKVError(f"kv8: scales must be fp32 [{B}, {KVH}, >= {-(-rows // block)}] of one layout, last dimension contiguous")
+    return abi.Kv8Cache(fmt, block, B, KVH, d, rows, k8.data_ptr(), v8.data_ptr(), strides[0], strides[1], strides[2],
+                        k_scale.data_ptr(), v_scale.data_ptr(), steps[0], steps[1])
 
 
-def _dt16(t_or_dtype, what: str) -> int:
-    dt = t_or_dtype if isinstance(t_or_dtype, torch.dtype) else t_or_dtype.dtype
-    if dt not in (torch.bfloat16, torch.float16):
-        raise abi.OmniKVError(f"{what} must be bfloat16 or float16, got {dt}")
-    return _DT[dt]
+def _dt16(dtype: torch.dtype, what: str) -> int:
+    dt = _DT16.get(dtype)
+    if dt is None:
+        raise abi.OmniKVError(f"{what} must be bfloat16 or float16, got {dtype}")
+    return dt
 
 
 def kv8_alloc(B: int, KVH: int, rows: int, *, block: int, dtype: torch.dtype, device, tokens_first: bool = False):
@@ -593,34 +613,30 @@ def kv8_store(k: torch.Tensor, v: torch.Tensor, k8, v8, k_scale, v_scale, *, blo
               lens: Optional[torch.Tensor] = None, start: int = 0) -> None:
     """``omnikv_kv8_store``: 16-bit k, v ``[B,KVH,n,128]`` into rows ``[start, start + n)`` of an 8-bit cache (``start`` a
     multiple of ``block``); ``lens`` int32 ``[B]`` on the device: only the first ``lens[b]`` of them exist."""
-    dev = _on(k, v, k8, v8, k_scale, v_scale, lens)
+    dev = _on(k8, k, v, v8, k_scale, v_scale, lens)
     c = _kv8_cache(k8, v8, k_scale, v_scale, block)
-    dt = _dt16(k, "kv8_store: k and v")
-    if k.dtype != v.dtype or k.shape != v.shape or k.dim() != 4 or k.shape[:2] != k8.shape[:2] or k.shape[3] != 128:
+    dt, shape = _dt16(k.dtype, "kv8_store: k and v"), k.shape
+    if v.dtype is not k.dtype or v.shape != shape or len(shape) != 4 or shape[0] != c.B or shape[1] != c.KVH or shape[3] != 128:
         raise abi.OmniKVError("kv8_store: k and v must be [B, KVH, n, 128] of one dtype")
-    n = k.shape[2]
-    if start < 0 or start % block or start + n > k8.shape[2]:
-        raise abi.OmniKVError(f"kv8_store: rows [{start}, {start + n}) must start at a multiple of {block} inside the cache's {k8.shape[2]} rows")
-    _need_i32(k.shape[0], lens=lens)
-    if n == 0:
-        return
-    ks, vs = _kv_strides(k), _kv_strides(v)
-    _launch(dev, lambda st: abi.lib().omnikv_kv8_store(C.byref(c), dt, k.data_ptr(), *ks, v.data_ptr(), *vs, start, n,
-                                                       _ptr(lens), st), "omnikv_kv8_store")
+    n = shape[2]
+    if start < 0 or start % block or start + n > c.rows:
+        raise abi.OmniKVError(f"kv8_store: rows [{start}, {start + n}) must start at a multiple of {block} inside the cache's {c.rows} rows")
+    lens_ptr = _need_i32("lens", c.B, lens)
+    if n:
+        _launch(dev, "omnikv_kv8_store", c, dt, k.data_ptr(), *_kv_strides(k), v.data_ptr(), *_kv_strides(v), start, n, lens_ptr)
 
 
 def kv8_append(k_new: torch.Tensor, v_new: torch.Tensor, k8, v8, k_scale, v_scale, pos: torch.Tensor, *, block: int) -> None:
     """``omnikv_kv8_append``: 16-bit k_new, v_new ``[B,KVH,128]`` at row ``pos[b]`` (int32, device; negative: skipped).
     A block whose scale has to grow for the new row is re-coded up to that row."""
-    dev = _on(k_new, v_new, k8, v8, k_scale, v_scale, pos)
+    dev = _on(k8, k_new, v_new, v8, k_scale, v_scale, pos)
     c = _kv8_cache(k8, v8, k_scale, v_scale, block)
-    dt = _dt16(k_new, "kv8_append: k_new and v_new")
-    if k_new.shape != (c.B, c.KVH, 128) or v_new.shape != k_new.shape or v_new.dtype != k_new.dtype \
-            or k_new.stride() != v_new.stride() or k_new.stride(2) != 1:
+    dt, strides = _dt16(k_new.dtype, "kv8_append: k_new and v_new"), k_new.stride()
+    if k_new.shape != (c.B, c.KVH, 128) or v_new.shape != k_new.shape or v_new.dtype is not k_new.dtype \
+            or v_new.stride() != strides or strides[2] != 1:
         raise abi.OmniKVError("kv8_append: k_new and v_new must be [B, KVH, 128] of one dtype and layout")
-    _need_i32(c.B, pos=pos)
-    _launch(dev, lambda st: abi.lib().omnikv_kv8_append(C.byref(c), dt, k_new.data_ptr(), v_new.data_ptr(), k_new.stride(0),
-                                                        k_new.stride(1), pos.data_ptr(), st), "omnikv_kv8_append")
+    _launch(dev, "omnikv_kv8_append", c, dt, k_new.data_ptr(), v_new.data_ptr(), strides[0], strides[1],
+            _need_i32("pos", c.B, pos))
 
 
 def kv8_load(k8, v8, k_scale, v_scale, *, block: int, dtype: torch.dtype, start: int = 0, rows: Optional[int] = None,
@@ -629,20 +645,20 @@ def kv8_load(k8, v8, k_scale, v_scale, *, block: int, dtype: torch.dtype, start:
     the end of the cache), or rows ``idx[b]`` (int32 ``[B, n]``; one outside the cache reads as zeros)."""
     dev = _on(k8, v8, k_scale, v_scale, idx)
     c = _kv8_cache(k8, v8, k_scale, v_scale, block)
-    dt = _dt16(dtype, "kv8_load: dtype")
+    dt, B, KVH = _dt16(dtype, "kv8_load: dtype"), c.B, c.KVH
     if idx is not None:
-        if idx.dtype != torch.int32 or idx.dim() != 2 or idx.shape[0] != c.B or idx.stride(1) != 1 or start or rows is not None:
+        shape = idx.shape
+        if idx.dtype is not torch.int32 or len(shape) != 2 or shape[0] != B or idx.stride(1) != 1 or start or rows is not None:
             raise abi.OmniKVError("kv8_load: idx must be int32 [B, n] with contiguous rows, without start and rows")
-        n = idx.shape[1]
+        n, idx_ptr, idx_stride = shape[1], idx.data_ptr(), idx.stride(0)
     else:
-        n = c.rows - start if rows is None else rows
+        n, idx_ptr, idx_stride = (c.rows - start if rows is None else rows), None, 0
         if start < 0 or n < 0 or start + n > c.rows:
             raise abi.OmniKVError(f"kv8_load: rows [{start}, {start + n}) are not inside the cache's {c.rows}")
-    k, v = torch.empty(2, c.B, c.KVH, n, 128, dtype=dtype, device=dev)
+    k = torch.empty((B, KVH, n, 128), dtype=dtype, device=k8.device)
+    v = torch.empty_like(k)
     if n:
-        _launch(dev, lambda st: abi.lib().omnikv_kv8_load(C.byref(c), dt, start, n, _ptr(idx), 0 if idx is None else idx.stride(0),
-                                                          k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), k.stride(2), st),
-                "omnikv_kv8_load")
+        _launch(dev, "omnikv_kv8_load", c, dt, start, n, idx_ptr, idx_stride, k.data_ptr(), v.data_ptr(), KVH * n * 128, n * 128, 128)
     return k, v
 
 
@@ -658,47 +674,44 @@ def kv8_decode_attn(q: torch.Tensor, k8, v8, k_scale, v_scale, len_a: torch.Tens
     selector-``last`` scores of positions ``< score_len[b]``.  ``n_splits``: CTAs per (sequence, KV head) on average
     (default: as many as the GPU holds); ``max_rows`` (default: all) is only a hint for that number."""
     dev = _on(q, k8, v8, k_scale, v_scale, len_a, idx, tail_start, tail_len, out, score_out, score_len, ws)
-    p = abi.Kv8AttnParams()
-    p.cache = c = _kv8_cache(k8, v8, k_scale, v_scale, block)
-    p.dtype = _dt16(q, "kv8_decode_attn: q")
-    B, KVH = c.B, c.KVH
-    if q.dim() != 3 or q.shape[0] != B or q.shape[2] != 128 or q.stride(2) != 1 or q.shape[1] % KVH:
+    c = _kv8_cache(k8, v8, k_scale, v_scale, block)
+    dt, B, KVH, rows = _dt16(q.dtype, "kv8_decode_attn: q"), c.B, c.KVH, c.rows
+    shape, strides = q.shape, q.stride()
+    if len(shape) != 3 or shape[0] != B or shape[2] != 128 or strides[2] != 1 or shape[1] % KVH:
         raise abi.OmniKVError("kv8_decode_attn: q must be [B, H, 128] with contiguous head vectors, H a multiple of KVH")
-    p.H = H = q.shape[1]
-    p.scale = float(scale if scale is not None else 1.0 / math.sqrt(128))
+    H = shape[1]
     if out is None:
         out = torch.empty_like(q)
-    if out.shape != q.shape or out.stride() != q.stride() or out.dtype != q.dtype:
+    if out.shape != shape or out.stride() != strides or out.dtype is not q.dtype:
         raise abi.OmniKVError("kv8_decode_attn: out must have the shape, strides and dtype of q")
-    p.q, p.q_stride_b, p.q_stride_h, p.out = q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr()
-    _need_i32(B, len_a=len_a, tail_start=tail_start, tail_len=tail_len, score_len=score_len)
-    p.len = len_a.data_ptr()
-    cap = c.rows
+    idx_ptr, idx_stride, idx_cap, cap = None, 0, 0, rows
     if idx is not None:
-        if idx.dtype != torch.int32 or idx.dim() != 2 or idx.shape[0] != B or idx.shape[1] == 0 or idx.stride(1) != 1:
+        if idx.dtype is not torch.int32 or idx.dim() != 2 or idx.shape[0] != B or idx.shape[1] == 0 or idx.stride(1) != 1:
             raise abi.OmniKVError("kv8_decode_attn: idx must be int32 [B, cap] with contiguous rows")
-        p.idx, p.idx_stride, p.idx_cap = idx.data_ptr(), idx.stride(0), idx.shape[1]
-        cap = idx.shape[1]
+        idx_ptr, idx_stride, idx_cap = idx.data_ptr(), idx.stride(0), idx.shape[1]
+        cap = idx_cap
     if (tail_len is None) != (tail_start is None):
         raise abi.OmniKVError("kv8_decode_attn: tail_start and tail_len go together")
     if tail_len is not None:
-        p.tail_start, p.tail_len = tail_start.data_ptr(), tail_len.data_ptr()
-        cap += c.rows
+        cap += rows
+    score_ptr, score_stride = None, 0
     if score_out is not None:
         if idx is not None or tail_len is not None or score_len is None:
             raise abi.OmniKVError("kv8_decode_attn: scores need score_len, and neither idx nor a tail")
-        if score_out.dtype != torch.float32 or score_out.dim() != 3 or score_out.shape[:2] != (KVH, B) \
+        if score_out.dtype is not torch.float32 or score_out.dim() != 3 or score_out.shape[:2] != (KVH, B) \
                 or not score_out.is_contiguous() or score_out.shape[2] == 0:
             raise abi.OmniKVError("kv8_decode_attn: score_out must be contiguous fp32 [KVH, B, stride]")
-        p.score_out, p.score_stride, p.score_len = score_out.data_ptr(), score_out.shape[2], score_len.data_ptr()
+        score_ptr, score_stride = score_out.data_ptr(), score_out.shape[2]
     # two CTAs per SM, each with at least four tiles of 32 rows (the kernel cuts the rows that there are into equal pieces)
-    p.n_ctas = n_splits * B * KVH if n_splits else min(2 * sm_count(dev), max(1, (max_rows or cap) // 128 + 1) * B * KVH)
-    need = abi.lib().omnikv_kv8_attn_workspace_bytes(B, H, KVH, p.n_ctas)
+    n_ctas = n_splits * B * KVH if n_splits else min(2 * sm_count(dev), ((max_rows or cap) // 128 + 1) * B * KVH)
     if ws is None:
-        ws = _own_workspace(dev, need, "kv8_attn")
-    p.workspace, p.workspace_bytes = ws.data_ptr(), ws.numel() * ws.element_size()
-    p.status = status_word(dev).data_ptr()
-    _launch(dev, lambda st: abi.lib().omnikv_kv8_decode_attn(C.byref(p), st), "omnikv_kv8_decode_attn")
+        ws = _own_workspace(dev, abi.lib().omnikv_kv8_attn_workspace_bytes(B, H, KVH, n_ctas), "kv8_attn")
+    p = abi.Kv8AttnParams(c, dt, H, scale if scale is not None else 0.08838834764831845, q.data_ptr(), strides[0], strides[1],
+                          out.data_ptr(), idx_ptr, idx_stride, idx_cap, _need_i32("len_a", B, len_a),
+                          _need_i32("tail_start", B, tail_start), _need_i32("tail_len", B, tail_len), score_ptr, score_stride,
+                          _need_i32("score_len", B, score_len), n_ctas, ws.data_ptr(), ws.numel() * ws.element_size(),
+                          _status_ptr(dev))
+    _launch(dev, "omnikv_kv8_decode_attn", p)
     return out
 
 
@@ -709,15 +722,14 @@ def quant_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """``omnikv_quant_rows``: 16-bit x ``[n, K]`` (K a multiple of 16, at most 32768) -> int8 codes ``[n, K]`` and fp32
     scales ``[n]`` with ``x ~ codes * scale[:, None]``: the tokens of a call, or a weight matrix's output channels."""
     dev = _on(x)
-    dt = _dt16(x, "quant_rows: x")
-    if x.dim() != 2 or x.stride(1) != 1 or x.shape[1] == 0 or x.shape[1] % 16:
+    dt, shape, strides = _dt16(x.dtype, "quant_rows: x"), x.shape, x.stride()
+    if len(shape) != 2 or strides[1] != 1 or shape[1] == 0 or shape[1] % 16:
         raise abi.OmniKVError("quant_rows: x must be [n, K] with contiguous rows and K a multiple of 16")
-    n, K = x.shape
-    codes = torch.empty(n, K, dtype=torch.int8, device=dev)
-    scale = torch.empty(n, dtype=torch.float32, device=dev)
+    n, K = shape
+    codes = torch.empty((n, K), dtype=torch.int8, device=x.device)
+    scale = torch.empty((n,), dtype=torch.float32, device=x.device)
     if n:
-        _launch(dev, lambda st: abi.lib().omnikv_quant_rows(dt, x.data_ptr(), x.stride(0), n, K, codes.data_ptr(), K,
-                                                            scale.data_ptr(), st), "omnikv_quant_rows")
+        _launch(dev, "omnikv_quant_rows", dt, x.data_ptr(), strides[0], n, K, codes.data_ptr(), K, scale.data_ptr())
     return codes, scale
 
 
@@ -728,38 +740,34 @@ def linear_w8a8(x8: torch.Tensor, x_scale: torch.Tensor, w8: torch.Tensor, w_sca
     ``x_scale[n]`` and ``w_scale[channels]`` (fp32), plus ``residual`` ``[n, channels]`` when given (``out`` may be the
     same tensor), rounded once to ``out_dtype`` (default: that of ``out`` or ``residual``, else bfloat16)."""
     dev = _on(x8, x_scale, w8, w_scale, residual, out)
-    for t in (x8, w8):
-        if t.dtype != torch.int8 or t.dim() != 2 or t.stride(1) != 1:
-            raise abi.OmniKVError("linear_w8a8: x8 [n, K] and w8 [channels, K] must be int8 with contiguous rows")
-    n, K = x8.shape
-    N = w8.shape[0]
-    if w8.shape[1] != K or K == 0 or K % 16:
+    xs, ws, x_st, w_st = x8.shape, w8.shape, x8.stride(), w8.stride()
+    if x8.dtype is not torch.int8 or w8.dtype is not torch.int8 or len(xs) != 2 or len(ws) != 2 or x_st[1] != 1 or w_st[1] != 1:
+        raise abi.OmniKVError("linear_w8a8: x8 [n, K] and w8 [channels, K] must be int8 with contiguous rows")
+    n, K = xs
+    N = ws[0]
+    if ws[1] != K or K == 0 or K % 16:
         raise abi.OmniKVError("linear_w8a8: x8 and w8 must share K, a multiple of 16")
-    for t, m in ((x_scale, n), (w_scale, N)):
-        if t.dtype != torch.float32 or t.shape != (m,) or not t.is_contiguous():
-            raise abi.OmniKVError("linear_w8a8: scales must be contiguous fp32, one per row of x8 and of w8")
+    if x_scale.dtype is not torch.float32 or w_scale.dtype is not torch.float32 or x_scale.shape != (n,) or w_scale.shape != (N,) \
+            or not x_scale.is_contiguous() or not w_scale.is_contiguous():
+        raise abi.OmniKVError("linear_w8a8: scales must be contiguous fp32, one per row of x8 and of w8")
     if out is None:
         dt = out_dtype or (residual.dtype if residual is not None else torch.bfloat16)
-        out = torch.empty(n, N, dtype=dt, device=dev)
+        out = torch.empty((n, N), dtype=dt, device=x8.device)
+    dt = out.dtype
     for t in (out, residual):
-        if t is not None and (t.shape != (n, N) or t.dtype != out.dtype or t.dtype not in _DT or t.stride(1) != 1
-                              or (out_dtype is not None and t.dtype != out_dtype)):
+        if t is not None and (t.shape != (n, N) or t.dtype is not dt or dt not in _DT or t.stride(1) != 1
+                              or (out_dtype is not None and dt is not out_dtype)):
             raise abi.OmniKVError("linear_w8a8: out and residual must be [n, channels] of one floating dtype, rows contiguous")
     if n == 0 or N == 0:
         return out
-    p = abi.LinearW8A8Params()
-    p.n_tokens, p.channels, p.K = n, N, K
-    p.x, p.x_stride_row, p.x_scale = x8.data_ptr(), x8.stride(0), x_scale.data_ptr()
-    p.w, p.w_stride_row, p.w_scale = w8.data_ptr(), w8.stride(0), w_scale.data_ptr()
-    p.out_dtype, p.out, p.out_stride_row = _DT[out.dtype], out.data_ptr(), out.stride(0)
-    if residual is not None:
-        p.residual, p.residual_stride_row = residual.data_ptr(), residual.stride(0)
-    need = abi.lib().omnikv_linear_w8a8_workspace_bytes(n, N, K)
+    need, work = abi.lib().omnikv_linear_w8a8_workspace_bytes(n, N, K), None
     if need:
-        ws = _own_workspace(dev, need, "linear_w8a8")
-        p.workspace, p.workspace_bytes = ws.data_ptr(), ws.numel()
-    p.status = status_word(dev).data_ptr()
-    _launch(dev, lambda st: abi.lib().omnikv_linear_w8a8(C.byref(p), st), "omnikv_linear_w8a8")
+        work = _own_workspace(dev, need, "linear_w8a8").data_ptr()
+    p = abi.LinearW8A8Params(n, N, K, x8.data_ptr(), x_st[0], x_scale.data_ptr(), w8.data_ptr(), w_st[0], w_scale.data_ptr(),
+                             _DT[dt], None if residual is None else residual.data_ptr(),
+                             0 if residual is None else residual.stride(0), out.data_ptr(), out.stride(0), work, need,
+                             _status_ptr(dev))
+    _launch(dev, "omnikv_linear_w8a8", p)
     return out
 
 
