@@ -526,7 +526,7 @@ int omnikv_decode_chain_supported(int dtype, int hidden, int inter, int H);
  * Codes are int8 (top = 127) or e4m3 (top = 448).  For a block whose rows hold the 16-bit values x, with a = max |x|:
  *     scale = a / top,   code = round(top * x / a)  to the nearest code, ties to even;     a = 0: all codes 0.
  * A block that holds an infinity or a NaN gets that scale and codes 0: all of it reads as NaN.  The e4m3 NaN codes
- * (0x7f, 0xff) are never written; attention reads them as +-480.
+ * (0x7f, 0xff) are never written.
  *
  * k, v: one byte per element, rows of head_dim contiguous codes; strides in elements, multiples of 16, bases 16-byte
  * aligned; [0, rows) is readable memory for every (sequence, head), at most 2^31 - 1 rows.  k_scale, v_scale:
@@ -594,7 +594,7 @@ typedef struct {
   float* score_out; /* [KVH, B, score_stride] or NULL */
   int64_t score_stride;
   const int32_t* score_len;
-  int32_t n_ctas; /* the work of all sequences is cut into at most this many equal pieces; 1..65536 */
+  int32_t n_ctas; /* the work of all sequences is cut into at most this many equal pieces; 1..32768 */
   void* workspace;
   size_t workspace_bytes;
   int32_t* status; /* optional device word: set to 5 if a bounded wait for a KV copy ran out */

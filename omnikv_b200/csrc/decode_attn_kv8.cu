@@ -2,13 +2,16 @@
 //
 // Mathematics.  With K = ck * sk, V = cv * sv (codes and per-block scales) a row j contributes, to one query head,
 //     x_j = (q . ck_j) * sk_j * scale * log2(e)          l = sum_j 2^(x_j - m)
-//     y_j = x_j + log2(sv_j)                              o = sum_j 2^(y_j - M + 15) cv_j
-//     out = o / l * 2^(M - m - 15)
-// m and M are running maxima of x and y.  The V scale rides in the exponent, so the weights that meet the codes lie in
-// [0, 2^15] whatever the scales: they round to fp16 (11 bits, three more than the bf16 weights of a 16-bit cache) and one
-// that is 2^-39 of the largest still counts.  The codes are fp16 numbers exactly (int8: 1024 + 128 + code by a byte
-// permutation, minus 1152; e4m3: exponent field moved, the factor 2^8 goes into the scale), the queries too after a power
-// of two per head.  Sums are fp32, in the MMA and outside.
+//     y_j = x_j + log2(sv_j)                              o = sum_j 2^(y_j - M + 11) cv_j
+//     out = o / l * 2^(M - m - 11)
+// with references m, M near the running maxima of x and y: they follow only when a value has outgrown them (x by 2^32, y
+// by 2^4, so that a weight stays below fp16's 2^16), which spares most tiles the reduction over the warp and the scaling
+// of o.  The V scale rides in the exponent, so the weights that meet the codes have one range whatever the scales: they
+// round to fp16 (11 bits, three more than the bf16 weights of a 16-bit cache) and one that is 2^-35 of the largest still
+// counts.
+//
+// The codes are fp16 numbers exactly (e4m3: the conversion instruction; int8: a byte permutation and a subtraction), the
+// queries too after a power of two per head.  Sums are fp32, in the MMA and outside.
 //
 // Layout.  A warp works alone: its own ring of 32-row tiles, its own mbarriers, no CTA barrier until the end of a segment.
 // Rows are the M side of both products (S^T = K q^T and O^T = V^T P^T with m16n8k16), the query heads of a KV head the N
@@ -17,8 +20,8 @@
 // pairs (byte permutations), P^T comes from S^T by movmatrix.
 //
 // Work.  The 32-row tiles of all (sequence, KV head) segments form one list that is cut into equal pieces, one per CTA
-// (two CTAs per SM, at least four tiles each), whatever the lengths: a CTA may end one segment and begin the next.  Every
-// CTA leaves one partial (o, M, m, l) per segment that it touches, and the one that arrives last at a segment merges.
+// (one CTA of twelve warps per SM), whatever the lengths: a CTA may end one segment and begin the next.  Every CTA leaves
+// one partial (o, M, m, l) per segment that it touches, and the one that arrives last at a segment merges.
 //
 // Bound: HBM, 256 bytes of codes and 8 / block bytes of scales per (row, KV head).
 #include "kv8.cuh"
@@ -29,9 +32,9 @@ namespace omnikv {
 namespace {
 
 constexpr int MAX_G = 16;
-constexpr int NW = 4, NT = NW * 32;
+constexpr int kWarps[3] = {0, 12, 8};        // warps of a CTA by column blocks: 168 and 255 registers a thread
 constexpr int TILE = 32;                     // rows per tile: one lane per row when rows are fetched one by one
-constexpr int STAGES = 3;
+constexpr int STAGES = 2;
 constexpr int BOX = TILE * kHeadDim;         // bytes of a K or V tile
 constexpr int PITCH = 2 * kHeadDim + 16;     // row pitch of a tile fetched row by row (K | V | pad): conflict-free
 constexpr int ROWS_STAGE = TILE * PITCH, TMA_STAGE = 2 * BOX;
@@ -87,16 +90,33 @@ struct Cursor {
     list = row_list(a, b);
     nt = list.tiles();
   }
-  __device__ __forceinline__ void forward(const A8Args& a, int by) {
+  // false: still in the same segment
+  __device__ __forceinline__ bool forward(const A8Args& a, int by) {
     tile += by;
-    while (tile >= nt) {
+    if (tile < nt) return false;
+    do {
       tile -= nt;
       if (++kvh == a.KVH) {
         kvh = 0;
-        if (++b >= a.B) return;
+        if (++b >= a.B) return true;
         load(a);
       }
-    }
+    } while (tile >= nt);
+    return true;
+  }
+};
+// Where a segment's codes, scales and index list begin.
+struct Sources {
+  const unsigned char *k, *v;
+  const float *ks, *vs;
+  const int* idx;
+  __device__ __forceinline__ void of(const A8Args& a, int b, int kvh) {
+    const int64_t at = (int64_t)b * a.sb + (int64_t)kvh * a.sh, sat = (int64_t)b * a.ssb + (int64_t)kvh * a.ssh;
+    k = a.k + at;
+    v = a.v + at;
+    ks = a.ks + sat;
+    vs = a.vs + sat;
+    idx = a.idx ? a.idx + (int64_t)b * a.idx_stride : nullptr;
   }
 };
 
@@ -121,8 +141,8 @@ __device__ __forceinline__ unsigned sub_h2(unsigned a, unsigned b) {
   return y;
 }
 
-// Bytes 0, 1 (hi = false) or 2, 3 of w as two fp16 numbers.  int8: the code.  e4m3: the value times 2^-8 (sign kept,
-// exponent and mantissa moved to fp16's fields; subnormals come out right, the NaN codes as 480 * 2^-8).
+// Bytes 0, 1 (hi = false) or 2, 3 of w as two fp16 numbers, exactly.  int8: w ^ 0x80808080 holds code + 128, which under the
+// exponent byte 0x64 is the number 1024 + 128 + code.
 template <int FMT>
 __device__ __forceinline__ unsigned prepare_word(unsigned w) {
   return FMT == kInt8 ? w ^ 0x80808080u : w;
@@ -132,19 +152,16 @@ __device__ __forceinline__ unsigned half2_of(unsigned w) {
   if constexpr (FMT == kInt8) {
     return sub_h2(__byte_perm(w, 0x64646464u, HI ? 0x4342 : 0x4140), 0x64806480u);
   } else {
-    const unsigned x = __byte_perm(w, 0, HI ? 0x3424 : 0x1404);
-    return ((x >> 1) & 0x3f803f80u) | (x & 0x80008000u);
+    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(HI ? w >> 16 : w & 0xffffu), __NV_E4M3);
+    return (unsigned)h.x | (unsigned)h.y << 16;
   }
-}
-template <int FMT>
-__host__ __device__ constexpr float half2_unit() {  // what the conversion leaves to be multiplied
-  return FMT == kInt8 ? 1.f : 256.f;
 }
 
 __device__ __forceinline__ void cp_async4(void* smem_dst, const void* gmem_src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;\n" ::"r"(smem_u32(smem_dst)), "l"(gmem_src) : "memory");
 }
 
+template <int NW>
 struct Shared {
   uint64_t full[NW][STAGES];
   float scale[NW][STAGES][2][TILE];  // K and V scale of each row of a tile
@@ -156,10 +173,11 @@ struct Shared {
 // COLS: n8 column blocks of query heads (1: up to 8 heads per KV head, 2: up to 16).  TMA: tiles as boxes of a tensor map
 // (rows that follow one another), else rows fetched one by one.
 template <typename T, int FMT, int COLS, bool TMA>
-__global__ void __launch_bounds__(NT, 2)
+__global__ void __launch_bounds__(kWarps[COLS] * 32, 1)
 decode_attn_kv8_kernel(const A8Args a, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
+  constexpr int NW = kWarps[COLS], NT = NW * 32;
   extern __shared__ __align__(128) unsigned char smem_raw[];
-  __shared__ Shared sh;
+  __shared__ Shared<NW> sh;
   constexpr int STAGE_BYTES = TMA ? TMA_STAGE : ROWS_STAGE;
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -169,6 +187,10 @@ decode_attn_kv8_kernel(const A8Args a, const __grid_constant__ CUtensorMap tm_k,
 
   if (lane < STAGES) mbar_init(&sh.full[warp][lane], 1);
   asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+  if (TMA && tid == 0) {
+    asm volatile("prefetch.tensormap [%0];\n" ::"l"(&tm_k) : "memory");
+    asm volatile("prefetch.tensormap [%0];\n" ::"l"(&tm_v) : "memory");
+  }
   __syncwarp();
   pdl_wait();
 
@@ -178,18 +200,27 @@ decode_attn_kv8_kernel(const A8Args a, const __grid_constant__ CUtensorMap tm_k,
     const int mine = b0 + lane < a.B ? row_list(a, b0 + lane).tiles() : 0;
     per_head += __reduce_add_sync(0xffffffffu, mine);
   }
-  const long long W = (long long)per_head * a.KVH;
-  const long long C = max(1ll, min((long long)gridDim.x, W / NW));
-  const int c = blockIdx.x;
+  // Pieces.  One per segment when four tiles per warp do a segment: a merge across CTAs costs more than it saves then.
+  // Else as many as there are CTAs, a multiple of the segments where that leaves few CTAs idle: the pieces of equal
+  // segments then end where the segments end.
+  const int segs = a.B * a.KVH, W = per_head * a.KVH;
+  int C = min((int)gridDim.x, W <= segs * NW * 4 ? segs : max(W / NW, segs));
+  if (C > segs && C % segs <= C / 16) C -= C % segs;
+  const int each = W / C, more = W - each * C, c = blockIdx.x;
   if (c >= C) return;
-  const long long w0 = W * c / C, w1 = W * (c + 1) / C;
-  const auto owner = [&](long long tile) { return (int)(((tile + 1) * C - 1) / W); };  // the CTA that has this tile
+  const auto piece_lo = [&](int i) { return i * each + i * more / C; };  // i * more < 2^30
+  const int w0 = piece_lo(c), w1 = piece_lo(c + 1);
+  const auto owner = [&](int tile) {  // the CTA that has this tile
+    int i = min(C - 1, (int)(((float)tile + 0.5f) * (float)C / (float)W));
+    while (piece_lo(i) > tile) --i;
+    while (piece_lo(i + 1) <= tile) ++i;
+    return i;
+  };
   Cursor seg;  // the segment being worked on; tile = 0
-  long long seg_lo;
+  int seg_lo;
   {
-    long long before = 0;  // tiles of the sequences in front
-    int b0 = 0, found = -1, in_front = 0;
-    for (; found < 0; b0 += 32) {
+    int before = 0, found = -1;  // tiles per KV head of the sequences in front
+    for (int b0 = 0; found < 0; b0 += 32) {
       const int mine = b0 + lane < a.B ? row_list(a, b0 + lane).tiles() : 0;
       int sum = mine;
 #pragma unroll
@@ -198,30 +229,27 @@ decode_attn_kv8_kernel(const A8Args a, const __grid_constant__ CUtensorMap tm_k,
         if (lane >= off) sum += x;
       }
       const unsigned hit = __ballot_sync(0xffffffffu, (before + sum) * a.KVH > w0);
-      if (hit) {
-        found = b0 + __ffs(hit) - 1;
-        in_front = __shfl_sync(0xffffffffu, sum - mine, __ffs(hit) - 1);
-      } else {
-        before += __shfl_sync(0xffffffffu, sum, 31);
-      }
+      const int at = hit ? __ffs(hit) - 1 : 31;
+      before += __shfl_sync(0xffffffffu, hit ? sum - mine : sum, at);
+      if (hit) found = b0 + at;
     }
     seg.b = found;
     seg.load(a);
-    const long long first = (before + in_front) * a.KVH;
-    seg.kvh = (int)((w0 - first) / seg.nt);
+    seg.kvh = (w0 - before * a.KVH) / seg.nt;
     seg.tile = 0;
-    seg_lo = first + (long long)seg.kvh * seg.nt;
+    seg_lo = before * a.KVH + seg.kvh * seg.nt;
   }
 
   // ---- the warp's stream of tiles: every NW-th of the piece ----
   Cursor ahead = seg;  // the next tile to ask for
-  long long ahead_w = w0 + warp;
+  Sources from;
+  int ahead_w = w0 + warp;
   int asked = 0, pos = -1;
   const auto find_row = [&]() {  // the cache position of this lane's row in the tile to ask for, -1: none
     pos = -1;
     if (ahead_w < w1) {
       const int r = ahead.tile * TILE + lane;
-      if (r < ahead.list.nA) pos = a.idx ? a.idx[(size_t)ahead.b * a.idx_stride + r] : r;
+      if (r < ahead.list.nA) pos = from.idx ? from.idx[r] : r;
       else if (r < ahead.list.n()) pos = ahead.list.t0 + (r - ahead.list.nA);
     }
   };
@@ -229,52 +257,49 @@ decode_attn_kv8_kernel(const A8Args a, const __grid_constant__ CUtensorMap tm_k,
     if (ahead_w < w1) {
       const int s = asked % STAGES;
       unsigned char* dst = ring + s * STAGE_BYTES;
-      const bool ok = pos >= 0 && pos < a.rows;
-      if constexpr (TMA) {
-        if (lane == 0) {
-          mbar_expect_tx(&sh.full[warp][s], TMA_STAGE);
+      const bool ok = (unsigned)pos < (unsigned)a.rows;
+      const unsigned valid = __ballot_sync(0xffffffffu, ok);
+      if (lane == 0) {
+        sh.valid[warp][s] = valid;
+        mbar_expect_tx(&sh.full[warp][s], TMA ? TMA_STAGE : __popc(valid) * 2 * kHeadDim);
+        if constexpr (TMA) {
           tma_load_4d(dst, &tm_k, 0, ahead.tile * TILE, ahead.kvh, ahead.b, &sh.full[warp][s]);
           tma_load_4d(dst + BOX, &tm_v, 0, ahead.tile * TILE, ahead.kvh, ahead.b, &sh.full[warp][s]);
         }
       }
-      const unsigned valid = __ballot_sync(0xffffffffu, ok);
-      if (lane == 0) {
-        sh.valid[warp][s] = valid;
-        if constexpr (!TMA) mbar_expect_tx(&sh.full[warp][s], __popc(valid) * 2 * kHeadDim);
-      }
       __syncwarp();
       if (ok) {
         if constexpr (!TMA) {
-          const int64_t at = (int64_t)ahead.b * a.sb + (int64_t)ahead.kvh * a.sh + (int64_t)pos * a.sr;
+          const int64_t at = (int64_t)pos * a.sr;
           if (a.pair) {
-            tma_bulk_g2s(dst + lane * PITCH, a.k + at, 2 * kHeadDim, &sh.full[warp][s]);
+            tma_bulk_g2s(dst + lane * PITCH, from.k + at, 2 * kHeadDim, &sh.full[warp][s]);
           } else {
-            tma_bulk_g2s(dst + lane * PITCH, a.k + at, kHeadDim, &sh.full[warp][s]);
-            tma_bulk_g2s(dst + lane * PITCH + kHeadDim, a.v + at, kHeadDim, &sh.full[warp][s]);
+            tma_bulk_g2s(dst + lane * PITCH, from.k + at, kHeadDim, &sh.full[warp][s]);
+            tma_bulk_g2s(dst + lane * PITCH + kHeadDim, from.v + at, kHeadDim, &sh.full[warp][s]);
           }
         }
-        const int64_t sat = (int64_t)ahead.b * a.ssb + (int64_t)ahead.kvh * a.ssh + (pos >> a.shift);
-        cp_async4(&sh.scale[warp][s][0][lane], a.ks + sat);
-        cp_async4(&sh.scale[warp][s][1][lane], a.vs + sat);
+        cp_async4(&sh.scale[warp][s][0][lane], from.ks + (pos >> a.shift));
+        cp_async4(&sh.scale[warp][s][1][lane], from.vs + (pos >> a.shift));
       }
       ++asked;
       ahead_w += NW;
-      if (ahead_w < w1) ahead.forward(a, NW);
+      if (ahead_w < w1 && ahead.forward(a, NW)) from.of(a, ahead.b, ahead.kvh);
     }
     cp_async_commit();
     find_row();
   };
-  ahead.tile = (int)(w0 - seg_lo);
+  ahead.tile = w0 - seg_lo;
   if (ahead_w < w1) ahead.forward(a, warp);
+  from.of(a, min(ahead.b, a.B - 1), ahead.kvh);
   find_row();
 #pragma unroll
   for (int s = 0; s < STAGES - 1; ++s) ask();
 
   int used = 0;
   bool dead = false;
-  long long next_w = w0 + warp;  // the warp's next tile
-  for (long long lo = w0; lo < w1;) {
-    const long long seg_hi = seg_lo + seg.nt, hi = min(w1, seg_hi);  // this CTA's tiles of the segment: [lo, hi)
+  int next_w = w0 + warp;  // the warp's next tile
+  for (int lo = w0; lo < w1;) {
+    const int seg_hi = seg_lo + seg.nt, hi = min(w1, seg_hi);  // this CTA's tiles of the segment: [lo, hi)
     const int b = seg.b, kvh = seg.kvh;
 
     // ---- queries: fragments of q * 2^e (largest element in [2^13, 2^14)), e folded into the head's factor ----
@@ -304,7 +329,7 @@ decode_attn_kv8_kernel(const A8Args a, const __grid_constant__ CUtensorMap tm_k,
         qf[cb][j][0] = pack2<__half>(x.x * up, x.y * up);
         qf[cb][j][1] = pack2<__half>(y.x * up, y.y * up);
       }
-      const float f = down * a.scale * half2_unit<FMT>();
+      const float f = down * a.scale * kLog2e;
       qs[cb][0] = __shfl_sync(0xffffffffu, f, 8 * t);
       qs[cb][1] = __shfl_sync(0xffffffffu, f, 8 * t + 4);
     }
@@ -362,7 +387,7 @@ decode_attn_kv8_kernel(const A8Args a, const __grid_constant__ CUtensorMap tm_k,
         }
       }
       // ---- scales, mask, scores ----
-      const int row0 = (int)(next_w - seg_lo) * TILE;
+      const int row0 = (next_w - seg_lo) * TILE;
       float lv[2][2];
 #pragma unroll
       for (int i = 0; i < 2; ++i)
@@ -372,63 +397,78 @@ decode_attn_kv8_kernel(const A8Args a, const __grid_constant__ CUtensorMap tm_k,
           const float ks = __shfl_sync(0xffffffffu, my_ks, r);
           lv[i][u] = __shfl_sync(0xffffffffu, my_lv, r);
           const bool ok = (valid >> r) & 1u;
-          float best = -INFINITY;
+          if (!ok) lv[i][u] = 0.f;  // a scale that was not read
 #pragma unroll
           for (int cb = 0; cb < COLS; ++cb)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              const float z = x[i][cb][2 * u + e] * ks * qs[cb][e];
-              if (cb * 8 + 2 * t + e < G) best = max_nan(best, z);
-              x[i][cb][2 * u + e] = ok ? z * kLog2e : -INFINITY;
+              float& z = x[i][cb][2 * u + e];
+              z = ok ? z * ks * qs[cb][e] : -INFINITY;
             }
           if (a.score_out) {
+            float best = -INFINITY;
+#pragma unroll
+            for (int cb = 0; cb < COLS; ++cb)
+#pragma unroll
+              for (int e = 0; e < 2; ++e)
+                if (cb * 8 + 2 * t + e < G) best = max_nan(best, x[i][cb][2 * u + e]);
             best = max_nan(best, __shfl_xor_sync(0xffffffffu, best, 1));
             best = max_nan(best, __shfl_xor_sync(0xffffffffu, best, 2));
-            if (t == 0 && row0 + r < score_lim) score_row[row0 + r] = best;
+            if (t == 0 && row0 + r < score_lim) score_row[row0 + r] = best * (1.f / kLog2e);
           }
-          if (!ok) lv[i][u] = 0.f;  // a scale that was not read
         }
       // ---- weights ----
       unsigned pb[2][COLS][2];
 #pragma unroll
       for (int cb = 0; cb < COLS; ++cb) {
-        float corr[2];
+        float mx[2], My[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float mx = m[cb][e], My = M[cb][e];
+          mx[e] = My[e] = -INFINITY;
 #pragma unroll
           for (int i = 0; i < 2; ++i)
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-              mx = fmaxf(mx, x[i][cb][2 * u + e]);
-              My = fmaxf(My, x[i][cb][2 * u + e] + lv[i][u]);
+              mx[e] = fmaxf(mx[e], x[i][cb][2 * u + e]);
+              My[e] = fmaxf(My[e], x[i][cb][2 * u + e] + lv[i][u]);
             }
+        }
+        const bool outgrown = mx[0] > m[cb][0] + 32.f || mx[1] > m[cb][1] + 32.f || My[0] > M[cb][0] + 4.f || My[1] > M[cb][1] + 4.f;
+        if (__any_sync(0xffffffffu, outgrown)) {
+          float corr[2];
 #pragma unroll
-          for (int off = 4; off < 32; off <<= 1) {
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-            My = fmaxf(My, __shfl_xor_sync(0xffffffffu, My, off));
+          for (int e = 0; e < 2; ++e) {
+#pragma unroll
+            for (int off = 4; off < 32; off <<= 1) {
+              mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], off));
+              My[e] = fmaxf(My[e], __shfl_xor_sync(0xffffffffu, My[e], off));
+            }
+            mx[e] = fmaxf(m[cb][e], mx[e]);
+            My[e] = fmaxf(M[cb][e], My[e]);
+            l[cb][e] *= m[cb][e] == mx[e] ? 1.f : ex2(m[cb][e] - mx[e]);
+            corr[e] = M[cb][e] == My[e] ? 1.f : ex2(M[cb][e] - My[e]);
+            m[cb][e] = mx[e];
+            M[cb][e] = My[e];
           }
-          const float mu = mx == -INFINITY ? 0.f : mx, Mu = My == -INFINITY ? 0.f : My;
-          float sum = 0.f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            o[cb][i][0] *= corr[0];
+            o[cb][i][1] *= corr[1];
+            o[cb][i][2] *= corr[0];
+            o[cb][i][3] *= corr[1];
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float mu = m[cb][e] == -INFINITY ? 0.f : m[cb][e], Mu = M[cb][e] == -INFINITY ? 0.f : M[cb][e] - 11.f;
 #pragma unroll
           for (int i = 0; i < 2; ++i)
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
               float& z = x[i][cb][2 * u + e];
-              sum += ex2(z - mu);
-              z = ex2(z + lv[i][u] - Mu + 15.f);
+              l[cb][e] += ex2(z - mu);
+              z = ex2(z + lv[i][u] - Mu);
             }
-          l[cb][e] = fmaf(l[cb][e], ex2(m[cb][e] - mu), sum);
-          corr[e] = ex2(M[cb][e] - Mu);
-          m[cb][e] = mx;
-          M[cb][e] = My;
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          o[cb][i][0] *= corr[0];
-          o[cb][i][1] *= corr[1];
-          o[cb][i][2] *= corr[0];
-          o[cb][i][3] *= corr[1];
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -439,8 +479,17 @@ decode_attn_kv8_kernel(const A8Args a, const __grid_constant__ CUtensorMap tm_k,
       // ---- O^T += V^T P^T: thread (g, t) holds dimensions 16 g .. 16 g + 15 of four rows ----
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const uint4 v0 = piece(1, 16 * i + 2 * t, g), v1 = piece(1, 16 * i + 2 * t + 1, g);
-        const uint4 v2 = piece(1, 16 * i + 8 + 2 * t, g), v3 = piece(1, 16 * i + 9 + 2 * t, g);
+        uint4 v0 = piece(1, 16 * i + 2 * t, g), v1 = piece(1, 16 * i + 2 * t + 1, g);
+        uint4 v2 = piece(1, 16 * i + 8 + 2 * t, g), v3 = piece(1, 16 * i + 9 + 2 * t, g);
+        if (FMT == kE4m3 && valid != 0xffffffffu) {  // what lies in the place of a missing row may be a NaN code
+          const auto keep = [&](uint4& v, int r) {
+            if (!((valid >> r) & 1u)) v = make_uint4(0, 0, 0, 0);
+          };
+          keep(v0, 16 * i + 2 * t);
+          keep(v1, 16 * i + 2 * t + 1);
+          keep(v2, 16 * i + 8 + 2 * t);
+          keep(v3, 16 * i + 9 + 2 * t);
+        }
         const unsigned* w0p = reinterpret_cast<const unsigned*>(&v0);
         const unsigned* w1p = reinterpret_cast<const unsigned*>(&v1);
         const unsigned* w2p = reinterpret_cast<const unsigned*>(&v2);
@@ -460,8 +509,11 @@ decode_attn_kv8_kernel(const A8Args a, const __grid_constant__ CUtensorMap tm_k,
       ++used;
     }
 
-    // ---- the CTA's partial of the segment: the warps add up in turn, in warp order ----
-    if (hi == w1) pdl_trigger();
+    // ---- the CTA's partial of the segment ----
+    // Behind the CTA's last segment the rings are free and every warp leaves its sums in its own; before that the warps add
+    // theirs up in turn in one buffer (next tiles are on their way into the rings meanwhile).  Either way in warp order.
+    const bool last_seg = hi == w1;
+    if (last_seg) pdl_trigger();
 #pragma unroll
     for (int cb = 0; cb < COLS; ++cb)
 #pragma unroll
@@ -475,116 +527,161 @@ decode_attn_kv8_kernel(const A8Args a, const __grid_constant__ CUtensorMap tm_k,
           sh.ml[warp][h][2] = l[cb][e];
         }
       }
-    __syncthreads();
-#pragma unroll 1
-    for (int turn = 0; turn < NW; ++turn) {
-      if (warp == turn) {
+    const auto leave = [&](float* to, bool add, bool scaled) {
 #pragma unroll
-        for (int cb = 0; cb < COLS; ++cb)
+      for (int cb = 0; cb < COLS; ++cb)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int h = cb * 8 + 2 * t + e;
-            if (h >= G) continue;
+        for (int e = 0; e < 2; ++e) {
+          const int h = cb * 8 + 2 * t + e;
+          if (h >= G) continue;
+          float f = 1.f;
+          if (scaled) {
             float Ms = -INFINITY;
 #pragma unroll
             for (int w = 0; w < NW; ++w) Ms = fmaxf(Ms, sh.ml[w][h][0]);
-            const float f = M[cb][e] == -INFINITY && Ms == -INFINITY ? 1.f : ex2(M[cb][e] - Ms);
-            float4* dst = reinterpret_cast<float4*>(o_s + h * OS_PITCH + 16 * g);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              float4 y = make_float4(o[cb][2 * i][e] * f, o[cb][2 * i][2 + e] * f, o[cb][2 * i + 1][e] * f, o[cb][2 * i + 1][2 + e] * f);
-              if (turn) {
-                const float4 old = dst[i];
-                y.x += old.x, y.y += old.y, y.z += old.z, y.w += old.w;
-              }
-              dst[i] = y;
-            }
+            f = M[cb][e] == Ms ? 1.f : ex2(M[cb][e] - Ms);
           }
-      }
+          float4* dst = reinterpret_cast<float4*>(to + h * OS_PITCH + 16 * g);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float4 y = make_float4(o[cb][2 * i][e] * f, o[cb][2 * i][2 + e] * f, o[cb][2 * i + 1][e] * f, o[cb][2 * i + 1][2 + e] * f);
+            if (add) {
+              const float4 old = dst[i];
+              y.x += old.x, y.y += old.y, y.z += old.z, y.w += old.w;
+            }
+            dst[i] = y;
+          }
+        }
+    };
+    if (last_seg) {
+      __syncwarp();
+      leave(reinterpret_cast<float*>(ring), false, false);
       __syncthreads();
+    } else {
+      __syncthreads();
+#pragma unroll 1
+      for (int turn = 0; turn < NW; ++turn) {
+        if (warp == turn) leave(o_s, turn > 0, true);
+        __syncthreads();
+      }
     }
     const int seg_no = b * a.KVH + kvh;
     const int c_lo = owner(seg_lo), parts = owner(seg_hi - 1) - c_lo + 1;
-    const auto finish = [](float acc, float Ms, float ms, float L) {  // a head without rows: zero
-      return L == 0.f ? 0.f : acc / L * exp2f(Ms - ms - 15.f);
+    const auto write_out = [&](int h, const float4& acc, float Ms, float ms, float L) {  // a head without rows: zero
+      const float f = L == 0.f ? 0.f : exp2f(Ms - ms - 11.f) / L;
+      T* dst = static_cast<T*>(a.out) + (size_t)b * a.q_sb + (size_t)(kvh * G + h) * a.q_sh + lane * 4;
+      *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(acc.x * f, acc.y * f), pack2<T>(acc.z * f, acc.w * f));
     };
-    for (int h = 0; h < G; ++h) {
-      float Ms = -INFINITY, ms = -INFINITY, L = 0.f;
-#pragma unroll
-      for (int w = 0; w < NW; ++w) {
-        Ms = fmaxf(Ms, sh.ml[w][h][0]);
-        ms = fmaxf(ms, sh.ml[w][h][1]);
+    for (int h = warp; h < G; h += NW) {  // a head per warp: lane w holds the factors of warp w's sums
+      float Mw = -INFINITY, mw = -INFINITY, L = 0.f;
+      if (lane < NW) {
+        Mw = sh.ml[lane][h][0];
+        mw = sh.ml[lane][h][1];
+        L = sh.ml[lane][h][2];
       }
+      float Ms = Mw, ms = mw;
 #pragma unroll
-      for (int w = 0; w < NW; ++w)
-        if (sh.ml[w][h][2] != 0.f) L = fmaf(sh.ml[w][h][2], ex2(sh.ml[w][h][1] - ms), L);
-      const float acc = o_s[h * OS_PITCH + tid];
+      for (int off = 8; off > 0; off >>= 1) {
+        Ms = fmaxf(Ms, __shfl_xor_sync(0xffffffffu, Ms, off));
+        ms = fmaxf(ms, __shfl_xor_sync(0xffffffffu, ms, off));
+      }
+      Ms = __shfl_sync(0xffffffffu, Ms, 0);
+      ms = __shfl_sync(0xffffffffu, ms, 0);
+      if (L != 0.f && mw != ms) L *= ex2(mw - ms);
+      const float f = Mw == Ms ? 1.f : ex2(Mw - Ms);
+#pragma unroll
+      for (int off = 8; off > 0; off >>= 1) L += __shfl_xor_sync(0xffffffffu, L, off);
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (last_seg) {
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+          const float4 v = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(smem + w * STAGES * STAGE_BYTES) + h * OS_PITCH + lane * 4);
+          const float fw = __shfl_sync(0xffffffffu, f, w);
+          acc.x = fmaf(v.x, fw, acc.x), acc.y = fmaf(v.y, fw, acc.y), acc.z = fmaf(v.z, fw, acc.z), acc.w = fmaf(v.w, fw, acc.w);
+        }
+      } else {
+        acc = *reinterpret_cast<const float4*>(o_s + h * OS_PITCH + lane * 4);
+      }
       if (parts == 1) {
-        static_cast<T*>(a.out)[(size_t)b * a.q_sb + (size_t)(kvh * G + h) * a.q_sh + tid] = from_float<T>(finish(acc, Ms, ms, L) * half2_unit<FMT>());
+        write_out(h, acc, Ms, ms, __shfl_sync(0xffffffffu, L, 0));
       } else {
         const size_t slot = (size_t)(c + seg_no) * G + h;  // (CTA, segment) pairs walk a staircase: their sum is unique
-        a.ws_o[slot * kHeadDim + tid] = acc;
-        if (tid == 0) a.ws_ml[slot] = make_float4(Ms, ms, L, 0.f);
+        *reinterpret_cast<float4*>(a.ws_o + slot * kHeadDim + lane * 4) = acc;
+        if (lane == 0) a.ws_ml[slot] = make_float4(Ms, ms, L, 0.f);
       }
     }
     if (parts > 1) {
-      __threadfence();
       __syncthreads();
-      if (tid == 0) sh.last = atomicAdd(a.ws_cnt + seg_no, 1u) == (unsigned)(parts - 1);
+      if (tid == 0) {
+        __threadfence();  // the CTA's stores, ordered before the barrier, are visible before its arrival is
+        sh.last = atomicAdd(a.ws_cnt + seg_no, 1u) == (unsigned)(parts - 1);
+        __threadfence();
+      }
       __syncthreads();
       if (sh.last) {
-        __threadfence();
-        // one warp per head, four dimensions per lane
-        for (int h = warp; h < G; h += NW) {
-          const size_t base = (size_t)(c_lo + seg_no) * G + h;
-          const float4* op = reinterpret_cast<const float4*>(a.ws_o + base * kHeadDim) + lane;
-          const float4* mp = a.ws_ml + base;
-          const int o_step = G * (kHeadDim / 4);
-          constexpr int PRE = 16;
-          float4 first_o[PRE];  // asked for together with the maxima
-#pragma unroll
-          for (int p = 0; p < PRE; ++p) first_o[p] = p < parts ? __ldcg(op + (size_t)p * o_step) : make_float4(0.f, 0.f, 0.f, 0.f);
-          float Ms = -INFINITY, ms = -INFINITY;
-          for (int p = lane; p < parts; p += 32) {
-            const float4 v = __ldcg(mp + (size_t)p * G);
-            Ms = fmaxf(Ms, v.x);
-            ms = fmaxf(ms, v.y);
-          }
-#pragma unroll
-          for (int off = 16; off > 0; off >>= 1) {
-            Ms = fmaxf(Ms, __shfl_xor_sync(0xffffffffu, Ms, off));
-            ms = fmaxf(ms, __shfl_xor_sync(0xffffffffu, ms, off));
-          }
-          float L = 0.f;
+        // `per` warps share a head, each with every per-th partial, four dimensions per lane; their sums meet in o_s
+        const int per = max(1, NW / G);
+        for (int h0 = 0; h0 < G; h0 += NW / per) {
+          const int h = h0 + warp / per, part = warp % per;
+          const bool on = h < min(G, h0 + NW / per);
+          float Ms = -INFINITY, ms = -INFINITY, L = 0.f;
           float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-          const auto add = [&](const float4& v, float f) {
-            acc.x = fmaf(v.x, f, acc.x), acc.y = fmaf(v.y, f, acc.y), acc.z = fmaf(v.z, f, acc.z), acc.w = fmaf(v.w, f, acc.w);
-          };
-          for (int p0 = 0; p0 < parts; p0 += 32) {
-            float f = 0.f;
-            if (p0 + lane < parts) {
-              const float4 v = __ldcg(mp + (size_t)(p0 + lane) * G);
-              f = v.x == -INFINITY && Ms == -INFINITY ? 1.f : ex2(v.x - Ms);
-              if (v.z != 0.f) L = fmaf(v.z, ex2(v.y - ms), L);
-            }
-            const int n = min(32, parts - p0);
-            if (p0 == 0) {
+          if (on) {
+            const size_t base = (size_t)(c_lo + seg_no) * G + h;
+            const float4* op = reinterpret_cast<const float4*>(a.ws_o + base * kHeadDim) + lane;
+            const float4* mp = a.ws_ml + base;
+            const int o_step = G * (kHeadDim / 4);
+            constexpr int PRE = 8;
+            float4 first_o[PRE];  // this warp's partials part, part + per, ...: asked for together with the maxima
 #pragma unroll
-              for (int p = 0; p < PRE; ++p) add(first_o[p], __shfl_sync(0xffffffffu, f, p));
-#pragma unroll 16
-              for (int p = PRE; p < n; ++p) add(__ldcg(op + (size_t)p * o_step), __shfl_sync(0xffffffffu, f, p));
-            } else {
-#pragma unroll 16
-              for (int p = 0; p < n; ++p) add(__ldcg(op + (size_t)(p0 + p) * o_step), __shfl_sync(0xffffffffu, f, p));
+            for (int i = 0; i < PRE; ++i) first_o[i] = part + i * per < parts ? __ldcg(op + (size_t)(part + i * per) * o_step) : acc;
+            const float4 none = make_float4(-INFINITY, -INFINITY, 0.f, 0.f);
+            const float4 first_ml = lane < parts ? __ldcg(mp + (size_t)lane * G) : none;
+            Ms = first_ml.x;
+            ms = first_ml.y;
+            for (int p = lane + 32; p < parts; p += 32) {
+              const float4 v = __ldcg(mp + (size_t)p * G);
+              Ms = fmaxf(Ms, v.x);
+              ms = fmaxf(ms, v.y);
             }
+#pragma unroll
+            for (int off = 16; off > 0; off >>= 1) {
+              Ms = fmaxf(Ms, __shfl_xor_sync(0xffffffffu, Ms, off));
+              ms = fmaxf(ms, __shfl_xor_sync(0xffffffffu, ms, off));
+            }
+            const auto add = [&](const float4& v, float f) {
+              acc.x = fmaf(v.x, f, acc.x), acc.y = fmaf(v.y, f, acc.y), acc.z = fmaf(v.z, f, acc.z), acc.w = fmaf(v.w, f, acc.w);
+            };
+            int p = part;
+            for (int p0 = 0; p0 < parts; p0 += 32) {  // lane p - p0 holds the factor of partial p
+              float4 v = first_ml;
+              if (p0) v = p0 + lane < parts ? __ldcg(mp + (size_t)(p0 + lane) * G) : none;
+              const float f = v.x == Ms ? 1.f : ex2(v.x - Ms);
+              if (v.z != 0.f) L = fmaf(v.z, v.y == ms ? 1.f : ex2(v.y - ms), L);
+              const int end = min(parts, p0 + 32);
+              if (p0 == 0) {
+#pragma unroll
+                for (int i = 0; i < PRE; ++i) {
+                  if (p >= end) continue;
+                  add(first_o[i], __shfl_sync(0xffffffffu, f, p));
+                  p += per;
+                }
+              }
+#pragma unroll 8
+              for (; p < end; p += per) add(__ldcg(op + (size_t)p * o_step), __shfl_sync(0xffffffffu, f, p - p0));
+            }
+#pragma unroll
+            for (int off = 16; off > 0; off >>= 1) L += __shfl_xor_sync(0xffffffffu, L, off);
+            if (per > 1) *reinterpret_cast<float4*>(o_s + warp * OS_PITCH + lane * 4) = acc;
           }
-#pragma unroll
-          for (int off = 16; off > 0; off >>= 1) L += __shfl_xor_sync(0xffffffffu, L, off);
-          T* dst = static_cast<T*>(a.out) + (size_t)b * a.q_sb + (size_t)(kvh * G + h) * a.q_sh + lane * 4;
-          dst[0] = from_float<T>(finish(acc.x, Ms, ms, L) * half2_unit<FMT>());
-          dst[1] = from_float<T>(finish(acc.y, Ms, ms, L) * half2_unit<FMT>());
-          dst[2] = from_float<T>(finish(acc.z, Ms, ms, L) * half2_unit<FMT>());
-          dst[3] = from_float<T>(finish(acc.w, Ms, ms, L) * half2_unit<FMT>());
+          if (per > 1) __syncthreads();
+          if (on && part == 0) {
+            for (int w = 1; w < per; ++w) {
+              const float4 v = *reinterpret_cast<const float4*>(o_s + (warp + w) * OS_PITCH + lane * 4);
+              acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
+            }
+            write_out(h, acc, Ms, ms, L);
+          }
         }
         if (tid == 0) a.ws_cnt[seg_no] = 0u;
       }
@@ -603,19 +700,19 @@ decode_attn_kv8_kernel(const A8Args a, const __grid_constant__ CUtensorMap tm_k,
     for (int i = used; i < asked; ++i) mbar_wait(&sh.full[warp][i % STAGES], (i / STAGES) & 1);
 }
 
-constexpr int smem_bytes(bool tma, int G) {
-  return NW * STAGES * (tma ? TMA_STAGE : ROWS_STAGE) + G * OS_PITCH * 4 + 1024;
+constexpr int smem_bytes(bool tma, int cols) {
+  return kWarps[cols] * STAGES * (tma ? TMA_STAGE : ROWS_STAGE) + 16 * OS_PITCH * 4 + 1024;
 }
 
 template <typename T, int FMT, int COLS, bool TMA>
 int launch(const A8Args& a, int ctas, const CUtensorMap& tm_k, const CUtensorMap& tm_v, cudaStream_t st) {
   static std::atomic<unsigned long long> done{0};
   auto kern = decode_attn_kv8_kernel<T, FMT, COLS, TMA>;
-  if (const int rc = allow_smem(kern, smem_bytes(TMA, 8 * COLS), done)) return rc;
+  if (const int rc = allow_smem(kern, smem_bytes(TMA, COLS), done)) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas);
-  cfg.blockDim = dim3(NT);
-  cfg.dynamicSmemBytes = smem_bytes(TMA, a.G);
+  cfg.blockDim = dim3(kWarps[COLS] * 32);
+  cfg.dynamicSmemBytes = smem_bytes(TMA, COLS);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -632,7 +729,7 @@ int launch_any(const A8Args& a, int ctas, bool tma, const CUtensorMap& tm_k, con
   return tma ? launch<T, FMT, 2, true>(a, ctas, tm_k, tm_v, st) : launch<T, FMT, 2, false>(a, ctas, tm_k, tm_v, st);
 }
 
-constexpr long long kMaxCtas = 65536;
+constexpr int kMaxCtas = 32768;
 
 inline long long slots_of(int B, int KVH, int ctas) { return (long long)ctas + (long long)B * KVH; }
 
@@ -657,6 +754,8 @@ extern "C" int omnikv_kv8_decode_attn(const omnikv_kv8_attn_params* p, void* str
   if (p->tail_len && !p->tail_start) return OMNIKV_E_BADARG;
   if (p->score_out && (p->idx || p->tail_len || !p->score_len || p->score_stride <= 0)) return OMNIKV_E_BADARG;
   if (!is_16bit(p->dtype) || p->H / c.KVH > MAX_G) return OMNIKV_E_UNSUPPORTED;
+  const int64_t most = (p->idx ? p->idx_cap : (int64_t)c.rows) + (p->tail_len ? c.rows : 0);
+  if ((most / TILE + 2) * c.B * c.KVH > 0x7fffffff) return OMNIKV_E_UNSUPPORTED;  // tiles are counted in 32 bits
   if (p->n_ctas > kMaxCtas || (size_t)c.B * c.KVH * 4 > kAttnCntBytes) return OMNIKV_E_UNSUPPORTED;
   if (!p->workspace || p->workspace_bytes < omnikv_kv8_attn_workspace_bytes(c.B, p->H, c.KVH, p->n_ctas)) return OMNIKV_E_WORKSPACE;
   if (bad16(p->workspace)) return OMNIKV_E_BADARG;

@@ -702,8 +702,8 @@ def kv8_decode_attn(q: torch.Tensor, k8, v8, k_scale, v_scale, len_a: torch.Tens
                 or not score_out.is_contiguous() or score_out.shape[2] == 0:
             raise abi.OmniKVError("kv8_decode_attn: score_out must be contiguous fp32 [KVH, B, stride]")
         score_ptr, score_stride = score_out.data_ptr(), score_out.shape[2]
-    # two CTAs per SM, each with at least four tiles of 32 rows (the kernel cuts the rows that there are into equal pieces)
-    n_ctas = n_splits * B * KVH if n_splits else min(2 * sm_count(dev), ((max_rows or cap) // 128 + 1) * B * KVH)
+    # one CTA per SM; fewer when there are fewer (sequence, KV head) pairs and not a tile of 32 rows for each of twelve warps
+    n_ctas = n_splits * B * KVH if n_splits else min(sm_count(dev), ((max_rows or cap) // 384 + 1) * B * KVH)
     if ws is None:
         ws = _own_workspace(dev, abi.lib().omnikv_kv8_attn_workspace_bytes(B, H, KVH, n_ctas), "kv8_attn")
     p = abi.Kv8AttnParams(c, dt, H, scale if scale is not None else 0.08838834764831845, q.data_ptr(), strides[0], strides[1],

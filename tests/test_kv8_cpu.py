@@ -57,7 +57,7 @@ def test_attention_arguments_are_checked():
                    dict(tail_len=256), dict(score_out=256), dict(score_out=256, score_len=256, score_stride=8, idx=256, idx_cap=4),
                    dict(workspace=264)):
         assert call(**change) == -1, change
-    for change in (dict(dtype=abi.F32), dict(H=136), dict(n_ctas=65537)):
+    for change in (dict(dtype=abi.F32), dict(H=136), dict(n_ctas=32769)):
         assert call(**change) == -2, change
     assert call(workspace_bytes=16384) == -3 and call(workspace=None) == -3
     assert lib.omnikv_kv8_decode_attn(None, None) == -1

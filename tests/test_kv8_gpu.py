@@ -290,6 +290,7 @@ def test_what_lies_behind_a_sequence_does_not_matter(fmt):
         t[:, :, 5:] = float("nan")  # blocks behind row 80
     for t in cache[:2]:
         t[:, :, n:].copy_(x[:, :, n:].to(CODES[fmt]) if fmt == "e4m3" else torch.full_like(t[:, :, n:], -128))
+        t.view(torch.int8)[:, :, n:, ::3] = 127  # a NaN code in e4m3
     assert torch.equal(ops().kv8_decode_attn(q, *cache, i32([n]), block=block), want)
     cache[1].view(torch.int8)[:, :, 32:48], cache[3][:, :, 2] = 0, float("inf")  # a block inside it that reads as NaN
     assert torch.isnan(ops().kv8_decode_attn(q, *cache, i32([n]), block=block)).all()
