@@ -300,7 +300,8 @@ decode_attn_kv8_kernel(const A8Args a, const __grid_constant__ CUtensorMap tm_k,
   int next_w = w0 + warp;  // the warp's next tile
   for (int lo = w0; lo < w1;) {
     const int seg_hi = seg_lo + seg.nt, hi = min(w1, seg_hi);  // this CTA's tiles of the segment: [lo, hi)
-    const int b = seg.b, kvh = seg.kvh;
+    const int b = seg.b, kvh = seg.kvh, seg_no = b * a.KVH + kvh;
+    const int c_lo = owner(seg_lo), parts = owner(seg_hi - 1) - c_lo + 1;  // the CTAs that share it
 
     // ---- queries: fragments of q * 2^e (largest element in [2^13, 2^14)), e folded into the head's factor ----
     unsigned qf[COLS][8][2];
@@ -565,8 +566,6 @@ decode_attn_kv8_kernel(const A8Args a, const __grid_constant__ CUtensorMap tm_k,
         __syncthreads();
       }
     }
-    const int seg_no = b * a.KVH + kvh;
-    const int c_lo = owner(seg_lo), parts = owner(seg_hi - 1) - c_lo + 1;
     const auto write_out = [&](int h, const float4& acc, float Ms, float ms, float L) {  // a head without rows: zero
       const float f = L == 0.f ? 0.f : exp2f(Ms - ms - 11.f) / L;
       T* dst = static_cast<T*>(a.out) + (size_t)b * a.q_sb + (size_t)(kvh * G + h) * a.q_sh + lane * 4;

@@ -21,8 +21,10 @@ inline Kv8View view_of(const omnikv_kv8_cache* c) {
 }
 
 // ---- store ------------------------------------------------------------------------------------------------------
-// A CTA takes PASSES * 16 rows of one (sequence, head) of K or V: sixteen lanes hold a row, eight elements each, in
-// registers between the two steps (maximum of the block, codes), so every element is read once.
+// A CTA takes 128 rows (256 where a scale block is that long) of one (sequence, head) of K or V: sixteen lanes hold a row,
+// eight elements each, in registers between the two steps (maximum of the block, codes), so every element is read once.
+// One thread per scale block turns its maximum into the rule for its codes: the divisions that takes were a third of the
+// instructions when every thread did it (131072 rows of 8 heads: 149 -> 123 us).
 constexpr int ST_THREADS = 256, ST_ROWS = ST_THREADS / 16;
 
 struct StoreArgs {
@@ -33,11 +35,14 @@ struct StoreArgs {
   const int* lens;
 };
 
-template <typename T, int FMT, int PASSES>
+// PPB: passes of 16 rows per scale block; 0: blocks shorter than a pass.
+template <typename T, int FMT, int PASSES, int PPB>
 __global__ void __launch_bounds__(ST_THREADS) kv8_store_kernel(const StoreArgs a) {
-  constexpr int R = PASSES * ST_ROWS;
-  __shared__ unsigned top[R];  // largest magnitude per scale block of this CTA (one per row at most)
+  constexpr int R = PASSES * ST_ROWS, WARPS = ST_THREADS / 32, BLOCKS = PPB ? PASSES / PPB : R;
+  __shared__ unsigned top[BLOCKS][PPB ? WARPS : 1];  // largest magnitude of each scale block, by warp
+  __shared__ float2 rules[BLOCKS];
   pdl_wait();
+  pdl_trigger();
   const int tid = threadIdx.x, lane16 = tid & 15, row16 = tid >> 4;
   const int h = blockIdx.y >> 1, b = blockIdx.z;
   const bool is_v = blockIdx.y & 1;
@@ -45,41 +50,52 @@ __global__ void __launch_bounds__(ST_THREADS) kv8_store_kernel(const StoreArgs a
   const int r0 = blockIdx.x * R;
   if (r0 >= n) return;
   const int shift = 31 - __clz(a.c.block);
-  const T* src = static_cast<const T*>(is_v ? a.v : a.k) + (size_t)b * (is_v ? a.v_sb : a.k_sb) + (size_t)h * (is_v ? a.v_sh : a.k_sh);
   const int64_t s_sr = is_v ? a.v_sr : a.k_sr;
-  for (int i = tid; i < R; i += ST_THREADS) top[i] = 0;
+  const T* src = static_cast<const T*>(is_v ? a.v : a.k) + (size_t)b * (is_v ? a.v_sb : a.k_sb) + (size_t)h * (is_v ? a.v_sh : a.k_sh) +
+                 (int64_t)(r0 + row16) * s_sr + lane16 * 8;
   uint4 x[PASSES];
 #pragma unroll
   for (int p = 0; p < PASSES; ++p) {
-    const int r = r0 + p * ST_ROWS + row16;
     x[p] = make_uint4(0, 0, 0, 0);
-    if (r < n) x[p] = reinterpret_cast<const uint4*>(src + (size_t)r * s_sr)[lane16];
+    if (r0 + p * ST_ROWS + row16 < n) x[p] = *reinterpret_cast<const uint4*>(src + p * ST_ROWS * s_sr);
+  }
+  if constexpr (PPB > 0) {
+#pragma unroll
+    for (int i = 0; i < BLOCKS; ++i) {
+      unsigned m2 = 0;
+#pragma unroll
+      for (int p = i * PPB; p < (i + 1) * PPB; ++p) m2 = max_abs2<T>(m2, x[p]);
+      const unsigned m = __reduce_max_sync(0xffffffffu, abs_bits_of<T>(m2));
+      if ((tid & 31) == 0) top[i][tid >> 5] = m;
+    }
+  } else {
+    for (int i = tid; i < R; i += ST_THREADS) top[i][0] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int p = 0; p < PASSES; ++p) {
+      unsigned m = abs_bits_of<T>(max_abs2<T>(0u, x[p]));
+#pragma unroll
+      for (int off = 8; off > 0; off >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, off));
+      if (lane16 == 0 && m) atomicMax(&top[(p * ST_ROWS + row16) >> shift][0], m);
+    }
   }
   __syncthreads();
+  if (tid < (PPB ? BLOCKS : R >> shift)) {
+    unsigned m = top[tid][0];
+    if constexpr (PPB > 0)
 #pragma unroll
-  for (int p = 0; p < PASSES; ++p) {
-    const unsigned* w = reinterpret_cast<const unsigned*>(&x[p]);
-    unsigned m2 = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) m2 = max_abs2(m2, w[i]);
-    unsigned m = abs_bits_of<T>(m2);
-#pragma unroll
-    for (int off = 8; off > 0; off >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, off));
-    if (lane16 == 0 && m) atomicMax(&top[(p * ST_ROWS + row16) >> shift], m);
+      for (int w = 1; w < WARPS; ++w) m = max(m, top[tid][w]);
+    const CodeRule rule = code_rule<FMT>(m);
+    rules[tid] = shared_rule<FMT>(rule, m);
+    float* scale = (is_v ? a.c.vs : a.c.ks) + (size_t)b * a.c.ssb + (size_t)h * a.c.ssh + ((a.start + r0) >> shift);
+    if (r0 + (tid << shift) < n) scale[tid] = rule.scale;
   }
   __syncthreads();
-  unsigned char* dst = (is_v ? a.c.v : a.c.k) + (size_t)b * a.c.sb + (size_t)h * a.c.sh;
-  float* scale = (is_v ? a.c.vs : a.c.ks) + (size_t)b * a.c.ssb + (size_t)h * a.c.ssh;
+  unsigned char* dst = (is_v ? a.c.v : a.c.k) + (size_t)b * a.c.sb + (size_t)h * a.c.sh + ((int64_t)a.start + r0 + row16) * a.c.sr + lane16 * 8;
 #pragma unroll
   for (int p = 0; p < PASSES; ++p) {
-    const int lr = p * ST_ROWS + row16, r = r0 + lr;
-    if (r >= n) continue;
-    const CodeRule rule = code_rule<FMT>(top[lr >> shift]);
-    const unsigned* w = reinterpret_cast<const unsigned*>(&x[p]);
-    const int64_t at = (int64_t)a.start + r;
-    *reinterpret_cast<uint2*>(dst + at * a.c.sr + lane16 * 8) =
-        make_uint2(code4<FMT>(rule, unpack16<T>(w[0]), unpack16<T>(w[1])), code4<FMT>(rule, unpack16<T>(w[2]), unpack16<T>(w[3])));
-    if (lane16 == 0 && (r & (a.c.block - 1)) == 0) scale[at >> shift] = rule.scale;
+    const int lr = p * ST_ROWS + row16;
+    if (r0 + lr < n) *reinterpret_cast<uint2*>(dst + p * ST_ROWS * a.c.sr) = code8<T, FMT>(rules[PPB ? p / (PPB ? PPB : 1) : lr >> shift], x[p]);
   }
 }
 
@@ -93,6 +109,7 @@ template <typename T, int FMT>
 __global__ void __launch_bounds__(AP_THREADS) kv8_append_kernel(const Kv8View c, const T* k_new, const T* v_new,
                                                                 int64_t n_sb, int64_t n_sh, const int* pos_dev) {
   pdl_wait();
+  pdl_trigger();
   const int tid = threadIdx.x, lane = tid & 31;
   const int h = blockIdx.x >> 1, b = blockIdx.y;
   const bool is_v = blockIdx.x & 1;
@@ -152,6 +169,7 @@ __global__ void __launch_bounds__(LD_THREADS) kv8_load_kernel(const Kv8View c, i
                                                               int64_t idx_stride, T* k_out, T* v_out, int64_t o_sb,
                                                               int64_t o_sh, int64_t o_sr) {
   pdl_wait();
+  pdl_trigger();
   const int i = blockIdx.x * (LD_THREADS / 8) + (threadIdx.x >> 3), piece = threadIdx.x & 7;
   if (i >= n) return;
   const int h = blockIdx.y >> 1, b = blockIdx.z;
@@ -182,10 +200,14 @@ int launch_store(const StoreArgs& a, int B, cudaStream_t st) {
     OMNIKV_CUDA_OK(launch_pdl(kern, dim3(ceil_div(a.n, rows), 2 * a.KVH, B), dim3(ST_THREADS), 0, st, a));
     return OMNIKV_OK;
   };
-  // 64 rows per CTA: four 16-byte loads per thread in flight; a longer block needs a CTA of its own
-  if (a.c.block <= 64) return go(kv8_store_kernel<T, FMT, 4>, 64);
-  if (a.c.block == 128) return go(kv8_store_kernel<T, FMT, 8>, 128);
-  return go(kv8_store_kernel<T, FMT, 16>, 256);
+  switch (a.c.block) {
+    case 16: return go(kv8_store_kernel<T, FMT, 8, 1>, 128);
+    case 32: return go(kv8_store_kernel<T, FMT, 8, 2>, 128);
+    case 64: return go(kv8_store_kernel<T, FMT, 8, 4>, 128);
+    case 128: return go(kv8_store_kernel<T, FMT, 8, 8>, 128);
+    case 256: return go(kv8_store_kernel<T, FMT, 16, 16>, 256);
+    default: return go(kv8_store_kernel<T, FMT, 8, 0>, 128);
+  }
 }
 
 // kernel<element type, format> for the two 16-bit types and the two formats

@@ -39,14 +39,18 @@ __device__ __forceinline__ float code_value(unsigned byte) {
 // with X < 2^11; e4m3: 2^-16), so the rounded fp32 quotient lies on the true side and the code is that of exact arithmetic.
 // (top x could overflow for a >= 2^64: both sides are scaled down by a power of two there.)
 //
-// Four values (code4): x * (top / a) is within 2^-23 of the quotient, which is the true side for every quotient but an
-// exact middle, and exact middles do occur (x = a / 2).  Rounding that product to 21 bits puts those, which have at most
-// 8, back in place and moves no other quotient by more than 2^-20.6: five instructions per value instead of a division's
-// thirty (a store of 131072 rows of 8 heads: 269 -> 194 us).
+// Four values (code4), a third of a division's instructions (a store of 131072 rows of 8 heads: 269 -> 123 us).  A
+// product with the rounded factor top / a is within 2^-23 of the quotient, which is the true side for every quotient but an
+// exact middle; and exact middles do occur.
+//   int8: (2k+1) A 2^m = 254 X has, unless 127 divides A, the one solution 2k+1 = 127, x = a / 2, which rounds to the even 64,
+//   away from zero: so the factor is rounded up.  Where 127 divides A the factor is a power of two and nothing is rounded, or
+//   (fp16 only) the values are divided.  The sum with 1.5 * 2^23 rounds the exact product to an integer, ties to even.
+//   e4m3: middles fall to both sides.  Rounding the product to 21 bits puts those, which have at most 8 bits, back in their
+//   place and moves no other quotient by more than 2^-20.6.
 struct CodeRule {
   float mul, den, scale, factor;
   bool live;  // false: all codes are zero (nothing but zeros, or something that is not finite)
-  bool tiny;  // top / a could overflow: code4 divides
+  bool divide;  // code4 divides: top / a could overflow, or see above
 };
 template <int FMT>
 __device__ __forceinline__ CodeRule code_rule(unsigned a_bits) {
@@ -57,45 +61,24 @@ __device__ __forceinline__ CodeRule code_rule(unsigned a_bits) {
   const float f = a >= 18446744073709551616.f ? 5.421010862427522e-20f : 1.f;  // 2^64, 2^-64
   r.mul = code_top<FMT>() * f;
   r.den = r.live ? a * f : 1.f;
-  r.tiny = a < 7.888609052210118e-31f;  // 2^-100
-  r.factor = r.live && !r.tiny ? __fdiv_rn(code_top<FMT>(), a) : 0.f;
+  r.divide = a < 7.888609052210118e-31f;  // 2^-100
+  r.factor = 0.f;
+  if (r.live && !r.divide) {
+    r.factor = FMT == kInt8 ? __fdiv_ru(127.f, a) : __fdiv_rn(code_top<FMT>(), a);
+    if (FMT == kInt8 && fmaf(r.scale, 127.f, -a) == 0.f && fmaf(r.factor, a, -127.f) != 0.f) r.divide = true;
+  }
   return r;
 }
 template <int FMT>
 __device__ __forceinline__ unsigned code_with(const CodeRule& r, float x) {
   return r.live ? code_of<FMT>(__fdiv_rn(x * r.mul, r.den)) : 0u;
 }
-__device__ __forceinline__ float to_21_bits(float x) { return __uint_as_float((__float_as_uint(x) + 4u) & ~7u); }
-// The codes of four values, packed.
+// What the threads of a CTA share of a rule: {factor, a}; factor 0: all codes zero, negative: divide.
 template <int FMT>
-__device__ __forceinline__ unsigned code4(const CodeRule& r, float2 x, float2 y) {
-  if (r.tiny) return code_with<FMT>(r, x.x) | code_with<FMT>(r, x.y) << 8 | code_with<FMT>(r, y.x) << 16 | code_with<FMT>(r, y.y) << 24;
-  const float q0 = to_21_bits(x.x * r.factor), q1 = to_21_bits(x.y * r.factor);
-  const float q2 = to_21_bits(y.x * r.factor), q3 = to_21_bits(y.y * r.factor);
-  unsigned w;
-  if constexpr (FMT == kInt8) {  // adding 1.5 * 2^23 rounds to an integer (ties to even) and leaves it in the low byte
-    constexpr float kBig = 12582912.f;
-    const unsigned lo = __byte_perm(__float_as_uint(q0 + kBig), __float_as_uint(q1 + kBig), 0x0040);
-    const unsigned hi = __byte_perm(__float_as_uint(q2 + kBig), __float_as_uint(q3 + kBig), 0x0040);
-    w = __byte_perm(lo, hi, 0x5410);
-  } else {
-    w = (unsigned)__nv_cvt_float2_to_fp8x2(make_float2(q0, q1), __NV_SATFINITE, __NV_E4M3) |
-        (unsigned)__nv_cvt_float2_to_fp8x2(make_float2(q2, q3), __NV_SATFINITE, __NV_E4M3) << 16;
-  }
-  return r.live ? w : 0u;
+__device__ __forceinline__ float2 shared_rule(const CodeRule& r, unsigned a_bits) {
+  return make_float2(!r.live ? 0.f : r.divide ? -1.f : r.factor, __uint_as_float(a_bits));
 }
-
-// Largest magnitude of the two 16-bit elements of a word, and of two words, as 16-bit patterns side by side: the order of
-// the patterns without the sign is the order of the magnitudes (NaN above infinity), in both 16-bit types.
-__device__ __forceinline__ unsigned max_abs2(unsigned m, unsigned w) { return __vmaxu2(m, w & 0x7fff7fffu); }
-// ... as the bits of a float
-template <typename T>
-__device__ __forceinline__ unsigned abs_bits_of(unsigned m2) {
-  const unsigned m = max(m2 & 0xffffu, m2 >> 16);
-  if constexpr (std::is_same<T, __half>::value) return abs_bits(__half2float(__ushort_as_half((unsigned short)m)));
-  else return m << 16;
-}
-
+__device__ __forceinline__ float to_21_bits(float x) { return __uint_as_float((__float_as_uint(x) + 4u) & ~7u); }
 // Two 16-bit elements of a 32-bit word as floats.
 template <typename T>
 __device__ __forceinline__ float2 unpack16(unsigned u);
@@ -106,6 +89,53 @@ __device__ __forceinline__ float2 unpack16<__nv_bfloat16>(unsigned u) {
 template <>
 __device__ __forceinline__ float2 unpack16<__half>(unsigned u) {
   return __half22float2(*reinterpret_cast<__half2*>(&u));
+}
+
+// The codes of four values, packed.
+template <int FMT>
+__device__ __forceinline__ unsigned code4(const float2& rule, float2 x, float2 y) {
+  const float f = rule.x;
+  if (f <= 0.f) {
+    if (f == 0.f) return 0u;
+    const CodeRule r = code_rule<FMT>(__float_as_uint(rule.y));
+    return code_with<FMT>(r, x.x) | code_with<FMT>(r, x.y) << 8 | code_with<FMT>(r, y.x) << 16 | code_with<FMT>(r, y.y) << 24;
+  }
+  if constexpr (FMT == kInt8) {
+    constexpr float kBig = 12582912.f;
+    const unsigned q0 = __float_as_uint(fmaf(x.x, f, kBig)), q1 = __float_as_uint(fmaf(x.y, f, kBig));
+    const unsigned q2 = __float_as_uint(fmaf(y.x, f, kBig)), q3 = __float_as_uint(fmaf(y.y, f, kBig));
+    return __byte_perm(__byte_perm(q0, q1, 0x0040), __byte_perm(q2, q3, 0x0040), 0x5410);
+  } else {
+    return (unsigned)__nv_cvt_float2_to_fp8x2(make_float2(to_21_bits(x.x * f), to_21_bits(x.y * f)), __NV_SATFINITE, __NV_E4M3) |
+           (unsigned)__nv_cvt_float2_to_fp8x2(make_float2(to_21_bits(y.x * f), to_21_bits(y.y * f)), __NV_SATFINITE, __NV_E4M3) << 16;
+  }
+}
+// ... of the eight 16-bit elements of a 16-byte piece
+template <typename T, int FMT>
+__device__ __forceinline__ uint2 code8(const float2& rule, const uint4& v) {
+  return make_uint2(code4<FMT>(rule, unpack16<T>(v.x), unpack16<T>(v.y)), code4<FMT>(rule, unpack16<T>(v.z), unpack16<T>(v.w)));
+}
+
+// Running largest magnitudes of the two 16-bit elements of a word, side by side (a NaN stays), and the larger of both as
+// the bits of a float.
+template <typename T>
+__device__ __forceinline__ unsigned max_abs2(unsigned m, unsigned w) {
+  unsigned r;
+  if constexpr (std::is_same<T, __half>::value)
+    asm("max.NaN.f16x2 %0, %1, %2;\n" : "=r"(r) : "r"(m), "r"(w & 0x7fff7fffu));
+  else
+    asm("max.NaN.bf16x2 %0, %1, %2;\n" : "=r"(r) : "r"(m), "r"(w & 0x7fff7fffu));
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ unsigned max_abs2(unsigned m, const uint4& v) {
+  return max_abs2<T>(max_abs2<T>(max_abs2<T>(max_abs2<T>(m, v.x), v.y), v.z), v.w);
+}
+template <typename T>
+__device__ __forceinline__ unsigned abs_bits_of(unsigned m2) {
+  const unsigned m = max(m2 & 0x7fffu, (m2 >> 16) & 0x7fffu);  // the order of the patterns is the order of the magnitudes
+  if constexpr (std::is_same<T, __half>::value) return abs_bits(__half2float(__ushort_as_half((unsigned short)m)));
+  else return m << 16;
 }
 
 // Host: an omnikv_kv8_cache that the kernels can read.

@@ -18,42 +18,43 @@ namespace {
 // ---- rows to codes ------------------------------------------------------------------------------------------------
 // One CTA per row; the row stays in registers between the maximum and the codes, so it is read once and with one round
 // of loads in flight (a single token's row is a latency chain: load, maximum, store).
-constexpr int QR_VEC = 8;  // 16-byte pieces per thread at most
-
-template <typename T, int THREADS>
-__global__ void __launch_bounds__(THREADS) quant_rows_kernel(const T* x, int64_t x_sr, int K, int8_t* codes, int64_t c_sr,
+// VEC: 16-byte pieces per thread at most.
+template <typename T, int THREADS, int VEC>
+__global__ void __launch_bounds__(THREADS, THREADS > 512 ? 1 : 1024 / THREADS) quant_rows_kernel(const T* x, int64_t x_sr, int K, int8_t* codes, int64_t c_sr,
                                                              float* scale) {
   __shared__ unsigned top[THREADS / 32];
+  __shared__ float2 shared;
   pdl_wait();
   pdl_trigger();  // the product behind it may set itself up; it waits for this grid before it reads anything
   const int row = blockIdx.x, tid = threadIdx.x, nvec = K / 8;
   const uint4* src = reinterpret_cast<const uint4*>(x + (size_t)row * x_sr);
-  uint4 v[QR_VEC];
+  uint4 v[VEC];
 #pragma unroll
-  for (int u = 0; u < QR_VEC; ++u) {
+  for (int u = 0; u < VEC; ++u) {
     v[u] = make_uint4(0, 0, 0, 0);
     if (tid + u * THREADS < nvec) v[u] = src[tid + u * THREADS];
   }
   unsigned m2 = 0;
 #pragma unroll
-  for (int u = 0; u < QR_VEC; ++u) {
-    m2 = max_abs2(max_abs2(m2, v[u].x), v[u].y);
-    m2 = max_abs2(max_abs2(m2, v[u].z), v[u].w);
-  }
+  for (int u = 0; u < VEC; ++u) m2 = max_abs2<T>(m2, v[u]);
   unsigned m = abs_bits_of<T>(m2);
   m = __reduce_max_sync(0xffffffffu, m);
   if ((tid & 31) == 0) top[tid >> 5] = m;
   __syncthreads();
+  if (tid == 0) {  // the divisions of a rule once per row
 #pragma unroll
-  for (int i = 0; i < THREADS / 32; ++i) m = max(m, top[i]);
-  const CodeRule rule = code_rule<kInt8>(m);
-  if (tid == 0) scale[row] = rule.scale;
+    for (int i = 1; i < THREADS / 32; ++i) m = max(m, top[i]);
+    const CodeRule rule = code_rule<kInt8>(m);
+    shared = shared_rule<kInt8>(rule, m);
+    scale[row] = rule.scale;
+  }
+  __syncthreads();
+  const float2 rule = shared;
   uint2* dst = reinterpret_cast<uint2*>(codes + (size_t)row * c_sr);
 #pragma unroll
-  for (int u = 0; u < QR_VEC; ++u) {
+  for (int u = 0; u < VEC; ++u) {
     if (tid + u * THREADS >= nvec) continue;
-    dst[tid + u * THREADS] = make_uint2(code4<kInt8>(rule, unpack16<T>(v[u].x), unpack16<T>(v[u].y)),
-                                        code4<kInt8>(rule, unpack16<T>(v[u].z), unpack16<T>(v[u].w)));
+    dst[tid + u * THREADS] = code8<T, kInt8>(rule, v[u]);
   }
 }
 
@@ -407,20 +408,253 @@ linear_tile_kernel(const LinArgs a, const __grid_constant__ CUtensorMap tm_w, co
   }
 }
 
+// ---- many tokens: 256 channels x up to 256 tokens on a pair of SMs --------------------------------------------------------
+// The same kernel on cta_group::2.  A tile of 128 x 256 on one SM asks for 48 KB of operands per 128 bytes of K, more than
+// L2 delivers at the tensor cores' pace; a pair shares the operands of a 256 x 256 tile (each CTA loads half of the
+// channels and half of the tokens) and asks for 32 KB per SM.  CTA 0 of the pair issues the MMAs; its barriers count both
+// CTAs' bytes, and a commit reports to both.  The token count BN of a tile is a run-time choice (a multiple of 32), made so
+// that the last round of tiles is nearly full.  Eight epilogue warps: two per quarter of the TMEM lanes, half of the tokens each.
+constexpr int PK_THREADS = 320, PK_STAGES = 6, PK_HALF = 128 * TK_KB, PK_STAGE = 2 * PK_HALF, PK_SMEM = PK_STAGES * PK_STAGE + 1024;
+
+__device__ __forceinline__ unsigned cluster_rank() {
+  unsigned r;
+  asm volatile("mov.u32 %0, %cluster_ctarank;\n" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ unsigned in_cta(unsigned addr, unsigned rank) {  // a shared-memory address in CTA `rank` of the cluster
+  unsigned r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync_all() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
+__device__ __forceinline__ void pair_load(void* dst, const CUtensorMap* map, int col, int row, unsigned bar_cluster) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], [%4];\n" ::
+          "r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(col), "r"(row), "r"(bar_cluster)
+      : "memory");
+}
+__device__ __forceinline__ void pair_mma_i8(unsigned d_tmem, uint64_t a_desc, uint64_t b_desc, unsigned idesc, unsigned accumulate) {
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      "setp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n"
+      "}\n" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void pair_commit(uint64_t* bar) {  // arrives at this offset in both CTAs
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n" ::"r"(smem_u32(bar)),
+               "h"((unsigned short)3)
+               : "memory");
+}
+__device__ __forceinline__ void remote_arrive(unsigned bar_cluster) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(bar_cluster) : "memory");
+}
+
+struct PkShared {
+  float x_scale[256];
+  uint64_t full[PK_STAGES], empty[PK_STAGES], acc_full[2], acc_empty[2];
+  unsigned tmem_base;
+  int fail, issued;
+};
+
+template <typename T>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PK_THREADS, 1)
+linear_pair_kernel(const LinArgs a, const int BN, const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x) {
+  extern __shared__ __align__(128) unsigned char smem_raw[];
+  __shared__ PkShared sh;
+  unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rank = (int)cluster_rank(), pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const int units = ceil_div(a.N, 2 * TK_M) * a.token_tiles;
+
+  if (tid == 0) {
+    sh.fail = 0;
+    sh.issued = 0;
+    for (int i = 0; i < PK_STAGES; ++i) {
+      mbar_init(&sh.full[i], 1);
+      mbar_init(&sh.empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sh.acc_full[i], 1);
+      mbar_init(&sh.acc_empty[i], 16);  // the epilogue warps of both CTAs
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+  }
+  __syncwarp();
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;\n" ::"r"(smem_u32(&sh.tmem_base)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();  // the barriers of both CTAs are there before either is signalled from the other side
+  tc_fence_after();
+  const unsigned tmem = sh.tmem_base;
+  pdl_wait();
+  pdl_trigger();
+
+  if (warp == 8) {
+    if (lane == 0) {
+      int it = 0;
+      for (int u = pair; u < units && !sh.fail; u += pairs) {
+        const int tt = u % a.token_tiles, ct = u / a.token_tiles;
+        for (int k = 0; k < a.chunks; ++k, ++it) {
+          const int st = it % PK_STAGES;
+          if (!mbar_wait(&sh.empty[st], ((it / PK_STAGES) & 1) ^ 1, &sh.fail)) {
+            if (!sh.fail && a.status) atomicExch(a.status, 7);
+            sh.fail = 1;
+            break;
+          }
+          unsigned char* dst = ring + (size_t)st * PK_STAGE;
+          const unsigned bar = in_cta(smem_u32(&sh.full[st]), 0);
+          if (rank == 0) mbar_expect_tx(&sh.full[st], 2 * (TK_M + BN / 2) * TK_KB);
+          pair_load(dst, &tm_w, k * TK_KB, (2 * ct + rank) * TK_M, bar);
+          pair_load(dst + PK_HALF, &tm_x, k * TK_KB, tt * BN + rank * (BN / 2), bar);
+          sh.issued = it + 1;
+        }
+      }
+    }
+  } else if (warp == 9) {
+    if (lane == 0 && rank == 0) {
+      const unsigned idesc = i8_instr_desc(2 * TK_M, BN);
+      bool ok = true;
+      int it = 0, n = 0;
+      for (int u = pair; ok && u < units; u += pairs, ++n) {
+        const int buf = n & 1;
+        if (!mbar_wait(&sh.acc_empty[buf], ((n >> 1) & 1) ^ 1, &sh.fail)) { ok = false; break; }
+        tc_fence_after();
+        const unsigned d_tmem = tmem + (unsigned)buf * 256;
+        for (int k = 0; k < a.chunks; ++k, ++it) {
+          const int st = it % PK_STAGES;
+          if (!mbar_wait(&sh.full[st], (it / PK_STAGES) & 1, &sh.fail)) { ok = false; break; }
+          tc_fence_after();
+          const unsigned w_base = smem_u32(ring + (size_t)st * PK_STAGE), x_base = w_base + PK_HALF;
+#pragma unroll
+          for (int j = 0; j < TK_KB / 32; ++j)
+            pair_mma_i8(d_tmem, smem_desc_sw128(w_base + j * 32), smem_desc_sw128(x_base + j * 32), idesc, (k || j) ? 1u : 0u);
+          pair_commit(&sh.empty[st]);
+        }
+        if (ok) pair_commit(&sh.acc_full[buf]);
+      }
+      if (!ok) {
+        if (!sh.fail && a.status) atomicExch(a.status, 7);
+        sh.fail = 1;
+      }
+    }
+  } else {
+    const int quarter = warp & 3, half = warp >> 2;
+    int n = 0;
+    for (int u = pair; u < units; u += pairs, ++n) {
+      const int buf = n & 1, t0 = (u % a.token_tiles) * BN, c = (2 * (u / a.token_tiles) + rank) * TK_M + quarter * 32 + lane;
+      const int tokens = min(BN, a.n - t0), j_lo = half * (BN / 2), j_hi = min(tokens, j_lo + BN / 2);
+      const float ws = c < a.N ? a.w_scale[c] : 0.f;
+      for (int j = tid; j < tokens; j += 256) sh.x_scale[j] = a.x_scale[t0 + j];  // the unit before ended with a barrier
+      const T* res = c < a.N ? static_cast<const T*>(a.res) : nullptr;
+      T r[16];
+      const auto ask = [&](int j0) {
+        if (res)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) r[j] = res[(size_t)(t0 + min(j0 + j, tokens - 1)) * a.res_sr + c];
+      };
+      if (j_lo < j_hi) ask(j_lo);
+      const bool got = mbar_wait(&sh.acc_full[buf], (n >> 1) & 1, &sh.fail);
+      unsigned any;  // the 256 threads leave together
+      asm volatile(
+          "{\n"
+          ".reg .pred p, q;\n"
+          "setp.ne.b32 p, %1, 0;\n"
+          "barrier.cta.red.or.pred q, 1, 256, p;\n"
+          "selp.u32 %0, 1, 0, q;\n"
+          "}\n"
+          : "=r"(any)
+          : "r"((unsigned)!got)
+          : "memory");
+      if (any) {
+        if (!sh.fail && a.status) atomicExch(a.status, 7);
+        sh.fail = 1;
+        break;
+      }
+      tc_fence_after();
+      const unsigned src = tmem + ((unsigned)(quarter * 32) << 16) + (unsigned)buf * 256;
+#pragma unroll 1
+      for (int j0 = j_lo; j0 < j_hi; j0 += 16) {
+        int v[16];
+        tmem_ld16i(src + j0, v);
+        tmem_ld_wait();
+        float y[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          y[j] = (float)v[j] * sh.x_scale[j0 + j] * ws;
+          if (res) y[j] += to_float(r[j]);
+        }
+        if (j0 + 16 < j_hi) ask(j0 + 16);
+        T* out = static_cast<T*>(a.out) + (size_t)(t0 + j0) * a.out_sr + c;
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          if (c < a.N && j0 + j < j_hi) out[(size_t)j * a.out_sr] = from_float<T>(y[j]);
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) remote_arrive(in_cta(smem_u32(&sh.acc_empty[buf]), 0));
+      asm volatile("bar.sync 1, 256;\n" ::: "memory");  // sh.x_scale is used again
+    }
+  }
+
+  // ---- teardown: neither CTA leaves while the other may still signal it ----
+  tc_fence_before();
+  __syncthreads();
+  if (sh.fail && tid == 256 && rank == 0) {  // wait (bounded) for the last requested tile of every stage
+    for (int st = 0; st < PK_STAGES; ++st) {
+      const int last = sh.issued - 1 - ((sh.issued - 1 - st) % PK_STAGES + PK_STAGES) % PK_STAGES;
+      if (sh.issued > st && last >= 0) mbar_wait(&sh.full[st], (last / PK_STAGES) & 1);
+    }
+  }
+  __syncwarp();
+  cluster_sync_all();
+  if (warp == 0) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;\n" ::"r"(tmem) : "memory");
+  }
+}
+
 // ---- which kernel, and how K is cut -------------------------------------------------------------------------------------
 constexpr int kStreamTokens = 16;
 
 struct TilePlan {
   int BN, token_tiles, tiles, S, chunks;
+  bool pair;
 };
 inline TilePlan tile_plan(int n, int N, int K) {
   TilePlan p;
-  p.BN = n <= 32 ? 32 : n <= 64 ? 64 : n <= 128 ? 128 : 256;
-  p.token_tiles = ceil_div(n, p.BN);
-  p.tiles = p.token_tiles * ceil_div(N, TK_M);
   p.chunks = ceil_div(K, TK_KB);
+  p.S = 1;
+  p.pair = n > 128;
+  if (p.pair) {
+    // The token count whose rounds of tiles over the SM pairs take least.  A round goes by the operands' way from L2 rather
+    // than by its MMAs: measured 10.3, 11.3, 13.0 us for 128, 192, 256 tokens at K = 4096, i.e. in proportion to BN + 360.
+    const int channel_tiles = ceil_div(N, 2 * TK_M);
+    long long best = -1;
+    for (int BN = 256; BN >= 128; BN -= 32) {
+      const long long cost = (long long)ceil_div(channel_tiles * ceil_div(n, BN), TK_CTAS / 2) * (BN + 360);
+      if (best < 0 || cost < best) {
+        best = cost;
+        p.BN = BN;
+      }
+    }
+    p.token_tiles = ceil_div(n, p.BN);
+    p.tiles = channel_tiles * p.token_tiles;
+    return p;
+  }
+  p.BN = n <= 32 ? 32 : n <= 64 ? 64 : 128;
+  p.token_tiles = 1;
+  p.tiles = ceil_div(N, TK_M);
   // slices: as many as keep all SMs busy, of four chunks at least
-  p.S = p.tiles >= TK_CTAS ? 1 : max(1, min(TK_CTAS / p.tiles, p.chunks / 4));
+  if (p.tiles < TK_CTAS) p.S = max(1, min(TK_CTAS / p.tiles, p.chunks / 4));
   return p;
 }
 inline size_t tile_workspace(const TilePlan& p) {
@@ -442,17 +676,29 @@ int launch_tile(const LinArgs& a, const TilePlan& pl, cudaStream_t st) {
 }
 
 template <typename T>
+int launch_pair(const LinArgs& a, const TilePlan& pl, cudaStream_t st) {
+  static std::atomic<unsigned long long> done{0};
+  auto kern = linear_pair_kernel<T>;
+  if (const int rc = allow_smem(kern, PK_SMEM, done)) return rc;
+  CUtensorMap tm_w, tm_x;
+  if (!make_bytes_tensor_map(&tm_w, a.w, a.N, a.K, a.w_sr, TK_M) || !make_bytes_tensor_map(&tm_x, a.x, a.n, a.K, a.x_sr, pl.BN / 2))
+    return OMNIKV_E_UNSUPPORTED;
+  OMNIKV_CUDA_OK(launch_pdl_smem_args(kern, dim3(2 * min(TK_CTAS / 2, pl.tiles)), dim3(PK_THREADS), PK_SMEM, st, a, pl.BN, tm_w, tm_x));
+  return OMNIKV_OK;
+}
+
+template <typename T>
 int launch_linear(const LinArgs& a, const TilePlan& pl, cudaStream_t st) {
   if (a.n <= kStreamTokens) {
     auto kern = a.n <= 8 ? linear_stream_kernel<T, 1> : linear_stream_kernel<T, 2>;
     OMNIKV_CUDA_OK(launch_pdl(kern, dim3(ceil_div(a.N, SK_ROWS)), dim3(SK_THREADS), 0, st, a));
     return OMNIKV_OK;
   }
+  if (pl.pair) return launch_pair<T>(a, pl, st);
   switch (pl.BN) {
     case 32: return launch_tile<T, 32>(a, pl, st);
     case 64: return launch_tile<T, 64>(a, pl, st);
-    case 128: return launch_tile<T, 128>(a, pl, st);
-    default: return launch_tile<T, 256>(a, pl, st);
+    default: return launch_tile<T, 128>(a, pl, st);
   }
 }
 
@@ -467,18 +713,19 @@ extern "C" int omnikv_quant_rows(int dtype, const void* x, int64_t x_stride_row,
     return OMNIKV_E_BADARG;
   if (!is_16bit(dtype) || K > 32768) return OMNIKV_E_UNSUPPORTED;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const auto go = [&](auto tag, auto threads) -> int {
-    using T = decltype(tag);
-    constexpr int TH = decltype(threads)::value;
-    OMNIKV_CUDA_OK(launch_pdl_args(quant_rows_kernel<T, TH>, dim3(n), dim3(TH), st, static_cast<const T*>(x), x_stride_row, K,
-                                   codes, code_stride_row, scale));
+  const auto go = [&](auto kern, int threads, auto tag) -> int {
+    OMNIKV_CUDA_OK(launch_pdl_args(kern, dim3(n), dim3(threads), st, static_cast<const decltype(tag)*>(x), x_stride_row, K, codes,
+                                   code_stride_row, scale));
     return OMNIKV_OK;
   };
-  using Small = std::integral_constant<int, 128>;
-  using Large = std::integral_constant<int, 512>;
-  const bool small = K <= 128 * 8 * QR_VEC;
-  if (dtype == OMNIKV_BF16) return small ? go(__nv_bfloat16(), Small()) : go(__nv_bfloat16(), Large());
-  return small ? go(__half(), Small()) : go(__half(), Large());
+  const auto pick = [&](auto tag) -> int {  // few pieces per thread: a row is one round of loads, and several rows share an SM
+    using T = decltype(tag);
+    if (K <= 256 * 8 * 2) return go(quant_rows_kernel<T, 256, 2>, 256, tag);
+    if (K <= 512 * 8 * 2) return go(quant_rows_kernel<T, 512, 2>, 512, tag);
+    if (K <= 512 * 8 * 4) return go(quant_rows_kernel<T, 512, 4>, 512, tag);
+    return go(quant_rows_kernel<T, 1024, 4>, 1024, tag);
+  };
+  return dtype == OMNIKV_BF16 ? pick(__nv_bfloat16()) : pick(__half());
 }
 
 extern "C" size_t omnikv_linear_w8a8_workspace_bytes(int n_tokens, int channels, int K) {

@@ -146,6 +146,26 @@ def test_store_of_extreme_values(fmt):
     assert math.isinf(cache[2][0, 0, 4].item()) and math.isnan(cache[2][0, 0, 3].item())
 
 
+@pytest.mark.parametrize("dtype,bits", [(torch.bfloat16, 8), (torch.float16, 11)])
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+def test_store_of_every_maximum(dtype, bits, fmt):
+    """All mantissas of a block's maximum against values in the middle between two codes, and their neighbours."""
+    lo = 1 << (bits - 1)
+    a = torch.arange(lo, 2 * lo, dtype=torch.float64, device="cuda")[:, None]
+    half = torch.arange(126, dtype=torch.float64, device="cuda")[None] + 0.5
+    if fmt == "e4m3":  # (16 + j) / 32 2^e: the middles of every binade, and those of the subnormals
+        j = torch.arange(1, 16, 2, dtype=torch.float64, device="cuda")
+        half = torch.cat([(16 + j) * 2.0 ** e for e in range(-11, 4)] + [j * 2.0 ** -10])[None, :126]
+    top = ko.TOP[fmt]
+    near = (half * a / top).to(dtype)
+    step = torch.tensor([1], dtype=torch.int16, device="cuda")
+    for other in (near, (near.view(torch.int16) + step).view(dtype), -(near.view(torch.int16) - step).view(dtype)):
+        x = torch.cat([a.to(dtype), other, (a / 2).to(dtype)], 1)[None, None]
+        cache = ops().kv8_alloc(1, 1, lo, block=1, dtype=CODES[fmt], device="cuda")
+        ops().kv8_store(x, x, *cache, block=1)
+        assert torch.equal(cache[0].float().double(), ko.quantise(x.double(), 1, fmt)[0])
+
+
 def test_load_by_index():
     B, KVH, rows, block = 2, 3, 150, 16
     cache, k, v = filled(B, KVH, rows, "int8", torch.float16, block, 11, tokens_first=True)

@@ -47,6 +47,25 @@ def test_quant_rows(dtype, n, K):
     assert ((scale.double() - scales[:, 0]).abs() <= 2.0 ** -24 * scales[:, 0]).all()
 
 
+@pytest.mark.parametrize("dtype,bits", [(torch.bfloat16, 8), (torch.float16, 11)])
+def test_quant_rows_of_every_maximum(dtype, bits):
+    """All mantissas of the row's maximum against values that hit the middles between two codes: odd multiples of a / 254
+    where those are numbers of the type, a / 2, and their neighbours."""
+    lo = 1 << (bits - 1)
+    a = torch.arange(lo, 2 * lo, dtype=torch.float64, device="cuda")[:, None]
+    mids = (torch.arange(0, 127, dtype=torch.float64, device="cuda")[None] + 0.5) * a / 127
+    near = mids.to(dtype)
+    step = torch.tensor([1], dtype=torch.int16, device="cuda")
+    below, above = ((near.view(torch.int16) + d * step).view(dtype) for d in (-1, 1))
+    x = torch.cat([a.to(dtype), near, -near, below, above, (a / 2).to(dtype), torch.zeros(len(a), 2, dtype=dtype, device="cuda")], 1)
+    assert x.shape[1] == 512
+    for scale in (1.0, 2.0 ** -20 if dtype == torch.float16 else 2.0 ** -100):
+        xs = x * scale
+        codes, _ = ops().quant_rows(xs)
+        want, _ = ko.quantise(xs.double()[:, None], 1, "int8")
+        assert torch.equal(codes.double(), want[:, 0])
+
+
 def test_quant_rows_of_extreme_values():
     x = torch.randn(7, 64, device="cuda").to(torch.bfloat16)
     x[0] = 0
