@@ -623,7 +623,7 @@ linear_pair_kernel(const LinArgs a, const int BN, const __grid_constant__ CUtens
 }
 
 // ---- which kernel, and how K is cut -------------------------------------------------------------------------------------
-constexpr int kStreamTokens = 16;
+constexpr int kStreamTokens = OMNIKV_LINEAR_STREAM_TOKENS;
 
 struct TilePlan {
   int BN, token_tiles, tiles, S, chunks;

@@ -547,7 +547,7 @@ def _own_workspace(dev: int, nbytes: int, tag: str) -> torch.Tensor:
     graphs, or a graph and eager calls, may run at the same time).  One that was outgrown is kept: a captured graph
     may still use it."""
     stream = torch._C._cuda_getCurrentRawStream(dev)
-    key = (dev, tag, stream, abi.lib().omnikv_capture_id(stream))
+    key = (dev, tag, stream, abi.lib().omnikv_capture_id(stream) if torch._C._cuda_isCurrentStreamCapturing() else 0)
     kept = _own_workspaces.get(key)
     if kept is None or kept[-1].numel() < nbytes:
         kept = _own_workspaces.setdefault(key, [])
@@ -655,7 +655,7 @@ def kv8_load(k8, v8, k_scale, v_scale, *, block: int, dtype: torch.dtype, start:
         n, idx_ptr, idx_stride = (c.rows - start if rows is None else rows), None, 0
         if start < 0 or n < 0 or start + n > c.rows:
             raise abi.OmniKVError(f"kv8_load: rows [{start}, {start + n}) are not inside the cache's {c.rows}")
-    k = torch.empty((B, KVH, n, 128), dtype=dtype, device=k8.device)
+    k = torch.empty_strided((B, KVH, n, 128), (KVH * n * 128, n * 128, 128, 1), dtype=dtype, device=k8.device)
     v = torch.empty_like(k)
     if n:
         _launch(dev, "omnikv_kv8_load", c, dt, start, n, idx_ptr, idx_stride, k.data_ptr(), v.data_ptr(), KVH * n * 128, n * 128, 128)
@@ -681,8 +681,8 @@ def kv8_decode_attn(q: torch.Tensor, k8, v8, k_scale, v_scale, len_a: torch.Tens
         raise abi.OmniKVError("kv8_decode_attn: q must be [B, H, 128] with contiguous head vectors, H a multiple of KVH")
     H = shape[1]
     if out is None:
-        out = torch.empty_like(q)
-    if out.shape != shape or out.stride() != strides or out.dtype is not q.dtype:
+        out = torch.empty_strided(shape, strides, dtype=q.dtype, device=q.device)
+    elif out.shape != shape or out.stride() != strides or out.dtype is not q.dtype:
         raise abi.OmniKVError("kv8_decode_attn: out must have the shape, strides and dtype of q")
     idx_ptr, idx_stride, idx_cap, cap = None, 0, 0, rows
     if idx is not None:
@@ -705,7 +705,7 @@ def kv8_decode_attn(q: torch.Tensor, k8, v8, k_scale, v_scale, len_a: torch.Tens
     # one CTA per SM; fewer when there are fewer (sequence, KV head) pairs and not a tile of 32 rows for each of twelve warps
     n_ctas = n_splits * B * KVH if n_splits else min(sm_count(dev), ((max_rows or cap) // 384 + 1) * B * KVH)
     if ws is None:
-        ws = _own_workspace(dev, abi.lib().omnikv_kv8_attn_workspace_bytes(B, H, KVH, n_ctas), "kv8_attn")
+        ws = _own_workspace(dev, abi.kv8_attn_workspace_bytes(B, H, KVH, n_ctas), "kv8_attn")
     p = abi.Kv8AttnParams(c, dt, H, scale if scale is not None else 0.08838834764831845, q.data_ptr(), strides[0], strides[1],
                           out.data_ptr(), idx_ptr, idx_stride, idx_cap, _need_i32("len_a", B, len_a),
                           _need_i32("tail_start", B, tail_start), _need_i32("tail_len", B, tail_len), score_ptr, score_stride,
@@ -726,8 +726,8 @@ def quant_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     if len(shape) != 2 or strides[1] != 1 or shape[1] == 0 or shape[1] % 16:
         raise abi.OmniKVError("quant_rows: x must be [n, K] with contiguous rows and K a multiple of 16")
     n, K = shape
-    codes = torch.empty((n, K), dtype=torch.int8, device=x.device)
-    scale = torch.empty((n,), dtype=torch.float32, device=x.device)
+    codes = torch.empty_strided((n, K), (K, 1), dtype=torch.int8, device=x.device)
+    scale = torch.empty_strided((n,), (1,), dtype=torch.float32, device=x.device)
     if n:
         _launch(dev, "omnikv_quant_rows", dt, x.data_ptr(), strides[0], n, K, codes.data_ptr(), K, scale.data_ptr())
     return codes, scale
@@ -750,21 +750,25 @@ def linear_w8a8(x8: torch.Tensor, x_scale: torch.Tensor, w8: torch.Tensor, w_sca
     if x_scale.dtype is not torch.float32 or w_scale.dtype is not torch.float32 or x_scale.shape != (n,) or w_scale.shape != (N,) \
             or not x_scale.is_contiguous() or not w_scale.is_contiguous():
         raise abi.OmniKVError("linear_w8a8: scales must be contiguous fp32, one per row of x8 and of w8")
-    if out is None:
-        dt = out_dtype or (residual.dtype if residual is not None else torch.bfloat16)
-        out = torch.empty((n, N), dtype=dt, device=x8.device)
-    dt = out.dtype
+    dt = out_dtype
+    if dt is None:
+        dt = out.dtype if out is not None else residual.dtype if residual is not None else torch.bfloat16
     for t in (out, residual):
-        if t is not None and (t.shape != (n, N) or t.dtype is not dt or dt not in _DT or t.stride(1) != 1
-                              or (out_dtype is not None and dt is not out_dtype)):
+        if t is not None and (t.shape != (n, N) or t.dtype is not dt or t.stride(1) != 1):
             raise abi.OmniKVError("linear_w8a8: out and residual must be [n, channels] of one floating dtype, rows contiguous")
+    out_code = _DT.get(dt)
+    if out_code is None:
+        raise abi.OmniKVError(f"linear_w8a8: the result is float32, bfloat16 or float16, not {dt}")
+    if out is None:
+        out = torch.empty_strided((n, N), (N, 1), dtype=dt, device=x8.device)
     if n == 0 or N == 0:
         return out
-    need, work = abi.lib().omnikv_linear_w8a8_workspace_bytes(n, N, K), None
-    if need:
-        work = _own_workspace(dev, need, "linear_w8a8").data_ptr()
+    work = need = 0
+    if n > abi.STREAM_TOKENS:
+        need = abi.lib().omnikv_linear_w8a8_workspace_bytes(n, N, K)
+        work = _own_workspace(dev, need, "linear_w8a8").data_ptr() if need else 0
     p = abi.LinearW8A8Params(n, N, K, x8.data_ptr(), x_st[0], x_scale.data_ptr(), w8.data_ptr(), w_st[0], w_scale.data_ptr(),
-                             _DT[dt], None if residual is None else residual.data_ptr(),
+                             out_code, None if residual is None else residual.data_ptr(),
                              0 if residual is None else residual.stride(0), out.data_ptr(), out.stride(0), work, need,
                              _status_ptr(dev))
     _launch(dev, "omnikv_linear_w8a8", p)

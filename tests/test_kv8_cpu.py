@@ -63,6 +63,16 @@ def test_attention_arguments_are_checked():
     assert lib.omnikv_kv8_decode_attn(None, None) == -1
 
 
+def test_workspace_rules_agree_with_the_library():
+    from omnikv_b200 import abi
+    lib = abi.lib()
+    for B, H, KVH, n in ((1, 32, 8, 148), (16, 8, 8, 1), (3, 16, 1, 700)):
+        assert abi.kv8_attn_workspace_bytes(B, H, KVH, n) == lib.omnikv_kv8_attn_workspace_bytes(B, H, KVH, n)
+    assert lib.omnikv_kv8_attn_workspace_bytes(1, 30, 8, 4) == 0
+    assert lib.omnikv_linear_w8a8_workspace_bytes(abi.STREAM_TOKENS, 512, 14336) == 0
+    assert lib.omnikv_linear_w8a8_workspace_bytes(abi.STREAM_TOKENS + 1, 512, 14336) > 0
+
+
 def test_linear_arguments_are_checked():
     from omnikv_b200 import abi
     lib = abi.lib()
