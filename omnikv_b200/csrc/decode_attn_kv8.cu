@@ -68,7 +68,7 @@ struct A8Args {
 struct RowList {
   int nA, nB, t0;
   __device__ __forceinline__ int n() const { return nA + nB; }
-  __device__ __forceinline__ int tiles() const { return max(1, ceil_div(nA + nB, TILE)); }  // an empty one is written too
+  __device__ __forceinline__ int tiles() const { return ceil_div(nA + nB, TILE); }
 };
 __device__ __forceinline__ RowList row_list(const A8Args& a, int b) {
   RowList r;
@@ -195,15 +195,24 @@ decode_attn_kv8_kernel(const A8Args a, const __grid_constant__ CUtensorMap tm_k,
   pdl_wait();
 
   // ---- this CTA's piece of the list: tiles [w0, w1) of W ----
-  int per_head = 0;  // tiles of all sequences, per KV head
+  int per_head = 0, filled = 0;  // tiles of all sequences, per KV head; sequences that have any
   for (int b0 = 0; b0 < a.B; b0 += 32) {
     const int mine = b0 + lane < a.B ? row_list(a, b0 + lane).tiles() : 0;
     per_head += __reduce_add_sync(0xffffffffu, mine);
+    filled += __popc(__ballot_sync(0xffffffffu, mine > 0));
+  }
+  if (filled < a.B) {  // a sequence without rows: zeros, written by one CTA
+    for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
+      if (row_list(a, b).n() > 0) continue;
+      for (int i = tid; i < a.H * (kHeadDim / 2); i += NT)
+        reinterpret_cast<unsigned*>(static_cast<T*>(a.out) + (size_t)b * a.q_sb + (size_t)(i >> 6) * a.q_sh)[i & 63] = 0u;
+    }
+    if (filled == 0) return;
   }
   // Pieces.  One per segment when four tiles per warp do a segment: a merge across CTAs costs more than it saves then.
   // Else as many as there are CTAs, a multiple of the segments where that leaves few CTAs idle: the pieces of equal
   // segments then end where the segments end.
-  const int segs = a.B * a.KVH, W = per_head * a.KVH;
+  const int segs = filled * a.KVH, W = per_head * a.KVH;
   int C = min((int)gridDim.x, W <= segs * NW * 4 ? segs : max(W / NW, segs));
   if (C > segs && C % segs <= C / 16) C -= C % segs;
   const int each = W / C, more = W - each * C, c = blockIdx.x;
@@ -406,18 +415,26 @@ decode_attn_kv8_kernel(const A8Args a, const __grid_constant__ CUtensorMap tm_k,
               float& z = x[i][cb][2 * u + e];
               z = ok ? z * ks * qs[cb][e] : -INFINITY;
             }
-          if (a.score_out) {
-            float best = -INFINITY;
-#pragma unroll
-            for (int cb = 0; cb < COLS; ++cb)
-#pragma unroll
-              for (int e = 0; e < 2; ++e)
-                if (cb * 8 + 2 * t + e < G) best = max_nan(best, x[i][cb][2 * u + e]);
-            best = max_nan(best, __shfl_xor_sync(0xffffffffu, best, 1));
-            best = max_nan(best, __shfl_xor_sync(0xffffffffu, best, 2));
-            if (t == 0 && row0 + r < score_lim) score_row[row0 + r] = best * (1.f / kLog2e);
-          }
         }
+      if (a.score_out) {
+        // largest over the heads: a thread holds two heads of four rows (8 j + g); the four threads of a row group trade
+        // halves twice, after which thread t has row 8 t + g
+        float best[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          best[j] = -INFINITY;
+#pragma unroll
+          for (int cb = 0; cb < COLS; ++cb)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              if (cb * 8 + 2 * t + e < G) best[j] = max_nan(best[j], x[j >> 1][cb][2 * (j & 1) + e]);
+        }
+        const float s0 = (t & 2) ? best[0] : best[2], s1 = (t & 2) ? best[1] : best[3];
+        const float k0 = max_nan((t & 2) ? best[2] : best[0], __shfl_xor_sync(0xffffffffu, s0, 2));
+        const float k1 = max_nan((t & 2) ? best[3] : best[1], __shfl_xor_sync(0xffffffffu, s1, 2));
+        const float mine = max_nan((t & 1) ? k1 : k0, __shfl_xor_sync(0xffffffffu, (t & 1) ? k0 : k1, 1));
+        if (row0 + 8 * t + g < score_lim) score_row[row0 + 8 * t + g] = mine * (1.f / kLog2e);
+      }
       // ---- weights ----
       unsigned pb[2][COLS][2];
 #pragma unroll
@@ -512,8 +529,9 @@ decode_attn_kv8_kernel(const A8Args a, const __grid_constant__ CUtensorMap tm_k,
 
     // ---- the CTA's partial of the segment ----
     // Behind the CTA's last segment the rings are free and every warp leaves its sums in its own; before that the warps add
-    // theirs up in turn in one buffer (next tiles are on their way into the rings meanwhile).  Either way in warp order.
+    // theirs up in turns in the few buffers that o_s holds (next tiles are on their way into the rings meanwhile).
     const bool last_seg = hi == w1;
+    const int bufs = min(NW, MAX_G / G);
     if (last_seg) pdl_trigger();
 #pragma unroll
     for (int cb = 0; cb < COLS; ++cb)
@@ -561,8 +579,9 @@ decode_attn_kv8_kernel(const A8Args a, const __grid_constant__ CUtensorMap tm_k,
     } else {
       __syncthreads();
 #pragma unroll 1
-      for (int turn = 0; turn < NW; ++turn) {
-        if (warp == turn) leave(o_s, turn > 0, true);
+      for (int turn = 0; turn * bufs < NW; ++turn) {
+        const int buf = warp - turn * bufs;
+        if (buf >= 0 && buf < bufs) leave(o_s + buf * G * OS_PITCH, turn > 0, true);
         __syncthreads();
       }
     }
@@ -599,7 +618,10 @@ decode_attn_kv8_kernel(const A8Args a, const __grid_constant__ CUtensorMap tm_k,
           acc.x = fmaf(v.x, fw, acc.x), acc.y = fmaf(v.y, fw, acc.y), acc.z = fmaf(v.z, fw, acc.z), acc.w = fmaf(v.w, fw, acc.w);
         }
       } else {
-        acc = *reinterpret_cast<const float4*>(o_s + h * OS_PITCH + lane * 4);
+        for (int buf = 0; buf < bufs; ++buf) {
+          const float4 v = *reinterpret_cast<const float4*>(o_s + (buf * G + h) * OS_PITCH + lane * 4);
+          acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
+        }
       }
       if (parts == 1) {
         write_out(h, acc, Ms, ms, __shfl_sync(0xffffffffu, L, 0));

@@ -161,37 +161,57 @@ __global__ void __launch_bounds__(AP_THREADS) kv8_append_kernel(const Kv8View c,
 }
 
 // ---- load -------------------------------------------------------------------------------------------------------
-// Sixteen codes per thread, eight threads per row.
+// Eight threads per row of 128 codes, sixteen codes each; a CTA takes K and V of 16 * STEPS rows of a head.  The heads of
+// the same rows are neighbours in the grid: where a token's heads lie together (the layout of layers that read selected
+// tokens), the scattered reads of a token then come close in time.
 constexpr int LD_THREADS = 256;
+constexpr int kLoadIdxSteps = 4;  // rows per thread of scattered reads (2048 of 20000 rows, 16 sequences: 39.4, 35.5, 34.7 us for 1, 2, 4)
 
-template <typename T, int FMT>
-__global__ void __launch_bounds__(LD_THREADS) kv8_load_kernel(const Kv8View c, int start, int n, const int* idx,
+template <typename T, int FMT, int STEPS>
+__global__ void __launch_bounds__(LD_THREADS) kv8_load_kernel(const Kv8View c, int KVH, int start, int n, const int* idx,
                                                               int64_t idx_stride, T* k_out, T* v_out, int64_t o_sb,
                                                               int64_t o_sh, int64_t o_sr) {
   pdl_wait();
   pdl_trigger();
-  const int i = blockIdx.x * (LD_THREADS / 8) + (threadIdx.x >> 3), piece = threadIdx.x & 7;
-  if (i >= n) return;
-  const int h = blockIdx.y >> 1, b = blockIdx.z;
-  const bool is_v = blockIdx.y & 1;
-  const int64_t row = idx ? (int64_t)idx[(size_t)b * idx_stride + i] : (int64_t)start + i;
-  uint4 q = make_uint4(0, 0, 0, 0);
-  float s = 0.f;
-  if (row >= 0 && row < c.rows) {
-    const int shift = 31 - __clz(c.block);
-    q = *reinterpret_cast<const uint4*>((is_v ? c.v : c.k) + (size_t)b * c.sb + (size_t)h * c.sh + row * c.sr + piece * 16);
-    s = ((is_v ? c.vs : c.ks) + (size_t)b * c.ssb + (size_t)h * c.ssh)[row >> shift];
-  }
-  const unsigned* w = reinterpret_cast<const unsigned*>(&q);
-  unsigned o[8];
+  const int h = blockIdx.x % KVH, i0 = (blockIdx.x / KVH) * (16 * STEPS) + (threadIdx.x >> 4), b = blockIdx.y;
+  const bool is_v = (threadIdx.x >> 3) & 1;
+  const int piece = threadIdx.x & 7, shift = 31 - __clz(c.block);
+  const unsigned char* code = (is_v ? c.v : c.k) + (size_t)b * c.sb + (size_t)h * c.sh + piece * 16;
+  const float* scale = (is_v ? c.vs : c.ks) + (size_t)b * c.ssb + (size_t)h * c.ssh;
+  T* out = (is_v ? v_out : k_out) + (size_t)b * o_sb + (size_t)h * o_sh + piece * 16;
+  int64_t row[STEPS];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const unsigned two = w[j >> 1] >> (16 * (j & 1));
-    o[j] = pack2<T>(code_value<FMT>(two & 0xffu) * s, code_value<FMT>((two >> 8) & 0xffu) * s);
+  for (int u = 0; u < STEPS; ++u) {
+    const int i = i0 + 16 * u;
+    row[u] = i >= n ? -1 : idx ? (int64_t)idx[(size_t)b * idx_stride + i] : (int64_t)start + i;
+    if (row[u] >= c.rows) row[u] = -1;
   }
-  uint4* dst = reinterpret_cast<uint4*>((is_v ? v_out : k_out) + (size_t)b * o_sb + (size_t)h * o_sh + (size_t)i * o_sr + piece * 16);
-  dst[0] = make_uint4(o[0], o[1], o[2], o[3]);
-  dst[1] = make_uint4(o[4], o[5], o[6], o[7]);
+  uint4 q[STEPS];
+  float s[STEPS];
+#pragma unroll
+  for (int u = 0; u < STEPS; ++u) {
+    q[u] = make_uint4(0, 0, 0, 0);
+    s[u] = 0.f;
+    if (row[u] >= 0) {
+      q[u] = *reinterpret_cast<const uint4*>(code + row[u] * c.sr);
+      s[u] = scale[row[u] >> shift];
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < STEPS; ++u) {
+    const int i = i0 + 16 * u;
+    if (i >= n) continue;
+    const unsigned* w = reinterpret_cast<const unsigned*>(&q[u]);
+    unsigned o[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const unsigned two = w[j >> 1] >> (16 * (j & 1));
+      o[j] = pack2<T>(code_value<FMT>(two & 0xffu) * s[u], code_value<FMT>((two >> 8) & 0xffu) * s[u]);
+    }
+    uint4* dst = reinterpret_cast<uint4*>(out + (int64_t)i * o_sr);
+    dst[0] = make_uint4(o[0], o[1], o[2], o[3]);
+    dst[1] = make_uint4(o[4], o[5], o[6], o[7]);
+  }
 }
 
 template <typename T, int FMT>
@@ -264,13 +284,18 @@ extern "C" int omnikv_kv8_load(const omnikv_kv8_cache* c, int dtype, int start, 
   if (out_stride_b % 8 || out_stride_h % 8 || out_stride_row % 8 || out_stride_row < kHeadDim) return OMNIKV_E_BADARG;
   if (!is_16bit(dtype)) return OMNIKV_E_UNSUPPORTED;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const dim3 grid(ceil_div(n, LD_THREADS / 8), 2 * c->KVH, c->B);
-#define OMNIKV_CALL(T, F)                                                                                             \
-  launch_pdl_args(kv8_load_kernel<T, F>, grid, dim3(LD_THREADS), st, view_of(c), start, n, idx, idx_stride,          \
-                  static_cast<T*>(k_out), static_cast<T*>(v_out), out_stride_b, out_stride_h, out_stride_row)
-  OMNIKV_CUDA_OK(OMNIKV_KV8_DISPATCH(dtype, c->format, OMNIKV_CALL));
+  const int steps = idx ? kLoadIdxSteps : 1;
+  const int64_t blocks = ((int64_t)n + 16 * steps - 1) / (16 * steps) * c->KVH;
+  if (blocks > 0x7fffffff) return OMNIKV_E_UNSUPPORTED;
+  const auto go = [&](auto kern, auto tag) -> int {
+    using T = decltype(tag);
+    OMNIKV_CUDA_OK(launch_pdl_args(kern, dim3((unsigned)blocks, c->B), dim3(LD_THREADS), st, view_of(c), c->KVH, start, n, idx, idx_stride,
+                                   static_cast<T*>(k_out), static_cast<T*>(v_out), out_stride_b, out_stride_h, out_stride_row));
+    return OMNIKV_OK;
+  };
+#define OMNIKV_CALL(T, F) (idx ? go(kv8_load_kernel<T, F, kLoadIdxSteps>, T()) : go(kv8_load_kernel<T, F, 1>, T()))
+  return OMNIKV_KV8_DISPATCH(dtype, c->format, OMNIKV_CALL);
 #undef OMNIKV_CALL
-  return OMNIKV_OK;
 }
 
 extern "C" unsigned long long omnikv_capture_id(void* stream) {

@@ -70,18 +70,18 @@ struct LinArgs {
   void* out;
   int64_t out_sr;
   int n, N, K;
-  int* counters;  // tile kernel with slices of K: [tiles] arrivals, zero between launches
-  int* part;      // [tiles][slices][tokens of a tile][128]
+  int* counters;  // tile kernel: [CTAs] arrivals at the tile that a CTA is the first to work on, zero between launches
+  int* part;      // tile kernel: [CTAs + tiles][tokens of a tile][128]
   int* status;
-  int S, token_tiles, chunks;
+  int token_tiles, chunks;
 };
 
 // ---- up to 16 tokens: a stream of the weights -------------------------------------------------------------------------
 // A CTA owns 16 channels, its eight warps take 64-byte chunks of K in turn.  The fragments of m16n8k32 come straight from
 // global memory with 16-byte loads: inside a chunk of 64 the order of k is free as long as both operands agree, so thread
 // (g, t) takes bytes 16 t .. 16 t + 15 of rows g and g + 8 (weights) and of token g, and their words 0..3 are two MMAs.
-// Four chunks are asked for while the four before them are multiplied.  The eight integer sums meet in shared memory.
-constexpr int SK_THREADS = 256, SK_WARPS = SK_THREADS / 32, SK_ROWS = 16, SK_DEPTH = 4;
+// DEPTH chunks are asked for while the DEPTH before them are multiplied.  The eight integer sums meet in shared memory.
+constexpr int SK_THREADS = 256, SK_WARPS = SK_THREADS / 32, SK_ROWS = 16;
 
 __device__ __forceinline__ void mma_i8(int (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
   asm volatile(
@@ -97,7 +97,8 @@ __device__ __forceinline__ uint4 ld_stream(const int8_t* p) {  // weights: read 
 
 // NB: blocks of eight tokens
 template <typename T, int NB>
-__global__ void __launch_bounds__(SK_THREADS, 2) linear_stream_kernel(const LinArgs a) {
+__global__ void __launch_bounds__(SK_THREADS, NB == 1 ? 3 : 2) linear_stream_kernel(const LinArgs a) {
+  constexpr int SK_DEPTH = NB == 1 ? 2 : 3;
   __shared__ int sums[SK_WARPS][NB * 8][SK_ROWS + 1];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int c0 = blockIdx.x * SK_ROWS;
@@ -163,18 +164,20 @@ __global__ void __launch_bounds__(SK_THREADS, 2) linear_stream_kernel(const LinA
   static_cast<T*>(a.out)[(size_t)tok * a.out_sr + c] = from_float<T>(y);
 }
 
-// ---- more tokens: tiles of 128 channels x BN tokens on tcgen05 -----------------------------------------------------------
+// ---- up to 128 tokens: tiles of 128 channels x BN tokens on tcgen05 ---------------------------------------------------------
+// Still a stream of the weights.  The chunks (128 bytes of K) of all tiles form one list that is cut into equal pieces, one
+// per CTA: a CTA may end one tile and begin the next.  The integer sums of a tile that several CTAs share go to the
+// workspace, and the one that arrives last adds them up.
 // Warp 4 fetches 128-byte wide boxes of weights and tokens (TMA, 128-byte swizzle), warp 5 issues the MMAs (K = 32 bytes
 // each), int32 accumulators in tensor memory, two of them so that the epilogue of a tile runs under the next tile's MMAs.
 // Warps 0-3 read a tile back: thread = channel (TMEM lane), columns = tokens, so a warp's store is 32 neighbouring channels
-// of a token whatever the alignment of the output.  When there are too few tiles for the GPU, K is cut into slices: their
-// integer sums go to the workspace and the CTA that arrives last at a tile adds them up.
+// of a token whatever the alignment of the output.
 constexpr int TK_M = 128, TK_KB = 128, TK_THREADS = 192, TK_CTAS = 148;
 
 template <int BN>
 struct TkShape {
   static constexpr int STAGE = (TK_M + BN) * TK_KB;
-  static constexpr int STAGES = BN >= 256 ? 4 : (BN >= 128 ? 6 : 8);
+  static constexpr int STAGES = BN >= 128 ? 6 : 8;
   static constexpr int SMEM = STAGES * STAGE + 1024;
 };
 
@@ -216,8 +219,51 @@ __device__ __forceinline__ bool epilogue_any(bool pred) {  // OR over the 128 ep
   return r != 0;
 }
 
+// The results of 16 tokens of one channel: 32 neighbouring channels of a token per warp and store.  What the residual needs
+// from memory is asked for one step ahead (`ask`), the full and the ragged step have code of their own.
+template <typename T>
+struct Channel {
+  const T* res;  // this channel's first token, or nullptr
+  T* out;        // nullptr: a channel past the end
+  int64_t res_sr, out_sr;
+  int tokens;
+  float w_scale;
+  T r[16];
+  __device__ __forceinline__ void ask(int j0) {
+    if (!res || j0 >= tokens) return;
+    const T* p = res + (int64_t)j0 * res_sr;
+    if (j0 + 16 <= tokens) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) r[j] = p[j * res_sr];
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) r[j] = p[min(j, tokens - 1 - j0) * res_sr];
+    }
+  }
+  __device__ __forceinline__ void put(int j0, const int (&v)[16], const float* x_scale) {
+    if (!out) return;
+    float y[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) y[j] = (float)v[j] * x_scale[j0 + j] * w_scale;
+    if (res) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) y[j] += to_float(r[j]);
+      ask(j0 + 16);
+    }
+    T* p = out + (int64_t)j0 * out_sr;
+    if (j0 + 16 <= tokens) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) p[j * out_sr] = from_float<T>(y[j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        if (j0 + j < tokens) p[j * out_sr] = from_float<T>(y[j]);
+    }
+  }
+};
+
 struct TkShared {
-  float x_scale[256];
+  float x_scale[128];
   uint64_t full[8], empty[8], acc_full[2], acc_empty[2];
   unsigned tmem_base;
   int fail, issued, last;
@@ -232,7 +278,6 @@ linear_tile_kernel(const LinArgs a, const __grid_constant__ CUtensorMap tm_w, co
   constexpr unsigned TMEM_COLS = 2 * BN;
   unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int S = a.S, units = ceil_div(a.N, TK_M) * a.token_tiles * S;
 
   if (tid == 0) {
     sh.fail = 0;
@@ -258,27 +303,29 @@ linear_tile_kernel(const LinArgs a, const __grid_constant__ CUtensorMap tm_w, co
   const unsigned tmem = sh.tmem_base;
   pdl_wait();
   pdl_trigger();
-  // unit u: slice u % S of tile u / S; the tiles of a block of channels follow one another
-  const auto slice_lo = [&](int s) { return (int)((long long)s * a.chunks / S); };
+  // this CTA's piece [lo, hi) of the list of chunks (the host keeps their count below 2^31)
+  const int chunks = a.chunks, total = ceil_div(a.N, TK_M) * chunks, C = gridDim.x, cta = blockIdx.x;
+  const auto piece_lo = [&](int i) { return (int)((long long)i * total / C); };
+  const int lo = piece_lo(cta), hi = piece_lo(cta + 1);
 
   if (warp == 4) {
     if (lane == 0) {
-      int it = 0;
-      for (int u = blockIdx.x; u < units && !sh.fail; u += gridDim.x) {
-        const int s = u % S, tile = u / S, tt = tile % a.token_tiles, ct = tile / a.token_tiles;
-        const int k1 = slice_lo(s + 1);
-        for (int k = slice_lo(s); k < k1; ++k, ++it) {
-          const int st = it % STAGES;
-          if (!mbar_wait(&sh.empty[st], ((it / STAGES) & 1) ^ 1, &sh.fail)) {
-            if (!sh.fail && a.status) atomicExch(a.status, 7);
-            sh.fail = 1;
-            break;
-          }
-          unsigned char* dst = ring + (size_t)st * STAGE;
-          mbar_expect_tx(&sh.full[st], STAGE);
-          tma_load_2d(dst, &tm_w, k * TK_KB, ct * TK_M, &sh.full[st]);
-          tma_load_2d(dst + TK_M * TK_KB, &tm_x, k * TK_KB, tt * BN, &sh.full[st]);
-          sh.issued = it + 1;
+      int ct = lo / chunks, k = lo % chunks;
+      for (int it = 0; it < hi - lo; ++it) {
+        const int st = it % STAGES;
+        if (!mbar_wait(&sh.empty[st], ((it / STAGES) & 1) ^ 1, &sh.fail)) {
+          if (!sh.fail && a.status) atomicExch(a.status, 7);
+          sh.fail = 1;
+          break;
+        }
+        unsigned char* dst = ring + (size_t)st * STAGE;
+        mbar_expect_tx(&sh.full[st], STAGE);
+        tma_load_2d(dst, &tm_w, k * TK_KB, ct * TK_M, &sh.full[st]);
+        tma_load_2d(dst + TK_M * TK_KB, &tm_x, k * TK_KB, 0, &sh.full[st]);
+        sh.issued = it + 1;
+        if (++k == chunks) {
+          k = 0;
+          ++ct;
         }
       }
     }
@@ -287,19 +334,19 @@ linear_tile_kernel(const LinArgs a, const __grid_constant__ CUtensorMap tm_w, co
       constexpr unsigned idesc = i8_instr_desc(TK_M, BN);
       bool ok = true;
       int it = 0, n = 0;
-      for (int u = blockIdx.x; ok && u < units; u += gridDim.x, ++n) {
-        const int buf = n & 1, s = u % S, k0 = slice_lo(s), k1 = slice_lo(s + 1);
+      for (int at = lo; ok && at < hi; ++n) {
+        const int buf = n & 1, end = min(hi, (at / chunks + 1) * chunks);
         if (!mbar_wait(&sh.acc_empty[buf], ((n >> 1) & 1) ^ 1, &sh.fail)) { ok = false; break; }
         tc_fence_after();
         const unsigned d_tmem = tmem + (unsigned)buf * BN;
-        for (int k = k0; k < k1; ++k, ++it) {
+        for (int first = at; at < end; ++at, ++it) {
           const int st = it % STAGES;
           if (!mbar_wait(&sh.full[st], (it / STAGES) & 1, &sh.fail)) { ok = false; break; }
           tc_fence_after();
           const unsigned w_base = smem_u32(ring + (size_t)st * STAGE), x_base = w_base + TK_M * TK_KB;
 #pragma unroll
           for (int j = 0; j < TK_KB / 32; ++j)
-            tc_mma_i8(d_tmem, smem_desc_sw128(w_base + j * 32), smem_desc_sw128(x_base + j * 32), idesc, (k > k0 || j) ? 1u : 0u);
+            tc_mma_i8(d_tmem, smem_desc_sw128(w_base + j * 32), smem_desc_sw128(x_base + j * 32), idesc, (at > first || j) ? 1u : 0u);
           tc_commit(&sh.empty[st]);
         }
         if (ok) tc_commit(&sh.acc_full[buf]);
@@ -310,34 +357,17 @@ linear_tile_kernel(const LinArgs a, const __grid_constant__ CUtensorMap tm_w, co
       }
     }
   } else {
+    const int tokens = a.n;
+    for (int j = tid; j < tokens; j += 128) sh.x_scale[j] = a.x_scale[j];
     int n = 0;
-    for (int u = blockIdx.x; u < units; u += gridDim.x, ++n) {
-      const int buf = n & 1, s = u % S, tile = u / S, t0 = (tile % a.token_tiles) * BN, c = (tile / a.token_tiles) * TK_M + tid;
-      const int tokens = min(BN, a.n - t0);
-      const float ws = c < a.N ? a.w_scale[c] : 0.f;
-      for (int j = tid; j < tokens; j += 128) sh.x_scale[j] = a.x_scale[t0 + j];  // the unit before ended with a barrier
-      const T* res = c < a.N ? static_cast<const T*>(a.res) : nullptr;
-      // 16 tokens of this thread's channel; what they need from memory is asked for one step ahead
-      T r[16];
-      const auto ask = [&](int j0) {
-        if (res)
-#pragma unroll
-          for (int j = 0; j < 16; ++j) r[j] = res[(size_t)(t0 + min(j0 + j, tokens - 1)) * a.res_sr + c];
-      };
-      const auto finish = [&](int j0, const int (&v)[16]) {
-        float y[16];
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          y[j] = (float)v[j] * sh.x_scale[j0 + j] * ws;
-          if (res) y[j] += to_float(r[j]);
-        }
-        if (j0 + 16 < tokens) ask(j0 + 16);
-        T* out = static_cast<T*>(a.out) + (size_t)(t0 + j0) * a.out_sr + c;
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-          if (c < a.N && j0 + j < tokens) out[(size_t)j * a.out_sr] = from_float<T>(y[j]);
-      };
-      if (S == 1) ask(0);
+    for (int at = lo; at < hi; ++n) {
+      const int buf = n & 1, tile = at / chunks, end = min(hi, (tile + 1) * chunks), c = tile * TK_M + tid;
+      const bool whole = end - at == chunks;
+      at = end;
+      const bool in = c < a.N;
+      Channel<T> ch{in && a.res ? static_cast<const T*>(a.res) + c : nullptr, in ? static_cast<T*>(a.out) + c : nullptr,
+                    a.res_sr, a.out_sr, tokens, in ? a.w_scale[c] : 0.f};
+      if (whole) ch.ask(0);
       const bool got = mbar_wait(&sh.acc_full[buf], (n >> 1) & 1, &sh.fail);
       if (epilogue_any(!got)) {  // the 128 threads leave together
         if (!sh.fail && a.status) atomicExch(a.status, 7);
@@ -346,14 +376,14 @@ linear_tile_kernel(const LinArgs a, const __grid_constant__ CUtensorMap tm_w, co
       }
       tc_fence_after();
       const unsigned src = tmem + ((unsigned)(warp * 32) << 16) + (unsigned)buf * BN;
-      int* part = a.part + ((size_t)tile * S + s) * BN * TK_M + tid;
+      int* part = a.part + (size_t)(cta + tile) * BN * TK_M + tid;  // (CTA, tile) pairs walk a staircase: their sum is unique
 #pragma unroll 1
       for (int j0 = 0; j0 < tokens; j0 += 16) {
         int v[16];
         tmem_ld16i(src + j0, v);
         tmem_ld_wait();
-        if (S == 1) {
-          finish(j0, v);
+        if (whole) {
+          ch.put(j0, v, sh.x_scale);
         } else {
 #pragma unroll
           for (int j = 0; j < 16; ++j) __stcg(part + (j0 + j) * TK_M, v[j]);
@@ -361,32 +391,52 @@ linear_tile_kernel(const LinArgs a, const __grid_constant__ CUtensorMap tm_w, co
       }
       tc_fence_before();
       mbar_arrive(&sh.acc_empty[buf]);
-      if (S > 1) {
-        __threadfence();
+      if (!whole) {
+        // the CTAs that share the tile: from the one that has its first chunk to the one that has its last
+        const auto owner = [&](int chunk) {
+          int i = min(C - 1, (int)(((float)chunk + 0.5f) * (float)C / (float)total));
+          while (piece_lo(i) > chunk) --i;
+          while (piece_lo(i + 1) <= chunk) ++i;
+          return i;
+        };
+        const int first = owner(tile * chunks), parts = owner((tile + 1) * chunks - 1) - first + 1;
         epilogue_bar();
         if (tid == 0) {
-          sh.last = atomicAdd(a.counters + tile, 1) == S - 1;
-          if (sh.last) a.counters[tile] = 0;  // nobody else touches it any more in this call
+          __threadfence();  // the stores, ordered before the barrier, are visible before the arrival is
+          sh.last = atomicAdd(a.counters + first, 1) == parts - 1;
+          if (sh.last) a.counters[first] = 0;  // nobody else touches it any more in this call
+          __threadfence();
         }
         epilogue_bar();
         if (sh.last) {
-          __threadfence();
-          const int* all = a.part + (size_t)tile * S * BN * TK_M + tid;
-          ask(0);
+          const int* all = a.part + (size_t)(first + tile) * BN * TK_M + tid;
+          const auto fetch = [&](int q, int j0, int (&v)[16]) {  // 16 tokens of partial q (the columns behind the tokens are there too)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] = q < parts && j0 < tokens ? __ldcg(all + ((size_t)q * BN + j0 + j) * TK_M) : 0;
+          };
+          int v0[16], v1[16], n0[16], n1[16];  // the first two partials are asked for one step ahead
+          ch.ask(0);
+          fetch(0, 0, v0);
+          fetch(1, 0, v1);
 #pragma unroll 1
           for (int j0 = 0; j0 < tokens; j0 += 16) {
-            int v[16];
+            fetch(0, j0 + 16, n0);
+            fetch(1, j0 + 16, n1);
 #pragma unroll
-            for (int j = 0; j < 16; ++j) v[j] = 0;
-#pragma unroll 4
-            for (int q = 0; q < S; ++q)
+            for (int j = 0; j < 16; ++j) v0[j] += v1[j];
+#pragma unroll 1
+            for (int q = 2; q < parts; ++q) {
+              fetch(q, j0, v1);
 #pragma unroll
-              for (int j = 0; j < 16; ++j) v[j] += __ldcg(all + ((size_t)q * BN + j0 + j) * TK_M);
-            finish(j0, v);
+              for (int j = 0; j < 16; ++j) v0[j] += v1[j];
+            }
+            ch.put(j0, v0, sh.x_scale);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v0[j] = n0[j], v1[j] = n1[j];
           }
         }
+        epilogue_bar();  // sh.last is used again
       }
-      epilogue_bar();  // sh.x_scale and sh.last are used again
     }
   }
 
@@ -552,16 +602,11 @@ linear_pair_kernel(const LinArgs a, const int BN, const __grid_constant__ CUtens
     for (int u = pair; u < units; u += pairs, ++n) {
       const int buf = n & 1, t0 = (u % a.token_tiles) * BN, c = (2 * (u / a.token_tiles) + rank) * TK_M + quarter * 32 + lane;
       const int tokens = min(BN, a.n - t0), j_lo = half * (BN / 2), j_hi = min(tokens, j_lo + BN / 2);
-      const float ws = c < a.N ? a.w_scale[c] : 0.f;
       for (int j = tid; j < tokens; j += 256) sh.x_scale[j] = a.x_scale[t0 + j];  // the unit before ended with a barrier
-      const T* res = c < a.N ? static_cast<const T*>(a.res) : nullptr;
-      T r[16];
-      const auto ask = [&](int j0) {
-        if (res)
-#pragma unroll
-          for (int j = 0; j < 16; ++j) r[j] = res[(size_t)(t0 + min(j0 + j, tokens - 1)) * a.res_sr + c];
-      };
-      if (j_lo < j_hi) ask(j_lo);
+      const bool in = c < a.N;
+      Channel<T> ch{in && a.res ? static_cast<const T*>(a.res) + (int64_t)t0 * a.res_sr + c : nullptr,
+                    in ? static_cast<T*>(a.out) + (int64_t)t0 * a.out_sr + c : nullptr, a.res_sr, a.out_sr, j_hi, in ? a.w_scale[c] : 0.f};
+      ch.ask(j_lo);
       const bool got = mbar_wait(&sh.acc_full[buf], (n >> 1) & 1, &sh.fail);
       unsigned any;  // the 256 threads leave together
       asm volatile(
@@ -586,17 +631,7 @@ linear_pair_kernel(const LinArgs a, const int BN, const __grid_constant__ CUtens
         int v[16];
         tmem_ld16i(src + j0, v);
         tmem_ld_wait();
-        float y[16];
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          y[j] = (float)v[j] * sh.x_scale[j0 + j] * ws;
-          if (res) y[j] += to_float(r[j]);
-        }
-        if (j0 + 16 < j_hi) ask(j0 + 16);
-        T* out = static_cast<T*>(a.out) + (size_t)(t0 + j0) * a.out_sr + c;
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-          if (c < a.N && j0 + j < j_hi) out[(size_t)j * a.out_sr] = from_float<T>(y[j]);
+        ch.put(j0, v, sh.x_scale);
       }
       tc_fence_before();
       __syncwarp();
@@ -626,13 +661,12 @@ linear_pair_kernel(const LinArgs a, const int BN, const __grid_constant__ CUtens
 constexpr int kStreamTokens = OMNIKV_LINEAR_STREAM_TOKENS;
 
 struct TilePlan {
-  int BN, token_tiles, tiles, S, chunks;
+  int BN, token_tiles, tiles, chunks, ctas;
   bool pair;
 };
 inline TilePlan tile_plan(int n, int N, int K) {
   TilePlan p;
   p.chunks = ceil_div(K, TK_KB);
-  p.S = 1;
   p.pair = n > 128;
   if (p.pair) {
     // The token count whose rounds of tiles over the SM pairs take least.  A round goes by the operands' way from L2 rather
@@ -648,17 +682,20 @@ inline TilePlan tile_plan(int n, int N, int K) {
     }
     p.token_tiles = ceil_div(n, p.BN);
     p.tiles = channel_tiles * p.token_tiles;
+    p.ctas = 2 * min(TK_CTAS / 2, p.tiles);
     return p;
   }
   p.BN = n <= 32 ? 32 : n <= 64 ? 64 : 128;
   p.token_tiles = 1;
   p.tiles = ceil_div(N, TK_M);
-  // slices: as many as keep all SMs busy, of four chunks at least
-  if (p.tiles < TK_CTAS) p.S = max(1, min(TK_CTAS / p.tiles, p.chunks / 4));
+  // a piece of sixteen chunks takes about as long as sharing a tile does; pieces that end with the tiles where that leaves
+  // few SMs idle
+  p.ctas = (int)min((long long)TK_CTAS, max((long long)p.tiles, (long long)p.tiles * p.chunks / 16));
+  if (p.ctas > p.tiles && p.ctas % p.tiles <= p.ctas / 6) p.ctas -= p.ctas % p.tiles;
   return p;
 }
-inline size_t tile_workspace(const TilePlan& p) {
-  return p.S == 1 ? 0 : 1024 + (size_t)p.tiles * p.S * p.BN * TK_M * sizeof(int);  // counters: tiles < 148
+inline size_t tile_workspace(const TilePlan& p) {  // nothing is shared when every CTA has whole tiles
+  return p.pair || p.tiles % p.ctas == 0 ? 0 : 1024 + (size_t)(p.ctas + p.tiles) * p.BN * TK_M * sizeof(int);
 }
 
 inline bool bad16(const void* p) { return !p || (reinterpret_cast<uintptr_t>(p) & 15); }
@@ -671,7 +708,7 @@ int launch_tile(const LinArgs& a, const TilePlan& pl, cudaStream_t st) {
   CUtensorMap tm_w, tm_x;
   if (!make_bytes_tensor_map(&tm_w, a.w, a.N, a.K, a.w_sr, TK_M) || !make_bytes_tensor_map(&tm_x, a.x, a.n, a.K, a.x_sr, BN))
     return OMNIKV_E_UNSUPPORTED;
-  OMNIKV_CUDA_OK(launch_pdl_smem_args(kern, dim3(min(TK_CTAS, pl.tiles * pl.S)), dim3(TK_THREADS), TkShape<BN>::SMEM, st, a, tm_w, tm_x));
+  OMNIKV_CUDA_OK(launch_pdl_smem_args(kern, dim3(pl.ctas), dim3(TK_THREADS), TkShape<BN>::SMEM, st, a, tm_w, tm_x));
   return OMNIKV_OK;
 }
 
@@ -683,7 +720,7 @@ int launch_pair(const LinArgs& a, const TilePlan& pl, cudaStream_t st) {
   CUtensorMap tm_w, tm_x;
   if (!make_bytes_tensor_map(&tm_w, a.w, a.N, a.K, a.w_sr, TK_M) || !make_bytes_tensor_map(&tm_x, a.x, a.n, a.K, a.x_sr, pl.BN / 2))
     return OMNIKV_E_UNSUPPORTED;
-  OMNIKV_CUDA_OK(launch_pdl_smem_args(kern, dim3(2 * min(TK_CTAS / 2, pl.tiles)), dim3(PK_THREADS), PK_SMEM, st, a, pl.BN, tm_w, tm_x));
+  OMNIKV_CUDA_OK(launch_pdl_smem_args(kern, dim3(pl.ctas), dim3(PK_THREADS), PK_SMEM, st, a, pl.BN, tm_w, tm_x));
   return OMNIKV_OK;
 }
 
@@ -744,13 +781,13 @@ extern "C" int omnikv_linear_w8a8(const omnikv_linear_w8a8_params* p, void* stre
   LinArgs a{p->x, p->x_stride_row, p->x_scale, p->w, p->w_stride_row, p->w_scale, p->residual, p->residual_stride_row,
             p->out, p->out_stride_row, p->n_tokens, p->channels, p->K};
   const TilePlan pl = tile_plan(a.n, a.N, a.K);
+  if ((long long)pl.tiles * pl.chunks > 0x7fffffff) return OMNIKV_E_UNSUPPORTED;
   const size_t need = a.n <= kStreamTokens ? 0 : tile_workspace(pl);
   if (need && (!p->workspace || p->workspace_bytes < need)) return OMNIKV_E_WORKSPACE;
   if (need && bad16(p->workspace)) return OMNIKV_E_BADARG;
   a.counters = static_cast<int*>(p->workspace);
   a.part = a.counters + 256;
   a.status = p->status;
-  a.S = pl.S;
   a.token_tiles = pl.token_tiles;
   a.chunks = pl.chunks;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
