@@ -30,6 +30,7 @@ from .. import ops, tensor_tools
 from .omnikv_config import logger
 from .spec_cache import OmniKVMultiStageCache, WOPackCache, full_attn_layers_of, get_cache_cls  # noqa: F401
 
+_KV_DTYPES = {"int8": torch.int8, "fp8_e4m3": torch.float8_e4m3fn}  # config key kv_cache_dtype
 _last_call_t = time.time()
 
 
@@ -223,6 +224,8 @@ def select_tokens_by_attn_universal(raw_attn, hidden_states, position_ids, past_
     k_cache = past_key_value.key_cache[raw_attn.layer_idx]
     if not k_cache.is_cuda:
         raise ValueError("the filter layer's keys must be on the GPU (filter layers are never offloaded)")
+    if k_cache.dtype in (torch.int8, torch.float8_e4m3fn):
+        raise NotImplementedError("the selector function scores keys in the model's type, not the codes of an 8-bit cache")
     q = q.to(k_cache.dtype)
     dev = k_cache.device
     n_dev = torch.full((bsz,), int(consider_len), dtype=torch.int32, device=dev)
@@ -264,6 +267,18 @@ class _ProjView:
         return F.linear(x, self.weight)
 
 
+def _project(x: torch.Tensor, owner: nn.Module, name: str, rows: Optional[int] = None) -> torch.Tensor:
+    """``x @ owner.<name>_weight.T`` (its first ``rows`` rows) for x ``[..., K]``: the library product, or the 8-bit integer
+    one when the weight is held as int8 codes (``OmniKVMulLM.quantize_weights_``)."""
+    codes = getattr(owner, name + "_codes", None)
+    if codes is None:
+        w = getattr(owner, name + "_weight")
+        return F.linear(x, w if rows is None else w[:rows])
+    x8, x_scale = ops.quant_rows(x.reshape(-1, x.shape[-1]))
+    y = ops.linear_w8a8(x8, x_scale, codes[:rows], getattr(owner, name + "_scale")[:rows], out_dtype=x.dtype)
+    return y.view(*x.shape[:-1], -1)
+
+
 class OmniKVAttention(nn.Module):
     """The ``self_attn`` object of a layer: Llama attention with fused QKV weights whose decode path
     runs in ``omnikv_decode_attn`` through the cache."""
@@ -296,7 +311,7 @@ class OmniKVAttention(nn.Module):
         """x ``[B, n, hidden]`` -> rotated q ``[B,H,n,d]``, rotated k and v ``[B,KVH,n,d]``."""
         B, n, _ = x.shape
         nq, nkv = self.num_heads * self.head_dim, self.num_key_value_heads * self.head_dim
-        qkv = F.linear(x, self.qkv_weight)
+        qkv = _project(x, self, "qkv")
         q = qkv[..., :nq].view(B, n, self.num_heads, self.head_dim).transpose(1, 2)
         k = qkv[..., nq:nq + nkv].view(B, n, self.num_key_value_heads, self.head_dim).transpose(1, 2)
         v = qkv[..., nq + nkv:].view(B, n, self.num_key_value_heads, self.head_dim).transpose(1, 2)
@@ -310,16 +325,17 @@ class OmniKVAttention(nn.Module):
             # decode: rotate q and k and append k, v to the cache in one kernel, straight from the fused projection
             tc = _tc_linear_ok(self.config, hidden_states)
             x2 = hidden_states.view(B, -1)
-            qkv = ops.batched_linear(x2, self.qkv_weight) if tc else F.linear(x2, self.qkv_weight)
+            qkv = ops.batched_linear(x2, self.qkv_weight) if tc else _project(x2, self, "qkv")
             q = torch.empty(B, self.num_heads, self.head_dim, dtype=qkv.dtype, device=qkv.device)
             k_buf, v_buf, pos = past_key_value.write_target_batch(self.layer_idx)
             ops.rope_append(qkv, self.num_heads, self.num_key_value_heads, self.rotary_emb.inv_freq, rope_pos, q,
                             k_buf, v_buf, pos)
+            past_key_value.row_written(self.layer_idx)
             o = past_key_value.attend(q, self.layer_idx, score_out=score_out, score_len=score_len)
             if tc:
                 o = ops.batched_linear(o.view(B, self.num_heads * self.head_dim), self.o_weight).view(B, 1, -1)
             else:
-                o = F.linear(o.view(B, 1, self.num_heads * self.head_dim), self.o_weight)
+                o = _project(o.view(B, 1, self.num_heads * self.head_dim), self, "o")
             return self.tp.all_reduce_sum(o) if self.tp is not None else o
         cos, sin = position_embeddings
         q, k, v = self.qkv(hidden_states, cos, sin)
@@ -336,7 +352,7 @@ class OmniKVAttention(nn.Module):
             o = past_key_value.attend(q[:, :, 0].contiguous(), self.layer_idx, score_out=score_out,
                                       score_len=score_len)
             o = o.view(B, 1, self.num_heads * self.head_dim)
-        o = F.linear(o, self.o_weight)
+        o = _project(o, self, "o")
         return self.tp.all_reduce_sum(o) if self.tp is not None else o
 
 
@@ -344,7 +360,8 @@ def _tc_linear_ok(config, x, inter=64) -> bool:
     """Decode-sized activations (at most 16 tokens, 16-bit, on the GPU) and ``tcgen05_linear`` switched on: the
     projections go through ``omnikv_batched_linear`` instead of the library GEMM."""
     return (x.is_cuda and x.dtype in (torch.bfloat16, torch.float16) and x.shape[-2] == 1 and x.numel() // x.shape[-1] <= 16
-            and inter % 64 == 0 and x.shape[-1] % 8 == 0 and config.get("tcgen05_linear", False))
+            and inter % 64 == 0 and x.shape[-1] % 8 == 0 and config.get("tcgen05_linear", False)
+            and config.get("linear_dtype", None) is None)
 
 
 class OmniKVMLP(nn.Module):
@@ -365,13 +382,13 @@ class OmniKVMLP(nn.Module):
             act = ops.batched_linear(x2, self.gate_up_weight, epilogue="swiglu")
             o = ops.batched_linear(act, self.down_weight).view(*x.shape[:-1], -1)
             return self.tp.all_reduce_sum(o) if self.tp is not None else o
-        gu = F.linear(x, self.gate_up_weight)
+        gu = _project(x, self, "gate_up")
         if x.is_cuda and x.shape[-2] == 1:  # decode: one kernel for silu(gate) * up
             act = ops.silu_mul(gu.view(-1, 2 * self.intermediate_size)).view(*x.shape[:-1], self.intermediate_size)
         else:
             g, u = gu[..., : self.intermediate_size], gu[..., self.intermediate_size:]
             act = F.silu(g) * u
-        o = F.linear(act, self.down_weight)
+        o = _project(act, self, "down")
         return self.tp.all_reduce_sum(o) if self.tp is not None else o
 
 
@@ -443,7 +460,7 @@ class OmniKVMulLayer(nn.Module):
                 self.hidden_state_window = win.contiguous()
             window_hs = self.hidden_state_window
         W = window_hs.shape[1]
-        q = F.linear(window_hs, attn.q_proj.weight)
+        q = _project(window_hs, attn, "qkv", attn.num_heads * attn.head_dim)
         rope_pos = getattr(cache, "rope_pos_dev", None)
         if (rope_pos is not None and q.is_cuda and attn.head_dim == 128 and attn.rotary_emb.attention_scaling == 1.0
                 and self.config.get("fused_small_ops", True)):
@@ -493,7 +510,8 @@ class OmniKVMulLayer(nn.Module):
         if ok is None:
             a = self.self_attn
             # the fused QKV kernel rotates with cos/sin of pos * inv_freq: no attention scaling (yarn, longrope)
-            ok = self.config.get("fused_decode", True) and a.rotary_emb.attention_scaling == 1.0 and ops.fused_decode_supported(
+            ok = self.config.get("fused_decode", True) and self.config.get("linear_dtype", None) is None \
+                and a.rotary_emb.attention_scaling == 1.0 and ops.fused_decode_supported(
                 key, self.config.hidden_size, self.mlp.intermediate_size, a.num_heads * a.head_dim, 8)
             self._fused_cache[key] = ok
         return ok
@@ -579,6 +597,7 @@ class OmniKVMulLayer(nn.Module):
                 ops.decode_qkv(h, self.input_layernorm.weight, self.input_layernorm.variance_epsilon, attn.qkv_weight,
                                attn.num_heads, attn.num_key_value_heads, attn.rotary_emb.inv_freq, cache.pos_dev, bufs.q,
                                k_seq, v_seq, pos)
+            cache.row_written(self.layer_idx)
             cache.attend(bufs.q, self.layer_idx, out=bufs.o, score_out=score_out, score_len=score_len)
             self._decode_select_end(cache, score_out)
             ops.decode_gemv_residual(attn.o_weight, bufs.o.view(-1), None, None, tp_out=xc.at(2 * self.layer_idx))
@@ -590,6 +609,7 @@ class OmniKVMulLayer(nn.Module):
         ops.decode_qkv(h, self.input_layernorm.weight, self.input_layernorm.variance_epsilon, attn.qkv_weight,
                        attn.num_heads, attn.num_key_value_heads, attn.rotary_emb.inv_freq, cache.pos_dev, bufs.q,
                        k_seq, v_seq, pos)
+        cache.row_written(self.layer_idx)
         cache.attend(bufs.q, self.layer_idx, out=bufs.o, score_out=score_out, score_len=score_len)
         self._decode_select_end(cache, score_out)
         lead = tp is None or tp.rank == 0  # with tensor parallelism only one rank adds the residual before the SUM
@@ -802,6 +822,7 @@ class OmniKVMulLM(nn.Module):
         m.eval()
         if seed is not None:
             m.init_random_(seed)
+            m._apply_linear_dtype()
         return m
 
     @classmethod
@@ -820,11 +841,40 @@ class OmniKVMulLM(nn.Module):
                 for k in f.keys():
                     sd[k] = f.get_tensor(k)
         m.load_hf_state_dict(sd)
+        m._apply_linear_dtype()
         return m
+
+    def _apply_linear_dtype(self) -> None:
+        """The config key ``linear_dtype``: None (the model's type) or "int8"."""
+        kind = self.config.get("linear_dtype", None)
+        if kind not in (None, "int8"):
+            raise NotImplementedError(f"linear_dtype={kind!r}: only None and 'int8' are implemented")
+        if kind == "int8":
+            self.quantize_weights_()
+
+    @torch.no_grad()
+    def quantize_weights_(self) -> "OmniKVMulLM":
+        """Hold the projections of every layer (QKV, output, gate/up, down) as int8 codes with one scale per output channel
+        and multiply them with per-token int8 activations (``omnikv_linear_w8a8``); the 16-bit matrices are given up.
+        Embedding, norms and lm_head stay.  Decoding then runs through the modules (the fused batch-1 kernels stream 16-bit
+        weights)."""
+        for layer in self.model.layers:
+            for owner, names in ((layer.self_attn, ("qkv", "o")), (layer.mlp, ("gate_up", "down"))):
+                for name in names:
+                    w = owner._parameters.pop(name + "_weight", None)
+                    if w is None:  # already done
+                        continue
+                    codes, scale = ops.quant_rows(w)
+                    owner.register_buffer(name + "_codes", codes, persistent=False)
+                    owner.register_buffer(name + "_scale", scale, persistent=False)
+            layer._fused_cache.clear()
+        self.config.linear_dtype = "int8"
+        return self
 
     @torch.no_grad()
     def load_hf_state_dict(self, sd):
         tp = self.tp
+        self._need_weights()
 
         def put(dst, src, dim=None):
             """Copy the full tensor, or this rank's slice of dimension ``dim`` when sharded."""
@@ -849,6 +899,7 @@ class OmniKVMulLM(nn.Module):
 
     def hf_state_dict(self):
         """Weights under their Hugging Face Llama names (views of the fused tensors)."""
+        self._need_weights()
         sd = {"model.embed_tokens.weight": self.model.embed_tokens.weight, "model.norm.weight": self.model.norm.weight,
               "lm_head.weight": self.lm_head.weight}
         for i, layer in enumerate(self.model.layers):
@@ -860,6 +911,10 @@ class OmniKVMulLM(nn.Module):
             sd[p + "input_layernorm.weight"] = layer.input_layernorm.weight
             sd[p + "post_attention_layernorm.weight"] = layer.post_attention_layernorm.weight
         return sd
+
+    def _need_weights(self) -> None:
+        if getattr(self.model.layers[0].self_attn, "qkv_codes", None) is not None:
+            raise RuntimeError("the projections are held as int8 codes (quantize_weights_): load or read weights before that")
 
     @torch.no_grad()
     def prepare_synthetic_decode(self, batch: int, seed: int = 0) -> None:
@@ -885,6 +940,14 @@ class OmniKVMulLM(nn.Module):
         kwargs = {}
         if cache_cls_name == "lazy":  # modeling/offload_select_once.py:275-276
             kwargs["skip_threshold"] = self.config.get("skip_threshold", 0.4)
+        kv_dtype = self.config.get("kv_cache_dtype", None)
+        if kv_dtype is not None:
+            if kv_dtype not in _KV_DTYPES:
+                raise NotImplementedError(f"kv_cache_dtype={kv_dtype!r}: only None and {sorted(_KV_DTYPES)} are implemented")
+            selector = self.config.get("selector_cls", "softmax_before_last")
+            kwargs.update(kv_dtype=_KV_DTYPES[kv_dtype], kv_block=self.config.get("kv_cache_block", 64),
+                          # the window selectors read the filter layers' keys in the model's type
+                          keep_layers=() if selector == "last" else do_sel_layers)
         return self.cache_cls.from_dynamic_cache(
             past_key_values,
             full_attn_layers=full_attn_layers_of(do_sel_layers, self.config.num_hidden_layers),
@@ -993,6 +1056,7 @@ class OmniKVMulLM(nn.Module):
         hs = h.view(1, 1, -1)
         for i, layer in enumerate(layers):
             score_out, score_len = layer._decode_select_begin(hs, cache, None)
+            cache.row_written(i)
             cache.attend(fb.q, i, out=fb.o, score_out=score_out, score_len=score_len)
             layer._decode_select_end(cache, score_out)
             tail = (qkv_args(layers[i + 1]) if i + 1 < len(layers) else

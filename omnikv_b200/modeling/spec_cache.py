@@ -19,6 +19,11 @@ Same public surface -- ``from_dynamic_cache``, ``update``, ``set_idx_on_gpu``, `
   selected tokens over the host link into staged device rows.  ``WOPackCache`` keeps one host
   buffer per layer and gathers inside each sparse layer, without overlap (:426-429, :477-483).
 
+With ``kv_dtype`` (torch.int8 or torch.float8_e4m3fn) the layers' K/V are held in 8 bits with one scale per ``kv_block`` rows
+and head: a prompt is stored by ``omnikv_kv8_store``, a token by ``omnikv_kv8_append``, and attention reads the codes
+(``omnikv_kv8_decode_attn``).  Layers named in ``keep_layers`` stay in the model's type (filter layers whose window selector
+scores 16-bit keys).  Not together with ``real_offload``.
+
 Batches: the reference flattens the batch of the index list (:292), which is only meaningful at
 batch 1; here every sequence has its own index list, lengths and tail.
 """
@@ -59,7 +64,15 @@ def make_layer_state(full_attn_layers, num_hidden_layers, num_wait_layers) -> Di
 class OmniKVMultiStageCache:
     pack_gather = True  # one gather per filter group on a side stream
 
-    def __init__(self, full_attn_layers: List, num_hidden_layers, num_wait_load_layers=2, real_offload=True):
+    def __init__(self, full_attn_layers: List, num_hidden_layers, num_wait_load_layers=2, real_offload=True,
+                 kv_dtype: Optional[torch.dtype] = None, kv_block: int = 64, keep_layers: Sequence[int] = ()):
+        if kv_dtype not in (None, torch.int8, torch.float8_e4m3fn):
+            raise ValueError(f"kv_dtype must be None, torch.int8 or torch.float8_e4m3fn, got {kv_dtype}")
+        if kv_dtype is not None and real_offload:
+            raise NotImplementedError("an 8-bit KV cache is held on the GPU: kv_dtype needs real_offload=False")
+        self.kv_dtype, self.kv_block, self.keep_layers = kv_dtype, int(kv_block), frozenset(keep_layers)
+        self._kv8: Dict[int, Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]] = {}  # codes and scales
+        self._new_row: Optional[Tuple[torch.Tensor, torch.Tensor]] = None  # 16-bit K, V of the token on its way into an 8-bit layer
         self.stage = "prefill"
         self.full_attn_layers = list(full_attn_layers)
         self.num_hidden_layers = num_hidden_layers
@@ -103,13 +116,13 @@ class OmniKVMultiStageCache:
     # ------------------------------------------------------------------------------------------
     @staticmethod
     def from_dynamic_cache(cache, full_attn_layers: List, num_hidden_layers, num_wait_load_layers=2,
-                           real_offload=True):
+                           real_offload=True, **kv8):
         """modeling/spec_cache.py:371-385.  ``cache`` may be None, an object with empty ``key_cache`` /
         ``value_cache`` lists (the usual case: the prefill then runs through this cache), or one that already holds
         a prompt -- CUDA tensors ``[B, KVH, P, d]`` for every layer: they are taken over as if that prompt had just
         been prefilled (copied into the preallocated layout; with ``real_offload`` the sparse layers' rows go to
-        pinned host memory), and decoding continues from there."""
-        c = OmniKVMultiStageCache(full_attn_layers, num_hidden_layers, num_wait_load_layers, real_offload)
+        pinned host memory), and decoding continues from there.  ``kv8``: ``kv_dtype``, ``kv_block``, ``keep_layers``."""
+        c = OmniKVMultiStageCache(full_attn_layers, num_hidden_layers, num_wait_load_layers, real_offload, **kv8)
         c._adopt(cache)
         return c
 
@@ -140,6 +153,9 @@ class OmniKVMultiStageCache:
     def is_offloaded(self, layer_idx: int) -> bool:
         return self.real_offload and self.layer_state[layer_idx][0]
 
+    def is_kv8(self, layer_idx: int) -> bool:
+        return self.kv_dtype is not None and layer_idx not in self.keep_layers
+
     def _host_key(self, layer_idx: int) -> Tuple[int, int]:
         """(key of the host/staged buffer, slot of the layer inside it)."""
         if self.pack_gather:
@@ -162,7 +178,14 @@ class OmniKVMultiStageCache:
 
     def _alloc_layer(self, layer_idx: int, B: int, KVH: int, d: int, dtype, device) -> None:
         P = self.prefill_len
-        if self.is_offloaded(layer_idx):
+        if self.is_kv8(layer_idx):
+            from .. import ops
+            cap = -(-(P + self.reserve) // self.kv_block) * self.kv_block
+            self._kv8[layer_idx] = ops.kv8_alloc(B, KVH, cap, block=self.kv_block, dtype=self.kv_dtype, device=device,
+                                                 tokens_first=self.is_sparse(layer_idx))
+            if self._new_row is None or self._new_row[0].shape[:2] != (B, KVH) or self._new_row[0].dtype != dtype:
+                self._new_row = tuple(torch.zeros(B, KVH, 1, d, dtype=dtype, device=device) for _ in range(2))
+        elif self.is_offloaded(layer_idx):
             if B != 1:
                 raise NotImplementedError("real_offload keeps one sequence's prompt KV on the host (batch 1)")
             key, slot = self._host_key(layer_idx)
@@ -180,6 +203,8 @@ class OmniKVMultiStageCache:
             key, slot = self._host_key(layer_idx)
             self.key_cache[layer_idx] = self._host[key][:, slot, 0].permute(1, 0, 2).unsqueeze(0)
             self.value_cache[layer_idx] = self._host[key][:, slot, 1].permute(1, 0, 2).unsqueeze(0)
+        elif self.is_kv8(layer_idx):  # the codes: kv8_rows() has the values
+            self.key_cache[layer_idx], self.value_cache[layer_idx] = self._kv8[layer_idx][:2]
         else:
             self.key_cache[layer_idx] = self._k[layer_idx]
             self.value_cache[layer_idx] = self._v[layer_idx]
@@ -211,7 +236,13 @@ class OmniKVMultiStageCache:
         P = self.prefill_len
         for layer in range(self.num_hidden_layers):
             self._alloc_layer(layer, B, KVH, d, dtype, device)
-            if self.is_offloaded(layer):
+            if self.is_kv8(layer):
+                from .. import ops
+                for b in range(B):
+                    k, v = (torch.randn(1, KVH, prefill_lens[b], d, generator=g, device=device, dtype=torch.float32).to(dtype)
+                            for _ in range(2))
+                    ops.kv8_store(k, v, *(t[b:b + 1] for t in self._kv8[layer]), block=self.kv_block)
+            elif self.is_offloaded(layer):
                 key, slot = self._host_key(layer)
                 step = 65536
                 for s in range(0, P, step):
@@ -256,7 +287,10 @@ class OmniKVMultiStageCache:
             self._init_meta(B, [P] * B, key_states.device)
             self._seen_tokens += P
         self._alloc_layer(layer_idx, B, KVH, d, key_states.dtype, key_states.device)
-        if self.is_offloaded(layer_idx):
+        if self.is_kv8(layer_idx):
+            from .. import ops
+            ops.kv8_store(key_states, value_states, *self._kv8[layer_idx], block=self.kv_block)
+        elif self.is_offloaded(layer_idx):
             key, slot = self._host_key(layer_idx)
             last = layer_idx == self.num_hidden_layers - 1  # the reference blocks on the last layer (:320-329)
             self._host[key][:, slot, 0].copy_(key_states[0].transpose(0, 1), non_blocking=not last)
@@ -281,26 +315,46 @@ class OmniKVMultiStageCache:
                 "set cache.reserve (rows kept free behind the prompt) before the prefill")
 
     def append_kv(self, k_new: torch.Tensor, v_new: torch.Tensor, layer_idx: int) -> None:
-        """Write the current token's rows ``[B, KVH, d]`` in place (``omnikv_kv_append``)."""
+        """Write the current token's rows ``[B, KVH, d]`` in place (``omnikv_kv_append``, ``omnikv_kv8_append``)."""
         from .. import ops
+        if self.is_kv8(layer_idx):
+            ops.kv8_append(k_new, v_new, *self._kv8[layer_idx], self.pos_dev, block=self.kv_block)
+            return
         pos = self.tail_pos_dev if self.is_offloaded(layer_idx) else self.pos_dev
         ops.kv_append(k_new, v_new, self._k[layer_idx], self._v[layer_idx], pos)
 
     def write_target_batch(self, layer_idx: int):
         """(k buffer, v buffer, row index tensor) for the current token of every sequence: the layer's
-        ``[B, KVH, rows, d]`` views and the int32 device positions (tail-relative for offloaded layers)."""
+        ``[B, KVH, rows, d]`` views and the int32 device positions (tail-relative for offloaded layers).  For an 8-bit
+        layer that is a single 16-bit row, and ``row_written`` takes it from there."""
+        if self.is_kv8(layer_idx):
+            return self._new_row[0], self._new_row[1], self.zero_dev
         pos = self.tail_pos_dev if self.is_offloaded(layer_idx) else self.pos_dev
         return self._k[layer_idx], self._v[layer_idx], pos
 
     def write_target(self, layer_idx: int):
         """(k rows, v rows, row index tensor) the current token of sequence 0 is written to: ``[KVH, rows, d]``
-        views of the layer's buffer and the int32 device position (tail-relative for offloaded layers)."""
-        pos = self.tail_pos_dev if self.is_offloaded(layer_idx) else self.pos_dev
-        return self._k[layer_idx][0], self._v[layer_idx][0], pos
+        views of the layer's buffer and the int32 device position (tail-relative for offloaded layers); see
+        ``write_target_batch`` for an 8-bit layer."""
+        k, v, pos = self.write_target_batch(layer_idx)
+        return k[0], v[0], pos
+
+    def row_written(self, layer_idx: int) -> None:
+        """The kernel that was given ``write_target`` has written the token's row: an 8-bit layer codes it now."""
+        if self.is_kv8(layer_idx):
+            self.append_kv(self._new_row[0][:, :, 0], self._new_row[1][:, :, 0], layer_idx)
+
+    def kv8_rows(self, layer_idx: int, start: int = 0, rows: Optional[int] = None, idx: Optional[torch.Tensor] = None):
+        """K, V ``[B, KVH, n, d]`` of an 8-bit layer in the model's type: rows ``[start, start + rows)``, or the rows
+        ``idx`` (int32 ``[B, n]``)."""
+        from .. import ops
+        return ops.kv8_load(*self._kv8[layer_idx], block=self.kv_block, dtype=self._new_row[0].dtype, start=start, rows=rows, idx=idx)
 
     def _compat_kv(self, layer_idx):
         n = self._seen_tokens
         P = self.prefill_len
+        if self.is_kv8(layer_idx):
+            return self._compat_kv8(layer_idx, n, P)
         if not self.is_sparse(layer_idx):
             return self._k[layer_idx][:, :, :n], self._v[layer_idx][:, :, :n]
         left = self.layer_state[layer_idx][1]
@@ -322,6 +376,20 @@ class OmniKVMultiStageCache:
         self.part_key[layer_idx], self.part_value[layer_idx] = pk, pv
         self.tail_k[layer_idx], self.tail_v[layer_idx] = tk, tv
         return (ks[0], vs[0]) if len(ks) == 1 else (torch.cat(ks, 0), torch.cat(vs, 0))
+
+    def _compat_kv8(self, layer_idx, n, P):
+        if not self.is_sparse(layer_idx):
+            return self.kv8_rows(layer_idx, rows=n)
+        idx, count = self._idx[self.layer_state[layer_idx][1]]
+        if int(count.min()) != int(count.max()):
+            raise ValueError("update() returns one tensor per layer: the sequences must have selected equally many rows")
+        sel = idx[:, :int(count.max())]
+        tail = torch.arange(P, n, dtype=torch.int32, device=idx.device).expand(idx.shape[0], -1)
+        k, v = self.kv8_rows(layer_idx, idx=torch.cat([sel, tail], 1))
+        m = sel.shape[1]
+        self.part_key[layer_idx], self.part_value[layer_idx] = k[:, :, :m], v[:, :, :m]
+        self.tail_k[layer_idx], self.tail_v[layer_idx] = k[:, :, m:], v[:, :, m:]
+        return k, v
 
     def set_idx_on_gpu(self, idx: torch.Tensor, sel_layer_idx: int) -> None:
         """modeling/spec_cache.py:290-306.  ``idx`` ``[B, k]`` ascending (int64 as the reference's
@@ -383,6 +451,14 @@ class OmniKVMultiStageCache:
         would have returned, computed by ``omnikv_decode_attn``.  ``score_out`` (filter layers):
         per-KV-head selector-``last`` score planes for positions ``< score_len``."""
         from .. import ops
+        if self.is_kv8(layer_idx):
+            cache = self._kv8[layer_idx]
+            if not self.is_sparse(layer_idx):
+                return ops.kv8_decode_attn(q, *cache, self.cur_len_dev, block=self.kv_block, out=out, score_out=score_out,
+                                           score_len=score_len)
+            idx32, count = self._idx[self.layer_state[layer_idx][1]]
+            return ops.kv8_decode_attn(q, *cache, count, block=self.kv_block, idx=idx32, tail_start=self.prefill_len_dev,
+                                       tail_len=self.tail_len_dev, out=out, max_rows=idx32.shape[1] + self.reserve)
         if not self.is_sparse(layer_idx):
             return ops.decode_attn(q, self._k[layer_idx], self._v[layer_idx], self.cur_len_dev, out=out,
                                    score_out=score_out, score_len=score_len)
@@ -415,8 +491,8 @@ class WOPackCache(OmniKVMultiStageCache):
 
     @staticmethod
     def from_dynamic_cache(cache, full_attn_layers: List, num_hidden_layers, num_wait_load_layers=2,
-                           real_offload=True):
-        c = WOPackCache(full_attn_layers, num_hidden_layers, num_wait_load_layers, real_offload)
+                           real_offload=True, **kv8):
+        c = WOPackCache(full_attn_layers, num_hidden_layers, num_wait_load_layers, real_offload, **kv8)
         c._adopt(cache)
         return c
 
@@ -439,9 +515,9 @@ class OmniKVLazyCache(OmniKVMultiStageCache):
 
     @staticmethod
     def from_dynamic_cache(cache, full_attn_layers: List, num_hidden_layers, num_wait_load_layers=2,
-                           real_offload=True, skip_threshold=0.4):
+                           real_offload=True, skip_threshold=0.4, **kv8):
         c = OmniKVLazyCache(full_attn_layers, num_hidden_layers, num_wait_load_layers, real_offload,
-                            skip_threshold=skip_threshold)
+                            skip_threshold=skip_threshold, **kv8)
         c._adopt(cache)
         return c
 

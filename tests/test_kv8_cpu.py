@@ -127,3 +127,15 @@ def test_appending_rows_in_falling_order_equals_storing_them(fmt):
     want, ws = ko.quantise(x, 8, fmt)
     assert torch.allclose(scales, ws, rtol=1e-15)
     assert ((codes - want).abs() <= 1e-9).float().mean() > 0.999  # a tie may fall to either side of the last bit
+
+
+def test_cache_options_are_checked():
+    from omnikv_b200.modeling import OmniKVLazyCache, OmniKVMultiStageCache, WOPackCache
+    for cls in (OmniKVMultiStageCache, WOPackCache, OmniKVLazyCache):
+        c = cls.from_dynamic_cache(None, [0, 1, 4], 4, 1, False, kv_dtype=torch.int8, kv_block=32, keep_layers=[1])
+        assert [c.is_kv8(i) for i in range(4)] == [True, False, True, True] and c.kv_block == 32
+        assert not any(cls.from_dynamic_cache(None, [0, 1, 4], 4, 1, False).is_kv8(i) for i in range(4))
+        with pytest.raises(NotImplementedError):
+            cls.from_dynamic_cache(None, [0, 1, 4], 4, 1, True, kv_dtype=torch.int8)
+        with pytest.raises(ValueError):
+            cls.from_dynamic_cache(None, [0, 1, 4], 4, 1, False, kv_dtype=torch.uint8)
