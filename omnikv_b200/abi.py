@@ -112,12 +112,6 @@ class ChainParams(C.Structure):
 
 
 KV8_INT8, KV8_E4M3 = 0, 1
-STREAM_TOKENS = 16  # OMNIKV_LINEAR_STREAM_TOKENS: projections of up to this many tokens need no workspace
-
-
-def kv8_attn_workspace_bytes(B: int, H: int, KVH: int, n_ctas: int) -> int:
-    """``omnikv_kv8_attn_workspace_bytes`` without the call: counters, then one partial per (CTA, segment) pair."""
-    return 16384 + (n_ctas + B * KVH) * (H // KVH) * 528
 
 
 class Kv8Cache(C.Structure):

@@ -7,7 +7,10 @@ result on its own: if the library is missing, every call raises.
 from __future__ import annotations
 
 import ctypes as C
+import importlib.machinery
+import importlib.util
 import math
+from pathlib import Path
 from typing import Optional, Tuple
 
 import torch
@@ -25,7 +28,7 @@ _launches = 0
 
 def launch_count() -> int:
     """Kernels of this library launched so far by this process (each ABI call adds what it launches)."""
-    return _launches
+    return _launches + (_bind_module.launches() if _bind_module is not None else 0)
 
 
 def _count(n: int) -> None:
@@ -511,86 +514,29 @@ def host_device_pointer(t: torch.Tensor) -> int:
 # ------------------------------------------------------------------------------------------------
 # KV cache held in 8 bits
 # ------------------------------------------------------------------------------------------------
-# A call of this section costs the host a few microseconds, of the order of its kernel for a single token, so what a
-# check needs is read from a tensor once and the C structs are filled by position.
-_KV8 = {torch.int8: abi.KV8_INT8, torch.float8_e4m3fn: abi.KV8_E4M3}
-_DT16 = {torch.bfloat16: abi.BF16, torch.float16: abi.F16}
-_own_workspaces = {}
+# Tensors are checked, results allocated and the C ABI called by the extension ``_omnikv_bind`` (csrc/host/bind.cpp): these
+# calls are a few microseconds on the GPU.
+_KV8 = (torch.int8, torch.float8_e4m3fn)
+_BIND_ABI = ("omnikv_kv8_store", "omnikv_kv8_append", "omnikv_kv8_load", "omnikv_kv8_attn_workspace_bytes", "omnikv_kv8_decode_attn",
+             "omnikv_quant_rows", "omnikv_linear_w8a8_workspace_bytes", "omnikv_linear_w8a8", "omnikv_capture_id")
+_bind_module = None
 
 
-def _on(first: torch.Tensor, *others) -> int:
-    """The ordinal of the device that all given tensors (None entries allowed) are on; raises for CPU tensors or several devices."""
-    dev = first.get_device()
-    for t in others:
-        if t is not None and t.get_device() != dev:
-            raise abi.OmniKVError("all tensors of a call must be on one CUDA device")
-    if dev < 0:
-        raise abi.OmniKVError("omnikv_b200 kernels need CUDA tensors; there is no CPU path")
-    return dev
-
-
-def _launch(dev: int, what: str, *args) -> None:
-    """Calls the C entry point ``what`` on the current stream of device ``dev``, with that device current."""
-    fn = getattr(abi.lib(), what)
-    if dev == torch._C._cuda_getDevice():
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
-    else:
-        with torch.cuda.device(dev):
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
-    if rc:
-        abi.check(rc, what)
-    _count(1)
-
-
-def _own_workspace(dev: int, nbytes: int, tag: str) -> torch.Tensor:
-    """A zero-filled workspace for calls that follow one another: one per stream, and one per captured graph (two
-    graphs, or a graph and eager calls, may run at the same time).  One that was outgrown is kept: a captured graph
-    may still use it."""
-    stream = torch._C._cuda_getCurrentRawStream(dev)
-    key = (dev, tag, stream, abi.lib().omnikv_capture_id(stream) if torch._C._cuda_isCurrentStreamCapturing() else 0)
-    kept = _own_workspaces.get(key)
-    if kept is None or kept[-1].numel() < nbytes:
-        kept = _own_workspaces.setdefault(key, [])
-        kept.append(torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=f"cuda:{dev}"))
-    return kept[-1]
-
-
-def _status_ptr(dev: int) -> int:
-    word = _status.get(dev)
-    return (status_word(dev) if word is None else word).data_ptr()
-
-
-def _need_i32(what: str, B: int, t: Optional[torch.Tensor]) -> Optional[int]:
-    """Address of a contiguous int32 ``[B]`` tensor (None stays None)."""
-    if t is None:
-        return None
-    if t.dtype is not torch.int32 or t.shape != (B,) or not t.is_contiguous():
-        raise abi.OmniKVError(f"{what} must be contiguous int32 [{B}]")
-    return t.data_ptr()
-
-
-def _kv8_cache(k8, v8, k_scale, v_scale, block: int) -> abi.Kv8Cache:
-    """The C description of a cache: codes ``[B,KVH,rows,128]`` (int8 or float8_e4m3fn) and fp32 scales ``[B,KVH,>=ceil(rows/block)]``."""
-    fmt, shape, strides = _KV8.get(k8.dtype), k8.shape, k8.stride()
-    if fmt is None or v8.dtype is not k8.dtype or len(shape) != 4 or v8.shape != shape or shape[3] != 128 \
-            or strides[3] != 1 or v8.stride() != strides:
-        raise abi.OmniKVError("kv8: k8 and v8 must be int8 or float8_e4m3fn [B, KVH, rows, 128] of one layout, rows contiguous")
-    if block < 1 or block > 256 or block & (block - 1):
-        raise abi.OmniKVError(f"kv8: block must be a power of two between 1 and 256, got {block}")
-    B, KVH, rows, d = shape
-    scales, steps = k_scale.shape, k_scale.stride()
-    if k_scale.dtype is not torch.float32 or v_scale.dtype is not torch.float32 or len(scales) != 3 or scales[0] != B \
-            or scales[1] != KVH or scales[2] * block < rows or steps[2] != 1 or v_scale.shape != scales or v_scale.stride() != steps:
-        raise abi.OmniKVError(f"kv8: scales must be fp32 [{B}, {KVH}, >= {-(-rows // block)}] of one layout, last dimension contiguous")
-    return abi.Kv8Cache(fmt, block, B, KVH, d, rows, k8.data_ptr(), v8.data_ptr(), strides[0], strides[1], strides[2],
-                        k_scale.data_ptr(), v_scale.data_ptr(), steps[0], steps[1])
-
-
-def _dt16(dtype: torch.dtype, what: str) -> int:
-    dt = _DT16.get(dtype)
-    if dt is None:
-        raise abi.OmniKVError(f"{what} must be bfloat16 or float16, got {dtype}")
-    return dt
+def _bind():
+    """The loaded extension.  Raises when it has not been built: there is no other code path."""
+    global _bind_module
+    if _bind_module is None:
+        lib, path = abi.lib(), Path(__file__).resolve().parent / "_lib" / "_omnikv_bind.so"
+        if not path.exists():
+            raise RuntimeError(f"{path} is missing: build it with `python -m omnikv_b200.build`")
+        loader = importlib.machinery.ExtensionFileLoader("_omnikv_bind", str(path))
+        spec = importlib.util.spec_from_file_location("_omnikv_bind", str(path), loader=loader)
+        module = importlib.util.module_from_spec(spec)
+        loader.exec_module(module)
+        module.init(tuple(C.cast(getattr(lib, name), C.c_void_p).value for name in _BIND_ABI), abi.OmniKVError, abi.check,
+                    lambda dev: (sm_count(dev), status_word(dev).data_ptr()))
+        _bind_module = module
+    return _bind_module
 
 
 def kv8_alloc(B: int, KVH: int, rows: int, *, block: int, dtype: torch.dtype, device, tokens_first: bool = False):
@@ -611,55 +557,23 @@ def kv8_alloc(B: int, KVH: int, rows: int, *, block: int, dtype: torch.dtype, de
 
 def kv8_store(k: torch.Tensor, v: torch.Tensor, k8, v8, k_scale, v_scale, *, block: int,
               lens: Optional[torch.Tensor] = None, start: int = 0) -> None:
-    """``omnikv_kv8_store``: 16-bit k, v ``[B,KVH,n,128]`` into rows ``[start, start + n)`` of an 8-bit cache (``start`` a
-    multiple of ``block``); ``lens`` int32 ``[B]`` on the device: only the first ``lens[b]`` of them exist."""
-    dev = _on(k8, k, v, v8, k_scale, v_scale, lens)
-    c = _kv8_cache(k8, v8, k_scale, v_scale, block)
-    dt, shape = _dt16(k.dtype, "kv8_store: k and v"), k.shape
-    if v.dtype is not k.dtype or v.shape != shape or len(shape) != 4 or shape[0] != c.B or shape[1] != c.KVH or shape[3] != 128:
-        raise abi.OmniKVError("kv8_store: k and v must be [B, KVH, n, 128] of one dtype")
-    n = shape[2]
-    if start < 0 or start % block or start + n > c.rows:
-        raise abi.OmniKVError(f"kv8_store: rows [{start}, {start + n}) must start at a multiple of {block} inside the cache's {c.rows} rows")
-    lens_ptr = _need_i32("lens", c.B, lens)
-    if n:
-        _launch(dev, "omnikv_kv8_store", c, dt, k.data_ptr(), *_kv_strides(k), v.data_ptr(), *_kv_strides(v), start, n, lens_ptr)
+    """``omnikv_kv8_store``: 16-bit k, v ``[B,KVH,n,128]`` into rows ``[start, start + n)`` of an 8-bit cache: codes k8, v8
+    ``[B,KVH,rows,128]`` (int8 or float8_e4m3fn) and fp32 k_scale, v_scale ``[B,KVH,>=ceil(rows/block)]``.  ``start`` is a
+    multiple of ``block``; ``lens`` int32 ``[B]`` on the device: only the first ``lens[b]`` of the rows exist."""
+    (_bind_module or _bind()).kv8_store(k, v, k8, v8, k_scale, v_scale, block, lens, start)
 
 
 def kv8_append(k_new: torch.Tensor, v_new: torch.Tensor, k8, v8, k_scale, v_scale, pos: torch.Tensor, *, block: int) -> None:
     """``omnikv_kv8_append``: 16-bit k_new, v_new ``[B,KVH,128]`` at row ``pos[b]`` (int32, device; negative: skipped).
     A block whose scale has to grow for the new row is re-coded up to that row."""
-    dev = _on(k8, k_new, v_new, v8, k_scale, v_scale, pos)
-    c = _kv8_cache(k8, v8, k_scale, v_scale, block)
-    dt, strides = _dt16(k_new.dtype, "kv8_append: k_new and v_new"), k_new.stride()
-    if k_new.shape != (c.B, c.KVH, 128) or v_new.shape != k_new.shape or v_new.dtype is not k_new.dtype \
-            or v_new.stride() != strides or strides[2] != 1:
-        raise abi.OmniKVError("kv8_append: k_new and v_new must be [B, KVH, 128] of one dtype and layout")
-    _launch(dev, "omnikv_kv8_append", c, dt, k_new.data_ptr(), v_new.data_ptr(), strides[0], strides[1],
-            _need_i32("pos", c.B, pos))
+    (_bind_module or _bind()).kv8_append(k_new, v_new, k8, v8, k_scale, v_scale, pos, block)
 
 
 def kv8_load(k8, v8, k_scale, v_scale, *, block: int, dtype: torch.dtype, start: int = 0, rows: Optional[int] = None,
              idx: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """``omnikv_kv8_load``: (k, v) ``[B,KVH,n,128]`` in ``dtype`` (16-bit): rows ``[start, start + rows)`` (default: to
     the end of the cache), or rows ``idx[b]`` (int32 ``[B, n]``; one outside the cache reads as zeros)."""
-    dev = _on(k8, v8, k_scale, v_scale, idx)
-    c = _kv8_cache(k8, v8, k_scale, v_scale, block)
-    dt, B, KVH = _dt16(dtype, "kv8_load: dtype"), c.B, c.KVH
-    if idx is not None:
-        shape = idx.shape
-        if idx.dtype is not torch.int32 or len(shape) != 2 or shape[0] != B or idx.stride(1) != 1 or start or rows is not None:
-            raise abi.OmniKVError("kv8_load: idx must be int32 [B, n] with contiguous rows, without start and rows")
-        n, idx_ptr, idx_stride = shape[1], idx.data_ptr(), idx.stride(0)
-    else:
-        n, idx_ptr, idx_stride = (c.rows - start if rows is None else rows), None, 0
-        if start < 0 or n < 0 or start + n > c.rows:
-            raise abi.OmniKVError(f"kv8_load: rows [{start}, {start + n}) are not inside the cache's {c.rows}")
-    k = torch.empty_strided((B, KVH, n, 128), (KVH * n * 128, n * 128, 128, 1), dtype=dtype, device=k8.device)
-    v = torch.empty_like(k)
-    if n:
-        _launch(dev, "omnikv_kv8_load", c, dt, start, n, idx_ptr, idx_stride, k.data_ptr(), v.data_ptr(), KVH * n * 128, n * 128, 128)
-    return k, v
+    return (_bind_module or _bind()).kv8_load(k8, v8, k_scale, v_scale, block, dtype, start, rows, idx)
 
 
 def kv8_decode_attn(q: torch.Tensor, k8, v8, k_scale, v_scale, len_a: torch.Tensor, *, block: int,
@@ -672,47 +586,10 @@ def kv8_decode_attn(q: torch.Tensor, k8, v8, k_scale, v_scale, len_a: torch.Tens
     are positions ``[0, len_a[b])``, or ``idx[b][0..len_a[b])`` (int32 ``[B, cap]``) followed by the ``tail_len[b]``
     positions from ``tail_start[b]`` of the same cache.  ``score_out`` ``[KVH,B,stride]`` fp32 (without ``idx`` and tail):
     selector-``last`` scores of positions ``< score_len[b]``.  ``n_splits``: CTAs per (sequence, KV head) on average
-    (default: as many as the GPU holds); ``max_rows`` (default: all) is only a hint for that number."""
-    dev = _on(q, k8, v8, k_scale, v_scale, len_a, idx, tail_start, tail_len, out, score_out, score_len, ws)
-    c = _kv8_cache(k8, v8, k_scale, v_scale, block)
-    dt, B, KVH, rows = _dt16(q.dtype, "kv8_decode_attn: q"), c.B, c.KVH, c.rows
-    shape, strides = q.shape, q.stride()
-    if len(shape) != 3 or shape[0] != B or shape[2] != 128 or strides[2] != 1 or shape[1] % KVH:
-        raise abi.OmniKVError("kv8_decode_attn: q must be [B, H, 128] with contiguous head vectors, H a multiple of KVH")
-    H = shape[1]
-    if out is None:
-        out = torch.empty_strided(shape, strides, dtype=q.dtype, device=q.device)
-    elif out.shape != shape or out.stride() != strides or out.dtype is not q.dtype:
-        raise abi.OmniKVError("kv8_decode_attn: out must have the shape, strides and dtype of q")
-    idx_ptr, idx_stride, idx_cap, cap = None, 0, 0, rows
-    if idx is not None:
-        if idx.dtype is not torch.int32 or idx.dim() != 2 or idx.shape[0] != B or idx.shape[1] == 0 or idx.stride(1) != 1:
-            raise abi.OmniKVError("kv8_decode_attn: idx must be int32 [B, cap] with contiguous rows")
-        idx_ptr, idx_stride, idx_cap = idx.data_ptr(), idx.stride(0), idx.shape[1]
-        cap = idx_cap
-    if (tail_len is None) != (tail_start is None):
-        raise abi.OmniKVError("kv8_decode_attn: tail_start and tail_len go together")
-    if tail_len is not None:
-        cap += rows
-    score_ptr, score_stride = None, 0
-    if score_out is not None:
-        if idx is not None or tail_len is not None or score_len is None:
-            raise abi.OmniKVError("kv8_decode_attn: scores need score_len, and neither idx nor a tail")
-        if score_out.dtype is not torch.float32 or score_out.dim() != 3 or score_out.shape[:2] != (KVH, B) \
-                or not score_out.is_contiguous() or score_out.shape[2] == 0:
-            raise abi.OmniKVError("kv8_decode_attn: score_out must be contiguous fp32 [KVH, B, stride]")
-        score_ptr, score_stride = score_out.data_ptr(), score_out.shape[2]
-    # one CTA per SM; fewer when there are fewer (sequence, KV head) pairs and not a tile of 32 rows for each of twelve warps
-    n_ctas = n_splits * B * KVH if n_splits else min(sm_count(dev), ((max_rows or cap) // 384 + 1) * B * KVH)
-    if ws is None:
-        ws = _own_workspace(dev, abi.kv8_attn_workspace_bytes(B, H, KVH, n_ctas), "kv8_attn")
-    p = abi.Kv8AttnParams(c, dt, H, scale if scale is not None else 0.08838834764831845, q.data_ptr(), strides[0], strides[1],
-                          out.data_ptr(), idx_ptr, idx_stride, idx_cap, _need_i32("len_a", B, len_a),
-                          _need_i32("tail_start", B, tail_start), _need_i32("tail_len", B, tail_len), score_ptr, score_stride,
-                          _need_i32("score_len", B, score_len), n_ctas, ws.data_ptr(), ws.numel() * ws.element_size(),
-                          _status_ptr(dev))
-    _launch(dev, "omnikv_kv8_decode_attn", p)
-    return out
+    (default: as many as the GPU holds); ``max_rows`` (default: all) is only a hint for that number.  ``ws``: a zeroed
+    workspace of ``omnikv_kv8_attn_workspace_bytes``; by default every stream and every captured graph has its own."""
+    return (_bind_module or _bind()).kv8_decode_attn(q, k8, v8, k_scale, v_scale, len_a, block, idx, tail_start, tail_len, out,
+                                                     score_out, score_len, n_splits, max_rows, scale, ws)
 
 
 # ------------------------------------------------------------------------------------------------
@@ -721,16 +598,7 @@ def kv8_decode_attn(q: torch.Tensor, k8, v8, k_scale, v_scale, len_a: torch.Tens
 def quant_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """``omnikv_quant_rows``: 16-bit x ``[n, K]`` (K a multiple of 16, at most 32768) -> int8 codes ``[n, K]`` and fp32
     scales ``[n]`` with ``x ~ codes * scale[:, None]``: the tokens of a call, or a weight matrix's output channels."""
-    dev = _on(x)
-    dt, shape, strides = _dt16(x.dtype, "quant_rows: x"), x.shape, x.stride()
-    if len(shape) != 2 or strides[1] != 1 or shape[1] == 0 or shape[1] % 16:
-        raise abi.OmniKVError("quant_rows: x must be [n, K] with contiguous rows and K a multiple of 16")
-    n, K = shape
-    codes = torch.empty_strided((n, K), (K, 1), dtype=torch.int8, device=x.device)
-    scale = torch.empty_strided((n,), (1,), dtype=torch.float32, device=x.device)
-    if n:
-        _launch(dev, "omnikv_quant_rows", dt, x.data_ptr(), strides[0], n, K, codes.data_ptr(), K, scale.data_ptr())
-    return codes, scale
+    return (_bind_module or _bind()).quant_rows(x)
 
 
 def linear_w8a8(x8: torch.Tensor, x_scale: torch.Tensor, w8: torch.Tensor, w_scale: torch.Tensor, *,
@@ -739,40 +607,7 @@ def linear_w8a8(x8: torch.Tensor, x_scale: torch.Tensor, w8: torch.Tensor, w_sca
     """``omnikv_linear_w8a8``: int8 x8 ``[n, K]`` times int8 w8 ``[channels, K]`` transposed, an exact integer sum, times
     ``x_scale[n]`` and ``w_scale[channels]`` (fp32), plus ``residual`` ``[n, channels]`` when given (``out`` may be the
     same tensor), rounded once to ``out_dtype`` (default: that of ``out`` or ``residual``, else bfloat16)."""
-    dev = _on(x8, x_scale, w8, w_scale, residual, out)
-    xs, ws, x_st, w_st = x8.shape, w8.shape, x8.stride(), w8.stride()
-    if x8.dtype is not torch.int8 or w8.dtype is not torch.int8 or len(xs) != 2 or len(ws) != 2 or x_st[1] != 1 or w_st[1] != 1:
-        raise abi.OmniKVError("linear_w8a8: x8 [n, K] and w8 [channels, K] must be int8 with contiguous rows")
-    n, K = xs
-    N = ws[0]
-    if ws[1] != K or K == 0 or K % 16:
-        raise abi.OmniKVError("linear_w8a8: x8 and w8 must share K, a multiple of 16")
-    if x_scale.dtype is not torch.float32 or w_scale.dtype is not torch.float32 or x_scale.shape != (n,) or w_scale.shape != (N,) \
-            or not x_scale.is_contiguous() or not w_scale.is_contiguous():
-        raise abi.OmniKVError("linear_w8a8: scales must be contiguous fp32, one per row of x8 and of w8")
-    dt = out_dtype
-    if dt is None:
-        dt = out.dtype if out is not None else residual.dtype if residual is not None else torch.bfloat16
-    for t in (out, residual):
-        if t is not None and (t.shape != (n, N) or t.dtype is not dt or t.stride(1) != 1):
-            raise abi.OmniKVError("linear_w8a8: out and residual must be [n, channels] of one floating dtype, rows contiguous")
-    out_code = _DT.get(dt)
-    if out_code is None:
-        raise abi.OmniKVError(f"linear_w8a8: the result is float32, bfloat16 or float16, not {dt}")
-    if out is None:
-        out = torch.empty_strided((n, N), (N, 1), dtype=dt, device=x8.device)
-    if n == 0 or N == 0:
-        return out
-    work = need = 0
-    if n > abi.STREAM_TOKENS:
-        need = abi.lib().omnikv_linear_w8a8_workspace_bytes(n, N, K)
-        work = _own_workspace(dev, need, "linear_w8a8").data_ptr() if need else 0
-    p = abi.LinearW8A8Params(n, N, K, x8.data_ptr(), x_st[0], x_scale.data_ptr(), w8.data_ptr(), w_st[0], w_scale.data_ptr(),
-                             out_code, None if residual is None else residual.data_ptr(),
-                             0 if residual is None else residual.stride(0), out.data_ptr(), out.stride(0), work, need,
-                             _status_ptr(dev))
-    _launch(dev, "omnikv_linear_w8a8", p)
-    return out
+    return (_bind_module or _bind()).linear_w8a8(x8, x_scale, w8, w_scale, residual, out, out_dtype)
 
 
 # ------------------------------------------------------------------------------------------------

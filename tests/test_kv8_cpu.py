@@ -63,14 +63,25 @@ def test_attention_arguments_are_checked():
     assert lib.omnikv_kv8_decode_attn(None, None) == -1
 
 
-def test_workspace_rules_agree_with_the_library():
+def test_workspace_sizes():
     from omnikv_b200 import abi
     lib = abi.lib()
-    for B, H, KVH, n in ((1, 32, 8, 148), (16, 8, 8, 1), (3, 16, 1, 700)):
-        assert abi.kv8_attn_workspace_bytes(B, H, KVH, n) == lib.omnikv_kv8_attn_workspace_bytes(B, H, KVH, n)
+    # counters, then a partial (128 sums and four numbers) per head of every (CTA, segment) pair
+    assert lib.omnikv_kv8_attn_workspace_bytes(3, 16, 2, 700) == 16384 + (700 + 6) * 8 * 528
     assert lib.omnikv_kv8_attn_workspace_bytes(1, 30, 8, 4) == 0
-    assert lib.omnikv_linear_w8a8_workspace_bytes(abi.STREAM_TOKENS, 512, 14336) == 0
-    assert lib.omnikv_linear_w8a8_workspace_bytes(abi.STREAM_TOKENS + 1, 512, 14336) > 0
+    assert lib.omnikv_linear_w8a8_workspace_bytes(16, 512, 14336) == 0  # a stream of the weights
+    assert lib.omnikv_linear_w8a8_workspace_bytes(17, 512, 14336) > 0   # CTAs share tiles
+    assert lib.omnikv_linear_w8a8_workspace_bytes(200, 512, 14336) == 0
+
+
+def test_the_extension_is_built_and_checks_its_arguments():
+    from omnikv_b200 import ops
+    bind = ops._bind()
+    assert bind.launches() == 0 or torch.cuda.is_available()
+    with pytest.raises(TypeError):
+        bind.quant_rows()
+    with pytest.raises(ops.abi.OmniKVError, match="must be a tensor"):
+        ops.quant_rows([1.0])
 
 
 def test_linear_arguments_are_checked():
