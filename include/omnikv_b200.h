@@ -618,7 +618,6 @@ int omnikv_kv8_decode_attn(const omnikv_kv8_attn_params* p, void* stream);
  * The workspace of omnikv_linear_w8a8 (omnikv_linear_w8a8_workspace_bytes, may be 0 bytes) starts with 1 KiB of counters
  * that are ZERO before its first use and are left zero; calls that share it must not overlap.
  * ------------------------------------------------------------------------------------------ */
-#define OMNIKV_LINEAR_STREAM_TOKENS 16 /* calls of up to this many tokens are a stream of the weights, without workspace */
 int omnikv_quant_rows(int dtype, const void* x, int64_t x_stride_row, int n, int K, int8_t* codes, int64_t code_stride_row,
                       float* scale, void* stream);
 

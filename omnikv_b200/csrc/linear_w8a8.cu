@@ -74,6 +74,7 @@ struct LinArgs {
   int* part;      // tile kernel: [CTAs + tiles][tokens of a tile][128]
   int* status;
   int token_tiles, chunks;
+  int shared, sharers;  // tile kernel: how many tiles, the last ones, are cut into how many pieces (each of a chunk or more)
 };
 
 // ---- up to 16 tokens: a stream of the weights -------------------------------------------------------------------------
@@ -165,9 +166,10 @@ __global__ void __launch_bounds__(SK_THREADS, NB == 1 ? 3 : 2) linear_stream_ker
 }
 
 // ---- up to 128 tokens: tiles of 128 channels x BN tokens on tcgen05 ---------------------------------------------------------
-// Still a stream of the weights.  The chunks (128 bytes of K) of all tiles form one list that is cut into equal pieces, one
-// per CTA: a CTA may end one tile and begin the next.  The integer sums of a tile that several CTAs share go to the
-// workspace, and the one that arrives last adds them up.
+// Still a stream of the weights.  Of the tiles every CTA has as many whole ones as all can have.  The chunks (128 bytes of
+// K) of those left over form one list that is cut into equal pieces, one per CTA, which a CTA works on first: the integer
+// sums of a tile that several CTAs share go to the workspace, the one that arrives last adds them up, and all that happens
+// under the stream of the whole tiles.
 // Warp 4 fetches 128-byte wide boxes of weights and tokens (TMA, 128-byte swizzle), warp 5 issues the MMAs (K = 32 bytes
 // each), int32 accumulators in tensor memory, two of them so that the epilogue of a tile runs under the next tile's MMAs.
 // Warps 0-3 read a tile back: thread = channel (TMEM lane), columns = tokens, so a warp's store is 32 neighbouring channels
@@ -275,7 +277,7 @@ linear_tile_kernel(const LinArgs a, const __grid_constant__ CUtensorMap tm_w, co
   extern __shared__ __align__(128) unsigned char smem_raw[];
   __shared__ TkShared sh;
   constexpr int STAGES = TkShape<BN>::STAGES, STAGE = TkShape<BN>::STAGE;
-  constexpr unsigned TMEM_COLS = 2 * BN;
+  constexpr unsigned TMEM_COLS = BN < 16 ? 32 : 2 * BN;
   unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
@@ -303,29 +305,51 @@ linear_tile_kernel(const LinArgs a, const __grid_constant__ CUtensorMap tm_w, co
   const unsigned tmem = sh.tmem_base;
   pdl_wait();
   pdl_trigger();
-  // this CTA's piece [lo, hi) of the list of chunks (the host keeps their count below 2^31)
-  const int chunks = a.chunks, total = ceil_div(a.N, TK_M) * chunks, C = gridDim.x, cta = blockIdx.x;
-  const auto piece_lo = [&](int i) { return (int)((long long)i * total / C); };
+  // this CTA's work: the piece [lo, hi) of the shared tiles' chunks, then whole tiles
+  const int chunks = a.chunks, tiles = ceil_div(a.N, TK_M), whole_tiles = tiles - a.shared, C = gridDim.x, cta = blockIdx.x;
+  const int total = a.shared * chunks;  // the host keeps it below 2^31
+  const int S = a.sharers;
+  const auto piece_lo = [&](int i) { return S ? (int)((long long)min(i, S) * total / S) : 0; };
+  struct Unit {
+    int tile, k0, k1;
+  };
   const int lo = piece_lo(cta), hi = piece_lo(cta + 1);
+  const auto first_unit = [&](Unit& u) {  // false: no work
+    if (lo < hi) u = Unit{whole_tiles + lo / chunks, lo % chunks, min(chunks, lo % chunks + hi - lo)};
+    else u = Unit{cta, 0, chunks};
+    return lo < hi || cta < whole_tiles;
+  };
+  const auto next_unit = [&](Unit& u) {
+    if (u.tile >= whole_tiles) {
+      const int at = (u.tile - whole_tiles) * chunks + u.k1;
+      if (at < hi) {
+        u = Unit{u.tile + 1, 0, min(chunks, hi - at)};
+        return true;
+      }
+      u = Unit{cta, 0, chunks};
+    } else {
+      u.tile += C;
+    }
+    return u.tile < whole_tiles;
+  };
 
   if (warp == 4) {
     if (lane == 0) {
-      int ct = lo / chunks, k = lo % chunks;
-      for (int it = 0; it < hi - lo; ++it) {
-        const int st = it % STAGES;
-        if (!mbar_wait(&sh.empty[st], ((it / STAGES) & 1) ^ 1, &sh.fail)) {
-          if (!sh.fail && a.status) atomicExch(a.status, 7);
-          sh.fail = 1;
-          break;
-        }
-        unsigned char* dst = ring + (size_t)st * STAGE;
-        mbar_expect_tx(&sh.full[st], STAGE);
-        tma_load_2d(dst, &tm_w, k * TK_KB, ct * TK_M, &sh.full[st]);
-        tma_load_2d(dst + TK_M * TK_KB, &tm_x, k * TK_KB, 0, &sh.full[st]);
-        sh.issued = it + 1;
-        if (++k == chunks) {
-          k = 0;
-          ++ct;
+      int it = 0;
+      Unit u;
+      for (bool more = first_unit(u); more && !sh.fail; more = next_unit(u)) {
+        for (int k = u.k0; k < u.k1; ++k, ++it) {
+          const int st = it % STAGES;
+          if (!mbar_wait(&sh.empty[st], ((it / STAGES) & 1) ^ 1, &sh.fail)) {
+            if (!sh.fail && a.status) atomicExch(a.status, 7);
+            sh.fail = 1;
+            break;
+          }
+          unsigned char* dst = ring + (size_t)st * STAGE;
+          mbar_expect_tx(&sh.full[st], STAGE);
+          tma_load_2d(dst, &tm_w, k * TK_KB, u.tile * TK_M, &sh.full[st]);
+          tma_load_2d(dst + TK_M * TK_KB, &tm_x, k * TK_KB, 0, &sh.full[st]);
+          sh.issued = it + 1;
         }
       }
     }
@@ -334,19 +358,20 @@ linear_tile_kernel(const LinArgs a, const __grid_constant__ CUtensorMap tm_w, co
       constexpr unsigned idesc = i8_instr_desc(TK_M, BN);
       bool ok = true;
       int it = 0, n = 0;
-      for (int at = lo; ok && at < hi; ++n) {
-        const int buf = n & 1, end = min(hi, (at / chunks + 1) * chunks);
+      Unit u;
+      for (bool more = first_unit(u); ok && more; more = next_unit(u), ++n) {
+        const int buf = n & 1;
         if (!mbar_wait(&sh.acc_empty[buf], ((n >> 1) & 1) ^ 1, &sh.fail)) { ok = false; break; }
         tc_fence_after();
         const unsigned d_tmem = tmem + (unsigned)buf * BN;
-        for (int first = at; at < end; ++at, ++it) {
+        for (int k = u.k0; k < u.k1; ++k, ++it) {
           const int st = it % STAGES;
           if (!mbar_wait(&sh.full[st], (it / STAGES) & 1, &sh.fail)) { ok = false; break; }
           tc_fence_after();
           const unsigned w_base = smem_u32(ring + (size_t)st * STAGE), x_base = w_base + TK_M * TK_KB;
 #pragma unroll
           for (int j = 0; j < TK_KB / 32; ++j)
-            tc_mma_i8(d_tmem, smem_desc_sw128(w_base + j * 32), smem_desc_sw128(x_base + j * 32), idesc, (at > first || j) ? 1u : 0u);
+            tc_mma_i8(d_tmem, smem_desc_sw128(w_base + j * 32), smem_desc_sw128(x_base + j * 32), idesc, (k > u.k0 || j) ? 1u : 0u);
           tc_commit(&sh.empty[st]);
         }
         if (ok) tc_commit(&sh.acc_full[buf]);
@@ -360,10 +385,10 @@ linear_tile_kernel(const LinArgs a, const __grid_constant__ CUtensorMap tm_w, co
     const int tokens = a.n;
     for (int j = tid; j < tokens; j += 128) sh.x_scale[j] = a.x_scale[j];
     int n = 0;
-    for (int at = lo; at < hi; ++n) {
-      const int buf = n & 1, tile = at / chunks, end = min(hi, (tile + 1) * chunks), c = tile * TK_M + tid;
-      const bool whole = end - at == chunks;
-      at = end;
+    Unit u;
+    for (bool more = first_unit(u); more; more = next_unit(u), ++n) {
+      const int buf = n & 1, tile = u.tile, c = tile * TK_M + tid;
+      const bool whole = u.k1 - u.k0 == chunks;
       const bool in = c < a.N;
       Channel<T> ch{in && a.res ? static_cast<const T*>(a.res) + c : nullptr, in ? static_cast<T*>(a.out) + c : nullptr,
                     a.res_sr, a.out_sr, tokens, in ? a.w_scale[c] : 0.f};
@@ -376,7 +401,7 @@ linear_tile_kernel(const LinArgs a, const __grid_constant__ CUtensorMap tm_w, co
       }
       tc_fence_after();
       const unsigned src = tmem + ((unsigned)(warp * 32) << 16) + (unsigned)buf * BN;
-      int* part = a.part + (size_t)(cta + tile) * BN * TK_M + tid;  // (CTA, tile) pairs walk a staircase: their sum is unique
+      int* part = a.part + (size_t)(cta + tile - whole_tiles) * BN * TK_M + tid;  // (CTA, tile) pairs walk a staircase: their sum is unique
 #pragma unroll 1
       for (int j0 = 0; j0 < tokens; j0 += 16) {
         int v[16];
@@ -394,12 +419,12 @@ linear_tile_kernel(const LinArgs a, const __grid_constant__ CUtensorMap tm_w, co
       if (!whole) {
         // the CTAs that share the tile: from the one that has its first chunk to the one that has its last
         const auto owner = [&](int chunk) {
-          int i = min(C - 1, (int)(((float)chunk + 0.5f) * (float)C / (float)total));
+          int i = min(S - 1, (int)(((float)chunk + 0.5f) * (float)S / (float)total));
           while (piece_lo(i) > chunk) --i;
           while (piece_lo(i + 1) <= chunk) ++i;
           return i;
         };
-        const int first = owner(tile * chunks), parts = owner((tile + 1) * chunks - 1) - first + 1;
+        const int at = (tile - whole_tiles) * chunks, first = owner(at), parts = owner(at + chunks - 1) - first + 1;
         epilogue_bar();
         if (tid == 0) {
           __threadfence();  // the stores, ordered before the barrier, are visible before the arrival is
@@ -409,7 +434,7 @@ linear_tile_kernel(const LinArgs a, const __grid_constant__ CUtensorMap tm_w, co
         }
         epilogue_bar();
         if (sh.last) {
-          const int* all = a.part + (size_t)(first + tile) * BN * TK_M + tid;
+          const int* all = a.part + (size_t)(first + tile - whole_tiles) * BN * TK_M + tid;
           const auto fetch = [&](int q, int j0, int (&v)[16]) {  // 16 tokens of partial q (the columns behind the tokens are there too)
 #pragma unroll
             for (int j = 0; j < 16; ++j) v[j] = q < parts && j0 < tokens ? __ldcg(all + ((size_t)q * BN + j0 + j) * TK_M) : 0;
@@ -658,14 +683,18 @@ linear_pair_kernel(const LinArgs a, const int BN, const __grid_constant__ CUtens
 }
 
 // ---- which kernel, and how K is cut -------------------------------------------------------------------------------------
-constexpr int kStreamTokens = OMNIKV_LINEAR_STREAM_TOKENS;
+// Up to 16 tokens: the stream kernel starts and ends sooner, the tile kernel keeps more bytes in flight.  Measured with
+// weights that are not in L2, 16 tokens: 5.3 against 10.6 us for 17 MB, 13.6 against 16.1 for 59 MB, 17.2 against 16.7 for
+// 67 MB, 28.9 against 22.6 for 117 MB (one token: 25.6 against 22.8).
+inline bool is_stream(int n, int N, int K) { return n <= 16 && (long long)N * K <= 1ll << 26; }
 
 struct TilePlan {
-  int BN, token_tiles, tiles, chunks, ctas;
+  int BN, token_tiles, tiles, chunks, ctas, shared, sharers;
   bool pair;
 };
 inline TilePlan tile_plan(int n, int N, int K) {
   TilePlan p;
+  p.shared = p.sharers = 0;
   p.chunks = ceil_div(K, TK_KB);
   p.pair = n > 128;
   if (p.pair) {
@@ -685,17 +714,27 @@ inline TilePlan tile_plan(int n, int N, int K) {
     p.ctas = 2 * min(TK_CTAS / 2, p.tiles);
     return p;
   }
-  p.BN = n <= 32 ? 32 : n <= 64 ? 64 : 128;
+  p.BN = n <= 16 ? 16 : n <= 32 ? 32 : n <= 64 ? 64 : 128;
   p.token_tiles = 1;
   p.tiles = ceil_div(N, TK_M);
-  // a piece of sixteen chunks takes about as long as sharing a tile does; pieces that end with the tiles where that leaves
-  // few SMs idle
-  p.ctas = (int)min((long long)TK_CTAS, max((long long)p.tiles, (long long)p.tiles * p.chunks / 16));
-  if (p.ctas > p.tiles && p.ctas % p.tiles <= p.ctas / 6) p.ctas -= p.ctas % p.tiles;
+  // Tiles are shared where the SMs would idle for more than eight chunks' time otherwise, about what sharing costs.  Next
+  // to whole tiles in pieces of four chunks at least; where there are only shared tiles in pieces of sixteen, and in pieces
+  // that end with the tiles where that leaves few SMs idle.
+  const int left = p.tiles % TK_CTAS;
+  p.ctas = min(TK_CTAS, p.tiles);
+  if (left && (long long)(TK_CTAS - left) * p.chunks > 8 * TK_CTAS) {
+    p.shared = left;
+    if (p.tiles < TK_CTAS) {
+      p.ctas = (int)min((long long)TK_CTAS, max((long long)p.tiles, (long long)p.tiles * p.chunks / 16));
+      if (p.ctas % p.tiles <= p.ctas / 6) p.ctas -= p.ctas % p.tiles;
+      if (p.ctas == p.tiles) p.shared = 0;
+    }
+    p.sharers = p.shared ? (int)min((long long)p.ctas, max(1ll, (long long)p.shared * p.chunks / 4)) : 0;
+  }
   return p;
 }
-inline size_t tile_workspace(const TilePlan& p) {  // nothing is shared when every CTA has whole tiles
-  return p.pair || p.tiles % p.ctas == 0 ? 0 : 1024 + (size_t)(p.ctas + p.tiles) * p.BN * TK_M * sizeof(int);
+inline size_t tile_workspace(const TilePlan& p) {
+  return p.shared ? 1024 + (size_t)(p.sharers + p.shared) * p.BN * TK_M * sizeof(int) : 0;
 }
 
 inline bool bad16(const void* p) { return !p || (reinterpret_cast<uintptr_t>(p) & 15); }
@@ -726,13 +765,14 @@ int launch_pair(const LinArgs& a, const TilePlan& pl, cudaStream_t st) {
 
 template <typename T>
 int launch_linear(const LinArgs& a, const TilePlan& pl, cudaStream_t st) {
-  if (a.n <= kStreamTokens) {
+  if (is_stream(a.n, a.N, a.K)) {
     auto kern = a.n <= 8 ? linear_stream_kernel<T, 1> : linear_stream_kernel<T, 2>;
     OMNIKV_CUDA_OK(launch_pdl(kern, dim3(ceil_div(a.N, SK_ROWS)), dim3(SK_THREADS), 0, st, a));
     return OMNIKV_OK;
   }
   if (pl.pair) return launch_pair<T>(a, pl, st);
   switch (pl.BN) {
+    case 16: return launch_tile<T, 16>(a, pl, st);
     case 32: return launch_tile<T, 32>(a, pl, st);
     case 64: return launch_tile<T, 64>(a, pl, st);
     default: return launch_tile<T, 128>(a, pl, st);
@@ -767,7 +807,7 @@ extern "C" int omnikv_quant_rows(int dtype, const void* x, int64_t x_stride_row,
 
 extern "C" size_t omnikv_linear_w8a8_workspace_bytes(int n_tokens, int channels, int K) {
   using namespace omnikv;
-  if (n_tokens <= kStreamTokens || channels <= 0 || K <= 0) return 0;
+  if (n_tokens <= 0 || channels <= 0 || K <= 0 || is_stream(n_tokens, channels, K)) return 0;
   return tile_workspace(tile_plan(n_tokens, channels, K));
 }
 
@@ -782,13 +822,15 @@ extern "C" int omnikv_linear_w8a8(const omnikv_linear_w8a8_params* p, void* stre
             p->out, p->out_stride_row, p->n_tokens, p->channels, p->K};
   const TilePlan pl = tile_plan(a.n, a.N, a.K);
   if ((long long)pl.tiles * pl.chunks > 0x7fffffff) return OMNIKV_E_UNSUPPORTED;
-  const size_t need = a.n <= kStreamTokens ? 0 : tile_workspace(pl);
+  const size_t need = is_stream(a.n, a.N, a.K) ? 0 : tile_workspace(pl);
   if (need && (!p->workspace || p->workspace_bytes < need)) return OMNIKV_E_WORKSPACE;
   if (need && bad16(p->workspace)) return OMNIKV_E_BADARG;
   a.counters = static_cast<int*>(p->workspace);
   a.part = a.counters + 256;
   a.status = p->status;
   a.token_tiles = pl.token_tiles;
+  a.shared = pl.shared;
+  a.sharers = pl.sharers;
   a.chunks = pl.chunks;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   switch (p->out_dtype) {

@@ -87,7 +87,7 @@ def test_quant_rows_of_extreme_values():
 @pytest.mark.parametrize("n,N,K", [
     (1, 1, 16), (1, 6144, 4096), (2, 1000, 32), (7, 129, 4096), (8, 256, 128), (9, 64, 272), (16, 4096, 1040), (17, 33, 14336),
     (33, 700, 96), (64, 512, 512), (65, 1001, 2064), (77, 1001, 1040), (128, 256, 4096), (129, 257, 144), (200, 3000, 64),
-    (513, 640, 1024), (1000, 1024, 4096)])
+    (513, 640, 1024), (1000, 1024, 4096), (1, 16411, 4112), (16, 16411, 4112), (40, 19000, 1040), (100, 37900, 144)])
 def test_linear(out_dtype, n, N, K):
     ops_ = operands(n, N, K, seed=n + N + K)
     check(ops().linear_w8a8(*ops_, out_dtype=out_dtype), *ops_)
