@@ -550,7 +550,8 @@ typedef struct {
 /* Rows [start, start + n) of every (sequence, head) from 16-bit k, v [B, KVH, n, d] (element strides, multiples of 8,
  * bases 16-byte aligned): a prompt, or the next chunk of one.  start: a multiple of block.  lens (device [B] or NULL):
  * sequence b has min(lens[b], n) rows; what lies behind them is neither read nor written, their absence counts as
- * nothing in a block's maximum, and a block without rows keeps its scale. */
+ * nothing in a block's maximum, and a block without rows keeps its scale.  A cache that is written has memory of its own for
+ * every sequence and head (strides of 0 are refused, here and in omnikv_kv8_append). */
 int omnikv_kv8_store(const omnikv_kv8_cache* c, int dtype, const void* k, int64_t k_stride_b, int64_t k_stride_h,
                      int64_t k_stride_row, const void* v, int64_t v_stride_b, int64_t v_stride_h, int64_t v_stride_row,
                      int start, int n, const int32_t* lens, void* stream);
@@ -573,7 +574,8 @@ int omnikv_kv8_load(const omnikv_kv8_cache* c, int dtype, int start, int n, cons
  *   rows of sequence b: idx == NULL: positions [0, len[b]); else positions idx[b][0..len[b]); then the tail positions
  *   [tail_start[b], tail_start[b] + tail_len[b]) when tail_len is given.
  * len is taken into [0, rows] (with idx: [0, idx_cap]), the tail into the cache; an index outside [0, rows) counts as no
- * row.  No rows at all: the output is zero.  score_out (idx == NULL, no tail): as in omnikv_decode_attn.
+ * row.  No rows at all: the output is zero.  score_out (idx == NULL, no tail): as in omnikv_decode_attn, positions below
+ * min(score_len[b], len[b], score_stride).  The cache is only read: sequences or heads may share memory (strides of 0).
  * q, out [B, H, d] 16-bit; H / KVH at most 16.
  * The workspace (omnikv_kv8_attn_workspace_bytes) starts with 16 KiB of counters that are ZERO before its first use and
  * are left zero; calls that share it must not overlap. */
@@ -584,7 +586,8 @@ typedef struct {
   float scale;
   const void* q;
   int64_t q_stride_b, q_stride_h;
-  void* out; /* same strides as q */
+  void* out; /* may be q itself; heads must not overlap */
+  int64_t out_stride_b, out_stride_h;
   const int32_t* idx;
   int64_t idx_stride;
   int32_t idx_cap;
@@ -613,7 +616,7 @@ int omnikv_kv8_decode_attn(const omnikv_kv8_attn_params* p, void* stream);
  *
  * The sum is exact (32-bit integers, K <= 32768); the scales are applied in fp32 and the result is rounded once.  x, w:
  * int8, rows of K contiguous codes, K a multiple of 16, row strides (elements) multiples of 16, bases 16-byte aligned.
- * out: OMNIKV_F32 or a 16-bit type, residual of the same type (may alias out).  omnikv_quant_rows serves the activations
+ * out: OMNIKV_F32 or a 16-bit type, residual of the same type (may be out itself; a row stride of 0: one row for all tokens).  omnikv_quant_rows serves the activations
  * of a call and, once, a weight matrix [channels, K].
  * The workspace of omnikv_linear_w8a8 (omnikv_linear_w8a8_workspace_bytes, may be 0 bytes) starts with 1 KiB of counters
  * that are ZERO before its first use and are left zero; calls that share it must not overlap.

@@ -131,6 +131,7 @@ class Kv8AttnParams(C.Structure):
     _fields_ = [
         ("cache", Kv8Cache), ("dtype", C.c_int32), ("H", C.c_int32), ("scale", C.c_float),
         ("q", C.c_void_p), ("q_stride_b", C.c_int64), ("q_stride_h", C.c_int64), ("out", C.c_void_p),
+        ("out_stride_b", C.c_int64), ("out_stride_h", C.c_int64),
         ("idx", C.c_void_p), ("idx_stride", C.c_int64), ("idx_cap", C.c_int32), ("len", C.c_void_p),
         ("tail_start", C.c_void_p), ("tail_len", C.c_void_p),
         ("score_out", C.c_void_p), ("score_stride", C.c_int64), ("score_len", C.c_void_p),

@@ -49,6 +49,7 @@ struct A8Args {
   const void* q;
   int64_t q_sb, q_sh;
   void* out;
+  int64_t o_sb, o_sh;
   const int* idx;
   int64_t idx_stride;
   int idx_cap;
@@ -205,7 +206,7 @@ decode_attn_kv8_kernel(const A8Args a, const __grid_constant__ CUtensorMap tm_k,
     for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
       if (row_list(a, b).n() > 0) continue;
       for (int i = tid; i < a.H * (kHeadDim / 2); i += NT)
-        reinterpret_cast<unsigned*>(static_cast<T*>(a.out) + (size_t)b * a.q_sb + (size_t)(i >> 6) * a.q_sh)[i & 63] = 0u;
+        reinterpret_cast<unsigned*>(static_cast<T*>(a.out) + (size_t)b * a.o_sb + (size_t)(i >> 6) * a.o_sh)[i & 63] = 0u;
     }
     if (filled == 0) return;
   }
@@ -343,7 +344,7 @@ decode_attn_kv8_kernel(const A8Args a, const __grid_constant__ CUtensorMap tm_k,
       qs[cb][0] = __shfl_sync(0xffffffffu, f, 8 * t);
       qs[cb][1] = __shfl_sync(0xffffffffu, f, 8 * t + 4);
     }
-    const int score_lim = a.score_out ? min(a.score_len[b], seg.list.nA) : 0;
+    const int score_lim = a.score_out ? (int)min((int64_t)min(a.score_len[b], seg.list.nA), a.score_stride) : 0;
     float* score_row = a.score_out ? a.score_out + ((size_t)kvh * a.B + b) * a.score_stride : nullptr;
 
     float m[COLS][2], M[COLS][2], l[COLS][2], o[COLS][8][4];
@@ -587,7 +588,7 @@ decode_attn_kv8_kernel(const A8Args a, const __grid_constant__ CUtensorMap tm_k,
     }
     const auto write_out = [&](int h, const float4& acc, float Ms, float ms, float L) {  // a head without rows: zero
       const float f = L == 0.f ? 0.f : exp2f(Ms - ms - 11.f) / L;
-      T* dst = static_cast<T*>(a.out) + (size_t)b * a.q_sb + (size_t)(kvh * G + h) * a.q_sh + lane * 4;
+      T* dst = static_cast<T*>(a.out) + (size_t)b * a.o_sb + (size_t)(kvh * G + h) * a.o_sh + lane * 4;
       *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(acc.x * f, acc.y * f), pack2<T>(acc.z * f, acc.w * f));
     };
     for (int h = warp; h < G; h += NW) {  // a head per warp: lane w holds the factors of warp w's sums
@@ -770,7 +771,8 @@ extern "C" int omnikv_kv8_decode_attn(const omnikv_kv8_attn_params* p, void* str
   if (const int rc = check_kv8_cache(&c)) return rc;
   const auto bad16 = [](const void* q) { return !q || (reinterpret_cast<uintptr_t>(q) & 15); };
   if (bad16(p->q) || bad16(p->out) || !p->len || p->H <= 0 || p->H % c.KVH || p->n_ctas <= 0) return OMNIKV_E_BADARG;
-  if (p->q_stride_b % 8 || p->q_stride_h % 8) return OMNIKV_E_BADARG;
+  if (p->q_stride_b % 8 || p->q_stride_h % 8 || p->out_stride_b % 8 || p->out_stride_h % 8) return OMNIKV_E_BADARG;
+  if ((c.B > 1 && p->out_stride_b < kHeadDim) || (p->H > 1 && p->out_stride_h < kHeadDim)) return OMNIKV_E_BADARG;
   if (p->idx && (p->idx_cap <= 0 || p->idx_stride < 0)) return OMNIKV_E_BADARG;
   if (p->tail_len && !p->tail_start) return OMNIKV_E_BADARG;
   if (p->score_out && (p->idx || p->tail_len || !p->score_len || p->score_stride <= 0)) return OMNIKV_E_BADARG;
@@ -785,7 +787,8 @@ extern "C" int omnikv_kv8_decode_attn(const omnikv_kv8_attn_params* p, void* str
   a.sb = c.stride_b; a.sh = c.stride_h; a.sr = c.stride_row;
   a.ks = c.k_scale; a.vs = c.v_scale; a.ssb = c.scale_stride_b; a.ssh = c.scale_stride_h;
   a.shift = __builtin_ctz(c.block); a.rows = c.rows;
-  a.q = p->q; a.q_sb = p->q_stride_b; a.q_sh = p->q_stride_h; a.out = p->out;
+  a.q = p->q; a.q_sb = p->q_stride_b; a.q_sh = p->q_stride_h;
+  a.out = p->out; a.o_sb = p->out_stride_b; a.o_sh = p->out_stride_h;
   a.idx = p->idx; a.idx_stride = p->idx_stride; a.idx_cap = p->idx_cap;
   a.len = p->len; a.tail_start = p->tail_start; a.tail_len = p->tail_len;
   a.score_out = p->score_out; a.score_stride = p->score_stride; a.score_len = p->score_len;

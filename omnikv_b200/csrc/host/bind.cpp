@@ -88,23 +88,33 @@ const int32_t* ints(const at::Tensor* t, int64_t n, const char* name) {
   return static_cast<const int32_t*>(t->data_ptr());
 }
 
+// The step of a dimension (of one entry: any step will do).
+int64_t step(const at::Tensor& t, int d) { return t.size(d) > 1 ? t.stride(d) : t.size(t.dim() - 1); }
+bool same_layout(const at::Tensor& a, const at::Tensor& b) {
+  if (a.sizes() != b.sizes()) return false;
+  for (int d = 0; d < (int)a.dim(); ++d)
+    if (step(a, d) != step(b, d)) return false;
+  return true;
+}
+bool dense_rows(const at::Tensor& t) { return t.size(t.dim() - 1) < 2 || t.stride(t.dim() - 1) == 1; }
+
 // The C description of a cache: codes [B, KVH, rows, 128] (int8 or e4m3), fp32 scales [B, KVH, >= ceil(rows / block)].
 omnikv_kv8_cache cache_of(const at::Tensor& k8, const at::Tensor& v8, const at::Tensor& ks, const at::Tensor& vs, int64_t block) {
   const at::ScalarType t = k8.scalar_type();
-  if ((t != at::kChar && t != at::kFloat8_e4m3fn) || v8.scalar_type() != t || k8.dim() != 4 || v8.sizes() != k8.sizes() ||
-      k8.size(3) != 128 || k8.stride(3) != 1 || v8.strides() != k8.strides())
+  if ((t != at::kChar && t != at::kFloat8_e4m3fn) || v8.scalar_type() != t || k8.dim() != 4 || k8.size(3) != 128 ||
+      !dense_rows(k8) || !same_layout(k8, v8))
     refuse("kv8: k8 and v8 must be int8 or float8_e4m3fn [B, KVH, rows, 128] of one layout, rows contiguous");
   if (block < 1 || block > 256 || (block & (block - 1)))
     refuse("kv8: block must be a power of two between 1 and 256, got " + std::to_string(block));
   const int64_t B = k8.size(0), KVH = k8.size(1), rows = k8.size(2);
   if (B > INT32_MAX || KVH > INT32_MAX || rows > INT32_MAX) refuse("kv8: a cache has at most 2^31 - 1 rows");
   if (ks.scalar_type() != at::kFloat || vs.scalar_type() != at::kFloat || ks.dim() != 3 || ks.size(0) != B || ks.size(1) != KVH ||
-      ks.size(2) * block < rows || ks.stride(2) != 1 || vs.sizes() != ks.sizes() || vs.strides() != ks.strides())
+      ks.size(2) * block < rows || !dense_rows(ks) || !same_layout(ks, vs))
     refuse("kv8: scales must be fp32 [" + std::to_string(B) + ", " + std::to_string(KVH) + ", >= " +
            std::to_string((rows + block - 1) / block) + "] of one layout, last dimension contiguous");
   return omnikv_kv8_cache{t == at::kChar ? OMNIKV_KV8_INT8 : OMNIKV_KV8_E4M3, (int32_t)block, (int32_t)B, (int32_t)KVH, 128,
-                          (int32_t)rows, k8.data_ptr(), v8.data_ptr(), k8.stride(0), k8.stride(1), k8.stride(2),
-                          static_cast<float*>(ks.data_ptr()), static_cast<float*>(vs.data_ptr()), ks.stride(0), ks.stride(1)};
+                          (int32_t)rows, k8.data_ptr(), v8.data_ptr(), step(k8, 0), step(k8, 1), step(k8, 2),
+                          static_cast<float*>(ks.data_ptr()), static_cast<float*>(vs.data_ptr()), step(ks, 0), step(ks, 1)};
 }
 
 // ---- devices, streams, workspaces -----------------------------------------------------------------------------------------
@@ -170,17 +180,17 @@ PyObject* kv8_store(PyObject* const* a) {
   const omnikv_kv8_cache c = cache_of(k8, v8, ks, vs, block);
   const int dt = code_of_16bit(k.scalar_type(), "kv8_store: k and v");
   if (v.scalar_type() != k.scalar_type() || k.dim() != 4 || v.sizes() != k.sizes() || k.size(0) != c.B || k.size(1) != c.KVH ||
-      k.size(3) != 128 || k.stride(3) != 1 || v.stride(3) != 1)
+      k.size(3) != 128 || !dense_rows(k) || !dense_rows(v))
     refuse("kv8_store: k and v must be [B, KVH, n, 128] of one dtype, rows contiguous");
   const int64_t n = k.size(2);
   if (start < 0 || start % block || start > c.rows || n > c.rows - start)
-    refuse("kv8_store: rows [" + std::to_string(start) + ", " + std::to_string(start + n) + ") must start at a multiple of " +
-           std::to_string(block) + " inside the cache's " + std::to_string(c.rows) + " rows");
+    refuse("kv8_store: " + std::to_string(n) + " rows from " + std::to_string(start) + " must start at a multiple of " + std::to_string(block) +
+           " and lie inside the cache's " + std::to_string(c.rows));
   const int32_t* lens_ptr = ints(lens, c.B, "lens");
   if (n) {
     OnDevice on(dev);
-    done(abi.kv8_store(&c, dt, k.data_ptr(), k.stride(0), k.stride(1), k.stride(2), v.data_ptr(), v.stride(0), v.stride(1),
-                       v.stride(2), (int)start, (int)n, lens_ptr, on.stream),
+    done(abi.kv8_store(&c, dt, k.data_ptr(), step(k, 0), step(k, 1), step(k, 2), v.data_ptr(), step(v, 0), step(v, 1),
+                       step(v, 2), (int)start, (int)n, lens_ptr, on.stream),
          "omnikv_kv8_store");
   }
   Py_RETURN_NONE;
@@ -192,12 +202,12 @@ PyObject* kv8_append(PyObject* const* a) {
   const int dev = one_device(k8, {&k, &v, &v8, &ks, &vs, &pos});
   const omnikv_kv8_cache c = cache_of(k8, v8, ks, vs, integer(a[7]));
   const int dt = code_of_16bit(k.scalar_type(), "kv8_append: k_new and v_new");
-  if (k.dim() != 3 || k.size(0) != c.B || k.size(1) != c.KVH || k.size(2) != 128 || k.stride(2) != 1 || v.sizes() != k.sizes() ||
-      v.scalar_type() != k.scalar_type() || v.strides() != k.strides())
+  if (k.dim() != 3 || k.size(0) != c.B || k.size(1) != c.KVH || k.size(2) != 128 || !dense_rows(k) ||
+      v.scalar_type() != k.scalar_type() || !same_layout(k, v))
     refuse("kv8_append: k_new and v_new must be [B, KVH, 128] of one dtype and layout");
   const int32_t* at_row = ints(&pos, c.B, "pos");
   OnDevice on(dev);
-  done(abi.kv8_append(&c, dt, k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), at_row, on.stream), "omnikv_kv8_append");
+  done(abi.kv8_append(&c, dt, k.data_ptr(), v.data_ptr(), step(k, 0), step(k, 1), at_row, on.stream), "omnikv_kv8_append");
   Py_RETURN_NONE;
 }
 
@@ -211,15 +221,15 @@ PyObject* kv8_load(PyObject* const* a) {
   const int64_t start = integer(a[6]);
   int64_t n, idx_stride = 0;
   if (idx) {
-    if (idx->scalar_type() != at::kInt || idx->dim() != 2 || idx->size(0) != c.B || idx->stride(1) != 1 || start || a[7] != Py_None)
+    if (idx->scalar_type() != at::kInt || idx->dim() != 2 || idx->size(0) != c.B || !dense_rows(*idx) || start || a[7] != Py_None)
       refuse("kv8_load: idx must be int32 [B, n] with contiguous rows, without start and rows");
     n = idx->size(1);
-    idx_stride = idx->stride(0);
+    idx_stride = step(*idx, 0);
   } else {
-    n = a[7] == Py_None ? c.rows - start : integer(a[7]);
-    if (start < 0 || n < 0 || start > c.rows || n > c.rows - start)
-      refuse("kv8_load: rows [" + std::to_string(start) + ", " + std::to_string(start + n) + ") are not inside the cache's " +
-             std::to_string(c.rows));
+    n = a[7] == Py_None ? -1 : integer(a[7]);
+    if (start < 0 || start > c.rows || n > c.rows - start || (n < 0 && a[7] != Py_None))
+      refuse("kv8_load: " + std::to_string(n) + " rows from " + std::to_string(start) + " are not inside the cache's " + std::to_string(c.rows));
+    if (n < 0) n = c.rows - start;
   }
   if (n > INT32_MAX) refuse("kv8_load: at most 2^31 - 1 rows");
   const at::Tensor k = fresh({c.B, c.KVH, n, 128}, t, k8), v = fresh({c.B, c.KVH, n, 128}, t, k8);
@@ -247,7 +257,7 @@ PyObject* kv8_decode_attn(PyObject* const* a) {
   p.cache = cache_of(k8, v8, ks, vs, integer(a[6]));
   p.dtype = code_of_16bit(q.scalar_type(), "kv8_decode_attn: q");
   const int64_t B = p.cache.B, KVH = p.cache.KVH, rows = p.cache.rows;
-  if (q.dim() != 3 || q.size(0) != B || q.size(2) != 128 || q.stride(2) != 1 || KVH == 0 || q.size(1) % KVH || q.size(1) > INT32_MAX)
+  if (q.dim() != 3 || q.size(0) != B || q.size(2) != 128 || !dense_rows(q) || KVH == 0 || q.size(1) % KVH || q.size(1) > INT32_MAX)
     refuse("kv8_decode_attn: q must be [B, H, 128] with contiguous head vectors, H a multiple of KVH");
   p.H = (int32_t)q.size(1);
   p.scale = 0.08838834764831845f;  // 1 / sqrt(128)
@@ -255,16 +265,16 @@ PyObject* kv8_decode_attn(PyObject* const* a) {
     p.scale = (float)PyFloat_AsDouble(a[15]);
     if (PyErr_Occurred()) throw PythonError();
   }
-  if (out_arg && (out_arg->sizes() != q.sizes() || out_arg->strides() != q.strides() || out_arg->scalar_type() != q.scalar_type()))
-    refuse("kv8_decode_attn: out must have the shape, strides and dtype of q");
+  if (out_arg && (out_arg->sizes() != q.sizes() || !dense_rows(*out_arg) || out_arg->scalar_type() != q.scalar_type()))
+    refuse("kv8_decode_attn: out must have the shape and dtype of q, head vectors contiguous");
   p.len = ints(&len, B, "len_a");
   int64_t cap = rows;
   if (idx) {
     if (idx->scalar_type() != at::kInt || idx->dim() != 2 || idx->size(0) != B || idx->size(1) == 0 || idx->size(1) > INT32_MAX ||
-        idx->stride(1) != 1)
+        !dense_rows(*idx))
       refuse("kv8_decode_attn: idx must be int32 [B, cap] with contiguous rows");
     p.idx = static_cast<const int32_t*>(idx->data_ptr());
-    p.idx_stride = idx->stride(0);
+    p.idx_stride = step(*idx, 0);
     p.idx_cap = (int32_t)idx->size(1);
     cap = idx->size(1);
   }
@@ -285,15 +295,20 @@ PyObject* kv8_decode_attn(PyObject* const* a) {
   }
   // one CTA per SM; fewer when there are fewer (sequence, KV head) pairs and not a tile of 32 rows for each of twelve warps
   const Device& d = device(dev);
-  int64_t n = a[13] == Py_None ? 0 : integer(a[13]) * B * KVH;
-  if (a[13] == Py_None) n = std::min(d.sms, ((a[14] == Py_None ? cap : integer(a[14])) / 384 + 1) * B * KVH);
-  if (n < 1 || n > 32768) refuse("kv8_decode_attn: n_splits x B x KVH must lie in 1..32768");
+  if (a[14] != Py_None) cap = integer(a[14]);
+  const int64_t per = a[13] != Py_None ? integer(a[13]) : std::clamp<int64_t>(cap / 384, 0, d.sms) + 1;
+  const int64_t segments = B * KVH;
+  if (per < 1 || per > 32768 || segments < 1 || segments > 32768 || (a[13] != Py_None && per * segments > 32768))
+    refuse("kv8_decode_attn: n_splits x B x KVH must lie in 1..32768");
+  const int64_t n = a[13] != Py_None ? per * segments : std::min(d.sms, per * segments);
   p.n_ctas = (int32_t)n;
-  const at::Tensor out = out_arg ? *out_arg : at::empty_strided(q.sizes(), q.strides(), q.options());
+  const at::Tensor out = out_arg ? *out_arg : fresh(q.sizes(), q.scalar_type(), q);
   p.q = q.data_ptr();
-  p.q_stride_b = q.stride(0);
-  p.q_stride_h = q.stride(1);
+  p.q_stride_b = step(q, 0);
+  p.q_stride_h = step(q, 1);
   p.out = out.data_ptr();
+  p.out_stride_b = step(out, 0);
+  p.out_stride_h = step(out, 1);
   p.status = d.status;
   OnDevice on(dev);
   const at::Tensor& ws = ws_arg ? *ws_arg : workspace(dev, on.stream, 0, abi.kv8_attn_workspace_bytes((int)B, p.H, (int)KVH, p.n_ctas));
@@ -307,13 +322,13 @@ PyObject* quant_rows(PyObject* const* a) {
   const at::Tensor& x = tensor(a[0], "x");
   const int dev = one_device(x, {});
   const int dt = code_of_16bit(x.scalar_type(), "quant_rows: x");
-  if (x.dim() != 2 || x.stride(1) != 1 || x.size(1) == 0 || x.size(1) % 16 || x.size(0) > INT32_MAX || x.size(1) > INT32_MAX)
+  if (x.dim() != 2 || !dense_rows(x) || x.size(1) == 0 || x.size(1) % 16 || x.size(0) > INT32_MAX || x.size(1) > INT32_MAX)
     refuse("quant_rows: x must be [n, K] with contiguous rows and K a multiple of 16");
   const int64_t n = x.size(0), K = x.size(1);
   const at::Tensor codes = fresh({n, K}, at::kChar, x), scale = fresh({n}, at::kFloat, x);
   if (n) {
     OnDevice on(dev);
-    done(abi.quant_rows(dt, x.data_ptr(), x.stride(0), (int)n, (int)K, static_cast<int8_t*>(codes.data_ptr()), K,
+    done(abi.quant_rows(dt, x.data_ptr(), step(x, 0), (int)n, (int)K, static_cast<int8_t*>(codes.data_ptr()), K,
                         static_cast<float*>(scale.data_ptr()), on.stream),
          "omnikv_quant_rows");
   }
@@ -328,7 +343,7 @@ PyObject* linear_w8a8(PyObject* const* a) {
   const at::Tensor &x8 = tensor(a[0], "x8"), &xs = tensor(a[1], "x_scale"), &w8 = tensor(a[2], "w8"), &ws = tensor(a[3], "w_scale");
   const at::Tensor *res = maybe(a[4], "residual"), *out_arg = maybe(a[5], "out");
   const int dev = one_device(x8, {&xs, &w8, &ws, res, out_arg});
-  if (x8.scalar_type() != at::kChar || w8.scalar_type() != at::kChar || x8.dim() != 2 || w8.dim() != 2 || x8.stride(1) != 1 || w8.stride(1) != 1)
+  if (x8.scalar_type() != at::kChar || w8.scalar_type() != at::kChar || x8.dim() != 2 || w8.dim() != 2 || !dense_rows(x8) || !dense_rows(w8))
     refuse("linear_w8a8: x8 [n, K] and w8 [channels, K] must be int8 with contiguous rows");
   const int64_t n = x8.size(0), K = x8.size(1), N = w8.size(0);
   if (w8.size(1) != K || K == 0 || K % 16 || n > INT32_MAX || N > INT32_MAX || K > INT32_MAX)
@@ -341,7 +356,7 @@ PyObject* linear_w8a8(PyObject* const* a) {
                            : res           ? res->scalar_type()
                                            : at::kBFloat16;
   for (const at::Tensor* o : {out_arg, res})
-    if (o && (o->dim() != 2 || o->size(0) != n || o->size(1) != N || o->scalar_type() != t || o->stride(1) != 1))
+    if (o && (o->dim() != 2 || o->size(0) != n || o->size(1) != N || o->scalar_type() != t || !dense_rows(*o)))
       refuse("linear_w8a8: out and residual must be [n, channels] of one floating dtype, rows contiguous");
   if (t != at::kFloat && t != at::kBFloat16 && t != at::kHalf)
     refuse(std::string("linear_w8a8: the result is float32, bfloat16 or float16, not ") + c10::toString(t));
@@ -353,17 +368,17 @@ PyObject* linear_w8a8(PyObject* const* a) {
     p.channels = (int32_t)N;
     p.K = (int32_t)K;
     p.x = static_cast<const int8_t*>(x8.data_ptr());
-    p.x_stride_row = x8.stride(0);
+    p.x_stride_row = step(x8, 0);
     p.x_scale = static_cast<const float*>(xs.data_ptr());
     p.w = static_cast<const int8_t*>(w8.data_ptr());
-    p.w_stride_row = w8.stride(0);
+    p.w_stride_row = step(w8, 0);
     p.w_scale = static_cast<const float*>(ws.data_ptr());
     p.out_dtype = t == at::kFloat ? OMNIKV_F32 : t == at::kBFloat16 ? OMNIKV_BF16 : OMNIKV_F16;
     p.out = out.data_ptr();
-    p.out_stride_row = out.stride(0);
+    p.out_stride_row = step(out, 0);
     if (res) {
       p.residual = res->data_ptr();
-      p.residual_stride_row = res->stride(0);
+      p.residual_stride_row = step(*res, 0);
     }
     if (const size_t need = abi.linear_w8a8_workspace_bytes(p.n_tokens, p.channels, p.K)) {
       const at::Tensor& work = workspace(dev, on.stream, 1, need);

@@ -245,7 +245,7 @@ extern "C" int omnikv_kv8_store(const omnikv_kv8_cache* c, int dtype, const void
                                 int64_t v_stride_h, int64_t v_stride_row, int start, int n, const int32_t* lens,
                                 void* stream) {
   using namespace omnikv;
-  if (const int rc = check_kv8_cache(c)) return rc;
+  if (const int rc = check_kv8_written(c)) return rc;
   if (bad16(k) || bad16(v) || n <= 0 || start < 0 || start % c->block || n > c->rows - start) return OMNIKV_E_BADARG;
   if (!is_16bit(dtype)) return OMNIKV_E_UNSUPPORTED;
   if (k_stride_b % 8 || k_stride_h % 8 || k_stride_row % 8 || v_stride_b % 8 || v_stride_h % 8 || v_stride_row % 8)
@@ -261,7 +261,7 @@ extern "C" int omnikv_kv8_store(const omnikv_kv8_cache* c, int dtype, const void
 extern "C" int omnikv_kv8_append(const omnikv_kv8_cache* c, int dtype, const void* k_new, const void* v_new,
                                  int64_t new_stride_b, int64_t new_stride_h, const int32_t* pos, void* stream) {
   using namespace omnikv;
-  if (const int rc = check_kv8_cache(c)) return rc;
+  if (const int rc = check_kv8_written(c)) return rc;
   if (bad16(k_new) || bad16(v_new) || !pos || new_stride_b % 8 || new_stride_h % 8) return OMNIKV_E_BADARG;
   if (!is_16bit(dtype)) return OMNIKV_E_UNSUPPORTED;
   cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -150,6 +150,12 @@ inline int check_kv8_cache(const omnikv_kv8_cache* c) {
   if (c->B > 65535 || c->KVH > 32767) return OMNIKV_E_UNSUPPORTED;  // grid dimensions
   return OMNIKV_OK;
 }
+// ... and write: no two sequences or heads in the same memory.
+inline int check_kv8_written(const omnikv_kv8_cache* c) {
+  if (const int rc = check_kv8_cache(c)) return rc;
+  const auto shared = [](int n, int64_t codes, int64_t scales) { return n > 1 && (!codes || !scales); };
+  return shared(c->B, c->stride_b, c->scale_stride_b) || shared(c->KVH, c->stride_h, c->scale_stride_h) ? OMNIKV_E_BADARG : OMNIKV_OK;
+}
 // Tensor map over the codes of an 8-bit cache (false: the layout cannot be described as one).
 bool make_kv8_tensor_map(CUtensorMap* map, const void* base, int64_t rows, int KVH, int B, int64_t sr, int64_t sh,
                          int64_t sb, int box_rows);

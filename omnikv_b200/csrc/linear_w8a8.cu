@@ -816,7 +816,7 @@ extern "C" int omnikv_linear_w8a8(const omnikv_linear_w8a8_params* p, void* stre
   if (!p || bad16(p->x) || bad16(p->w) || !p->x_scale || !p->w_scale || !p->out) return OMNIKV_E_BADARG;
   if (p->n_tokens <= 0 || p->channels <= 0 || p->K <= 0 || p->K % 16) return OMNIKV_E_BADARG;
   if (p->x_stride_row % 16 || p->w_stride_row % 16 || p->x_stride_row < p->K || p->w_stride_row < p->K) return OMNIKV_E_BADARG;
-  if (p->out_stride_row < p->channels || (p->residual && p->residual_stride_row < p->channels)) return OMNIKV_E_BADARG;
+  if (p->out_stride_row < p->channels || (p->residual && p->residual_stride_row && p->residual_stride_row < p->channels)) return OMNIKV_E_BADARG;
   if (p->K > 32768 || (p->out_dtype != OMNIKV_F32 && !is_16bit(p->out_dtype))) return OMNIKV_E_UNSUPPORTED;
   LinArgs a{p->x, p->x_stride_row, p->x_scale, p->w, p->w_stride_row, p->w_scale, p->residual, p->residual_stride_row,
             p->out, p->out_stride_row, p->n_tokens, p->channels, p->K};

@@ -586,7 +586,8 @@ def kv8_decode_attn(q: torch.Tensor, k8, v8, k_scale, v_scale, len_a: torch.Tens
     are positions ``[0, len_a[b])``, or ``idx[b][0..len_a[b])`` (int32 ``[B, cap]``) followed by the ``tail_len[b]``
     positions from ``tail_start[b]`` of the same cache.  ``score_out`` ``[KVH,B,stride]`` fp32 (without ``idx`` and tail):
     selector-``last`` scores of positions ``< score_len[b]``.  ``n_splits``: CTAs per (sequence, KV head) on average
-    (default: as many as the GPU holds); ``max_rows`` (default: all) is only a hint for that number.  ``ws``: a zeroed
+    (default: as many as the GPU holds); ``max_rows`` (default: all) is only a hint for that number.  ``out`` (default: a
+    new contiguous tensor) may be q itself; q and the cache may be expanded over the batch.  ``ws``: a zeroed
     workspace of ``omnikv_kv8_attn_workspace_bytes``; by default every stream and every captured graph has its own."""
     return (_bind_module or _bind()).kv8_decode_attn(q, k8, v8, k_scale, v_scale, len_a, block, idx, tail_start, tail_len, out,
                                                      score_out, score_len, n_splits, max_rows, scale, ws)
@@ -606,7 +607,7 @@ def linear_w8a8(x8: torch.Tensor, x_scale: torch.Tensor, w8: torch.Tensor, w_sca
                 out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """``omnikv_linear_w8a8``: int8 x8 ``[n, K]`` times int8 w8 ``[channels, K]`` transposed, an exact integer sum, times
     ``x_scale[n]`` and ``w_scale[channels]`` (fp32), plus ``residual`` ``[n, channels]`` when given (``out`` may be the
-    same tensor), rounded once to ``out_dtype`` (default: that of ``out`` or ``residual``, else bfloat16)."""
+    same tensor, a residual may be one row expanded), rounded once to ``out_dtype`` (default: that of ``out`` or ``residual``, else bfloat16)."""
     return (_bind_module or _bind()).linear_w8a8(x8, x_scale, w8, w_scale, residual, out, out_dtype)
 
 

@@ -29,6 +29,9 @@ def test_cache_descriptions_are_checked():
     for change in (dict(dtype=abi.F32), dict(format=2), dict(block=48), dict(block=0), dict(block=512), dict(head_dim=64),
                    dict(KVH=40000), dict(B=70000)):
         assert store(**change) == -2, change
+    # two sequences, or two heads, in the same memory: not to be written
+    for name in ("stride_b", "stride_h", "scale_stride_b", "scale_stride_h"):
+        assert store(B=2, **{name: 0}) == -1, name
     assert lib.omnikv_kv8_store(None, 1, 256, 0, 0, 128, 256, 0, 0, 128, 0, 1, None, None) == -1
     c = _cache(abi)
     assert lib.omnikv_kv8_append(ctypes.byref(c), abi.BF16, 256, 256, 0, 128, None, None) == -1
@@ -48,6 +51,7 @@ def test_attention_arguments_are_checked():
         p.cache, p.dtype, p.H, p.scale = _cache(abi), abi.BF16, 32, 0.1
         p.q = p.out = p.len = p.workspace = 256
         p.q_stride_b, p.q_stride_h, p.n_ctas = 4096, 128, 4
+        p.out_stride_b, p.out_stride_h = 4096, 128
         p.workspace_bytes = lib.omnikv_kv8_attn_workspace_bytes(1, 32, 8, 4)
         for name, v in change.items():
             setattr(p, name, v)
@@ -55,7 +59,7 @@ def test_attention_arguments_are_checked():
 
     for change in (dict(q=None), dict(q=8), dict(len=None), dict(H=30), dict(n_ctas=0), dict(q_stride_h=4), dict(idx=256),
                    dict(tail_len=256), dict(score_out=256), dict(score_out=256, score_len=256, score_stride=8, idx=256, idx_cap=4),
-                   dict(workspace=264)):
+                   dict(workspace=264), dict(out_stride_h=4), dict(out_stride_h=0), dict(out=None)):
         assert call(**change) == -1, change
     for change in (dict(dtype=abi.F32), dict(H=136), dict(n_ctas=32769)):
         assert call(**change) == -2, change

@@ -471,6 +471,83 @@ def test_two_streams_at_once():
         assert all(torch.equal(x, want[i]) for x in got[i])
 
 
+def test_sequences_that_share_a_cache_and_a_query():
+    """Strides of 0, which reading allows: a shared prompt, one query for all sequences."""
+    B, H, KVH, rows, block = 3, 16, 4, 700, 32
+    cache, k, v = filled(1, KVH, rows, "int8", torch.bfloat16, block, 83)
+    q = draw((1, H, D), torch.bfloat16, 84, outliers=False)
+    lens = [700, 0, 401]
+    wide = [t.expand(B, *t.shape[1:]) for t in cache]
+    out = ops().kv8_decode_attn(q.expand(B, H, D), *wide, i32(lens), block=block)
+    check_attention(out, q.expand(B, H, D), k.expand(B, -1, -1, -1), v.expand(B, -1, -1, -1), [list(range(n)) for n in lens])
+    assert torch.equal(out, ops().kv8_decode_attn(q.repeat(B, 1, 1), *[t.repeat(B, *[1] * (t.dim() - 1)) for t in cache], i32(lens), block=block))
+    idx = torch.randperm(rows, device="cuda")[:300].int().expand(B, -1)
+    sel = ops().kv8_decode_attn(q.expand(B, H, D), *wide, i32([300, 7, 0]), block=block, idx=idx)
+    check_attention(sel, q.expand(B, H, D), k.expand(B, -1, -1, -1), v.expand(B, -1, -1, -1), [idx[0, :n].tolist() for n in (300, 7, 0)])
+    kk, _ = ops().kv8_load(*wide, block=block, dtype=torch.bfloat16)
+    assert torch.equal(kk[1], kk[0]) and torch.equal(kk[:1], ops().kv8_load(*cache, block=block, dtype=torch.bfloat16)[0])
+
+
+def test_results_in_place_and_in_strided_memory():
+    B, H, KVH, rows, block = 2, 24, 2, 3000, 64
+    cache, k, v = filled(B, KVH, rows, "e4m3", torch.float16, block, 85)
+    q = draw((B, H, D), torch.float16, 86, outliers=False)
+    lens = [rows, 0]
+    want = ops().kv8_decode_attn(q, *cache, i32(lens), block=block)
+    check_attention(want, q, k, v, [list(range(n)) for n in lens])
+    wide = torch.full((H + 2, B, D + 8), 7.0, dtype=torch.float16, device="cuda")
+    place = wide.permute(1, 0, 2)[:, 1:-1, :D]
+    assert ops().kv8_decode_attn(q, *cache, i32(lens), block=block, out=place).data_ptr() == place.data_ptr()
+    assert torch.equal(place, want)
+    place.fill_(7.0)
+    assert (wide == 7.0).all()
+    same = q.clone()
+    ops().kv8_decode_attn(same, *cache, i32(lens), block=block, out=same)
+    assert torch.equal(same, want)
+
+
+def test_scores_end_where_their_memory_ends():
+    B, H, KVH, rows, stride = 2, 8, 2, 500, 300
+    cache, _, _ = filled(B, KVH, rows, "int8", torch.bfloat16, 64, 87)
+    q = draw((B, H, D), torch.bfloat16, 88, outliers=False)
+    full = torch.zeros(KVH, B, rows, device="cuda")
+    ops().kv8_decode_attn(q, *cache, i32([rows, 250]), block=64, score_out=full, score_len=i32([rows, rows]))
+    flat = torch.full((KVH * B * stride + 1000,), 5.0, device="cuda")
+    narrow = flat[:KVH * B * stride].view(KVH, B, stride)
+    ops().kv8_decode_attn(q, *cache, i32([rows, 250]), block=64, score_out=narrow, score_len=i32([rows, rows]))
+    assert torch.equal(narrow[:, 0], full[:, 0, :stride]) and torch.equal(narrow[:, 1, :250], full[:, 1, :250])
+    assert (narrow[:, 1, 250:] == 5.0).all() and (flat[KVH * B * stride:] == 5.0).all()
+
+
+@pytest.mark.parametrize("B,KVH,H,splits", [(70, 1, 3, None), (70, 2, 8, 3), (200, 8, 32, None)])
+def test_many_sequences(B, KVH, H, splits):
+    g = torch.Generator().manual_seed(B)
+    lens = torch.randint(0, 90, (B,), generator=g).tolist()
+    lens[3], lens[33], lens[B - 1] = 1500, 0, 0
+    cache, k, v = filled(B, KVH, 1500, "int8", torch.bfloat16, 16, 89)
+    q = draw((B, H, D), torch.bfloat16, 90, outliers=False)
+    out = ops().kv8_decode_attn(q, *cache, i32(lens), block=16, n_splits=splits)
+    check_attention(out, q, k, v, [list(range(n)) for n in lens])
+
+
+def test_strides_of_single_entries_do_not_matter():
+    cache, _, _ = filled(1, 1, 60, "int8", torch.bfloat16, 64, 91)
+    q = draw((1, 4, D), torch.bfloat16, 92, outliers=False)
+    want = ops().kv8_decode_attn(q, *cache, i32([60]), block=64)
+    k8, v8, ks, vs = cache
+    odd = [t.as_strided(t.shape, (3, 5, t.stride(2), 1)) for t in (k8, v8)] + [ks.as_strided((1, 1, 1), (7, 11, 5)), vs.as_strided((1, 1, 1), (2, 9, 3))]
+    qo = q.as_strided(q.shape, (9, D, 1))
+    assert torch.equal(ops().kv8_decode_attn(qo, *odd, i32([60]), block=64), want)
+    row = draw((1, 1, D), torch.bfloat16, 93)
+    ops().kv8_append(row.as_strided(row.shape, (3, 1, 1)), row, *odd, i32([59]), block=64)
+    ops().kv8_append(row, row, *cache, i32([59]), block=64)  # the same row again changes nothing
+    got = [t.clone() for t in cache]
+    k = draw((1, 1, 60, D), torch.bfloat16, 91)
+    ops().kv8_store(k, draw((1, 1, 60, D), torch.bfloat16, 92), *odd, block=64)
+    ops().kv8_append(row, row, *odd, i32([59]), block=64)
+    assert all(torch.equal(a.float(), b.float()) for a, b in zip(cache, got))
+
+
 # ---------------------------------------------------------------------------------------------- refusals
 def test_refusals():
     from omnikv_b200.abi import OmniKVError
@@ -505,6 +582,14 @@ def test_refusals():
         lambda: o.kv8_decode_attn(q, *cache, n, block=16, score_out=torch.zeros(2, 2, 64, device="cuda")),
         lambda: o.kv8_decode_attn(q, *cache, n, block=16, out=torch.empty(2, 4, D, device="cuda")),
         lambda: o.kv8_decode_attn(q, *cache, n, block=16, n_splits=20000),
+        lambda: o.kv8_decode_attn(q, *cache, n, block=16, n_splits=2 ** 62),
+        lambda: o.kv8_decode_attn(q, *cache, n, block=16, n_splits=0),
+        lambda: o.kv8_decode_attn(q, *cache, n, block=16, out=q[:1].expand(2, 4, D)),  # sequences in the same memory
+        lambda: o.kv8_store(k, k, *[t[:1].expand(2, *t.shape[1:]) for t in cache], block=16),
+        lambda: o.kv8_append(k[:, :, 0], k[:, :, 0], *[t[:, :1].expand(2, 2, *t.shape[2:]) for t in cache], n, block=16),
+        lambda: o.kv8_load(*cache, block=16, dtype=torch.bfloat16, start=-2 ** 62),
+        lambda: o.kv8_load(*cache, block=16, dtype=torch.bfloat16, rows=-1),
+        lambda: o.kv8_load(*cache, block=16, dtype=torch.bfloat16, rows=2 ** 40),
         lambda: o.kv8_decode_attn(q, *cache, n, block=16, ws=torch.zeros(64, dtype=torch.uint8, device="cuda")),
         lambda: o.kv8_decode_attn(torch.zeros(2, 34, D, dtype=torch.bfloat16, device="cuda"), *cache, n, block=16),
         lambda: o.kv8_alloc(1, 1, 16, block=16, dtype=torch.uint8, device="cuda"),

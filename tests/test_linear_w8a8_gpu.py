@@ -159,6 +159,58 @@ def test_repeated_and_captured_calls_agree(n):
     assert all(torch.equal(got, want) for _, got in graphs)
 
 
+@pytest.mark.parametrize("N,K", [(1024, 8192), (18944 + 300, 1040)])  # tiles that CTAs share, alone and next to whole ones
+def test_shared_tiles_on_two_streams_and_in_graphs(N, K):
+    n = 40
+    x8, sx, w8, sw = operands(n, N, K)
+    want = ops().linear_w8a8(x8, sx, w8, sw)
+    check(want, x8, sx, w8, sw)
+    streams, got = [torch.cuda.Stream() for _ in range(2)], []
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(ops().linear_w8a8(x8, sx, w8, sw))
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got.append(ops().linear_w8a8(x8, sx, w8, sw))
+        graphs.append(graph)
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for s, graph in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                graph.replay()
+        got.append(ops().linear_w8a8(x8, sx, w8, sw))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want) for y in got)
+
+
+@pytest.mark.parametrize("n,N,K", [(1, 72, 64), (16, 500, 512), (40, 1024, 8192), (130, 300, 96)])
+def test_residual_in_place_and_one_row_for_all(n, N, K):
+    x8, sx, w8, sw = operands(n, N, K)
+    res = torch.randn(n, N, generator=torch.Generator(device="cuda").manual_seed(4), device="cuda").to(torch.bfloat16)
+    want = ops().linear_w8a8(x8, sx, w8, sw, residual=res)
+    check(want, x8, sx, w8, sw, res)
+    own = res.clone()
+    assert ops().linear_w8a8(x8, sx, w8, sw, residual=own, out=own).data_ptr() == own.data_ptr()
+    assert torch.equal(own, want)
+    bias = res[:1].expand(n, N)
+    assert torch.equal(ops().linear_w8a8(x8, sx, w8, sw, residual=bias), ops().linear_w8a8(x8, sx, w8, sw, residual=bias.contiguous()))
+
+
+def test_strides_of_a_single_row_do_not_matter():
+    x8, sx, w8, sw = operands(1, 200, 160)
+    want = ops().linear_w8a8(x8, sx, w8, sw)
+    out = torch.empty(200, dtype=torch.bfloat16, device="cuda").as_strided((1, 200), (1, 1))
+    assert torch.equal(ops().linear_w8a8(x8.as_strided(x8.shape, (7, 1)), sx, w8, sw, out=out), want)
+    x = torch.randn(1, 160, device="cuda").to(torch.bfloat16)
+    for a, b in zip(ops().quant_rows(x.as_strided(x.shape, (5, 1))), ops().quant_rows(x)):
+        assert torch.equal(a, b)
+
+
 def test_refusals():
     from omnikv_b200.abi import OmniKVError
     o = ops()
