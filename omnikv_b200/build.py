@@ -63,7 +63,7 @@ def build_bind(force: bool = False) -> Path:
                "-I", sysconfig.get_paths()["include"], "-I", str(torch_dir / "include"),
                "-I", str(torch_dir / "include" / "torch" / "csrc" / "api" / "include"), "-I", str(cuda / "include"),
                "-I", str(ROOT / "include"), str(src), "-o", str(BIND), "-L", str(torch_dir / "lib"),
-               f"-Wl,-rpath,{torch_dir / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+               f"-Wl,-rpath,{torch_dir / 'lib'}", "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"g++ failed on {src.name}:\n{r.stderr}")
