@@ -3,10 +3,13 @@
 //     out[t][c] = (sum_k x[t][k] w[c][k]) * x_scale[t] * w_scale[c] (+ residual[t][c])
 //
 // The sum is an integer (|sum| <= 128 * 128 * 32768 = 2^29), so it is exact and independent of the order in which slices
-// of K are added.  Up to 16 tokens the call is a stream of the weights (HBM bound: K * channels bytes) and runs on
-// mma.sync; more tokens run on tcgen05 (kind::i8) with the channels on the M side, which leaves the N side to a token
-// count of any size.
+// of K are added.  Four kernels: for few tokens a stream of the weights on mma.sync, which starts and ends soonest; for more
+// tcgen05 (kind::i8) with the channels on the M side, which leaves the N side to a token count of any size: tiles on single
+// SMs that stream a large matrix, tiles shared by a cluster of SMs where there are few of them, tiles on SM pairs for many
+// tokens.  linear_plan below chooses by estimates of their times.
+#include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <type_traits>
 
 #include "kv8.cuh"
@@ -73,15 +76,17 @@ struct LinArgs {
   int* counters;  // tile kernel: [CTAs] arrivals at the tile that a CTA is the first to work on, zero between launches
   int* part;      // tile kernel: [CTAs + tiles][tokens of a tile][128]
   int* status;
-  int token_tiles, chunks;
+  int token_tiles, chunks;  // tiles along the tokens, 128-byte steps of K
+  int cluster;              // cluster kernel: CTAs per tile
   int shared, sharers;  // tile kernel: how many tiles, the last ones, are cut into how many pieces (each of a chunk or more)
 };
 
-// ---- up to 16 tokens: a stream of the weights -------------------------------------------------------------------------
+// ---- few tokens: a stream of the weights -------------------------------------------------------------------------------
 // A CTA owns 16 channels, its eight warps take 64-byte chunks of K in turn.  The fragments of m16n8k32 come straight from
 // global memory with 16-byte loads: inside a chunk of 64 the order of k is free as long as both operands agree, so thread
 // (g, t) takes bytes 16 t .. 16 t + 15 of rows g and g + 8 (weights) and of token g, and their words 0..3 are two MMAs.
 // DEPTH chunks are asked for while the DEPTH before them are multiplied.  The eight integer sums meet in shared memory.
+// More tokens than a CTA takes go to other CTAs, which find the weights in L2.
 constexpr int SK_THREADS = 256, SK_WARPS = SK_THREADS / 32, SK_ROWS = 16;
 
 __device__ __forceinline__ void mma_i8(int (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
@@ -96,13 +101,13 @@ __device__ __forceinline__ uint4 ld_stream(const int8_t* p) {  // weights: read 
   return v;
 }
 
-// NB: blocks of eight tokens
+// NB: blocks of eight tokens of a CTA
 template <typename T, int NB>
 __global__ void __launch_bounds__(SK_THREADS, NB == 1 ? 3 : 2) linear_stream_kernel(const LinArgs a) {
-  constexpr int SK_DEPTH = NB == 1 ? 2 : 3;
+  constexpr int SK_DEPTH = NB == 2 ? 3 : 2;
   __shared__ int sums[SK_WARPS][NB * 8][SK_ROWS + 1];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const int c0 = blockIdx.x * SK_ROWS;
+  const int c0 = blockIdx.x * SK_ROWS, t0 = blockIdx.y * (NB * 8);
   // While the kernel before finishes, this CTA's weights start on their way into L2.  Nothing is read: weights that the
   // kernel before wrote would be wrong in registers, in L2 they are not.
   if (tid < SK_ROWS && c0 + tid < a.N)
@@ -113,7 +118,7 @@ __global__ void __launch_bounds__(SK_THREADS, NB == 1 ? 3 : 2) linear_stream_ker
   const int8_t* w1 = a.w + (size_t)min(c0 + g + 8, a.N - 1) * a.w_sr + 16 * t;
   const int8_t* xp[NB];
 #pragma unroll
-  for (int b = 0; b < NB; ++b) xp[b] = a.x + (size_t)min(b * 8 + g, a.n - 1) * a.x_sr + 16 * t;
+  for (int b = 0; b < NB; ++b) xp[b] = a.x + (size_t)min(t0 + b * 8 + g, a.n - 1) * a.x_sr + 16 * t;
   const int chunks = (a.K + 63) >> 6;
   int acc[NB][4];
 #pragma unroll
@@ -155,21 +160,27 @@ __global__ void __launch_bounds__(SK_THREADS, NB == 1 ? 3 : 2) linear_stream_ker
 #pragma unroll
     for (int e = 0; e < 4; ++e) sums[warp][b * 8 + 2 * t + (e & 1)][g + 8 * (e >> 1)] = acc[b][e];
   __syncthreads();
-  const int tok = tid / SK_ROWS, c = c0 + tid % SK_ROWS;
-  if (tok >= NB * 8 || tok >= a.n || c >= a.N) return;
-  int sum = 0;
+  const int c = c0 + tid % SK_ROWS;
+  if (c >= a.N) return;
+  const float w_scale = a.w_scale[c];
 #pragma unroll
-  for (int w = 0; w < SK_WARPS; ++w) sum += sums[w][tok][tid % SK_ROWS];
-  float y = (float)sum * a.x_scale[tok] * a.w_scale[c];
-  if (a.res) y += to_float(static_cast<const T*>(a.res)[(size_t)tok * a.res_sr + c]);
-  static_cast<T*>(a.out)[(size_t)tok * a.out_sr + c] = from_float<T>(y);
+  for (int at = tid / SK_ROWS; at < NB * 8; at += SK_THREADS / SK_ROWS) {
+    const int tok = t0 + at;
+    if (tok >= a.n) return;
+    int sum = 0;
+#pragma unroll
+    for (int w = 0; w < SK_WARPS; ++w) sum += sums[w][at][tid % SK_ROWS];
+    float y = (float)sum * a.x_scale[tok] * w_scale;
+    if (a.res) y += to_float(static_cast<const T*>(a.res)[(size_t)tok * a.res_sr + c]);
+    static_cast<T*>(a.out)[(size_t)tok * a.out_sr + c] = from_float<T>(y);
+  }
 }
 
-// ---- up to 128 tokens: tiles of 128 channels x BN tokens on tcgen05 ---------------------------------------------------------
-// Still a stream of the weights.  Of the tiles every CTA has as many whole ones as all can have.  The chunks (128 bytes of
-// K) of those left over form one list that is cut into equal pieces, one per CTA, which a CTA works on first: the integer
-// sums of a tile that several CTAs share go to the workspace, the one that arrives last adds them up, and all that happens
-// under the stream of the whole tiles.
+// ---- up to 128 tokens of a large matrix: tiles of 128 channels x BN tokens on tcgen05 ----------------------------------------
+// Still a stream of the weights.  Of the tiles every CTA has as many whole ones as all can have.  Where it pays (share_tiles
+// below) the chunks (128 bytes of K) of those left over form one list that is cut into equal pieces, at most one per CTA,
+// which a CTA works on first: the integer sums of a tile that several CTAs share go to the workspace, the one that arrives
+// last adds them up, and all that happens under the stream of the whole tiles.
 // Warp 4 fetches 128-byte wide boxes of weights and tokens (TMA, 128-byte swizzle), warp 5 issues the MMAs (K = 32 bytes
 // each), int32 accumulators in tensor memory, two of them so that the epilogue of a tile runs under the next tile's MMAs.
 // Warps 0-3 read a tile back: thread = channel (TMEM lane), columns = tokens, so a warp's store is 32 neighbouring channels
@@ -206,17 +217,18 @@ __device__ __forceinline__ void tmem_ld16i(unsigned taddr, int (&r)[16]) {
       : "r"(taddr));
 }
 __device__ __forceinline__ void epilogue_bar() { asm volatile("bar.sync 1, 128;\n" ::: "memory"); }
-__device__ __forceinline__ bool epilogue_any(bool pred) {  // OR over the 128 epilogue threads
+template <int THREADS>
+__device__ __forceinline__ bool epilogue_any(bool pred) {  // OR over the epilogue threads
   unsigned r;
   asm volatile(
       "{\n"
       ".reg .pred p, q;\n"
       "setp.ne.b32 p, %1, 0;\n"
-      "barrier.cta.red.or.pred q, 1, 128, p;\n"
+      "barrier.cta.red.or.pred q, 1, %2, p;\n"
       "selp.u32 %0, 1, 0, q;\n"
       "}\n"
       : "=r"(r)
-      : "r"((unsigned)pred)
+      : "r"((unsigned)pred), "n"(THREADS)
       : "memory");
   return r != 0;
 }
@@ -394,7 +406,7 @@ linear_tile_kernel(const LinArgs a, const __grid_constant__ CUtensorMap tm_w, co
                     a.res_sr, a.out_sr, tokens, in ? a.w_scale[c] : 0.f};
       if (whole) ch.ask(0);
       const bool got = mbar_wait(&sh.acc_full[buf], (n >> 1) & 1, &sh.fail);
-      if (epilogue_any(!got)) {  // the 128 threads leave together
+      if (epilogue_any<128>(!got)) {  // the 128 threads leave together
         if (!sh.fail && a.status) atomicExch(a.status, 7);
         sh.fail = 1;
         break;
@@ -633,18 +645,7 @@ linear_pair_kernel(const LinArgs a, const int BN, const __grid_constant__ CUtens
                     in ? static_cast<T*>(a.out) + (int64_t)t0 * a.out_sr + c : nullptr, a.res_sr, a.out_sr, j_hi, in ? a.w_scale[c] : 0.f};
       ch.ask(j_lo);
       const bool got = mbar_wait(&sh.acc_full[buf], (n >> 1) & 1, &sh.fail);
-      unsigned any;  // the 256 threads leave together
-      asm volatile(
-          "{\n"
-          ".reg .pred p, q;\n"
-          "setp.ne.b32 p, %1, 0;\n"
-          "barrier.cta.red.or.pred q, 1, 256, p;\n"
-          "selp.u32 %0, 1, 0, q;\n"
-          "}\n"
-          : "=r"(any)
-          : "r"((unsigned)!got)
-          : "memory");
-      if (any) {
+      if (epilogue_any<256>(!got)) {  // the 256 threads leave together
         if (!sh.fail && a.status) atomicExch(a.status, 7);
         sh.fail = 1;
         break;
@@ -682,100 +683,352 @@ linear_pair_kernel(const LinArgs a, const int BN, const __grid_constant__ CUtens
   }
 }
 
-// ---- which kernel, and how K is cut -------------------------------------------------------------------------------------
-// Up to 16 tokens: the stream kernel starts and ends sooner, the tile kernel keeps more bytes in flight.  Measured with
-// weights that are not in L2, 16 tokens: 5.3 against 10.6 us for 17 MB, 13.6 against 16.1 for 59 MB, 17.2 against 16.7 for
-// 67 MB, 28.9 against 22.6 for 117 MB (one token: 25.6 against 22.8).
-inline bool is_stream(int n, int N, int K) { return n <= 16 && (long long)N * K <= 1ll << 26; }
-
-struct TilePlan {
-  int BN, token_tiles, tiles, chunks, ctas, shared, sharers;
-  bool pair;
+// ---- few tiles: a cluster of CTAs per tile ------------------------------------------------------------------------------
+// K is cut into as many pieces as the cluster has CTAs.  Behind its MMAs a CTA sends each token's integer sums to the CTA
+// that finishes that token (token j: CTA j mod cluster), straight into its shared memory; one cluster barrier later every
+// CTA adds up what it was sent.  No workspace, no fences over global memory: partial sums by way of L2 and an arrival counter
+// took twice as long (64 x 8192 x 1024: 14.6 us, now 7.1; 128 x 4096 x 4096: 14.8, now 9.5; 77 x 1040 x 1001: 6.4, now 4.2).
+// Warps 0-7 read the sums out (two warps per quarter of the TMEM lanes, alternate groups of 16 tokens), 8 fetches, 9 issues.
+template <int BN>
+struct CkShape {
+  static constexpr int STAGE = (TK_M + BN) * TK_KB;
+  static constexpr int STAGES = BN >= 128 ? 4 : BN >= 64 ? 6 : 8;
+  static constexpr int SUMS = (BN + 8) * TK_M * 4;  // a column more per CTA where the cluster does not divide the columns
+  static constexpr int SMEM = STAGES * STAGE + SUMS + 1024;
 };
-inline TilePlan tile_plan(int n, int N, int K) {
-  TilePlan p;
-  p.shared = p.sharers = 0;
-  p.chunks = ceil_div(K, TK_KB);
-  p.pair = n > 128;
-  if (p.pair) {
-    // The token count whose rounds of tiles over the SM pairs take least.  A round goes by the operands' way from L2 rather
-    // than by its MMAs: measured 10.3, 11.3, 13.0 us for 128, 192, 256 tokens at K = 4096, i.e. in proportion to BN + 360.
-    const int channel_tiles = ceil_div(N, 2 * TK_M);
-    long long best = -1;
-    for (int BN = 256; BN >= 128; BN -= 32) {
-      const long long cost = (long long)ceil_div(channel_tiles * ceil_div(n, BN), TK_CTAS / 2) * (BN + 360);
-      if (best < 0 || cost < best) {
-        best = cost;
-        p.BN = BN;
+struct CkShared {
+  float x_scale[128];
+  uint64_t full[8], empty[8], done;
+  unsigned tmem_base;
+  int fail, issued;
+};
+__device__ __forceinline__ void st_cluster(unsigned addr, int v) {
+  asm volatile("st.shared::cluster.s32 [%0], %1;\n" ::"r"(addr), "r"(v) : "memory");
+}
+
+constexpr int CK_THREADS = 320;
+template <typename T, int BN>
+__global__ void __launch_bounds__(CK_THREADS, 1)
+linear_cluster_kernel(const LinArgs a, const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x) {
+  extern __shared__ __align__(128) unsigned char smem_raw[];
+  __shared__ CkShared sh;
+  constexpr int STAGES = CkShape<BN>::STAGES, STAGE = CkShape<BN>::STAGE;
+  constexpr unsigned TMEM_COLS = BN < 32 ? 32 : BN;
+  unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  int* sums = reinterpret_cast<int*>(ring + STAGES * STAGE);  // [source CTA][this CTA's columns][128]
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int cs = a.cluster, rank = (int)cluster_rank(), unit = blockIdx.x / cs;
+  const int tile = unit / a.token_tiles, t0 = (unit % a.token_tiles) * BN;
+  const int k0 = rank * a.chunks / cs, k1 = (rank + 1) * a.chunks / cs;
+  const int tokens = min(BN, a.n - t0), cols = (tokens + cs - 1) / cs;
+
+  if (tid == 0) {
+    sh.fail = 0;
+    sh.issued = 0;
+    for (int i = 0; i < STAGES; ++i) {
+      mbar_init(&sh.full[i], 1);
+      mbar_init(&sh.empty[i], 1);
+    }
+    mbar_init(&sh.done, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+  }
+  __syncwarp();
+  if (warp == 0) {
+    tmem_alloc(&sh.tmem_base, TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const unsigned tmem = sh.tmem_base;
+  asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");  // this CTA runs: its shared memory may be written
+  pdl_wait();
+  pdl_trigger();
+
+  if (warp == 8) {
+    if (lane == 0) {
+      for (int k = k0, it = 0; k < k1; ++k, ++it) {
+        const int st = it % STAGES;
+        if (!mbar_wait(&sh.empty[st], ((it / STAGES) & 1) ^ 1, &sh.fail)) {
+          if (!sh.fail && a.status) atomicExch(a.status, 7);
+          sh.fail = 1;
+          break;
+        }
+        unsigned char* dst = ring + (size_t)st * STAGE;
+        mbar_expect_tx(&sh.full[st], STAGE);
+        tma_load_2d(dst, &tm_w, k * TK_KB, tile * TK_M, &sh.full[st]);
+        tma_load_2d(dst + TK_M * TK_KB, &tm_x, k * TK_KB, t0, &sh.full[st]);
+        sh.issued = it + 1;
       }
     }
-    p.token_tiles = ceil_div(n, p.BN);
-    p.tiles = channel_tiles * p.token_tiles;
-    p.ctas = 2 * min(TK_CTAS / 2, p.tiles);
-    return p;
-  }
-  p.BN = n <= 16 ? 16 : n <= 32 ? 32 : n <= 64 ? 64 : 128;
-  p.token_tiles = 1;
-  p.tiles = ceil_div(N, TK_M);
-  // Tiles are shared where the SMs would idle for more than eight chunks' time otherwise, about what sharing costs.  Next
-  // to whole tiles in pieces of four chunks at least; where there are only shared tiles in pieces of sixteen, and in pieces
-  // that end with the tiles where that leaves few SMs idle.
-  const int left = p.tiles % TK_CTAS;
-  p.ctas = min(TK_CTAS, p.tiles);
-  if (left && (long long)(TK_CTAS - left) * p.chunks > 8 * TK_CTAS) {
-    p.shared = left;
-    if (p.tiles < TK_CTAS) {
-      p.ctas = (int)min((long long)TK_CTAS, max((long long)p.tiles, (long long)p.tiles * p.chunks / 16));
-      if (p.ctas % p.tiles <= p.ctas / 6) p.ctas -= p.ctas % p.tiles;
-      if (p.ctas == p.tiles) p.shared = 0;
+  } else if (warp == 9) {
+    if (lane == 0) {
+      constexpr unsigned idesc = i8_instr_desc(TK_M, BN);
+      bool ok = true;
+      for (int k = k0, it = 0; k < k1; ++k, ++it) {
+        const int st = it % STAGES;
+        if (!mbar_wait(&sh.full[st], (it / STAGES) & 1, &sh.fail)) { ok = false; break; }
+        tc_fence_after();
+        const unsigned w_base = smem_u32(ring + (size_t)st * STAGE), x_base = w_base + TK_M * TK_KB;
+#pragma unroll
+        for (int j = 0; j < TK_KB / 32; ++j)
+          tc_mma_i8(tmem, smem_desc_sw128(w_base + j * 32), smem_desc_sw128(x_base + j * 32), idesc, (it || j) ? 1u : 0u);
+        tc_commit(&sh.empty[st]);
+      }
+      if (ok) tc_commit(&sh.done);
+      else {
+        if (!sh.fail && a.status) atomicExch(a.status, 7);
+        sh.fail = 1;
+      }
     }
-    p.sharers = p.shared ? (int)min((long long)p.ctas, max(1ll, (long long)p.shared * p.chunks / 4)) : 0;
+  }
+  const int channel = (warp & 3) * 32 + lane, half = (warp >> 2) & 1, c = tile * TK_M + channel;
+  float w_scale = 0.f;
+  if (warp < 8) {
+    if (tid < tokens) sh.x_scale[tid] = a.x_scale[t0 + tid];
+    if (c < a.N) w_scale = a.w_scale[c];
+  }
+  __syncwarp();
+  asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+  if (warp < 8) {
+    const bool got = mbar_wait(&sh.done, 0, &sh.fail);
+    if (epilogue_any<256>(!got)) {
+      if (!sh.fail && a.status) atomicExch(a.status, 7);
+      sh.fail = 1;
+    } else {
+      tc_fence_after();
+      const unsigned mine = smem_u32(sums + (size_t)rank * cols * TK_M + channel);
+      int to = (half * 16) % cs, at = (half * 16) / cs;  // token j goes to CTA j % cs as its column j / cs
+#pragma unroll 1
+      for (int j0 = half * 16; j0 < tokens; j0 += 32) {
+        int v[16];
+        tmem_ld16i(tmem + ((unsigned)((warp & 3) * 32) << 16) + j0, v);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          if (j0 + j < tokens) st_cluster(in_cta(mine + (unsigned)at * (TK_M * 4), to), v[j]);
+          if (++to == cs) to = 0, ++at;
+        }
+        to += 16 % cs, at += 16 / cs;
+        if (to >= cs) to -= cs, ++at;
+      }
+      tc_fence_before();
+    }
+  }
+  __syncwarp();
+  cluster_sync_all();  // the sums of every CTA are where they are added up
+  if (warp < 8 && c < a.N) {
+    const T* res = static_cast<const T*>(a.res) + (int64_t)t0 * a.res_sr + c;
+    T* out = static_cast<T*>(a.out) + (int64_t)t0 * a.out_sr + c;
+    constexpr int U = 8;
+#pragma unroll 1
+    for (int i0 = half * U; rank + i0 * cs < tokens; i0 += 2 * U) {
+      int sum[U];
+      T r[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        sum[u] = 0;
+        if (a.res) r[u] = res[(int64_t)min(rank + (i0 + u) * cs, tokens - 1) * a.res_sr];
+      }
+      const int* from = sums + (size_t)i0 * TK_M + channel;
+#pragma unroll 2
+      for (int q = 0; q < cs; ++q, from += (size_t)cols * TK_M)
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (i0 + u < cols) sum[u] += from[u * TK_M];
+      float y[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int j = min(rank + (i0 + u) * cs, tokens - 1);
+        y[u] = (float)sum[u] * sh.x_scale[j] * w_scale;
+        if (a.res) y[u] += to_float(r[u]);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int j = rank + (i0 + u) * cs;
+        if (j < tokens) out[(int64_t)j * a.out_sr] = from_float<T>(y[u]);
+      }
+    }
+  }
+  __syncthreads();
+  if (sh.fail) {
+    if (tid == 256)
+      for (int st = 0; st < STAGES; ++st) {
+        const int last = sh.issued - 1 - ((sh.issued - 1 - st) % STAGES + STAGES) % STAGES;
+        if (sh.issued > st && last >= 0) mbar_wait(&sh.full[st], (last / STAGES) & 1);
+      }
+    __syncthreads();
+  }
+  if (warp == 0) {
+    tc_fence_after();
+    tmem_dealloc(tmem, TMEM_COLS);
+  }
+}
+
+// ---- which kernel -----------------------------------------------------------------------------------------------------------
+// The one whose estimated time is least.  The estimates are linear fits (in ns) to times measured with weights that are not
+// in L2, 1 to 512 tokens, 300 to 28672 channels, K = 512 to 14336, right to 4-6 % on average.  Both sides at some borders, us:
+//   stream against a cluster   16 x 4096 x 4096: 5.5, 7.1   64 x 4096 x 2048: 7.2, 6.7   1 x 14336 x 4096: 15.4, 13.1
+//   cluster against tiles      64 x 4096 x 6144: 10.1, 13.0   64 x 1024 x 8192: 6.7, 6.1
+//   stream against tiles       16 x 4096 x 14336: 17.3, 13.3   1 x 1024 x 8192: 3.6, 5.6
+//   cluster against pairs      256 x 8192 x 1024: 9.4, 22.6   512 x 1024 x 2048: 7.9, 6.4
+enum LinearKind { kStreamKernel, kTileKernel, kClusterKernel, kPairKernel };
+struct LinearPlan {
+  LinearKind kind;
+  int tokens, token_tiles;  // of a CTA (stream) or a tile, and how many of them
+  int tiles, ctas, chunks;  // tiles of both directions; CTAs; 128-byte steps of K
+  int cluster;              // CTAs per tile
+  int shared, sharers;      // tile kernel: see LinArgs
+};
+// Tile kernel: into how many pieces the tiles left over behind whole rounds are cut (0: none, they are a round of their own),
+// and what that saves (ns).  m pieces per tile save 1 - 1/m of a round and cost m partials' stores and additions; pieces
+// that end inside tiles, where there are too many tiles for two each, cost more.  Measured, us without and with: 16 x 4096 x
+// 19000 (149 tiles) 23.5, 16.8; 16 x 4096 x 28672 (224) 24.8, 22.8; 128 x 4096 x 28672 27.8, 34.4 (hence whole).
+struct Sharing {
+  int pieces;
+  double saves;
+};
+inline Sharing share_tiles(int n, long long tiles, long long chunks) {
+  const int left = (int)(tiles % TK_CTAS);
+  Sharing best = {0, 0.0};
+  if (tiles <= TK_CTAS || !left) return best;
+  for (int m = 2; m <= 6 && m * left <= TK_CTAS && m <= chunks; ++m) {
+    const double saves = 420.0 * chunks * (m - 1) / m - m * (450 + 18 * n);
+    if (saves > best.saves) best = Sharing{m * left, saves};
+  }
+  const double saves = 420.0 * chunks * (TK_CTAS - left) / TK_CTAS - 4000 - 70 * n;
+  if (2 * left > TK_CTAS && saves > best.saves) best = Sharing{TK_CTAS, saves};
+  return best;
+}
+inline LinearPlan linear_plan(int n, int N, int K) {
+  const long long chunks = ceil_div(K, TK_KB), channel_tiles = ceil_div(N, TK_M);
+  const double mega = ((double)N + n) * K * 1e-6;  // operand bytes
+  LinearPlan p = {};
+  double best = 1e300;
+  const auto offer = [&](double ns, LinearKind kind, int tokens, int cluster) {
+    if (ns >= best) return;
+    best = ns;
+    p.kind = kind;
+    p.tokens = tokens;
+    p.cluster = cluster;
+  };
+  // Stream, 8, 16 or 32 tokens per CTA: start, the bytes that an SM with the most CTAs fetches, CTAs, bytes of weights.
+  static constexpr double kStream[3][4] = {{1450, 12.6, 272, 53}, {1430, 10.4, 584, 42}, {1880, 11.1, 738, 13}};
+  for (int i = 0; i < 3 && n <= 128; ++i) {
+    const int tokens = 8 << i;
+    if (i && n <= tokens / 2) break;
+    const double ctas = (double)ceil_div(N, SK_ROWS) * ceil_div(n, tokens);
+    offer(kStream[i][0] + kStream[i][1] * std::ceil(ctas / TK_CTAS) * K * 1e-3 * (SK_ROWS + tokens) + kStream[i][2] * ctas / TK_CTAS +
+              kStream[i][3] * N * 1e-6 * K, kStreamKernel, tokens, 1);
+  }
+  // Tiles: start, tokens read out, rounds (by a CTA's operands from L2, or by all weights from HBM).
+  if (n <= 128) {
+    const int BN = n <= 16 ? 16 : n <= 32 ? 32 : n <= 64 ? 64 : 128;
+    const double whole = channel_tiles / TK_CTAS, rest = channel_tiles % TK_CTAS ? 1 : 0;
+    offer(3400 + 11.3 * n + chunks * (whole * std::max(1.25 * (TK_M + BN), 370.0) + rest * std::max(1.25 * (TK_M + BN), 270.0)) -
+              share_tiles(n, channel_tiles, chunks).saves, kTileKernel, BN, 1);
+  }
+  // Clusters, as many as can run at once: start, tokens read out and added up, the operands of a CTA, of all, the sums sent.
+  static constexpr int kCluster[5][2] = {{2, 74}, {3, 45}, {4, 33}, {6, 22}, {8, 15}};  // CTAs, clusters
+  for (int BN = 16; BN <= 128 && (BN == 16 || n > BN / 2); BN *= 2) {
+    const long long units = channel_tiles * ceil_div(n, BN);
+    for (const auto& c : kCluster) {
+      if (units > c[1] || c[0] > chunks) break;
+      const int tokens = min(n, BN);
+      offer(3180 + 8.6 * tokens + 16.9 * tokens / c[0] + 1.255 * ((chunks + c[0] - 1) / c[0]) * (TK_M + BN) + 82.6 * mega +
+                0.0586 * units * c[0] * tokens, kClusterKernel, BN, c[0]);
+    }
+  }
+  // Pairs: the token count whose rounds of tiles over the SM pairs take least.  A round goes by the operands' way from L2
+  // rather than by its MMAs: measured 10.3, 11.3, 13.0 us for 128, 192, 256 tokens at K = 4096.
+  for (int BN = 256; BN >= 32 && n > 16; BN -= 32) {
+    const double units = std::ceil(channel_tiles / 2.0) * ceil_div(n, BN);
+    const double round = chunks * (BN >= 128 ? 0.586 * BN + 211 : 0.16 * BN + 266);
+    offer(3380 + std::max(std::ceil(units / (TK_CTAS / 2)) * round, 170 * mega) + 5.6 * BN + 22 * mega, kPairKernel, BN, 2);
+  }
+  p.chunks = (int)chunks;
+  p.token_tiles = ceil_div(n, p.tokens);
+  const long long tiles = p.kind == kPairKernel ? (channel_tiles + 1) / 2 * p.token_tiles : channel_tiles * p.token_tiles;
+  p.tiles = (int)std::min<long long>(tiles, 0x7fffffff);
+  switch (p.kind) {
+    case kStreamKernel: break;  // a grid of its own
+    case kClusterKernel: p.ctas = p.tiles * p.cluster; break;
+    case kPairKernel: p.ctas = 2 * min(TK_CTAS / 2, p.tiles); break;
+    case kTileKernel:
+      p.ctas = min(TK_CTAS, p.tiles);
+      p.sharers = share_tiles(n, p.tiles, chunks).pieces;
+      if (p.sharers) p.shared = p.tiles % TK_CTAS;
   }
   return p;
 }
-inline size_t tile_workspace(const TilePlan& p) {
-  return p.shared ? 1024 + (size_t)(p.sharers + p.shared) * p.BN * TK_M * sizeof(int) : 0;
+inline size_t linear_workspace(const LinearPlan& p) {
+  return p.shared ? 1024 + (size_t)(p.sharers + p.shared) * p.tokens * TK_M * sizeof(int) : 0;
 }
 
 inline bool bad16(const void* p) { return !p || (reinterpret_cast<uintptr_t>(p) & 15); }
 
 template <typename T, int BN>
-int launch_tile(const LinArgs& a, const TilePlan& pl, cudaStream_t st) {
+int launch_tile(const LinArgs& a, const LinearPlan& pl, const CUtensorMap& tm_w, const CUtensorMap& tm_x, cudaStream_t st) {
   static std::atomic<unsigned long long> done{0};
   auto kern = linear_tile_kernel<T, BN>;
   if (const int rc = allow_smem(kern, TkShape<BN>::SMEM, done)) return rc;
-  CUtensorMap tm_w, tm_x;
-  if (!make_bytes_tensor_map(&tm_w, a.w, a.N, a.K, a.w_sr, TK_M) || !make_bytes_tensor_map(&tm_x, a.x, a.n, a.K, a.x_sr, BN))
-    return OMNIKV_E_UNSUPPORTED;
   OMNIKV_CUDA_OK(launch_pdl_smem_args(kern, dim3(pl.ctas), dim3(TK_THREADS), TkShape<BN>::SMEM, st, a, tm_w, tm_x));
   return OMNIKV_OK;
 }
 
+template <typename T, int BN>
+int launch_cluster(const LinArgs& a, const LinearPlan& pl, const CUtensorMap& tm_w, const CUtensorMap& tm_x, cudaStream_t st) {
+  static std::atomic<unsigned long long> done{0};
+  auto kern = linear_cluster_kernel<T, BN>;
+  if (const int rc = allow_smem(kern, CkShape<BN>::SMEM, done)) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(pl.ctas);
+  cfg.blockDim = dim3(CK_THREADS);
+  cfg.dynamicSmemBytes = CkShape<BN>::SMEM;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = pl.cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  OMNIKV_CUDA_OK(cudaLaunchKernelEx(&cfg, kern, a, tm_w, tm_x));
+  return OMNIKV_OK;
+}
+
+template <typename T, int BN>
+int launch_single(const LinArgs& a, const LinearPlan& pl, const CUtensorMap& tm_w, const CUtensorMap& tm_x, cudaStream_t st) {
+  return pl.kind == kClusterKernel ? launch_cluster<T, BN>(a, pl, tm_w, tm_x, st) : launch_tile<T, BN>(a, pl, tm_w, tm_x, st);
+}
+
 template <typename T>
-int launch_pair(const LinArgs& a, const TilePlan& pl, cudaStream_t st) {
+int launch_pair(const LinArgs& a, const LinearPlan& pl, const CUtensorMap& tm_w, const CUtensorMap& tm_x, cudaStream_t st) {
   static std::atomic<unsigned long long> done{0};
   auto kern = linear_pair_kernel<T>;
   if (const int rc = allow_smem(kern, PK_SMEM, done)) return rc;
-  CUtensorMap tm_w, tm_x;
-  if (!make_bytes_tensor_map(&tm_w, a.w, a.N, a.K, a.w_sr, TK_M) || !make_bytes_tensor_map(&tm_x, a.x, a.n, a.K, a.x_sr, pl.BN / 2))
-    return OMNIKV_E_UNSUPPORTED;
-  OMNIKV_CUDA_OK(launch_pdl_smem_args(kern, dim3(pl.ctas), dim3(PK_THREADS), PK_SMEM, st, a, pl.BN, tm_w, tm_x));
+  OMNIKV_CUDA_OK(launch_pdl_smem_args(kern, dim3(pl.ctas), dim3(PK_THREADS), PK_SMEM, st, a, pl.tokens, tm_w, tm_x));
   return OMNIKV_OK;
 }
 
 template <typename T>
-int launch_linear(const LinArgs& a, const TilePlan& pl, cudaStream_t st) {
-  if (is_stream(a.n, a.N, a.K)) {
-    auto kern = a.n <= 8 ? linear_stream_kernel<T, 1> : linear_stream_kernel<T, 2>;
-    OMNIKV_CUDA_OK(launch_pdl(kern, dim3(ceil_div(a.N, SK_ROWS)), dim3(SK_THREADS), 0, st, a));
+int launch_linear(const LinArgs& a, const LinearPlan& pl, cudaStream_t st) {
+  if (pl.kind == kStreamKernel) {
+    auto kern = pl.tokens == 8 ? linear_stream_kernel<T, 1> : pl.tokens == 16 ? linear_stream_kernel<T, 2> : linear_stream_kernel<T, 4>;
+    OMNIKV_CUDA_OK(launch_pdl(kern, dim3(ceil_div(a.N, SK_ROWS), pl.token_tiles), dim3(SK_THREADS), 0, st, a));
     return OMNIKV_OK;
   }
-  if (pl.pair) return launch_pair<T>(a, pl, st);
-  switch (pl.BN) {
-    case 16: return launch_tile<T, 16>(a, pl, st);
-    case 32: return launch_tile<T, 32>(a, pl, st);
-    case 64: return launch_tile<T, 64>(a, pl, st);
-    default: return launch_tile<T, 128>(a, pl, st);
+  CUtensorMap tm_w, tm_x;
+  if (!make_bytes_tensor_map(&tm_w, a.w, a.N, a.K, a.w_sr, TK_M) ||
+      !make_bytes_tensor_map(&tm_x, a.x, a.n, a.K, a.x_sr, pl.kind == kPairKernel ? pl.tokens / 2 : pl.tokens))
+    return OMNIKV_E_UNSUPPORTED;
+  if (pl.kind == kPairKernel) return launch_pair<T>(a, pl, tm_w, tm_x, st);
+  switch (pl.tokens) {
+    case 16: return launch_single<T, 16>(a, pl, tm_w, tm_x, st);
+    case 32: return launch_single<T, 32>(a, pl, tm_w, tm_x, st);
+    case 64: return launch_single<T, 64>(a, pl, tm_w, tm_x, st);
+    default: return launch_single<T, 128>(a, pl, tm_w, tm_x, st);
   }
 }
 
@@ -807,8 +1060,8 @@ extern "C" int omnikv_quant_rows(int dtype, const void* x, int64_t x_stride_row,
 
 extern "C" size_t omnikv_linear_w8a8_workspace_bytes(int n_tokens, int channels, int K) {
   using namespace omnikv;
-  if (n_tokens <= 0 || channels <= 0 || K <= 0 || is_stream(n_tokens, channels, K)) return 0;
-  return tile_workspace(tile_plan(n_tokens, channels, K));
+  if (n_tokens <= 0 || channels <= 0 || K <= 0) return 0;
+  return linear_workspace(linear_plan(n_tokens, channels, K));
 }
 
 extern "C" int omnikv_linear_w8a8(const omnikv_linear_w8a8_params* p, void* stream) {
@@ -820,9 +1073,9 @@ extern "C" int omnikv_linear_w8a8(const omnikv_linear_w8a8_params* p, void* stre
   if (p->K > 32768 || (p->out_dtype != OMNIKV_F32 && !is_16bit(p->out_dtype))) return OMNIKV_E_UNSUPPORTED;
   LinArgs a{p->x, p->x_stride_row, p->x_scale, p->w, p->w_stride_row, p->w_scale, p->residual, p->residual_stride_row,
             p->out, p->out_stride_row, p->n_tokens, p->channels, p->K};
-  const TilePlan pl = tile_plan(a.n, a.N, a.K);
-  if ((long long)pl.tiles * pl.chunks > 0x7fffffff) return OMNIKV_E_UNSUPPORTED;
-  const size_t need = is_stream(a.n, a.N, a.K) ? 0 : tile_workspace(pl);
+  const LinearPlan pl = linear_plan(a.n, a.N, a.K);
+  if (pl.tiles == 0x7fffffff) return OMNIKV_E_UNSUPPORTED;  // tiles are counted in 32 bits
+  const size_t need = linear_workspace(pl);
   if (need && (!p->workspace || p->workspace_bytes < need)) return OMNIKV_E_WORKSPACE;
   if (need && bad16(p->workspace)) return OMNIKV_E_BADARG;
   a.counters = static_cast<int*>(p->workspace);
@@ -832,6 +1085,7 @@ extern "C" int omnikv_linear_w8a8(const omnikv_linear_w8a8_params* p, void* stre
   a.shared = pl.shared;
   a.sharers = pl.sharers;
   a.chunks = pl.chunks;
+  a.cluster = pl.cluster;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   switch (p->out_dtype) {
     case OMNIKV_F32: return launch_linear<float>(a, pl, st);

@@ -74,7 +74,8 @@ def test_workspace_sizes():
     assert lib.omnikv_kv8_attn_workspace_bytes(3, 16, 2, 700) == 16384 + (700 + 6) * 8 * 528
     assert lib.omnikv_kv8_attn_workspace_bytes(1, 30, 8, 4) == 0
     assert lib.omnikv_linear_w8a8_workspace_bytes(16, 512, 14336) == 0  # a stream of the weights
-    assert lib.omnikv_linear_w8a8_workspace_bytes(17, 512, 14336) > 0   # CTAs share tiles
+    assert lib.omnikv_linear_w8a8_workspace_bytes(17, 512, 14336) == 0  # a cluster per tile
+    assert lib.omnikv_linear_w8a8_workspace_bytes(17, 28672, 4096) > 0  # CTAs share what is left behind whole tiles
     assert lib.omnikv_linear_w8a8_workspace_bytes(200, 512, 14336) == 0
 
 

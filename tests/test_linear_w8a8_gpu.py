@@ -87,7 +87,9 @@ def test_quant_rows_of_extreme_values():
 @pytest.mark.parametrize("n,N,K", [
     (1, 1, 16), (1, 6144, 4096), (2, 1000, 32), (7, 129, 4096), (8, 256, 128), (9, 64, 272), (16, 4096, 1040), (17, 33, 14336),
     (33, 700, 96), (64, 512, 512), (65, 1001, 2064), (77, 1001, 1040), (128, 256, 4096), (129, 257, 144), (200, 3000, 64),
-    (513, 640, 1024), (1000, 1024, 4096), (1, 16411, 4112), (16, 16411, 4112), (40, 19000, 1040), (100, 37900, 144)])
+    (513, 640, 1024), (1000, 1024, 4096), (1, 16411, 4112), (16, 16411, 4112), (40, 19000, 1040), (100, 37900, 144),
+    (24, 500, 4096), (31, 3000, 8192), (64, 1024, 8192), (90, 2048, 2064), (128, 4096, 4096), (130, 130, 8208), (200, 1001, 1040),
+    (256, 1024, 8192), (300, 4000, 14336), (500, 300, 4096), (16, 4096, 14336), (1, 4096, 14336), (5, 13, 32768), (100, 10241, 1040)])
 def test_linear(out_dtype, n, N, K):
     ops_ = operands(n, N, K, seed=n + N + K)
     check(ops().linear_w8a8(*ops_, out_dtype=out_dtype), *ops_)
@@ -159,7 +161,7 @@ def test_repeated_and_captured_calls_agree(n):
     assert all(torch.equal(got, want) for _, got in graphs)
 
 
-@pytest.mark.parametrize("N,K", [(1024, 8192), (18944 + 300, 1040)])  # tiles that CTAs share, alone and next to whole ones
+@pytest.mark.parametrize("N,K", [(1024, 8192), (18944 + 300, 1040)])  # a cluster per tile; tiles that CTAs share next to whole ones
 def test_shared_tiles_on_two_streams_and_in_graphs(N, K):
     n = 40
     x8, sx, w8, sw = operands(n, N, K)
