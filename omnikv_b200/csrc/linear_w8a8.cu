@@ -687,7 +687,7 @@ linear_pair_kernel(const LinArgs a, const int BN, const __grid_constant__ CUtens
 // K is cut into as many pieces as the cluster has CTAs.  Behind its MMAs a CTA sends each token's integer sums to the CTA
 // that finishes that token (token j: CTA j mod cluster), straight into its shared memory; one cluster barrier later every
 // CTA adds up what it was sent.  No workspace, no fences over global memory: partial sums by way of L2 and an arrival counter
-// took twice as long (64 x 8192 x 1024: 14.6 us, now 7.1; 128 x 4096 x 4096: 14.8, now 9.5; 77 x 1040 x 1001: 6.4, now 4.2).
+// took twice as long (64 x 8192 x 1024: 14.6 us, now 7.1; 128 x 4096 x 4096: 14.8, now 9.5; 256 x 8192 x 1024: 22.6, now 9.4).
 // Warps 0-7 read the sums out (two warps per quarter of the TMEM lanes, alternate groups of 16 tokens), 8 fetches, 9 issues.
 template <int BN>
 struct CkShape {
