@@ -288,10 +288,10 @@ PyObject* kv8_decode_attn(PyObject* const* a) {
     p.score_stride = score->size(2);
     p.score_len = ints(score_len, B, "score_len");
   }
-  // one CTA per SM; fewer when there are fewer (sequence, KV head) pairs and not a tile of 32 rows for each of twelve warps
+  // one CTA per SM; fewer when there are fewer (sequence, KV head) pairs and not three tiles of 32 rows for each
   const Device& d = device(dev);
   if (a[14] != Py_None) cap = integer(a[14]);
-  const int64_t per = a[13] != Py_None ? integer(a[13]) : std::clamp<int64_t>(cap / 384, 0, d.sms) + 1;
+  const int64_t per = a[13] != Py_None ? integer(a[13]) : std::clamp<int64_t>(cap / 96, 0, d.sms) + 1;
   const int64_t segments = B * KVH;
   if (per < 1 || per > 32768 || segments < 1 || segments > 32768 || (a[13] != Py_None && per * segments > 32768))
     refuse("kv8_decode_attn: n_splits x B x KVH must lie in 1..32768");

@@ -138,6 +138,24 @@ __device__ __forceinline__ unsigned abs_bits_of(unsigned m2) {
   else return m << 16;
 }
 
+// Thread-block clusters: this CTA's rank, a shared-memory address in CTA `rank`, and the barrier of all threads in two halves.
+__device__ __forceinline__ unsigned cluster_rank() {
+  unsigned r;
+  asm volatile("mov.u32 %0, %cluster_ctarank;\n" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ unsigned in_cta(unsigned addr, unsigned rank) {
+  unsigned r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory"); }
+__device__ __forceinline__ void cluster_sync_all() {
+  cluster_arrive();
+  cluster_wait();
+}
+
 // Host: an omnikv_kv8_cache that the kernels can read.
 inline int check_kv8_cache(const omnikv_kv8_cache* c) {
   const auto bad16 = [](const void* p) { return !p || (reinterpret_cast<uintptr_t>(p) & 15); };
@@ -163,14 +181,15 @@ bool make_kv8_tensor_map(CUtensorMap* map, const void* base, int64_t rows, int K
 // Tensor map over a row-major matrix of bytes: box 128 bytes x box_rows rows, 128-byte swizzle, zeros past its edges.
 bool make_bytes_tensor_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t ld, int box_rows);
 
-// cudaFuncSetAttribute once per kernel and device.
+// cudaFuncSetAttribute once per kernel and device (large_cluster: more than eight CTAs to a cluster, too).
 template <typename Kern>
-int allow_smem(Kern kern, int bytes, std::atomic<unsigned long long>& done) {
+int allow_smem(Kern kern, int bytes, std::atomic<unsigned long long>& done, bool large_cluster = false) {
   int dev = 0;
   OMNIKV_CUDA_OK(cudaGetDevice(&dev));
   const unsigned long long bit = 1ull << (dev & 63);
   if (done.load(std::memory_order_acquire) & bit) return OMNIKV_OK;
   OMNIKV_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  if (large_cluster) OMNIKV_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
   done.fetch_or(bit, std::memory_order_release);
   return OMNIKV_OK;
 }

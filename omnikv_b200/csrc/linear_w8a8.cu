@@ -503,19 +503,6 @@ linear_tile_kernel(const LinArgs a, const __grid_constant__ CUtensorMap tm_w, co
 // that the last round of tiles is nearly full.  Eight epilogue warps: two per quarter of the TMEM lanes, half of the tokens each.
 constexpr int PK_THREADS = 320, PK_STAGES = 6, PK_HALF = 128 * TK_KB, PK_STAGE = 2 * PK_HALF, PK_SMEM = PK_STAGES * PK_STAGE + 1024;
 
-__device__ __forceinline__ unsigned cluster_rank() {
-  unsigned r;
-  asm volatile("mov.u32 %0, %cluster_ctarank;\n" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ unsigned in_cta(unsigned addr, unsigned rank) {  // a shared-memory address in CTA `rank` of the cluster
-  unsigned r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(r) : "r"(addr), "r"(rank));
-  return r;
-}
-__device__ __forceinline__ void cluster_sync_all() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
-}
 __device__ __forceinline__ void pair_load(void* dst, const CUtensorMap* map, int col, int row, unsigned bar_cluster) {
   asm volatile(
       "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], [%4];\n" ::
@@ -741,7 +728,7 @@ linear_cluster_kernel(const LinArgs a, const __grid_constant__ CUtensorMap tm_w,
   __syncthreads();
   tc_fence_after();
   const unsigned tmem = sh.tmem_base;
-  asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");  // this CTA runs: its shared memory may be written
+  cluster_arrive();  // this CTA runs: its shared memory may be written
   pdl_wait();
   pdl_trigger();
 
@@ -789,7 +776,7 @@ linear_cluster_kernel(const LinArgs a, const __grid_constant__ CUtensorMap tm_w,
     if (c < a.N) w_scale = a.w_scale[c];
   }
   __syncwarp();
-  asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+  cluster_wait();
   if (warp < 8) {
     const bool got = mbar_wait(&sh.done, 0, &sh.fail);
     if (epilogue_any<256>(!got)) {

@@ -286,6 +286,31 @@ def test_selected_rows_and_tail(fmt, tokens_first, H, KVH, P, counts, tails, spl
     check_attention(no_tail, q, k, v, lists)
 
 
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("splits", [2, 3, 5, 7, 8, 9, 10, 13, 16, None])
+def test_one_to_sixteen_ctas_per_head(fmt, splits):
+    """A cluster of `splits` CTAs per (sequence, KV head) merges its partials, however many rows each of them gets."""
+    for B, KVH, G, lens in ((1, 1, 8, [1537]), (2, 1, 3, [70, 1500]), (1, 2, 5, [33]), (3, 1, 1, [0, 1, 1537]), (1, 7, 7, [1100])):
+        H, rows = KVH * G, 1537
+        cache, k, v = filled(B, KVH, rows, fmt, torch.float16, 64, 31)
+        q = draw((B, H, D), torch.float16, 32, outliers=False) * 2
+        score = torch.full((KVH, B, rows), 123.0, device="cuda")
+        out = ops().kv8_decode_attn(q, *cache, i32(lens), block=64, n_splits=splits, score_out=score, score_len=i32(lens))
+        check_attention(out, q, k, v, [list(range(n)) for n in lens])
+        for b in range(B):
+            _, _, logits, size = ko.attention(q[b].double(), k[b], v[b], list(range(lens[b])))
+            want = logits.view(KVH, G, -1).amax(1) if lens[b] else logits.new_zeros(KVH, 0)
+            assert ((score[:, b, :lens[b]].double() - want).abs() <= 2.0 ** -17 * size).all()
+            assert (score[:, b, lens[b]:] == 123.0).all()
+        idx = torch.randperm(rows, device="cuda")[:1200].int().expand(B, -1)
+        counts, tails = [min(n, 1200) for n in lens], [n % 50 for n in lens]
+        got = ops().kv8_decode_attn(q, *cache, i32(counts), block=64, n_splits=splits, idx=idx, tail_start=i32([100] * B), tail_len=i32(tails))
+        rows_of = [idx[0, :c].tolist() + list(range(100, 100 + t)) for c, t in zip(counts, tails)]
+        check_attention(got, q, k, v, rows_of)
+        assert torch.equal(got, ops().kv8_decode_attn(q, *cache, i32(counts), block=64, n_splits=splits, idx=idx,
+                                                       tail_start=i32([100] * B), tail_len=i32(tails)))
+
+
 def test_rows_outside_the_cache_count_as_none():
     """An index list with entries outside the cache, lengths and tails that reach past it: the rows that exist are used."""
     B, H, KVH, rows, block = 2, 8, 2, 100, 16
