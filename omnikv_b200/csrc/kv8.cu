@@ -21,11 +21,11 @@ inline Kv8View view_of(const omnikv_kv8_cache* c) {
 }
 
 // ---- store ------------------------------------------------------------------------------------------------------
-// A CTA takes 128 rows (256 where a scale block is that long) of one (sequence, head) of K or V: sixteen lanes hold a row,
-// eight elements each, in registers between the two steps (maximum of the block, codes), so every element is read once.
-// One thread per scale block turns its maximum into the rule for its codes: the divisions that takes were a third of the
-// instructions when every thread did it (131072 rows of 8 heads: 149 -> 123 us).
-constexpr int ST_THREADS = 256, ST_ROWS = ST_THREADS / 16;
+// A CTA takes 128 rows (256, and twice the threads, where a scale block is that long: 179 -> 140 us for 131072 rows of 8 heads
+// against twice the rows per thread) of one (sequence, head) of K or V: sixteen lanes hold a row, eight elements each, in
+// registers between the two steps (maximum of the block, codes), so every element is read once.  One thread per scale block
+// turns its maximum into the rule for its codes: the divisions that takes were a third of the instructions when every thread
+// did it (131072 rows of 8 heads, one tensor as K and V: 149 -> 123 us; two tensors: 128 us, 123 at the copy rate).
 
 struct StoreArgs {
   Kv8View c;
@@ -35,10 +35,11 @@ struct StoreArgs {
   const int* lens;
 };
 
-// PPB: passes of 16 rows per scale block; 0: blocks shorter than a pass.
-template <typename T, int FMT, int PASSES, int PPB>
+// PPB: passes of THREADS / 16 rows per scale block; 0: blocks shorter than a pass.
+constexpr int kStorePasses = 8;
+template <typename T, int FMT, int ST_THREADS, int PPB>
 __global__ void __launch_bounds__(ST_THREADS) kv8_store_kernel(const StoreArgs a) {
-  constexpr int R = PASSES * ST_ROWS, WARPS = ST_THREADS / 32, BLOCKS = PPB ? PASSES / PPB : R;
+  constexpr int PASSES = kStorePasses, ST_ROWS = ST_THREADS / 16, R = PASSES * ST_ROWS, WARPS = ST_THREADS / 32, BLOCKS = PPB ? PASSES / PPB : R;
   __shared__ unsigned top[BLOCKS][PPB ? WARPS : 1];  // largest magnitude of each scale block, by warp
   __shared__ float2 rules[BLOCKS];
   pdl_wait();
@@ -216,17 +217,17 @@ __global__ void __launch_bounds__(LD_THREADS) kv8_load_kernel(const Kv8View c, i
 
 template <typename T, int FMT>
 int launch_store(const StoreArgs& a, int B, cudaStream_t st) {
-  const auto go = [&](auto kern, int rows) -> int {
-    OMNIKV_CUDA_OK(launch_pdl(kern, dim3(ceil_div(a.n, rows), 2 * a.KVH, B), dim3(ST_THREADS), 0, st, a));
+  const auto go = [&](auto kern, int threads) -> int {
+    OMNIKV_CUDA_OK(launch_pdl(kern, dim3(ceil_div(a.n, kStorePasses * threads / 16), 2 * a.KVH, B), dim3(threads), 0, st, a));
     return OMNIKV_OK;
   };
   switch (a.c.block) {
-    case 16: return go(kv8_store_kernel<T, FMT, 8, 1>, 128);
-    case 32: return go(kv8_store_kernel<T, FMT, 8, 2>, 128);
-    case 64: return go(kv8_store_kernel<T, FMT, 8, 4>, 128);
-    case 128: return go(kv8_store_kernel<T, FMT, 8, 8>, 128);
-    case 256: return go(kv8_store_kernel<T, FMT, 16, 16>, 256);
-    default: return go(kv8_store_kernel<T, FMT, 8, 0>, 128);
+    case 16: return go(kv8_store_kernel<T, FMT, 256, 1>, 256);
+    case 32: return go(kv8_store_kernel<T, FMT, 256, 2>, 256);
+    case 64: return go(kv8_store_kernel<T, FMT, 256, 4>, 256);
+    case 128: return go(kv8_store_kernel<T, FMT, 256, 8>, 256);
+    case 256: return go(kv8_store_kernel<T, FMT, 512, 8>, 512);
+    default: return go(kv8_store_kernel<T, FMT, 256, 0>, 256);
   }
 }
 

@@ -39,9 +39,9 @@ __device__ __forceinline__ float code_value(unsigned byte) {
 // with X < 2^11; e4m3: 2^-16), so the rounded fp32 quotient lies on the true side and the code is that of exact arithmetic.
 // (top x could overflow for a >= 2^64: both sides are scaled down by a power of two there.)
 //
-// Four values (code4), a third of a division's instructions (a store of 131072 rows of 8 heads: 269 -> 123 us).  A
-// product with the rounded factor top / a is within 2^-23 of the quotient, which is the true side for every quotient but an
-// exact middle; and exact middles do occur.
+// Four values (code4), a third of a division's instructions (a store of 131072 rows of 8 heads, one tensor as K and V:
+// 269 -> 123 us).  A product with the rounded factor top / a is within 2^-23 of the quotient, which is the true side for
+// every quotient but an exact middle; and exact middles do occur.
 //   int8: (2k+1) A 2^m = 254 X has, unless 127 divides A, the one solution 2k+1 = 127, x = a / 2, which rounds to the even 64,
 //   away from zero: so the factor is rounded up.  Where 127 divides A the factor is a power of two and nothing is rounded, or
 //   (fp16 only) the values are divided.  The sum with 1.5 * 2^23 rounds the exact product to an integer, ties to even.
