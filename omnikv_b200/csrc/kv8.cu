@@ -35,7 +35,8 @@ struct StoreArgs {
   const int* lens;
 };
 
-// PPB: passes of THREADS / 16 rows per scale block; 0: blocks shorter than a pass.
+// PPB: passes of THREADS / 16 rows per scale block; 0: blocks shorter than a pass (one row: 165 us with a reduction per pass,
+// 144 with one for all passes).
 constexpr int kStorePasses = 8;
 template <typename T, int FMT, int ST_THREADS, int PPB>
 __global__ void __launch_bounds__(ST_THREADS) kv8_store_kernel(const StoreArgs a) {
@@ -70,14 +71,26 @@ __global__ void __launch_bounds__(ST_THREADS) kv8_store_kernel(const StoreArgs a
       if ((tid & 31) == 0) top[i][tid >> 5] = m;
     }
   } else {
-    for (int i = tid; i < R; i += ST_THREADS) top[i][0] = 0;
-    __syncthreads();
+    if (shift)
+      for (int i = tid; i < R; i += ST_THREADS) top[i][0] = 0;
+    // the rows' maxima over sixteen lanes: at each step a lane hands half of its passes over and keeps the other half
+    unsigned m[PASSES];
 #pragma unroll
-    for (int p = 0; p < PASSES; ++p) {
-      unsigned m = abs_bits_of<T>(max_abs2<T>(0u, x[p]));
+    for (int p = 0; p < PASSES; ++p) m[p] = abs_bits_of<T>(max_abs2<T>(0u, x[p]));
 #pragma unroll
-      for (int off = 8; off > 0; off >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, off));
-      if (lane16 == 0 && m) atomicMax(&top[(p * ST_ROWS + row16) >> shift][0], m);
+    for (int n = PASSES / 2, off = 8; n > 0; n >>= 1, off >>= 1)
+#pragma unroll
+      for (int p = 0; p < n; ++p) {
+        const unsigned keep = lane16 & off ? m[p + n] : m[p], give = lane16 & off ? m[p] : m[p + n];
+        m[p] = max(keep, __shfl_xor_sync(0xffffffffu, give, off));
+      }
+    m[0] = max(m[0], __shfl_xor_sync(0xffffffffu, m[0], 1));
+    const int row = (lane16 >> 1) * ST_ROWS + row16;  // bits 3, 2, 1 of the lane: the pass it has been left with
+    if (shift) {
+      __syncthreads();
+      if (!(lane16 & 1) && m[0]) atomicMax(&top[row >> shift][0], m[0]);
+    } else if (!(lane16 & 1)) {
+      top[row][0] = m[0];
     }
   }
   __syncthreads();
