@@ -315,8 +315,6 @@ linear_tile_kernel(const LinArgs a, const __grid_constant__ CUtensorMap tm_w, co
   __syncthreads();
   tc_fence_after();
   const unsigned tmem = sh.tmem_base;
-  pdl_wait();
-  pdl_trigger();
   // this CTA's work: the piece [lo, hi) of the shared tiles' chunks, then whole tiles
   const int chunks = a.chunks, tiles = ceil_div(a.N, TK_M), whole_tiles = tiles - a.shared, C = gridDim.x, cta = blockIdx.x;
   const int total = a.shared * chunks;  // the host keeps it below 2^31
@@ -344,6 +342,20 @@ linear_tile_kernel(const LinArgs a, const __grid_constant__ CUtensorMap tm_w, co
     }
     return u.tile < whole_tiles;
   };
+  // While the kernel before finishes, this CTA's first weights start on their way into L2 (16 x 4096 x 28672: 22.8 -> 21.8 us,
+  // 64 x 8192 x 20000: 34.5 -> 33.2); with fewer tiles than SMs it loses (16 x 4096 x 10240: 12.3, 13.1).
+  if (tid == 128 && tiles >= TK_CTAS) {
+    Unit u;
+    int n = 0;
+    for (bool more = first_unit(u); more && n < STAGES; more = next_unit(u))
+      for (int k = u.k0; k < u.k1 && n < STAGES; ++k, ++n)
+        asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];\n" ::"l"(reinterpret_cast<uint64_t>(&tm_w)),
+                     "r"(k * TK_KB), "r"(u.tile * TK_M)
+                     : "memory");
+  }
+  __syncwarp();
+  pdl_wait();
+  pdl_trigger();
 
   if (warp == 4) {
     if (lane == 0) {
