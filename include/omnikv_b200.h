@@ -597,7 +597,8 @@ typedef struct {
   float* score_out; /* [KVH, B, score_stride] or NULL */
   int64_t score_stride;
   const int32_t* score_len;
-  int32_t n_ctas; /* the work of all sequences is cut into at most this many equal pieces; 1..32768 */
+  int32_t n_ctas; /* 1..32768: the work of all sequences is cut into at most this many pieces, but for short caches, where
+                     every (sequence, KV head) has at least a CTA of its own */
   void* workspace;
   size_t workspace_bytes;
   int32_t* status; /* optional device word: set to 5 if a bounded wait for a KV copy ran out */

@@ -22,14 +22,15 @@
 // Work.  The 32-row tiles of all (sequence, KV head) segments form one list that is cut into equal pieces, one per CTA
 // (one CTA of twelve warps per SM), whatever the lengths: a CTA may end one segment and begin the next.  Every CTA leaves
 // one partial (o, M, m, l) per segment that it touches, and the one that arrives last at a segment merges.  Where segments are
-// few and short, a cluster of CTAs takes each (cluster_of below): its CTAs send their partials straight into the shared memory
-// of the one that finishes the head, which spares the merge three trips to L2.
+// short (ctas_per_segment below) each gets CTAs of its own instead: one, or a cluster whose CTAs send their partials straight
+// into the shared memory of the one that finishes the head, which spares the merge three trips to L2.
 //
 // Bound: HBM, 256 bytes of codes and 8 / block bytes of scales per (row, KV head).
 #include "kv8.cuh"
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 
 namespace omnikv {
 namespace {
@@ -65,7 +66,7 @@ struct A8Args {
   unsigned* ws_cnt; // [B * KVH] arrivals, zero between launches
   int* status;
   int B, H, KVH, G, pair;
-  int cluster;      // CTAs per segment where a cluster does one
+  int cluster;      // CTAs per segment where each has CTAs of its own
   float scale;
 };
 
@@ -179,7 +180,7 @@ struct Shared {
 };
 
 // COLS: n8 column blocks of query heads (1: up to 8 heads per KV head, 2: up to 16).  TMA: tiles as boxes of a tensor map
-// (rows that follow one another), else rows fetched one by one.  CLUSTER: a cluster of CTAs per segment.
+// (rows that follow one another), else rows fetched one by one.  CLUSTER: a cluster of a.cluster CTAs per segment.
 template <typename T, int FMT, int COLS, bool TMA, bool CLUSTER>
 __global__ void __launch_bounds__(kWarps[COLS] * 32, 1)
 decode_attn_kv8_kernel(const A8Args a, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
@@ -204,6 +205,7 @@ decode_attn_kv8_kernel(const A8Args a, const __grid_constant__ CUtensorMap tm_k,
 
   Cursor seg;  // the segment being worked on; tile = 0
   int seg_lo, w0, w1, W = 0, C = 1, each = 0, more = 0;
+  bool own = CLUSTER;  // the segment is this CTA's (or its cluster's) alone
   const int c = blockIdx.x, rank = CLUSTER ? (int)cluster_rank() : 0;
   const auto piece_lo = [&](int i) { return i * each + i * more / C; };  // i * more < 2^30
   const auto owner = [&](int tile) {  // the CTA that has this tile
@@ -243,20 +245,38 @@ decode_attn_kv8_kernel(const A8Args a, const __grid_constant__ CUtensorMap tm_k,
       }
       if (filled == 0) return;
   }
-    // Pieces.  One per segment when four tiles per warp do a segment: a merge across CTAs costs more than it saves then.
-    // Else as many as there are CTAs; with segments of one length a multiple of them, so that pieces end where segments end,
-    // where the CTAs that leaves idle cost less than that spares (5 us, or 2.3 tiles per warp; 16 x 3000 rows of 8 heads:
-    // 29.7 us with 148 pieces, 23.3 with 128).
-    const int segs = filled * a.KVH;
+    // Pieces.  Segments of different lengths, no more than there are CTAs and none much longer than a CTA's share: one CTA for
+    // each.  One piece per segment too when four tiles per warp do a segment: a merge across CTAs costs more than it saves
+    // then.  Else as many as there are CTAs; with segments of one length a multiple of them, so that pieces end where segments
+    // end, where the CTAs that leaves idle cost less than that spares (5 us, or 2.3 tiles per warp; 12 x 3000 rows of 8 heads:
+    // 29.7 us with 148 pieces, 23.3 with 96).
+    const int segs = filled * a.KVH, grid = gridDim.x;
+    const bool even = longest * filled == per_head;
     W = per_head * a.KVH;
-    C = min((int)gridDim.x, W <= segs * NW * 4 ? segs : max(W / NW, segs));
-    if (C > segs && longest * filled == per_head && (float)(C % segs) * (float)W <= 2.3f * NW * (float)C * (float)C) C -= C % segs;
-    each = W / C;
-    more = W - each * C;
+    own = !even && segs <= grid && longest <= W / grid + 32 + segs / 6;
+    C = min(grid, own || W <= segs * NW * 4 ? segs : max(W / NW, segs));
+    C = min(C, max(segs, (int)sqrtf(12.8f * (float)W * (float)segs / (float)G)));  // a tile costs 190 ns, a partial's head 15 in the merge
+    if (C > segs && even && (float)(C % segs) * (float)W <= 2.3f * NW * (float)C * (float)C) C -= C % segs;
     if (c >= C) return;
-    w0 = piece_lo(c);
-    w1 = piece_lo(c + 1);
-      int before = 0, found = -1;  // tiles per KV head of the sequences in front
+    int found = -1;
+    if (own) {
+      int at = c / a.KVH;  // among the sequences that have rows
+      for (int b0 = 0; found < 0; b0 += 32) {
+        const unsigned some = __ballot_sync(0xffffffffu, b0 + lane < a.B && row_list(a, min(b0 + lane, a.B - 1)).n() > 0);
+        if (at < __popc(some)) found = b0 + (int)__fns(some, 0, at + 1);
+        at -= __popc(some);
+      }
+      seg.kvh = c % a.KVH;
+      seg.b = found;
+      seg.load(a);
+      seg_lo = w0 = 0;
+      w1 = seg.nt;
+    } else {
+      each = W / C;
+      more = W - each * C;
+      w0 = piece_lo(c);
+      w1 = piece_lo(c + 1);
+      int before = 0;  // tiles per KV head of the sequences in front
       for (int b0 = 0; found < 0; b0 += 32) {
         const int mine = b0 + lane < a.B ? row_list(a, b0 + lane).tiles() : 0;
         int sum = mine;
@@ -273,8 +293,9 @@ decode_attn_kv8_kernel(const A8Args a, const __grid_constant__ CUtensorMap tm_k,
       seg.b = found;
       seg.load(a);
       seg.kvh = (w0 - before * a.KVH) / seg.nt;
-      seg.tile = 0;
       seg_lo = before * a.KVH + seg.kvh * seg.nt;
+    }
+    seg.tile = 0;
   }
 
   // ---- the warp's stream of tiles: every NW-th of the piece ----
@@ -338,7 +359,7 @@ decode_attn_kv8_kernel(const A8Args a, const __grid_constant__ CUtensorMap tm_k,
   for (int lo = w0; CLUSTER || lo < w1;) {
     const int seg_hi = seg_lo + seg.nt, hi = min(w1, seg_hi);  // this CTA's tiles of the segment: [lo, hi)
     const int b = seg.b, kvh = seg.kvh, seg_no = b * a.KVH + kvh;
-    const int c_lo = CLUSTER ? 0 : owner(seg_lo), parts = CLUSTER ? 1 : owner(seg_hi - 1) - c_lo + 1;  // the CTAs that share it
+    const int c_lo = own ? 0 : owner(seg_lo), parts = own ? 1 : owner(seg_hi - 1) - c_lo + 1;  // the CTAs that share it
 
     // ---- queries: fragments of q * 2^e (largest element in [2^13, 2^14)), e folded into the head's factor ----
     unsigned qf[COLS][8][2];
@@ -828,27 +849,45 @@ int launch(const A8Args& a, int ctas, const CUtensorMap& tm_k, const CUtensorMap
 
 template <typename T, int FMT>
 int launch_any(const A8Args& a, int ctas, bool tma, const CUtensorMap& tm_k, const CUtensorMap& tm_v, cudaStream_t st) {
-  if (a.G > 8) return tma ? launch<T, FMT, 2, true, false>(a, ctas, tm_k, tm_v, st) : launch<T, FMT, 2, false, false>(a, ctas, tm_k, tm_v, st);
-  if (a.cluster > 1) {
+  const auto go = [&](auto tiles, auto own) -> int {
+    constexpr bool TMA = decltype(tiles)::value, CLUSTER = decltype(own)::value;
+    return a.G <= 8 ? launch<T, FMT, 1, TMA, CLUSTER>(a, ctas, tm_k, tm_v, st) : launch<T, FMT, 2, TMA, CLUSTER>(a, ctas, tm_k, tm_v, st);
+  };
+  const std::true_type yes;
+  const std::false_type no;
+  if (a.cluster) {
     ctas = a.B * a.KVH * a.cluster;
-    return tma ? launch<T, FMT, 1, true, true>(a, ctas, tm_k, tm_v, st) : launch<T, FMT, 1, false, true>(a, ctas, tm_k, tm_v, st);
+    return tma ? go(yes, yes) : go(no, yes);
   }
-  return tma ? launch<T, FMT, 1, true, false>(a, ctas, tm_k, tm_v, st) : launch<T, FMT, 1, false, false>(a, ctas, tm_k, tm_v, st);
+  return tma ? go(yes, no) : go(no, no);
 }
 
 constexpr int kMaxCtas = 32768;
 
-// CTAs per segment, 1: no clusters.  As many as find three tiles each and run at once with those of the other segments (kMost:
-// clusters of so many CTAs that fit on a B200's 148 SMs), while a warp has three tiles at most; beyond that the list cut over
-// all SMs is faster.  Measured without and with, us, 8 segments: 100 rows 5.5, 5.7; 777 rows 10.3, 5.8; 2000 rows 11.2, 6.6;
-// 8781 rows 11.8, 11.1; 12000 rows 12.9, 13.2; 8781 selected rows 13.5, 12.8.
-inline int cluster_of(int segs, int G, int64_t rows, int n_ctas) {
-  static constexpr int kMost[17] = {0, 148, 74, 45, 33, 26, 22, 15, 15, 15, 11, 7, 7, 7, 7, 7, 7};
-  const int64_t tiles = (rows + TILE - 1) / TILE;
-  if (G > 8 || tiles <= 4) return 1;
-  int cs = (int)std::min<int64_t>({16, (tiles + 2) / 3, n_ctas / segs});
-  while (cs > 1 && segs > kMost[cs]) --cs;
-  return cs > 1 && tiles <= cs * kWarps[1] * 3 ? cs : 1;
+// CTAs per segment (1: a CTA for each, more: a cluster), or 0: the list cut over all SMs.  The one with the least estimated
+// time (ns), the rows being as many as they can be (four fifths of that on average): a start, 1 / warps of a round per tile,
+// what a cluster's exchange or the merges through L2 add (15 ns per head and partial of a segment).  kMost: clusters of so many CTAs that run at once on a B200's 148 SMs.  Measured, us, with 8 KV heads:
+//   one sequence, list or one CTA, cluster   100 rows 5.5, 5.7   777: 10.3, 5.8   2000: 11.2, 6.6   8781: 11.8, 11.1
+//                                            12000: 12.9, 13.2   8781 selected: 13.5, 12.8
+//   16 ragged sequences, list, CTA each      700 rows at most: 21.9, 9.9   3000: 30.2, 22.7   12000: 64.0, 70.7
+inline int ctas_per_segment(int B, int KVH, int G, int64_t rows, int n_ctas) {
+  static constexpr int kMost[17] = {0, 0, 74, 45, 33, 26, 22, 15, 15, 15, 11, 7, 7, 7, 7, 7, 7};
+  constexpr int kSms = 148;
+  const int segs = B * KVH;
+  const double tiles = (double)((rows + TILE - 1) / TILE), per_tile = 2300.0 / kWarps[G <= 8 ? 1 : 2];
+  const double all = tiles * segs, ctas = std::min({(double)kSms, all / kWarps[G <= 8 ? 1 : 2], std::sqrt(12.8 * all * segs / G)});
+  const double share = all / std::max(ctas, 1.0);
+  double best = 5800 + (B == 1 ? per_tile * share + 2000 + 15 * G * ctas / segs : 0.8 * per_tile * share + 8000 + 34 * segs);
+  int pick = 0;
+  for (int cs = 1; cs <= 16; ++cs) {
+    if (cs > 1 && (segs > kMost[cs] || (int64_t)cs * segs > n_ctas || cs * ceil_div(G, cs) > 16)) continue;
+    const double ns = ceil_div(segs, cs > 1 ? segs : kSms) * (5300 + per_tile * tiles / cs) + (cs > 1 ? 40 * cs : 0);
+    if (ns < best) {
+      best = ns;
+      pick = cs;
+    }
+  }
+  return pick;
 }
 
 inline long long slots_of(int B, int KVH, int ctas) { return (long long)ctas + (long long)B * KVH; }
@@ -896,7 +935,7 @@ extern "C" int omnikv_kv8_decode_attn(const omnikv_kv8_attn_params* p, void* str
   a.ws_o = reinterpret_cast<float*>(a.ws_ml + (size_t)slots_of(c.B, c.KVH, p->n_ctas) * a.G);
   a.status = p->status;
   a.scale = p->scale;
-  a.cluster = cluster_of(c.B * c.KVH, a.G, (p->idx ? (int64_t)p->idx_cap : (int64_t)c.rows), p->n_ctas);
+  a.cluster = ctas_per_segment(c.B, c.KVH, a.G, p->idx ? p->idx_cap : c.rows, p->n_ctas);  // a tail is taken to be short
   a.pair = a.v == a.k + kHeadDim;  // V rows right behind their K rows: one copy brings both
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   // rows that follow one another come as boxes of a tensor map (where the layout can be described as one)

@@ -290,7 +290,7 @@ def test_selected_rows_and_tail(fmt, tokens_first, H, KVH, P, counts, tails, spl
 @pytest.mark.parametrize("splits", [2, 3, 5, 7, 8, 9, 10, 13, 16, None])
 def test_one_to_sixteen_ctas_per_head(fmt, splits):
     """A cluster of `splits` CTAs per (sequence, KV head) merges its partials, however many rows each of them gets."""
-    for B, KVH, G, lens in ((1, 1, 8, [1537]), (2, 1, 3, [70, 1500]), (1, 2, 5, [33]), (3, 1, 1, [0, 1, 1537]), (1, 7, 7, [1100])):
+    for B, KVH, G, lens in ((1, 1, 8, [1537]), (1, 1, 16, [1537]), (2, 1, 11, [1537, 600]), (2, 1, 3, [70, 1500]), (1, 2, 5, [33]), (3, 1, 1, [0, 1, 1537]), (1, 7, 7, [1100])):
         H, rows = KVH * G, 1537
         cache, k, v = filled(B, KVH, rows, fmt, torch.float16, 64, 31)
         q = draw((B, H, D), torch.float16, 32, outliers=False) * 2
@@ -553,6 +553,20 @@ def test_many_sequences(B, KVH, H, splits):
     q = draw((B, H, D), torch.bfloat16, 90, outliers=False)
     out = ops().kv8_decode_attn(q, *cache, i32(lens), block=16, n_splits=splits)
     check_attention(out, q, k, v, [list(range(n)) for n in lens])
+
+
+@pytest.mark.parametrize("B,KVH,G,lens", [(4, 2, 4, [700, 300, 0, 1000]), (40, 3, 2, None), (5, 1, 16, [1, 0, 33, 900, 64])])
+def test_few_rows_of_different_numbers_in_a_large_cache(B, KVH, G, lens):
+    lens = lens or torch.randint(0, 900, (B,), generator=torch.Generator().manual_seed(7)).tolist()
+    cap, top = 40000, 1024
+    cache = ops().kv8_alloc(B, KVH, cap, block=64, dtype=torch.int8, device="cuda")
+    ops().kv8_store(draw((B, KVH, top, D), torch.bfloat16, 95), draw((B, KVH, top, D), torch.bfloat16, 96), *cache, block=64)
+    k, v = as_read(tuple(t[:, :, :top] for t in cache[:2]) + tuple(t[:, :, :top // 64] for t in cache[2:]), 64)
+    q = draw((B, KVH * G, D), torch.bfloat16, 97, outliers=False)
+    out = ops().kv8_decode_attn(q, *cache, i32(lens), block=64)
+    check_attention(out, q, k, v, [list(range(n)) for n in lens])
+    for n_splits in (1, 2, 9):
+        check_attention(ops().kv8_decode_attn(q, *cache, i32(lens), block=64, n_splits=n_splits), q, k, v, [list(range(n)) for n in lens])
 
 
 def test_strides_of_single_entries_do_not_matter():
