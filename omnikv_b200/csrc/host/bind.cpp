@@ -2,15 +2,15 @@
 // results and calls the C ABI on the current stream.
 //
 // The kernels behind these calls take one to ten microseconds for a single token, and checking a dozen tensors from Python
-// takes longer than that (attention 13.5, append 8.4, rows to codes 9.2 us of host time per call against 4.5, 2.9, 4.3 here).
+// takes longer than that (attention 13.5, append 8.4, rows to codes 9.2 us of host time per call against 4.2, 2.9, 3.6 here).
 // Nothing is kept between calls but workspaces (per device, stream and captured graph) and, per device, the SM count and
 // the status word's address.
 //
 // The library is not linked: `init` gets the addresses of its entry points, so that the one the process has loaded is used.
 #include <Python.h>
 
-#include <ATen/cuda/EmptyTensor.h>
 #include <ATen/ops/zeros.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -161,8 +161,19 @@ void done(int status, const char* what) {
   }
   ++g_launches;
 }
-at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType t, const at::Tensor& like) {  // contiguous; past the dispatcher
-  return at::Tensor(at::detail::empty_cuda(sizes, t, like.device(), std::nullopt));
+// New memory of the current device, and contiguous tensors in it (the two results of a call share one allocation: it and
+// its release are a third of the call).
+c10::Storage memory(size_t bytes) {
+  return c10::Storage(c10::Storage::use_byte_size_t(), bytes, c10::cuda::CUDACachingAllocator::get(), true);
+}
+at::Tensor tensor_in(const c10::Storage& s, size_t offset, at::IntArrayRef sizes, at::ScalarType t) {
+  at::Tensor r = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(s), c10::DispatchKeySet(c10::DispatchKey::CUDA), c10::scalarTypeToTypeMeta(t));
+  r.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+  r.unsafeGetTensorImpl()->set_storage_offset((int64_t)(offset / c10::elementSize(t)));
+  return r;
+}
+at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType t) {
+  return tensor_in(memory((size_t)c10::multiply_integers(sizes) * c10::elementSize(t)), 0, sizes, t);
 }
 
 // ---- the calls --------------------------------------------------------------------------------------------------------------
@@ -227,9 +238,11 @@ PyObject* kv8_load(PyObject* const* a) {
     if (n < 0) n = c.rows - start;
   }
   if (n > INT32_MAX) refuse("kv8_load: at most 2^31 - 1 rows");
-  const at::Tensor k = fresh({c.B, c.KVH, n, 128}, t, k8), v = fresh({c.B, c.KVH, n, 128}, t, k8);
+  OnDevice on(dev);
+  const size_t bytes = (size_t)c.B * c.KVH * n * 128 * 2;
+  const c10::Storage both = memory(2 * bytes);
+  const at::Tensor k = tensor_in(both, 0, {c.B, c.KVH, n, 128}, t), v = tensor_in(both, bytes, {c.B, c.KVH, n, 128}, t);
   if (n) {
-    OnDevice on(dev);
     done(abi.kv8_load(&c, dt, (int)start, (int)n, idx ? static_cast<const int32_t*>(idx->data_ptr()) : nullptr, idx_stride, k.data_ptr(),
                       v.data_ptr(), k.stride(0), k.stride(1), k.stride(2), on.stream),
          "omnikv_kv8_load");
@@ -297,7 +310,8 @@ PyObject* kv8_decode_attn(PyObject* const* a) {
     refuse("kv8_decode_attn: n_splits x B x KVH must lie in 1..32768");
   const int64_t n = a[13] != Py_None ? per * segments : std::min(d.sms, per * segments);
   p.n_ctas = (int32_t)n;
-  const at::Tensor out = out_arg ? *out_arg : fresh(q.sizes(), q.scalar_type(), q);
+  OnDevice on(dev);
+  const at::Tensor out = out_arg ? *out_arg : fresh(q.sizes(), q.scalar_type());
   p.q = q.data_ptr();
   p.q_stride_b = step(q, 0);
   p.q_stride_h = step(q, 1);
@@ -305,7 +319,6 @@ PyObject* kv8_decode_attn(PyObject* const* a) {
   p.out_stride_b = step(out, 0);
   p.out_stride_h = step(out, 1);
   p.status = d.status;
-  OnDevice on(dev);
   const at::Tensor& ws = ws_arg ? *ws_arg : workspace(dev, on.stream, 0, abi.kv8_attn_workspace_bytes((int)B, p.H, (int)KVH, p.n_ctas));
   p.workspace = ws.data_ptr();
   p.workspace_bytes = (size_t)ws.numel() * ws.element_size();
@@ -320,9 +333,11 @@ PyObject* quant_rows(PyObject* const* a) {
   if (x.dim() != 2 || !dense_rows(x) || x.size(1) == 0 || x.size(1) % 16 || x.size(0) > INT32_MAX || x.size(1) > INT32_MAX)
     refuse("quant_rows: x must be [n, K] with contiguous rows and K a multiple of 16");
   const int64_t n = x.size(0), K = x.size(1);
-  const at::Tensor codes = fresh({n, K}, at::kChar, x), scale = fresh({n}, at::kFloat, x);
+  OnDevice on(dev);
+  const size_t bytes = (size_t)n * K;  // a multiple of 16
+  const c10::Storage both = memory(bytes + n * sizeof(float));
+  const at::Tensor codes = tensor_in(both, 0, {n, K}, at::kChar), scale = tensor_in(both, bytes, {n}, at::kFloat);
   if (n) {
-    OnDevice on(dev);
     done(abi.quant_rows(dt, x.data_ptr(), step(x, 0), (int)n, (int)K, static_cast<int8_t*>(codes.data_ptr()), K,
                         static_cast<float*>(scale.data_ptr()), on.stream),
          "omnikv_quant_rows");
@@ -355,9 +370,9 @@ PyObject* linear_w8a8(PyObject* const* a) {
       refuse("linear_w8a8: out and residual must be [n, channels] of one floating dtype, rows contiguous");
   if (t != at::kFloat && t != at::kBFloat16 && t != at::kHalf)
     refuse(std::string("linear_w8a8: the result is float32, bfloat16 or float16, not ") + c10::toString(t));
-  const at::Tensor out = out_arg ? *out_arg : fresh({n, N}, t, x8);
+  OnDevice on(dev);
+  const at::Tensor out = out_arg ? *out_arg : fresh({n, N}, t);
   if (n && N) {
-    OnDevice on(dev);
     omnikv_linear_w8a8_params p = {};
     p.n_tokens = (int32_t)n;
     p.channels = (int32_t)N;
