@@ -10,7 +10,8 @@
 Cases: tp_timeline (one graph-replayed decode step of the benchmark on N GPUs, or on one: per-kernel %globaltimer
 stamps of the profiling build, with the wait for the peers' flags separated from the streaming time), dense_attn (filter layer: K and V of 8 KV heads x ctx rows, fused scores), sparse_attn
 (8781 selected rows + tail), topk (ctx scores, 8 planes), score_window (16-slot window, exp),
-offload_gather (30150 tokens x 12 layers from pinned host memory).  Each prints the CUDA-event time per launch.
+offload_gather (30150 tokens x 12 layers from pinned host memory), kv8 (8-bit KV cache: attention over ctx rows, selected rows and
+short caches, store and load), linear_w8a8 (the layer's projections in 8-bit integers).  Each prints the CUDA-event time per launch.
 """
 from __future__ import annotations
 
@@ -134,6 +135,74 @@ def batched_linear_cases(reps: int, n_tokens: int = 16, n_sets: int = 8):
                 torch.cuda.synchronize()
                 ms = a.elapsed_time(b) / n_sets
                 print(f"{name} [{leg}] rep {r}: {ms * 1e3:.1f} us per call, {nbytes / 1e6:.1f} MB, {nbytes / ms / 1e6:.0f} GB/s")
+    ops.check_status(dev)
+
+
+def _graph_us(fn, calls: int = 20) -> float:
+    """us per call of ``fn(i)``, ``calls`` calls back to back in a CUDA graph (median of five replays)."""
+    for i in range(3):
+        fn(i)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        for i in range(calls):
+            fn(i)
+    g.replay()
+    torch.cuda.synchronize()
+    ts = []
+    for _ in range(5):
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        g.replay()
+        b.record()
+        torch.cuda.synchronize()
+        ts.append(a.elapsed_time(b) / calls * 1e3)
+    return sorted(ts)[2]
+
+
+def kv8_cases(ctx: int):
+    """The 8-bit KV cache of one layer (8 KV heads, 32 query heads, 64 rows to a scale)."""
+    dev, KVH, H = "cuda", 8, 32
+    row_bytes = KVH * (256 + 8 / 64)
+    for codes in (torch.int8, torch.float8_e4m3fn):
+        k, v = (torch.randn(1, KVH, ctx, 128, device=dev).to(torch.bfloat16) for _ in range(2))
+        q = torch.randn(1, H, 128, device=dev).to(torch.bfloat16)
+        dense, sparse = (ops.kv8_alloc(1, KVH, ctx, block=64, dtype=codes, device=dev, tokens_first=t) for t in (False, True))
+        for cache in (dense, sparse):
+            ops.kv8_store(k, v, *cache, block=64)
+        scores = torch.empty(KVH, 1, ctx, dtype=torch.float32, device=dev)
+        length = torch.tensor([ctx], dtype=torch.int32, device=dev)
+        idx = torch.rand(1, ctx, device=dev).topk(int(0.067 * ctx), 1).indices.sort(1).values.int()
+        count = torch.tensor([idx.shape[1]], dtype=torch.int32, device=dev)
+        cases = {
+            "store": (lambda i: ops.kv8_store(k, v, *dense, block=64), 3 * ctx * KVH * 256),
+            "load": (lambda i: ops.kv8_load(*dense, block=64, dtype=torch.bfloat16), 3 * ctx * KVH * 256),
+            "attention, all rows": (lambda i: ops.kv8_decode_attn(q, *dense, length, block=64), ctx * row_bytes),
+            "attention, all rows, and scores": (lambda i: ops.kv8_decode_attn(q, *dense, length, block=64, score_out=scores, score_len=length),
+                                                ctx * (row_bytes + 4 * KVH)),
+            f"attention, {idx.shape[1]} selected rows": (lambda i: ops.kv8_decode_attn(q, *sparse, count, block=64, idx=idx),
+                                                         idx.shape[1] * row_bytes)}
+        for rows in (100, 777, 3000, 12000):
+            part, n = tuple(t[:, :, :rows] for t in dense[:2]) + dense[2:], torch.tensor([rows], dtype=torch.int32, device=dev)
+            cases[f"attention, {rows} rows"] = (lambda i, part=part, n=n: ops.kv8_decode_attn(q, *part, n, block=64), rows * row_bytes)
+        for name, (fn, nbytes) in cases.items():
+            us = _graph_us(fn)
+            print(f"{str(codes).split('.')[1]}: {name}: {us:.1f} us, {nbytes / 1e6:.1f} MB, {nbytes / us / 1e3:.0f} GB/s")
+    ops.check_status(dev)
+
+
+def linear_w8a8_cases(n_tokens: int):
+    """The four projections of a Llama-3-8B layer as 8-bit integer products, over weight sets larger than L2 together."""
+    dev = "cuda"
+    for name, K, N in (("qkv", 4096, 6144), ("o", 4096, 4096), ("gate_up", 4096, 28672), ("down", 14336, 4096)):
+        sets = [torch.randint(-127, 128, (N, K), device=dev, dtype=torch.int8) for _ in range(max(2, int(4e8 // (N * K))))]
+        scale = torch.ones(N, device=dev)
+        x = torch.randn(n_tokens, K, device=dev).to(torch.bfloat16)
+        x8, xs = ops.quant_rows(x)
+        us = _graph_us(lambda i: ops.linear_w8a8(x8, xs, sets[i % len(sets)], scale))
+        both = _graph_us(lambda i: ops.linear_w8a8(*ops.quant_rows(x), sets[i % len(sets)], scale))
+        print(f"{name} ({n_tokens} x {K} x {N}): {us:.1f} us, with the codes of its input {both:.1f} us; {N * K / 1e6:.1f} MB of weights, "
+              f"{N * K / us / 1e3:.0f} GB/s, {2 * n_tokens * N * K / us / 1e9:.3f} POP/s")
     ops.check_status(dev)
 
 
@@ -296,8 +365,8 @@ def prefill_case(ctx: int, reps: int, library: bool):
 def main():
     ap = argparse.ArgumentParser()
     ap.add_argument("case", choices=["dense_attn", "sparse_attn", "topk", "score_window", "offload_gather", "gemv", "operator",
-                                     "tp_timeline", "prefill_attn", "batched_linear"])
-    ap.add_argument("--tokens", type=int, default=16, help="batched_linear: sequences decoding together")
+                                     "tp_timeline", "prefill_attn", "batched_linear", "kv8", "linear_w8a8"])
+    ap.add_argument("--tokens", type=int, default=16, help="batched_linear, linear_w8a8: sequences decoding together")
     ap.add_argument("--reps", type=int, default=3)
     ap.add_argument("--ctx", type=int, default=131072)
     ap.add_argument("--splits", type=int, default=0)
@@ -322,6 +391,10 @@ def main():
         return gemv_cases(args.reps)
     if args.case == "batched_linear":
         return batched_linear_cases(args.reps, args.tokens)
+    if args.case == "kv8":
+        return kv8_cases(args.ctx)
+    if args.case == "linear_w8a8":
+        return linear_w8a8_cases(args.tokens)
     if args.case == "prefill_attn":
         return prefill_case(args.ctx if args.ctx != 131072 else 16384, args.reps, args.library)
     if args.case == "operator":
