@@ -650,6 +650,10 @@ int omnikv_linear_w8a8(const omnikv_linear_w8a8_params* p, void* stream);
  * captured graph: two graphs may be replayed at the same time). */
 unsigned long long omnikv_capture_id(void* stream);
 
+/* Calls release(arg) once the graph that `stream` records into, and every executable graph made from it, are destroyed (on a
+ * thread of the driver's, where CUDA must not be called): a workspace kept for that graph can go then. */
+int omnikv_capture_retain(void* stream, void (*release)(void*), void* arg);
+
 #ifdef __cplusplus
 }
 #endif

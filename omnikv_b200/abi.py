@@ -211,6 +211,7 @@ SIGNATURES = {
                                     C.c_void_p]),
     "omnikv_linear_w8a8_workspace_bytes": (C.c_size_t, [C.c_int, C.c_int, C.c_int]),
     "omnikv_linear_w8a8": (C.c_int, [C.POINTER(LinearW8A8Params), C.c_void_p]),
+    "omnikv_capture_retain": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
     "omnikv_capture_id": (C.c_ulonglong, [C.c_void_p]),
     "omnikv_kv_append": (C.c_int, [C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int,
                                    C.c_int, C.c_int64, C.c_int64, C.c_int64, C.c_int64, C.c_int64, C.c_void_p,

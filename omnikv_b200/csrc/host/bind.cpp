@@ -19,8 +19,10 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
+#include <climits>
 #include <cstring>
 #include <map>
+#include <mutex>
 #include <string>
 #include <tuple>
 #include <vector>
@@ -39,6 +41,7 @@ struct Abi {
   decltype(&omnikv_linear_w8a8_workspace_bytes) linear_w8a8_workspace_bytes;
   decltype(&omnikv_linear_w8a8) linear_w8a8;
   decltype(&omnikv_capture_id) capture_id;
+  decltype(&omnikv_capture_retain) capture_retain;
 } abi;
 PyObject *g_error, *g_check, *g_device_info;  // the exception class; check(status, what); device_info(ordinal) -> (SMs, status address)
 long long g_launches = 0;
@@ -137,12 +140,37 @@ const Device& device(int dev) {
   return it->second;
 }
 // A zero-filled workspace for calls that follow one another: one per stream, and one per captured graph (two graphs, or a
-// graph and eager calls, may run at the same time).  One that was outgrown is kept: a captured graph may still use it.
+// graph and eager calls, may run at the same time).  One that was outgrown is kept: a captured graph may still use it.  Those
+// of a captured graph go when the graph has been destroyed, of which a driver thread tells (graph_ended).
+struct Ended {
+  std::mutex lock;
+  std::vector<unsigned long long> ids;
+};
+Ended& ended() {
+  static auto& e = *new Ended;
+  return e;
+}
+void graph_ended(void* id) {
+  Ended& e = ended();
+  const std::lock_guard<std::mutex> hold(e.lock);
+  e.ids.push_back(reinterpret_cast<uintptr_t>(id));
+}
 const at::Tensor& workspace(int dev, cudaStream_t stream, int tag, size_t bytes) {
-  static auto& kept = *new std::map<std::tuple<int, int, cudaStream_t, unsigned long long>, std::vector<at::Tensor>>;
-  auto& own = kept[{dev, tag, stream, abi.capture_id(stream)}];
-  if (own.empty() || (size_t)own.back().numel() < bytes)
-    own.push_back(at::zeros({(int64_t)std::max(bytes, (size_t)1 << 20)}, at::TensorOptions().dtype(at::kByte).device(at::kCUDA, dev)));
+  static auto& kept = *new std::map<std::tuple<unsigned long long, int, int, cudaStream_t>, std::vector<at::Tensor>>;
+  const unsigned long long id = abi.capture_id(stream);
+  auto it = kept.find({id, dev, tag, stream});
+  if (it != kept.end() && (size_t)it->second.back().numel() >= bytes) return it->second.back();
+  std::vector<unsigned long long> gone;
+  {
+    const std::lock_guard<std::mutex> hold(ended().lock);
+    gone.swap(ended().ids);
+  }
+  for (const unsigned long long g : gone)
+    kept.erase(kept.lower_bound({g, INT_MIN, INT_MIN, nullptr}), kept.lower_bound({g + 1, INT_MIN, INT_MIN, nullptr}));
+  at::Tensor fresh_one = at::zeros({(int64_t)std::max(bytes, (size_t)1 << 20)}, at::TensorOptions().dtype(at::kByte).device(at::kCUDA, dev));
+  if (id && it == kept.end()) abi.capture_retain(stream, graph_ended, reinterpret_cast<void*>((uintptr_t)id));
+  auto& own = kept[{id, dev, tag, stream}];
+  own.push_back(std::move(fresh_one));
   return own.back();
 }
 struct OnDevice {  // the device of the call is current, its current stream at hand

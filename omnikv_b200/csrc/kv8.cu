@@ -321,3 +321,16 @@ extern "C" unsigned long long omnikv_capture_id(void* stream) {
   }
   return status == cudaStreamCaptureStatusActive ? id : 0;
 }
+
+extern "C" int omnikv_capture_retain(void* stream, void (*release)(void*), void* arg) {
+  using namespace omnikv;
+  if (!release) return OMNIKV_E_BADARG;
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  cudaGraph_t graph = nullptr;
+  OMNIKV_CUDA_OK(cudaStreamGetCaptureInfo(static_cast<cudaStream_t>(stream), &status, nullptr, &graph));
+  if (status != cudaStreamCaptureStatusActive || !graph) return OMNIKV_E_BADARG;
+  cudaUserObject_t object = nullptr;
+  OMNIKV_CUDA_OK(cudaUserObjectCreate(&object, arg, release, 1, cudaUserObjectNoDestructorSync));
+  OMNIKV_CUDA_OK(cudaGraphRetainUserObject(graph, object, 1, cudaGraphUserObjectMove));
+  return OMNIKV_OK;
+}

@@ -518,7 +518,7 @@ def host_device_pointer(t: torch.Tensor) -> int:
 # calls are a few microseconds on the GPU.
 _KV8 = (torch.int8, torch.float8_e4m3fn)
 _BIND_ABI = ("omnikv_kv8_store", "omnikv_kv8_append", "omnikv_kv8_load", "omnikv_kv8_attn_workspace_bytes", "omnikv_kv8_decode_attn",
-             "omnikv_quant_rows", "omnikv_linear_w8a8_workspace_bytes", "omnikv_linear_w8a8", "omnikv_capture_id")
+             "omnikv_quant_rows", "omnikv_linear_w8a8_workspace_bytes", "omnikv_linear_w8a8", "omnikv_capture_id", "omnikv_capture_retain")
 _bind_module = None
 
 

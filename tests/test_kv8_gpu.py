@@ -479,6 +479,24 @@ def test_prompt_then_steps_in_a_graph(fmt):
             assert torch.equal(res[2][:, :k_sel], want[t][2][:, :k_sel])
 
 
+def test_a_destroyed_graph_gives_its_workspace_back():
+    cache, _, _ = filled(2, 2, 9000, "int8", torch.bfloat16, 64, 79)
+    q, n = draw((2, 16, D), torch.bfloat16, 80, outliers=False), i32([9000, 5000])
+    ws = torch.zeros(ops().abi.lib().omnikv_kv8_attn_workspace_bytes(2, 16, 2, 148), dtype=torch.uint8, device="cuda")
+    want = ops().kv8_decode_attn(q, *cache, n, block=64, n_splits=37, ws=ws)
+    used = []
+    for _ in range(24):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = ops().kv8_decode_attn(q, *cache, n, block=64, n_splits=37)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        del graph, out
+        used.append(torch.cuda.memory_allocated())
+    assert max(used[4:]) - used[3] < 8 * (1 << 20), used  # not one of 1 MiB and more for each graph
+
+
 def test_two_streams_at_once():
     B, H, KVH, rows, block = 1, 32, 8, 20000, 64
     cache, _, _ = filled(B, KVH, rows, "int8", torch.bfloat16, block, 81)
