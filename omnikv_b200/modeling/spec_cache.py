@@ -70,6 +70,8 @@ class OmniKVMultiStageCache:
             raise ValueError(f"kv_dtype must be None, torch.int8 or torch.float8_e4m3fn, got {kv_dtype}")
         if kv_dtype is not None and real_offload:
             raise NotImplementedError("an 8-bit KV cache is held on the GPU: kv_dtype needs real_offload=False")
+        if not 1 <= int(kv_block) <= 256 or int(kv_block) & (int(kv_block) - 1):
+            raise ValueError(f"kv_block must be a power of two between 1 and 256, got {kv_block}")
         self.kv_dtype, self.kv_block, self.keep_layers = kv_dtype, int(kv_block), frozenset(keep_layers)
         self._kv8: Dict[int, Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]] = {}  # codes and scales
         self._new_row: Optional[Tuple[torch.Tensor, torch.Tensor]] = None  # 16-bit K, V of the token on its way into an 8-bit layer

@@ -544,6 +544,8 @@ def kv8_alloc(B: int, KVH: int, rows: int, *, block: int, dtype: torch.dtype, de
     heads first (a layer that reads whole heads) or tokens first (one that reads selected tokens)."""
     if dtype not in _KV8:
         raise abi.OmniKVError("kv8: codes are torch.int8 or torch.float8_e4m3fn")
+    if not 1 <= block <= 256 or block & (block - 1):
+        raise abi.OmniKVError(f"kv8: block must be a power of two between 1 and 256, got {block}")
     kw = dict(dtype=torch.int8, device=device)  # the all-zero byte is code 0 in both formats
     if tokens_first:
         kv = torch.zeros(B, rows, KVH, 2, 128, **kw).view(dtype)

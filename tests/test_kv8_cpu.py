@@ -155,3 +155,13 @@ def test_cache_options_are_checked():
             cls.from_dynamic_cache(None, [0, 1, 4], 4, 1, True, kv_dtype=torch.int8)
         with pytest.raises(ValueError):
             cls.from_dynamic_cache(None, [0, 1, 4], 4, 1, False, kv_dtype=torch.uint8)
+        for block in (0, 48, 512):
+            with pytest.raises(ValueError):
+                cls.from_dynamic_cache(None, [0, 1, 4], 4, 1, False, kv_dtype=torch.int8, kv_block=block)
+
+
+def test_allocation_checks_its_block():
+    from omnikv_b200 import abi, ops
+    for block in (0, 48, 512, -1):
+        with pytest.raises(abi.OmniKVError):
+            ops.kv8_alloc(1, 1, 64, block=block, dtype=torch.int8, device="cpu")
