@@ -291,7 +291,10 @@ class OmniKVMultiStageCache:
         self._alloc_layer(layer_idx, B, KVH, d, key_states.dtype, key_states.device)
         if self.is_kv8(layer_idx):
             from .. import ops
-            ops.kv8_store(key_states, value_states, *self._kv8[layer_idx], block=self.kv_block)
+            # rows as the kernel reads them: contiguous, 16-byte aligned
+            k, v = (t if t.stride(3) == 1 and not any(s % 8 for s in t.stride()[:3]) and t.data_ptr() % 16 == 0
+                    else t.clone(memory_format=torch.contiguous_format) for t in (key_states, value_states))
+            ops.kv8_store(k, v, *self._kv8[layer_idx], block=self.kv_block)
         elif self.is_offloaded(layer_idx):
             key, slot = self._host_key(layer_idx)
             last = layer_idx == self.num_hidden_layers - 1  # the reference blocks on the last layer (:320-329)

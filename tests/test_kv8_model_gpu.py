@@ -171,6 +171,20 @@ def test_cache_through_the_reference_api(kind, codes):
     assert cache.get_seq_length() == P + 3
 
 
+def test_a_prompt_of_any_layout_is_taken_over():
+    from omnikv_b200.modeling import OmniKVMultiStageCache
+    k, v = (torch.randn(1, 2, 70, 128, device="cuda").to(torch.bfloat16) for _ in range(2))
+    odd = torch.zeros(2 * 70 * 129 + 1, dtype=torch.bfloat16, device="cuda")[1:].view(1, 2, 70, 129)[..., :128]
+    odd.copy_(v)
+    got = []
+    for keys, values in ((k, v), (k.transpose(2, 3).contiguous().transpose(2, 3), odd)):
+        cache = OmniKVMultiStageCache([0, 2], 2, 0, False, kv_dtype=torch.int8, kv_block=16)
+        for i in range(2):
+            cache.update(keys, values, i)
+        got.append([t for i in range(2) for t in cache.kv8_rows(i, rows=70)])
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
 def test_synthetic_ragged_cache():
     from omnikv_b200.modeling import OmniKVMultiStageCache
     cache = OmniKVMultiStageCache([0, 3], 3, 0, False, kv_dtype=torch.int8, kv_block=16)
