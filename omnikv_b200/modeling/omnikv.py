@@ -448,6 +448,8 @@ class OmniKVMulLayer(nn.Module):
 
     def _select(self, hidden_states, position_embeddings, cache: OmniKVMultiStageCache) -> None:
         """Window selectors: scores from ``omnikv_score_window`` on the observation window's queries."""
+        if cache.is_kv8(self.layer_idx):
+            raise NotImplementedError(f"the window selectors read 16-bit keys: keep_layers of an 8-bit cache must name filter layer {self.layer_idx}")
         st, attn = cache.sel_state[self.layer_idx], self.self_attn
         B = hidden_states.shape[0]
         if "last" in self.selector_cls:  # "softmax_before_last": the current token only, no window bookkeeping

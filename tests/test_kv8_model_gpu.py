@@ -203,6 +203,8 @@ def test_refusals():
     with pytest.raises(NotImplementedError, match="8-bit"):
         select_tokens_by_attn_universal(attn, torch.zeros(1, 1, 512, device="cuda", dtype=torch.bfloat16),
                                         torch.zeros(1, 1, device="cuda"), out.past_key_values, 4, 40)
+    with pytest.raises(NotImplementedError, match="keep_layers"):
+        lm.model.layers[1]._select(torch.zeros(1, 1, 512, device="cuda", dtype=torch.bfloat16), None, out.past_key_values)
     with pytest.raises(NotImplementedError, match="kv_cache_dtype"):
         build(kv_cache_dtype="int4")(input_ids=tokens(1, 40, 0))
     with pytest.raises(NotImplementedError, match="real_offload"):
