@@ -859,7 +859,8 @@ class OmniKVMulLM(nn.Module):
         """Hold the projections of every layer (QKV, output, gate/up, down) as int8 codes with one scale per output channel
         and multiply them with per-token int8 activations (``omnikv_linear_w8a8``); the 16-bit matrices are given up.
         Embedding, norms and lm_head stay.  Decoding then runs through the modules (the fused batch-1 kernels stream 16-bit
-        weights)."""
+        weights).  ``state_dict`` holds codes and scales in the matrices' place; ``load_state_dict`` takes them into a model
+        that is quantised too."""
         for layer in self.model.layers:
             for owner, names in ((layer.self_attn, ("qkv", "o")), (layer.mlp, ("gate_up", "down"))):
                 for name in names:
@@ -867,8 +868,8 @@ class OmniKVMulLM(nn.Module):
                     if w is None:  # already done
                         continue
                     codes, scale = ops.quant_rows(w)
-                    owner.register_buffer(name + "_codes", codes, persistent=False)
-                    owner.register_buffer(name + "_scale", scale, persistent=False)
+                    owner.register_buffer(name + "_codes", codes)
+                    owner.register_buffer(name + "_scale", scale)
             layer._fused_cache.clear()
         self.config.linear_dtype = "int8"
         return self

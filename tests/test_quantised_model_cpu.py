@@ -1,0 +1,62 @@
+"""Projections held as int8 codes, on the host: what a model keeps, saves, loads and hands out.  The quantiser and the product
+are restated in plain torch (the kernels have no CPU path)."""
+import pytest
+import torch
+
+from oracle import kv8_oracle as ko
+
+
+def _quant_rows(x):
+    codes, scale = ko.quantise(x.double()[:, None], 1, "int8")
+    return codes[:, 0].to(torch.int8), scale[:, 0].float()
+
+
+def _linear_w8a8(x8, x_scale, w8, w_scale, *, out_dtype):
+    return ko.linear(x8, x_scale, w8, w_scale).to(out_dtype)
+
+
+@pytest.fixture(autouse=True)
+def on_the_host(monkeypatch):
+    from omnikv_b200 import ops
+    monkeypatch.setattr(ops, "quant_rows", _quant_rows)
+    monkeypatch.setattr(ops, "linear_w8a8", _linear_w8a8)
+
+
+def config(**omni):
+    from omnikv_b200.modeling import LlamaCompressorConfig
+    cfg = LlamaCompressorConfig(num_hidden_layers=2, hidden_size=256, intermediate_size=512, num_attention_heads=2,
+                                num_key_value_heads=1, vocab_size=64, head_dim=128)
+    cfg.set_config_of_compressor(model_cls="multi", cache_cls="multi", do_select_layers="1", num_wait_load_layers=0,
+                                 real_offload=False, dense_more=True, num_of_selected_tokens=0.25, selector_cls="last",
+                                 window_size=16, **omni)
+    return cfg
+
+
+def build(seed=0, dtype=torch.bfloat16, **omni):
+    from omnikv_b200.modeling import OmniKVMulLM
+    return OmniKVMulLM.from_config(config(**omni), dtype=dtype, device="cpu", seed=seed)
+
+
+OWNERS = (("self_attn", ("qkv", "o")), ("mlp", ("gate_up", "down")))
+
+
+def projections(lm):
+    return {f"{i}.{part}.{name}": (getattr(getattr(layer, part), name + "_codes"), getattr(getattr(layer, part), name + "_scale"))
+            for i, layer in enumerate(lm.model.layers) for part, names in OWNERS for name in names}
+
+
+def test_state_dict_holds_the_projections():
+    a, b = build(1, linear_dtype="int8"), build(2, linear_dtype="int8")
+    sd = a.state_dict()
+    assert sum(k.endswith("_codes") for k in sd) == sum(k.endswith("_scale") for k in sd) == 8
+    assert not all(torch.equal(x[0], y[0]) for x, y in zip(projections(a).values(), projections(b).values()))
+    b.load_state_dict(sd)
+    for name, (codes, scale) in projections(a).items():
+        assert torch.equal(codes, projections(b)[name][0]) and torch.equal(scale, projections(b)[name][1]), name
+
+
+@pytest.mark.parametrize("kinds", [(None, "int8"), ("int8", None)])
+def test_a_state_dict_of_the_other_kind_is_refused(kinds):
+    saved, target = (build(1, linear_dtype=kind) for kind in kinds)
+    with pytest.raises(RuntimeError, match="qkv_codes"):
+        target.load_state_dict(saved.state_dict())
