@@ -279,7 +279,19 @@ def _project(x: torch.Tensor, owner: nn.Module, name: str, rows: Optional[int] =
     return y.view(*x.shape[:-1], -1)
 
 
-class OmniKVAttention(nn.Module):
+class _Projections(nn.Module):
+    """A module whose fused matrices may be held as int8 codes with fp32 scales (``OmniKVMulLM.quantize_weights_``)."""
+
+    def _apply(self, fn, recurse=True):  # .to(), .half(): the scales move to another device but keep their 32 bits
+        scales = {name: t for name, t in self._buffers.items() if name.endswith("_scale")}
+        super()._apply(fn, recurse)
+        for name, t in scales.items():
+            if self._buffers[name].dtype != t.dtype:
+                self._buffers[name] = t.to(self._buffers[name].device)
+        return self
+
+
+class OmniKVAttention(_Projections):
     """The ``self_attn`` object of a layer: Llama attention with fused QKV weights whose decode path
     runs in ``omnikv_decode_attn`` through the cache."""
 
@@ -364,7 +376,7 @@ def _tc_linear_ok(config, x, inter=64) -> bool:
             and config.get("linear_dtype", None) is None)
 
 
-class OmniKVMLP(nn.Module):
+class OmniKVMLP(_Projections):
     def __init__(self, config, tp=None):
         super().__init__()
         self.tp = tp

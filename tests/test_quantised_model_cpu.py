@@ -60,3 +60,14 @@ def test_a_state_dict_of_the_other_kind_is_refused(kinds):
     saved, target = (build(1, linear_dtype=kind) for kind in kinds)
     with pytest.raises(RuntimeError, match="qkv_codes"):
         target.load_state_dict(saved.state_dict())
+
+
+@pytest.mark.parametrize("cast", [lambda m: m.to(torch.bfloat16), lambda m: m.half(), lambda m: m.double().to(torch.bfloat16),
+                                  lambda m: m.to("cpu", torch.float16)])
+def test_scales_stay_fp32_when_the_model_is_cast(cast):
+    lm = build(1, linear_dtype="int8")
+    before = {name: (c.clone(), s.clone()) for name, (c, s) in projections(lm).items()}
+    assert cast(lm) is lm
+    for name, (codes, scale) in projections(lm).items():
+        assert codes.dtype is torch.int8 and scale.dtype is torch.float32, name
+        assert torch.equal(codes, before[name][0]) and torch.equal(scale, before[name][1]), name
