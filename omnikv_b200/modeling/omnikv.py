@@ -254,28 +254,34 @@ class RMSNorm(nn.Module):
 
 
 class _ProjView:
-    """``q_proj`` / ``k_proj`` / ... as views of a fused weight: callable and with ``.weight``."""
+    """``q_proj`` / ``k_proj`` / ... as rows ``[lo, hi)`` of a fused matrix: callable, and with ``.weight`` where the matrix is
+    held in the model's type."""
 
     def __init__(self, owner, name, lo, hi):
         self._owner, self._name, self._lo, self._hi = owner, name, lo, hi
 
     @property
     def weight(self):
-        return getattr(self._owner, self._name)[self._lo:self._hi]
+        if getattr(self._owner, self._name + "_codes", None) is not None:
+            raise RuntimeError(_CODES_HELD)
+        return getattr(self._owner, self._name + "_weight")[self._lo:self._hi]
 
     def __call__(self, x):
-        return F.linear(x, self.weight)
+        return _project(x, self._owner, self._name, self._lo, self._hi)
 
 
-def _project(x: torch.Tensor, owner: nn.Module, name: str, rows: Optional[int] = None) -> torch.Tensor:
-    """``x @ owner.<name>_weight.T`` (its first ``rows`` rows) for x ``[..., K]``: the library product, or the 8-bit integer
+_CODES_HELD = "the projections are held as int8 codes (quantize_weights_): load or read weights before that"
+
+
+def _project(x: torch.Tensor, owner: nn.Module, name: str, lo: int = 0, hi: Optional[int] = None) -> torch.Tensor:
+    """``x @ owner.<name>_weight.T`` (its rows ``[lo, hi)``) for x ``[..., K]``: the library product, or the 8-bit integer
     one when the weight is held as int8 codes (``OmniKVMulLM.quantize_weights_``)."""
     codes = getattr(owner, name + "_codes", None)
     if codes is None:
         w = getattr(owner, name + "_weight")
-        return F.linear(x, w if rows is None else w[:rows])
+        return F.linear(x, w if hi is None else w[lo:hi])
     x8, x_scale = ops.quant_rows(x.reshape(-1, x.shape[-1]))
-    y = ops.linear_w8a8(x8, x_scale, codes[:rows], getattr(owner, name + "_scale")[:rows], out_dtype=x.dtype)
+    y = ops.linear_w8a8(x8, x_scale, codes[lo:hi], getattr(owner, name + "_scale")[lo:hi], out_dtype=x.dtype)
     return y.view(*x.shape[:-1], -1)
 
 
@@ -312,10 +318,10 @@ class OmniKVAttention(_Projections):
         nq, nkv = self.num_heads * self.head_dim, self.num_key_value_heads * self.head_dim
         self.qkv_weight = nn.Parameter(torch.empty(nq + 2 * nkv, self.hidden_size))
         self.o_weight = nn.Parameter(torch.empty(self.hidden_size, nq))
-        self.q_proj = _ProjView(self, "qkv_weight", 0, nq)
-        self.k_proj = _ProjView(self, "qkv_weight", nq, nq + nkv)
-        self.v_proj = _ProjView(self, "qkv_weight", nq + nkv, nq + 2 * nkv)
-        self.o_proj = _ProjView(self, "o_weight", 0, self.hidden_size)
+        self.q_proj = _ProjView(self, "qkv", 0, nq)
+        self.k_proj = _ProjView(self, "qkv", nq, nq + nkv)
+        self.v_proj = _ProjView(self, "qkv", nq + nkv, nq + 2 * nkv)
+        self.o_proj = _ProjView(self, "o", 0, self.hidden_size)
         # every layer reads the model's one rotary module (same frequencies everywhere, one dynamic update per step)
         self.rotary_emb = rotary_emb if rotary_emb is not None else OmniKVRotaryEmbedding(config)
 
@@ -384,9 +390,9 @@ class OmniKVMLP(_Projections):
         self.intermediate_size = config.intermediate_size // (tp.world if tp is not None else 1)  # local slice
         self.gate_up_weight = nn.Parameter(torch.empty(2 * self.intermediate_size, config.hidden_size))
         self.down_weight = nn.Parameter(torch.empty(config.hidden_size, self.intermediate_size))
-        self.gate_proj = _ProjView(self, "gate_up_weight", 0, self.intermediate_size)
-        self.up_proj = _ProjView(self, "gate_up_weight", self.intermediate_size, 2 * self.intermediate_size)
-        self.down_proj = _ProjView(self, "down_weight", 0, config.hidden_size)
+        self.gate_proj = _ProjView(self, "gate_up", 0, self.intermediate_size)
+        self.up_proj = _ProjView(self, "gate_up", self.intermediate_size, 2 * self.intermediate_size)
+        self.down_proj = _ProjView(self, "down", 0, config.hidden_size)
 
     def forward(self, x):
         if _tc_linear_ok(self.config, x, self.intermediate_size):  # opt-in: this package's tcgen05 weight stream
@@ -474,7 +480,7 @@ class OmniKVMulLayer(nn.Module):
                 self.hidden_state_window = win.contiguous()
             window_hs = self.hidden_state_window
         W = window_hs.shape[1]
-        q = _project(window_hs, attn, "qkv", attn.num_heads * attn.head_dim)
+        q = _project(window_hs, attn, "qkv", 0, attn.num_heads * attn.head_dim)
         rope_pos = getattr(cache, "rope_pos_dev", None)
         if (rope_pos is not None and q.is_cuda and attn.head_dim == 128 and attn.rotary_emb.attention_scaling == 1.0
                 and self.config.get("fused_small_ops", True)):
@@ -929,7 +935,7 @@ class OmniKVMulLM(nn.Module):
 
     def _need_weights(self) -> None:
         if getattr(self.model.layers[0].self_attn, "qkv_codes", None) is not None:
-            raise RuntimeError("the projections are held as int8 codes (quantize_weights_): load or read weights before that")
+            raise RuntimeError(_CODES_HELD)
 
     @torch.no_grad()
     def prepare_synthetic_decode(self, batch: int, seed: int = 0) -> None:

@@ -218,3 +218,19 @@ def test_refusals():
     from omnikv_b200.abi import OmniKVError
     with pytest.raises(OmniKVError, match="bfloat16 or float16"):
         build(torch.float32, kv_cache_dtype="int8")(input_ids=tokens(1, 40, 0))
+
+
+@pytest.mark.parametrize("selector", ["last", "exp"])
+def test_the_selector_function_reads_int8_projections(selector, monkeypatch):
+    """``select_tokens_by_attn_universal`` on a model with int8 projections and a 16-bit cache: the queries are those of the
+    8-bit product."""
+    from omnikv_b200.modeling import omnikv, select_tokens_by_attn_universal
+    lm = build(linear_dtype="int8", selector_cls=selector)
+    cache = lm(input_ids=tokens(1, 300, 8)).past_key_values
+    attn = lm.model.layers[1].self_attn
+    hs = torch.randn(1, 1 if selector == "last" else 16, 512, generator=torch.Generator().manual_seed(9)).cuda().to(torch.bfloat16)
+    pos = torch.full((1, 1), 300, device="cuda")
+    got = select_tokens_by_attn_universal(attn, hs, pos, cache, 40, 300, selector_cls=selector)
+    q = omnikv._project(hs, attn, "qkv")[..., :512]
+    monkeypatch.setattr(attn, "q_proj", lambda x: q)
+    assert got.shape == (1, 40) and torch.equal(got, select_tokens_by_attn_universal(attn, hs, pos, cache, 40, 300, selector_cls=selector))

@@ -71,3 +71,22 @@ def test_scales_stay_fp32_when_the_model_is_cast(cast):
     for name, (codes, scale) in projections(lm).items():
         assert codes.dtype is torch.int8 and scale.dtype is torch.float32, name
         assert torch.equal(codes, before[name][0]) and torch.equal(scale, before[name][1]), name
+
+
+@pytest.mark.parametrize("kind", [None, "int8"])
+def test_projection_views_multiply_with_what_is_held(kind):
+    from omnikv_b200.modeling.omnikv import _project
+    lm = build(3, linear_dtype=kind)
+    x = torch.randn(2, 5, 256, generator=torch.Generator().manual_seed(0)).to(torch.bfloat16)
+    act = torch.randn(2, 5, 512, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16)
+    for layer in lm.model.layers:
+        a, mlp = layer.self_attn, layer.mlp
+        assert torch.equal(torch.cat([a.q_proj(x), a.k_proj(x), a.v_proj(x)], -1), _project(x, a, "qkv"))
+        assert torch.equal(torch.cat([mlp.gate_proj(x), mlp.up_proj(x)], -1), _project(x, mlp, "gate_up"))
+        assert torch.equal(a.o_proj(x), _project(x, a, "o")) and torch.equal(mlp.down_proj(act), _project(act, mlp, "down"))
+        for view in (a.q_proj, a.k_proj, a.v_proj, a.o_proj, mlp.gate_proj, mlp.up_proj, mlp.down_proj):
+            if kind is None:
+                assert view.weight.dtype is torch.bfloat16
+                continue
+            with pytest.raises(RuntimeError, match="int8 codes"):
+                view.weight
