@@ -861,7 +861,6 @@ class OmniKVMulLM(nn.Module):
                 for k in f.keys():
                     sd[k] = f.get_tensor(k)
         m.load_hf_state_dict(sd)
-        m._apply_linear_dtype()
         return m
 
     def _apply_linear_dtype(self) -> None:
@@ -894,6 +893,7 @@ class OmniKVMulLM(nn.Module):
 
     @torch.no_grad()
     def load_hf_state_dict(self, sd):
+        """Weights under their Hugging Face Llama names; held as the config's ``linear_dtype`` says from then on."""
         tp = self.tp
         self._need_weights()
 
@@ -917,6 +917,7 @@ class OmniKVMulLM(nn.Module):
             put(mlp.down_proj.weight, sd[p + "mlp.down_proj.weight"], 1)
             put(layer.input_layernorm.weight, sd[p + "input_layernorm.weight"])
             put(layer.post_attention_layernorm.weight, sd[p + "post_attention_layernorm.weight"])
+        self._apply_linear_dtype()
 
     def hf_state_dict(self):
         """Weights under their Hugging Face Llama names (views of the fused tensors)."""

@@ -90,3 +90,14 @@ def test_projection_views_multiply_with_what_is_held(kind):
                 continue
             with pytest.raises(RuntimeError, match="int8 codes"):
                 view.weight
+
+
+def test_weights_loaded_later_are_quantised_as_the_config_says():
+    source, lm = build(4), build(seed=None, linear_dtype="int8")
+    lm.load_hf_state_dict(source.hf_state_dict())
+    want = projections(source.quantize_weights_())
+    for name, (codes, scale) in projections(lm).items():
+        assert torch.equal(codes, want[name][0]) and torch.equal(scale, want[name][1]), name
+    bad = build(seed=None, linear_dtype="int4")
+    with pytest.raises(NotImplementedError, match="linear_dtype"):
+        bad.load_hf_state_dict(build(4).hf_state_dict())
