@@ -881,10 +881,11 @@ class OmniKVMulLM(nn.Module):
         for layer in self.model.layers:
             for owner, names in ((layer.self_attn, ("qkv", "o")), (layer.mlp, ("gate_up", "down"))):
                 for name in names:
-                    w = owner._parameters.pop(name + "_weight", None)
+                    w = owner._parameters.get(name + "_weight")
                     if w is None:  # already done
                         continue
                     codes, scale = ops.quant_rows(w)
+                    del owner._parameters[name + "_weight"]
                     owner.register_buffer(name + "_codes", codes)
                     owner.register_buffer(name + "_scale", scale)
             layer._fused_cache.clear()

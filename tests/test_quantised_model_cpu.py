@@ -101,3 +101,27 @@ def test_weights_loaded_later_are_quantised_as_the_config_says():
     bad = build(seed=None, linear_dtype="int4")
     with pytest.raises(NotImplementedError, match="linear_dtype"):
         bad.load_hf_state_dict(build(4).hf_state_dict())
+
+
+def test_a_refused_quantisation_leaves_the_weights(monkeypatch):
+    from omnikv_b200 import ops
+    lm = build(5)
+    want = {k: v.clone() for k, v in lm.state_dict().items()}
+    calls = []
+
+    def refuse_the_third(w):
+        calls.append(w)
+        if len(calls) == 3:
+            raise ops.abi.OmniKVError("refused")
+        return _quant_rows(w)
+
+    monkeypatch.setattr(ops, "quant_rows", refuse_the_third)
+    with pytest.raises(ops.abi.OmniKVError):
+        lm.quantize_weights_()
+    first = lm.model.layers[0]
+    assert torch.equal(first.mlp.gate_up_weight, want["model.layers.0.mlp.gate_up_weight"])
+    assert first.mlp.gate_proj(torch.zeros(1, 256, dtype=torch.bfloat16)).shape == (1, 512)
+    assert torch.equal(lm.model.layers[1].self_attn.qkv_weight, want["model.layers.1.self_attn.qkv_weight"])
+    monkeypatch.setattr(ops, "quant_rows", _quant_rows)
+    for name, (codes, scale) in projections(lm.quantize_weights_()).items():
+        assert torch.equal(codes, projections(build(5).quantize_weights_())[name][0]), name
