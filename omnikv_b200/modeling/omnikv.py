@@ -288,6 +288,8 @@ def _project(x: torch.Tensor, owner: nn.Module, name: str, lo: int = 0, hi: Opti
 class _Projections(nn.Module):
     """A module whose fused matrices may be held as int8 codes with fp32 scales (``OmniKVMulLM.quantize_weights_``)."""
 
+    holds_codes = False  # some matrix of the model is: its layers then decode through the modules
+
     def _apply(self, fn, recurse=True):  # .to(), .half(): the scales move to another device but keep their 32 bits
         scales = {name: t for name, t in self._buffers.items() if name.endswith("_scale")}
         super()._apply(fn, recurse)
@@ -341,7 +343,7 @@ class OmniKVAttention(_Projections):
         if (n == 1 and rope_pos is not None and hidden_states.is_cuda and self.head_dim == 128
                 and self.rotary_emb.attention_scaling == 1.0):
             # decode: rotate q and k and append k, v to the cache in one kernel, straight from the fused projection
-            tc = _tc_linear_ok(self.config, hidden_states)
+            tc = not self.holds_codes and _tc_linear_ok(self.config, hidden_states)
             x2 = hidden_states.view(B, -1)
             qkv = ops.batched_linear(x2, self.qkv_weight) if tc else _project(x2, self, "qkv")
             q = torch.empty(B, self.num_heads, self.head_dim, dtype=qkv.dtype, device=qkv.device)
@@ -378,8 +380,7 @@ def _tc_linear_ok(config, x, inter=64) -> bool:
     """Decode-sized activations (at most 16 tokens, 16-bit, on the GPU) and ``tcgen05_linear`` switched on: the
     projections go through ``omnikv_batched_linear`` instead of the library GEMM."""
     return (x.is_cuda and x.dtype in (torch.bfloat16, torch.float16) and x.shape[-2] == 1 and x.numel() // x.shape[-1] <= 16
-            and inter % 64 == 0 and x.shape[-1] % 8 == 0 and config.get("tcgen05_linear", False)
-            and config.get("linear_dtype", None) is None)
+            and inter % 64 == 0 and x.shape[-1] % 8 == 0 and config.get("tcgen05_linear", False))
 
 
 class OmniKVMLP(_Projections):
@@ -395,7 +396,7 @@ class OmniKVMLP(_Projections):
         self.down_proj = _ProjView(self, "down", 0, config.hidden_size)
 
     def forward(self, x):
-        if _tc_linear_ok(self.config, x, self.intermediate_size):  # opt-in: this package's tcgen05 weight stream
+        if not self.holds_codes and _tc_linear_ok(self.config, x, self.intermediate_size):  # opt-in: this package's tcgen05 weight stream
             x2 = x.reshape(-1, x.shape[-1])
             act = ops.batched_linear(x2, self.gate_up_weight, epilogue="swiglu")
             o = ops.batched_linear(act, self.down_weight).view(*x.shape[:-1], -1)
@@ -434,6 +435,10 @@ class OmniKVMulLayer(nn.Module):
         self.decode_step = 0
         self.is_filter = layer_idx in self.do_select_layers
         self._fused_cache = {}
+
+    @property
+    def holds_codes(self) -> bool:
+        return self.self_attn.holds_codes
 
     # -- selection state -------------------------------------------------------------------------
     def _init_selection_state(self, cache: OmniKVMultiStageCache, device) -> None:
@@ -523,15 +528,14 @@ class OmniKVMulLayer(nn.Module):
 
     # -- batch-1 decode through the fused weight-streaming kernels -----------------------------------
     def _fused_ok(self, hidden_states) -> bool:
-        if hidden_states.shape[0] != 1 or hidden_states.shape[1] != 1 or not hidden_states.is_cuda:
+        if hidden_states.shape[0] != 1 or hidden_states.shape[1] != 1 or not hidden_states.is_cuda or self.holds_codes:
             return False
         key = hidden_states.dtype
         ok = self._fused_cache.get(key)
         if ok is None:
             a = self.self_attn
             # the fused QKV kernel rotates with cos/sin of pos * inv_freq: no attention scaling (yarn, longrope)
-            ok = self.config.get("fused_decode", True) and self.config.get("linear_dtype", None) is None \
-                and a.rotary_emb.attention_scaling == 1.0 and ops.fused_decode_supported(
+            ok = self.config.get("fused_decode", True) and a.rotary_emb.attention_scaling == 1.0 and ops.fused_decode_supported(
                 key, self.config.hidden_size, self.mlp.intermediate_size, a.num_heads * a.head_dim, 8)
             self._fused_cache[key] = ok
         return ok
@@ -885,11 +889,11 @@ class OmniKVMulLM(nn.Module):
                     if w is None:  # already done
                         continue
                     codes, scale = ops.quant_rows(w)
+                    for other in self.model.layers:
+                        other.self_attn.holds_codes = other.mlp.holds_codes = True
                     del owner._parameters[name + "_weight"]
                     owner.register_buffer(name + "_codes", codes)
                     owner.register_buffer(name + "_scale", scale)
-            layer._fused_cache.clear()
-        self.config.linear_dtype = "int8"
         return self
 
     @torch.no_grad()

@@ -234,3 +234,36 @@ def test_the_selector_function_reads_int8_projections(selector, monkeypatch):
     q = omnikv._project(hs, attn, "qkv")[..., :512]
     monkeypatch.setattr(attn, "q_proj", lambda x: q)
     assert got.shape == (1, 40) and torch.equal(got, select_tokens_by_attn_universal(attn, hs, pos, cache, 40, 300, selector_cls=selector))
+
+
+@pytest.mark.parametrize("part", [0, 5, 24])
+def test_a_model_quantised_in_part_decodes_as_its_modules_do(part, monkeypatch):
+    """Where the quantiser refuses a matrix the ones before it are codes and the rest 16-bit: batch-1 decoding then runs
+    through the modules for every layer (the fused kernels hand the residual stream on in another way)."""
+    from omnikv_b200 import ops
+    real = ops.quant_rows
+    ids, got = tokens(1, 200, 11), []
+    for fused in (True, False):
+        lm, calls = build(fused_decode=fused), []
+
+        def quant(w):
+            calls.append(w)
+            if len(calls) > part:
+                raise ops.abi.OmniKVError("refused")
+            return real(w)
+
+        with monkeypatch.context() as m:
+            m.setattr(ops, "quant_rows", quant)
+            if part == 24:
+                lm.quantize_weights_()
+            else:
+                with pytest.raises(ops.abi.OmniKVError):
+                    lm.quantize_weights_()
+        cache = lm(input_ids=ids).past_key_values
+        cache.stage = "decoding"
+        got.append(torch.stack([lm._decode_step(tokens(1, 1, 20 + t), cache)[0].clone() for t in range(6)]))
+        assert lm.model.layers[5].holds_codes is (part > 0)
+    if part:
+        assert torch.equal(*got)
+    else:  # nothing was changed: the fused kernels decode, whose sums run in another order
+        assert torch.nn.functional.cosine_similarity(got[0].flatten().double(), got[1].flatten().double(), 0) > 0.99

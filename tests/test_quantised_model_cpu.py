@@ -125,3 +125,14 @@ def test_a_refused_quantisation_leaves_the_weights(monkeypatch):
     monkeypatch.setattr(ops, "quant_rows", _quant_rows)
     for name, (codes, scale) in projections(lm.quantize_weights_()).items():
         assert torch.equal(codes, projections(build(5).quantize_weights_())[name][0]), name
+
+
+def test_quantising_one_model_leaves_the_config_and_others_alone():
+    from omnikv_b200.modeling import OmniKVMulLM
+    cfg = config()
+    a = OmniKVMulLM.from_config(cfg, device="cpu", seed=1).quantize_weights_()
+    assert cfg.get("linear_dtype", None) is None
+    b = OmniKVMulLM.from_config(cfg, device="cpu", seed=1)
+    assert "model.layers.0.mlp.down_codes" in a.state_dict() and "model.layers.0.mlp.down_weight" in b.state_dict()
+    for model, held in ((a, True), (b, False)):  # the fused kernels are kept from layers by what those hold
+        assert all(layer.holds_codes is held for layer in model.model.layers)
