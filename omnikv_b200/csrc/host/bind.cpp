@@ -362,9 +362,7 @@ PyObject* quant_rows(PyObject* const* a) {
     refuse("quant_rows: x must be [n, K] with contiguous rows and K a multiple of 16");
   const int64_t n = x.size(0), K = x.size(1);
   OnDevice on(dev);
-  const size_t bytes = (size_t)n * K;  // a multiple of 16
-  const c10::Storage both = memory(bytes + n * sizeof(float));
-  const at::Tensor codes = tensor_in(both, 0, {n, K}, at::kChar), scale = tensor_in(both, bytes, {n}, at::kFloat);
+  const at::Tensor codes = fresh({n, K}, at::kChar), scale = fresh({n}, at::kFloat);
   if (n) {
     done(abi.quant_rows(dt, x.data_ptr(), step(x, 0), (int)n, (int)K, static_cast<int8_t*>(codes.data_ptr()), K,
                         static_cast<float*>(scale.data_ptr()), on.stream),

@@ -235,3 +235,12 @@ def test_refusals():
             call()
             raise AssertionError(f"call {i} was not refused")
     assert o.linear_w8a8(x8[:0], sx[:0], w8, sw).shape == (0, 32)
+
+
+def test_codes_and_scales_have_memory_of_their_own(tmp_path):
+    """Results of a call can be saved together, and one of them does not hold the other's memory."""
+    codes, scale = ops().quant_rows(torch.randn(48, 640, device="cuda").to(torch.bfloat16))
+    assert codes.untyped_storage().nbytes() == 48 * 640 and scale.untyped_storage().nbytes() == 48 * 4
+    torch.save((codes, scale), tmp_path / "w.pt")
+    for a, b in zip(torch.load(tmp_path / "w.pt"), (codes, scale)):
+        assert torch.equal(a, b)
