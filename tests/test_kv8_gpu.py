@@ -181,6 +181,14 @@ def test_load_by_index():
     assert torch.equal(some_k, all_k[:, :, 33:83])
 
 
+def test_loaded_keys_and_values_have_memory_of_their_own():
+    cache, _, _ = filled(1, 2, 40, "int8", torch.bfloat16, 16, 13)
+    for pair in (ops().kv8_load(*cache, block=16, dtype=torch.bfloat16), ops().kv8_load(*cache, block=16, dtype=torch.bfloat16, rows=0),
+                 ops().kv8_load(*cache, block=16, dtype=torch.float16, idx=i32([[3, 1, 4]]))):
+        for t in pair:
+            assert t.is_contiguous() and t.untyped_storage().nbytes() == t.numel() * 2
+
+
 # ---------------------------------------------------------------------------------------------- append
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("fmt", ["int8", "e4m3"])
