@@ -14,6 +14,7 @@
 
 #include "kv8.cuh"
 #include "tc05.cuh"
+#include "tile_work.cuh"
 
 namespace omnikv {
 namespace {
@@ -315,39 +316,15 @@ linear_tile_kernel(const LinArgs a, const __grid_constant__ CUtensorMap tm_w, co
   __syncthreads();
   tc_fence_after();
   const unsigned tmem = sh.tmem_base;
-  // this CTA's work: the piece [lo, hi) of the shared tiles' chunks, then whole tiles
-  const int chunks = a.chunks, tiles = ceil_div(a.N, TK_M), whole_tiles = tiles - a.shared, C = gridDim.x, cta = blockIdx.x;
-  const int total = a.shared * chunks;  // the host keeps it below 2^31
-  const int S = a.sharers;
-  const auto piece_lo = [&](int i) { return S ? (int)((long long)min(i, S) * total / S) : 0; };
-  struct Unit {
-    int tile, k0, k1;
-  };
-  const int lo = piece_lo(cta), hi = piece_lo(cta + 1);
-  const auto first_unit = [&](Unit& u) {  // false: no work
-    if (lo < hi) u = Unit{whole_tiles + lo / chunks, lo % chunks, min(chunks, lo % chunks + hi - lo)};
-    else u = Unit{cta, 0, chunks};
-    return lo < hi || cta < whole_tiles;
-  };
-  const auto next_unit = [&](Unit& u) {
-    if (u.tile >= whole_tiles) {
-      const int at = (u.tile - whole_tiles) * chunks + u.k1;
-      if (at < hi) {
-        u = Unit{u.tile + 1, 0, min(chunks, hi - at)};
-        return true;
-      }
-      u = Unit{cta, 0, chunks};
-    } else {
-      u.tile += C;
-    }
-    return u.tile < whole_tiles;
-  };
+  const int tiles = ceil_div(a.N, TK_M);
+  const TileWork work(tiles, a.shared, a.sharers, a.chunks, gridDim.x, blockIdx.x);  // the host keeps shared * chunks below 2^31
+  using Unit = TileWork::Unit;
   // While the kernel before finishes, this CTA's first weights start on their way into L2 (16 x 4096 x 28672: 22.8 -> 21.8 us,
   // 64 x 8192 x 20000: 34.5 -> 33.2); with fewer tiles than SMs it loses (16 x 4096 x 10240: 12.3, 13.1).
   if (tid == 128 && tiles >= TK_CTAS) {
     Unit u;
     int n = 0;
-    for (bool more = first_unit(u); more && n < STAGES; more = next_unit(u))
+    for (bool more = work.first(u); more && n < STAGES; more = work.next(u))
       for (int k = u.k0; k < u.k1 && n < STAGES; ++k, ++n)
         asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];\n" ::"l"(reinterpret_cast<uint64_t>(&tm_w)),
                      "r"(k * TK_KB), "r"(u.tile * TK_M)
@@ -361,7 +338,7 @@ linear_tile_kernel(const LinArgs a, const __grid_constant__ CUtensorMap tm_w, co
     if (lane == 0) {
       int it = 0;
       Unit u;
-      for (bool more = first_unit(u); more && !sh.fail; more = next_unit(u)) {
+      for (bool more = work.first(u); more && !sh.fail; more = work.next(u)) {
         for (int k = u.k0; k < u.k1; ++k, ++it) {
           const int st = it % STAGES;
           if (!mbar_wait(&sh.empty[st], ((it / STAGES) & 1) ^ 1, &sh.fail)) {
@@ -383,7 +360,7 @@ linear_tile_kernel(const LinArgs a, const __grid_constant__ CUtensorMap tm_w, co
       bool ok = true;
       int it = 0, n = 0;
       Unit u;
-      for (bool more = first_unit(u); ok && more; more = next_unit(u), ++n) {
+      for (bool more = work.first(u); ok && more; more = work.next(u), ++n) {
         const int buf = n & 1;
         if (!mbar_wait(&sh.acc_empty[buf], ((n >> 1) & 1) ^ 1, &sh.fail)) { ok = false; break; }
         tc_fence_after();
@@ -410,9 +387,16 @@ linear_tile_kernel(const LinArgs a, const __grid_constant__ CUtensorMap tm_w, co
     for (int j = tid; j < tokens; j += 128) sh.x_scale[j] = a.x_scale[j];
     int n = 0;
     Unit u;
-    for (bool more = first_unit(u); more; more = next_unit(u), ++n) {
+    const auto arrive = [&](const TileWork::Party& p) {  // by one thread; true: the last of them
+      __threadfence();  // the stores, ordered before the barrier, are visible before the arrival is
+      const bool last = atomicAdd(a.counters + p.first, 1) == p.parts - 1;
+      if (last) a.counters[p.first] = 0;  // nobody else touches it any more in this call
+      __threadfence();
+      return last;
+    };
+    for (bool more = work.first(u); more; more = work.next(u), ++n) {
       const int buf = n & 1, tile = u.tile, c = tile * TK_M + tid;
-      const bool whole = u.k1 - u.k0 == chunks;
+      const bool whole = work.whole(u);
       const bool in = c < a.N;
       Channel<T> ch{in && a.res ? static_cast<const T*>(a.res) + c : nullptr, in ? static_cast<T*>(a.out) + c : nullptr,
                     a.res_sr, a.out_sr, tokens, in ? a.w_scale[c] : 0.f};
@@ -421,11 +405,12 @@ linear_tile_kernel(const LinArgs a, const __grid_constant__ CUtensorMap tm_w, co
       if (epilogue_any<128>(!got)) {  // the 128 threads leave together
         if (!sh.fail && a.status) atomicExch(a.status, 7);
         sh.fail = 1;
+        if (tid == 0) work.give_up(u, arrive);  // the counters end at zero whoever failed: the workspace is used again
         break;
       }
       tc_fence_after();
       const unsigned src = tmem + ((unsigned)(warp * 32) << 16) + (unsigned)buf * BN;
-      int* part = a.part + (size_t)(cta + tile - whole_tiles) * BN * TK_M + tid;  // (CTA, tile) pairs walk a staircase: their sum is unique
+      int* part = a.part + (size_t)(work.cta + tile - work.whole_tiles) * BN * TK_M + tid;  // (CTA, tile) pairs walk a staircase: their sum is unique
 #pragma unroll 1
       for (int j0 = 0; j0 < tokens; j0 += 16) {
         int v[16];
@@ -441,24 +426,13 @@ linear_tile_kernel(const LinArgs a, const __grid_constant__ CUtensorMap tm_w, co
       tc_fence_before();
       mbar_arrive(&sh.acc_empty[buf]);
       if (!whole) {
-        // the CTAs that share the tile: from the one that has its first chunk to the one that has its last
-        const auto owner = [&](int chunk) {
-          int i = min(S - 1, (int)(((float)chunk + 0.5f) * (float)S / (float)total));
-          while (piece_lo(i) > chunk) --i;
-          while (piece_lo(i + 1) <= chunk) ++i;
-          return i;
-        };
-        const int at = (tile - whole_tiles) * chunks, first = owner(at), parts = owner(at + chunks - 1) - first + 1;
+        const TileWork::Party p = work.party(tile);
+        const int parts = p.parts;
         epilogue_bar();
-        if (tid == 0) {
-          __threadfence();  // the stores, ordered before the barrier, are visible before the arrival is
-          sh.last = atomicAdd(a.counters + first, 1) == parts - 1;
-          if (sh.last) a.counters[first] = 0;  // nobody else touches it any more in this call
-          __threadfence();
-        }
+        if (tid == 0) sh.last = arrive(p);
         epilogue_bar();
         if (sh.last) {
-          const int* all = a.part + (size_t)(first + tile - whole_tiles) * BN * TK_M + tid;
+          const int* all = a.part + (size_t)(p.first + tile - work.whole_tiles) * BN * TK_M + tid;
           const auto fetch = [&](int q, int j0, int (&v)[16]) {  // 16 tokens of partial q (the columns behind the tokens are there too)
 #pragma unroll
             for (int j = 0; j < 16; ++j) v[j] = q < parts && j0 < tokens ? __ldcg(all + ((size_t)q * BN + j0 + j) * TK_M) : 0;
