@@ -279,7 +279,7 @@ struct Channel {
 
 struct TkShared {
   float x_scale[128];
-  uint64_t full[8], empty[8], acc_full[2], acc_empty[2];
+  uint64_t full[8], empty[8], acc_full[2], acc_empty[2], drained;
   unsigned tmem_base;
   int fail, issued, last;
 };
@@ -305,6 +305,7 @@ linear_tile_kernel(const LinArgs a, const __grid_constant__ CUtensorMap tm_w, co
       mbar_init(&sh.acc_full[i], 1);
       mbar_init(&sh.acc_empty[i], 128);
     }
+    mbar_init(&sh.drained, 1);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
   __syncwarp();
@@ -466,8 +467,12 @@ linear_tile_kernel(const LinArgs a, const __grid_constant__ CUtensorMap tm_w, co
   // ---- teardown ----
   tc_fence_before();
   __syncthreads();
-  if (sh.fail) {
-    if (tid == 128) {  // wait (bounded) for the last requested tile of every stage before the memory is given up
+  if (sh.fail) {  // wait (bounded) for what is in flight before the memories are given up:
+    if (tid == 160) {  // the MMAs, by the thread that issued them,
+      tc_commit(&sh.drained);
+      mbar_wait(&sh.drained, 0);
+    }
+    if (tid == 128) {  // and the last requested tile of every stage
       for (int st = 0; st < STAGES; ++st) {
         const int last = sh.issued - 1 - ((sh.issued - 1 - st) % STAGES + STAGES) % STAGES;
         if (sh.issued > st && last >= 0) mbar_wait(&sh.full[st], (last / STAGES) & 1);
@@ -511,13 +516,24 @@ __device__ __forceinline__ void pair_commit(uint64_t* bar) {  // arrives at this
                "h"((unsigned short)3)
                : "memory");
 }
+__device__ __forceinline__ void pair_commit_here(uint64_t* bar) {  // ... in this CTA only
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void st_cluster(unsigned addr, int v) {
+  asm volatile("st.shared::cluster.s32 [%0], %1;\n" ::"r"(addr), "r"(v) : "memory");
+}
+__device__ __forceinline__ int ld_cluster(unsigned addr) {
+  int v;
+  asm volatile("ld.shared::cluster.s32 %0, [%1];\n" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
 __device__ __forceinline__ void remote_arrive(unsigned bar_cluster) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(bar_cluster) : "memory");
 }
 
 struct PkShared {
   float x_scale[256];
-  uint64_t full[PK_STAGES], empty[PK_STAGES], acc_full[2], acc_empty[2];
+  uint64_t full[PK_STAGES], empty[PK_STAGES], acc_full[2], acc_empty[2], drained;
   unsigned tmem_base;
   int fail, issued;
 };
@@ -543,6 +559,7 @@ linear_pair_kernel(const LinArgs a, const int BN, const __grid_constant__ CUtens
       mbar_init(&sh.acc_full[i], 1);
       mbar_init(&sh.acc_empty[i], 16);  // the epilogue warps of both CTAs
     }
+    mbar_init(&sh.drained, 1);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
   __syncwarp();
@@ -557,6 +574,11 @@ linear_pair_kernel(const LinArgs a, const int BN, const __grid_constant__ CUtens
   const unsigned tmem = sh.tmem_base;
   pdl_wait();
   pdl_trigger();
+  const auto give_up = [&]() {  // a wait ran out: both CTAs of the pair stop
+    if (!sh.fail && a.status) atomicExch(a.status, 7);
+    sh.fail = 1;
+    st_cluster(in_cta(smem_u32(&sh.fail), rank ^ 1), 1);
+  };
 
   if (warp == 8) {
     if (lane == 0) {
@@ -566,8 +588,7 @@ linear_pair_kernel(const LinArgs a, const int BN, const __grid_constant__ CUtens
         for (int k = 0; k < a.chunks; ++k, ++it) {
           const int st = it % PK_STAGES;
           if (!mbar_wait(&sh.empty[st], ((it / PK_STAGES) & 1) ^ 1, &sh.fail)) {
-            if (!sh.fail && a.status) atomicExch(a.status, 7);
-            sh.fail = 1;
+            give_up();
             break;
           }
           unsigned char* dst = ring + (size_t)st * PK_STAGE;
@@ -601,10 +622,7 @@ linear_pair_kernel(const LinArgs a, const int BN, const __grid_constant__ CUtens
         }
         if (ok) pair_commit(&sh.acc_full[buf]);
       }
-      if (!ok) {
-        if (!sh.fail && a.status) atomicExch(a.status, 7);
-        sh.fail = 1;
-      }
+      if (!ok) give_up();
     }
   } else {
     const int quarter = warp & 3, half = warp >> 2;
@@ -619,8 +637,7 @@ linear_pair_kernel(const LinArgs a, const int BN, const __grid_constant__ CUtens
       ch.ask(j_lo);
       const bool got = mbar_wait(&sh.acc_full[buf], (n >> 1) & 1, &sh.fail);
       if (epilogue_any<256>(!got)) {  // the 256 threads leave together
-        if (!sh.fail && a.status) atomicExch(a.status, 7);
-        sh.fail = 1;
+        give_up();
         break;
       }
       tc_fence_after();
@@ -642,14 +659,22 @@ linear_pair_kernel(const LinArgs a, const int BN, const __grid_constant__ CUtens
   // ---- teardown: neither CTA leaves while the other may still signal it ----
   tc_fence_before();
   __syncthreads();
-  if (sh.fail && tid == 256 && rank == 0) {  // wait (bounded) for the last requested tile of every stage
-    for (int st = 0; st < PK_STAGES; ++st) {
-      const int last = sh.issued - 1 - ((sh.issued - 1 - st) % PK_STAGES + PK_STAGES) % PK_STAGES;
-      if (sh.issued > st && last >= 0) mbar_wait(&sh.full[st], (last / PK_STAGES) & 1);
-    }
-  }
-  __syncwarp();
   cluster_sync_all();
+  if (sh.fail) {  // in both CTAs; wait (bounded) for what is in flight before the memories are given up:
+    if (tid == 288 && rank == 0) {  // the MMAs, by the thread that issued them,
+      pair_commit_here(&sh.drained);
+      mbar_wait(&sh.drained, 0);
+    }
+    if (tid == 256 && rank == 0) {  // and the last tile of every stage that either CTA has requested its half of
+      const int issued = max(sh.issued, ld_cluster(in_cta(smem_u32(&sh.issued), 1)));
+      for (int st = 0; st < PK_STAGES; ++st) {
+        const int last = issued - 1 - ((issued - 1 - st) % PK_STAGES + PK_STAGES) % PK_STAGES;
+        if (issued > st && last >= 0) mbar_wait(&sh.full[st], (last / PK_STAGES) & 1);
+      }
+    }
+    __syncwarp();
+    cluster_sync_all();
+  }
   if (warp == 0) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;\n" ::"r"(tmem) : "memory");
@@ -671,13 +696,10 @@ struct CkShape {
 };
 struct CkShared {
   float x_scale[128];
-  uint64_t full[8], empty[8], done;
+  uint64_t full[8], empty[8], done, drained;
   unsigned tmem_base;
   int fail, issued;
 };
-__device__ __forceinline__ void st_cluster(unsigned addr, int v) {
-  asm volatile("st.shared::cluster.s32 [%0], %1;\n" ::"r"(addr), "r"(v) : "memory");
-}
 
 constexpr int CK_THREADS = 320;
 template <typename T, int BN>
@@ -703,6 +725,7 @@ linear_cluster_kernel(const LinArgs a, const __grid_constant__ CUtensorMap tm_w,
       mbar_init(&sh.empty[i], 1);
     }
     mbar_init(&sh.done, 1);
+    mbar_init(&sh.drained, 1);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
   __syncwarp();
@@ -824,7 +847,11 @@ linear_cluster_kernel(const LinArgs a, const __grid_constant__ CUtensorMap tm_w,
     }
   }
   __syncthreads();
-  if (sh.fail) {
+  if (sh.fail) {  // wait (bounded) for the MMAs and copies in flight
+    if (tid == 288) {
+      tc_commit(&sh.drained);
+      mbar_wait(&sh.drained, 0);
+    }
     if (tid == 256)
       for (int st = 0; st < STAGES; ++st) {
         const int last = sh.issued - 1 - ((sh.issued - 1 - st) % STAGES + STAGES) % STAGES;
