@@ -311,8 +311,9 @@ decode_attn_kv8_kernel(const A8Args a, const __grid_constant__ CUtensorMap tm_k,
       else if (r < ahead.list.n()) pos = ahead.list.t0 + (r - ahead.list.nA);
     }
   };
+  bool dead = false;  // a wait for a tile has run out: nothing more is asked for
   const auto ask = [&]() {  // copies of one tile, and of its rows' scales
-    if (ahead_w < w1) {
+    if (ahead_w < w1 && !dead) {
       const int s = asked % STAGES;
       unsigned char* dst = ring + s * STAGE_BYTES;
       const bool ok = (unsigned)pos < (unsigned)a.rows;
@@ -354,7 +355,6 @@ decode_attn_kv8_kernel(const A8Args a, const __grid_constant__ CUtensorMap tm_k,
   for (int s = 0; s < STAGES - 1; ++s) ask();
 
   int used = 0;
-  bool dead = false;
   int next_w = w0 + warp;  // the warp's next tile
   for (int lo = w0; CLUSTER || lo < w1;) {
     const int seg_hi = seg_lo + seg.nt, hi = min(w1, seg_hi);  // this CTA's tiles of the segment: [lo, hi)
@@ -409,11 +409,14 @@ decode_attn_kv8_kernel(const A8Args a, const __grid_constant__ CUtensorMap tm_k,
       __syncwarp();  // all lanes are done with the tile whose stage is refilled now
       ask();
       cp_async_wait<STAGES - 1>();
-      if (!dead && !mbar_wait(&sh.full[warp][s], (used / STAGES) & 1)) {
+      if (__any_sync(0xffffffffu, !dead && !mbar_wait(&sh.full[warp][s], (used / STAGES) & 1))) {
+        // The warp goes on, so that others get the partials and arrivals they count on, with what lies in its ring; the
+        // copies that it has asked for land first (a bounded wait each): the ring becomes a merge buffer, then another CTA's.
         dead = true;
-        if (a.status) atomicExch(a.status, 5);
+        if (lane == 0 && a.status) atomicExch(a.status, 5);
+        for (int i = used; i < asked; ++i) mbar_wait(&sh.full[warp][i % STAGES], (i / STAGES) & 1);
+        __syncwarp();
       }
-      __syncwarp();
       const unsigned char* tile = ring + s * STAGE_BYTES;
       // the 16-byte piece c of row r of the tile's K or V rows
       const auto piece = [&](int v, int r, int cc) {
@@ -801,8 +804,6 @@ decode_attn_kv8_kernel(const A8Args a, const __grid_constant__ CUtensorMap tm_k,
     }
   }
   cp_async_wait<0>();
-  if (dead)  // let every copy that was asked for land (bounded) before the shared memory is given up
-    for (int i = used; i < asked; ++i) mbar_wait(&sh.full[warp][i % STAGES], (i / STAGES) & 1);
 }
 
 constexpr int smem_bytes(bool tma, int cols) {
