@@ -645,7 +645,8 @@ def check_status(device) -> None:
     if code:
         status_word(device).zero_()
         what = {1: "a weight copy's ring slot (producer)", 2: "a weight copy (consumer)", 3: "the grid barrier",
-                4: "another rank's exchange flag", 5: "a K/V tile copy"}.get(code, "an unknown wait")
+                4: "another rank's exchange flag", 5: "a K/V tile copy", 6: "a tile or product of the prompt's attention",
+                7: "a tile or product of a projection"}.get(code, "an unknown wait")
         raise abi.OmniKVError(f"a decode kernel gave up waiting for {what} (status {code}); its results are incomplete")
 
 

@@ -165,3 +165,15 @@ def test_allocation_checks_its_block():
     for block in (0, 48, 512, -1):
         with pytest.raises(abi.OmniKVError):
             ops.kv8_alloc(1, 1, 64, block=block, dtype=torch.int8, device="cpu")
+
+
+def test_every_status_of_a_bounded_wait_is_named(monkeypatch):
+    from omnikv_b200 import ops
+    word = torch.zeros(1, dtype=torch.int32)
+    monkeypatch.setattr(ops, "status_word", lambda device: word)
+    ops.check_status("cuda")
+    for code in range(1, 8):
+        word.fill_(code)
+        with pytest.raises(ops.abi.OmniKVError, match=f"status {code}") as e:
+            ops.check_status("cuda")
+        assert "unknown" not in str(e.value) and int(word) == 0
