@@ -307,6 +307,7 @@ PyObject* kv8_decode_attn(PyObject* const* a) {
     p.idx_cap = (int32_t)idx->size(1);
     cap = idx->size(1);
   }
+  if (ws_arg && !ws_arg->is_contiguous()) refuse("kv8_decode_attn: ws must be contiguous");
   if (!tail_len != !tail_start) refuse("kv8_decode_attn: tail_start and tail_len go together");
   if (tail_len) {
     p.tail_start = ints(tail_start, B, "tail_start");

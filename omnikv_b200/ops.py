@@ -590,7 +590,7 @@ def kv8_decode_attn(q: torch.Tensor, k8, v8, k_scale, v_scale, len_a: torch.Tens
     selector-``last`` scores of positions ``< score_len[b]``.  ``n_splits``: CTAs per (sequence, KV head) on average
     (default: as many as the GPU holds); ``max_rows`` (default: all) is only a hint for that number.  ``out`` (default: a
     new contiguous tensor) may be q itself; q and the cache may be expanded over the batch.  ``ws``: a zeroed
-    workspace of ``omnikv_kv8_attn_workspace_bytes``; by default every stream and every captured graph has its own."""
+    contiguous workspace of ``omnikv_kv8_attn_workspace_bytes``; by default every stream and every captured graph has its own."""
     return (_bind_module or _bind()).kv8_decode_attn(q, k8, v8, k_scale, v_scale, len_a, block, idx, tail_start, tail_len, out,
                                                      score_out, score_len, n_splits, max_rows, scale, ws)
 

@@ -667,3 +667,17 @@ def test_refusals():
     with pytest.raises(OmniKVError):  # rows of codes that are not 16-byte aligned
         wide = torch.zeros(2, 2, 64, 2 * D + 1, dtype=torch.int8, device="cuda")
         o.kv8_load(wide[..., :D], wide[..., D:2 * D], ks, vs, block=16, dtype=torch.bfloat16)
+
+
+def test_a_workspace_that_is_not_one_piece_of_memory_is_refused():
+    from omnikv_b200.abi import OmniKVError
+    cache, k, v = filled(1, 2, 500, "int8", torch.bfloat16, 64, 101)
+    q, n = draw((1, 8, D), torch.bfloat16, 102, outliers=False), i32([500])
+    need = ops().abi.lib().omnikv_kv8_attn_workspace_bytes(1, 8, 2, 148)
+    whole = torch.zeros(2 * need, dtype=torch.uint8, device="cuda")
+    for ws in (whole[:1].expand(need), whole[::2], whole.view(2, -1).t()):
+        assert ws.numel() >= need
+        with pytest.raises(OmniKVError, match="contiguous"):
+            ops().kv8_decode_attn(q, *cache, n, block=64, ws=ws)
+    assert (whole == 0).all()
+    check_attention(ops().kv8_decode_attn(q, *cache, n, block=64, ws=whole), q, k, v, [list(range(500))])
