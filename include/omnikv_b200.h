@@ -576,7 +576,7 @@ int omnikv_kv8_load(const omnikv_kv8_cache* c, int dtype, int start, int n, cons
  * len is taken into [0, rows] (with idx: [0, idx_cap]), the tail into the cache; an index outside [0, rows) counts as no
  * row.  No rows at all: the output is zero.  score_out (idx == NULL, no tail): as in omnikv_decode_attn, positions below
  * min(score_len[b], len[b], score_stride).  The cache is only read: sequences or heads may share memory (strides of 0).
- * q, out [B, H, d] 16-bit; H / KVH at most 16.
+ * q, out [B, H, d] 16-bit; H / KVH at most 16, B * KVH at most 4096 (a counter of the workspace each).
  * The workspace (omnikv_kv8_attn_workspace_bytes) starts with 16 KiB of counters that are ZERO before its first use and
  * are left zero; calls that share it must not overlap. */
 typedef struct {

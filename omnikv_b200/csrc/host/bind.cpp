@@ -328,7 +328,8 @@ PyObject* kv8_decode_attn(PyObject* const* a) {
   if (a[14] != Py_None) cap = integer(a[14]);
   const int64_t per = a[13] != Py_None ? integer(a[13]) : std::clamp<int64_t>(cap / 96, 0, d.sms) + 1;
   const int64_t segments = B * KVH;
-  if (per < 1 || per > 32768 || segments < 1 || segments > 32768 || (a[13] != Py_None && per * segments > 32768))
+  if (segments > 4096) refuse("kv8_decode_attn: at most 4096 pairs of a sequence and a KV head, got " + std::to_string(segments));
+  if (per < 1 || per > 32768 || segments < 1 || (a[13] != Py_None && per * segments > 32768))
     refuse("kv8_decode_attn: n_splits x B x KVH must lie in 1..32768");
   const int64_t n = a[13] != Py_None ? per * segments : std::min(d.sms, per * segments);
   p.n_ctas = (int32_t)n;

@@ -584,7 +584,7 @@ def kv8_decode_attn(q: torch.Tensor, k8, v8, k_scale, v_scale, len_a: torch.Tens
                     score_out: Optional[torch.Tensor] = None, score_len: Optional[torch.Tensor] = None,
                     n_splits: Optional[int] = None, max_rows: Optional[int] = None, scale: Optional[float] = None,
                     ws: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """``omnikv_kv8_decode_attn``: ``decode_attn`` over an 8-bit cache.  q 16-bit ``[B,H,128]``; the rows of a sequence
+    """``omnikv_kv8_decode_attn``: ``decode_attn`` over an 8-bit cache.  q 16-bit ``[B,H,128]`` (B x KVH at most 4096); the rows of a sequence
     are positions ``[0, len_a[b])``, or ``idx[b][0..len_a[b])`` (int32 ``[B, cap]``) followed by the ``tail_len[b]``
     positions from ``tail_start[b]`` of the same cache.  ``score_out`` ``[KVH,B,stride]`` fp32 (without ``idx`` and tail):
     selector-``last`` scores of positions ``< score_len[b]``.  ``n_splits``: CTAs per (sequence, KV head) on average

@@ -681,3 +681,16 @@ def test_a_workspace_that_is_not_one_piece_of_memory_is_refused():
             ops().kv8_decode_attn(q, *cache, n, block=64, ws=ws)
     assert (whole == 0).all()
     check_attention(ops().kv8_decode_attn(q, *cache, n, block=64, ws=whole), q, k, v, [list(range(500))])
+
+
+def test_the_most_pairs_of_sequence_and_head():
+    """4096 pairs run, one more is refused by name."""
+    from omnikv_b200.abi import OmniKVError
+    cache, k, v = filled(1, 1, 40, "int8", torch.bfloat16, 16, 103)
+    q, lens = draw((4097, 2, D), torch.bfloat16, 104, outliers=False), torch.arange(4097, device="cuda").remainder(41).int()
+    wide = lambda B: [t.expand(B, *t.shape[1:]) for t in cache]  # noqa: E731
+    out = ops().kv8_decode_attn(q[:4096], *wide(4096), lens[:4096], block=16)
+    for b in (0, 40, 41, 2049, 4095):
+        check_attention(out[b:b + 1], q[b:b + 1], k, v, [list(range(b % 41))])
+    with pytest.raises(OmniKVError, match="4096"):
+        ops().kv8_decode_attn(q, *wide(4097), lens, block=16)
