@@ -262,7 +262,7 @@ class _ProjView:
 
     @property
     def weight(self):
-        if getattr(self._owner, self._name + "_codes", None) is not None:
+        if self._name + "_codes" in self._owner._buffers:
             raise RuntimeError(_CODES_HELD)
         return getattr(self._owner, self._name + "_weight")[self._lo:self._hi]
 
@@ -276,12 +276,12 @@ _CODES_HELD = "the projections are held as int8 codes (quantize_weights_): load 
 def _project(x: torch.Tensor, owner: nn.Module, name: str, lo: int = 0, hi: Optional[int] = None) -> torch.Tensor:
     """``x @ owner.<name>_weight.T`` (its rows ``[lo, hi)``) for x ``[..., K]``: the library product, or the 8-bit integer
     one when the weight is held as int8 codes (``OmniKVMulLM.quantize_weights_``)."""
-    codes = getattr(owner, name + "_codes", None)
+    codes = owner._buffers.get(name + "_codes")  # (a module's lookup of a missing name is slow: 0.87 against 0.09 us)
     if codes is None:
         w = getattr(owner, name + "_weight")
         return F.linear(x, w if hi is None else w[lo:hi])
     x8, x_scale = ops.quant_rows(x.reshape(-1, x.shape[-1]))
-    y = ops.linear_w8a8(x8, x_scale, codes[lo:hi], getattr(owner, name + "_scale")[lo:hi], out_dtype=x.dtype)
+    y = ops.linear_w8a8(x8, x_scale, codes[lo:hi], owner._buffers[name + "_scale"][lo:hi], out_dtype=x.dtype)
     return y.view(*x.shape[:-1], -1)
 
 
@@ -940,7 +940,7 @@ class OmniKVMulLM(nn.Module):
         return sd
 
     def _need_weights(self) -> None:
-        if getattr(self.model.layers[0].self_attn, "qkv_codes", None) is not None:
+        if self.model.layers[0].holds_codes:
             raise RuntimeError(_CODES_HELD)
 
     @torch.no_grad()

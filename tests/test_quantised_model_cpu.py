@@ -136,3 +136,24 @@ def test_quantising_one_model_leaves_the_config_and_others_alone():
     assert "model.layers.0.mlp.down_codes" in a.state_dict() and "model.layers.0.mlp.down_weight" in b.state_dict()
     for model, held in ((a, True), (b, False)):  # the fused kernels are kept from layers by what those hold
         assert all(layer.holds_codes is held for layer in model.model.layers)
+
+
+def test_a_16_bit_projection_asks_for_no_missing_attribute():
+    """A module's lookup of a name that it does not have costs a microsecond (an exception inside), four times per layer and
+    step: whether there are codes is read from the buffers."""
+    from omnikv_b200.modeling.omnikv import _project
+
+    class Owner(torch.nn.Module):
+        missed = 0
+
+        def __getattr__(self, name):
+            try:
+                return super().__getattr__(name)
+            except AttributeError:
+                Owner.missed += 1
+                raise
+
+    owner = Owner()
+    owner.qkv_weight = torch.nn.Parameter(torch.randn(8, 4))
+    x = torch.randn(3, 4)
+    assert torch.equal(_project(x, owner, "qkv"), torch.nn.functional.linear(x, owner.qkv_weight)) and Owner.missed == 0
