@@ -156,4 +156,5 @@ def test_a_16_bit_projection_asks_for_no_missing_attribute():
     owner = Owner()
     owner.qkv_weight = torch.nn.Parameter(torch.randn(8, 4))
     x = torch.randn(3, 4)
+    Owner.missed = 0  # setting a parameter looks its name up once
     assert torch.equal(_project(x, owner, "qkv"), torch.nn.functional.linear(x, owner.qkv_weight)) and Owner.missed == 0
