@@ -465,7 +465,7 @@ decode_attn_kv8_kernel(const A8Args a, const __grid_constant__ CUtensorMap tm_k,
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
               float& z = x[i][cb][2 * u + e];
-              z = ok ? z * ks * qs[cb][e] : -INFINITY;
+              z = ok ? z * (ks * qs[cb][e]) : -INFINITY;  // (z * ks may leave fp32's range where the logit is in it)
             }
         }
       if (a.score_out) {

@@ -402,6 +402,31 @@ def test_large_queries():
     assert torch.isnan(out[0, 1]).all() and torch.isfinite(out[0, [0, 2, 3]]).all()
 
 
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+def test_keys_and_queries_of_extreme_size(fmt):
+    """Products of a key's scale and its codes that leave fp32's range although the logits are in it."""
+    B, H, KVH, rows, block = 1, 4, 1, 300, 16
+    q = draw((B, H, D), torch.bfloat16, 15, outliers=False)
+    k, v = draw((B, KVH, rows, D), torch.bfloat16, 16), draw((B, KVH, rows, D), torch.bfloat16, 17)
+    tiny = q * 2.0 ** -120
+    cache = ops().kv8_alloc(B, KVH, rows, block=block, dtype=CODES[fmt], device="cuda")
+    ops().kv8_store(k * 2.0 ** 118, v, *cache, block=block)
+    check_attention(ops().kv8_decode_attn(tiny, *cache, i32([rows]), block=block), tiny, *as_read(cache, block), [list(range(rows))])
+    k[0, 0, 37, 5], q[0, :, 5] = 3e38, torch.tensor([0.5, -0.5, 0.25, 0.0], dtype=torch.bfloat16, device="cuda")
+    ops().kv8_store(k, v, *cache, block=block)
+    score = torch.zeros(KVH, B, rows, device="cuda")
+    out = ops().kv8_decode_attn(q, *cache, i32([rows]), block=block, score_out=score, score_len=i32([rows]))
+    kk, vv = as_read(cache, block)
+    # two heads see nothing but row 37, one everything else, one all rows (its products with that row are zero)
+    rest = [r for r in range(rows) if r != 37]
+    check_attention(out[:, :1], q[:, :1], kk, vv, [[37]])
+    check_attention(out[:, 2:3], q[:, 2:3], kk, vv, [[37]])
+    check_attention(out[:, 1:2], q[:, 1:2], kk, vv, [rest])
+    check_attention(out[:, 3:], q[:, 3:], kk, vv, [list(range(rows))])
+    want = kk[0, 0, 37, 5].item() * 0.5 / math.sqrt(D)
+    assert abs(score[0, 0, 37].item() - want) <= 2.0 ** -17 * want
+
+
 def test_offsets_past_32_bits():
     """A cache of more than 2^31 codes per sequence, read at its end."""
     KVH, rows, block = 8, 1_100_000, 64
