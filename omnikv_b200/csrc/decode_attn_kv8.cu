@@ -193,6 +193,7 @@ decode_attn_kv8_kernel(const A8Args a, const __grid_constant__ CUtensorMap tm_k,
   unsigned char* ring = smem + warp * STAGES * STAGE_BYTES;
   float* o_s = reinterpret_cast<float*>(smem + NW * STAGES * STAGE_BYTES);
   const int G = a.G;
+  const float factor = a.scale * kLog2e;
 
   if (lane < STAGES) mbar_init(&sh.full[warp][lane], 1);
   asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
@@ -361,9 +362,9 @@ decode_attn_kv8_kernel(const A8Args a, const __grid_constant__ CUtensorMap tm_k,
     const int b = seg.b, kvh = seg.kvh, seg_no = b * a.KVH + kvh;
     const int c_lo = own ? 0 : owner(seg_lo), parts = own ? 1 : owner(seg_hi - 1) - c_lo + 1;  // the CTAs that share it
 
-    // ---- queries: fragments of q * 2^e (largest element in [2^13, 2^14)), e folded into the head's factor ----
+    // ---- queries: fragments of q * 2^e (largest element in [2^13, 2^14)); a logit is z (ks 2^-e) scale log2(e) ----
     unsigned qf[COLS][8][2];
-    float qs[COLS][2];
+    float qs[COLS][2];  // 2^-e
 #pragma unroll
     for (int cb = 0; cb < COLS; ++cb) {
       const int h = cb * 8 + g;
@@ -388,9 +389,8 @@ decode_attn_kv8_kernel(const A8Args a, const __grid_constant__ CUtensorMap tm_k,
         qf[cb][j][0] = pack2<__half>(x.x * up, x.y * up);
         qf[cb][j][1] = pack2<__half>(y.x * up, y.y * up);
       }
-      const float f = down * a.scale * kLog2e;
-      qs[cb][0] = __shfl_sync(0xffffffffu, f, 8 * t);
-      qs[cb][1] = __shfl_sync(0xffffffffu, f, 8 * t + 4);
+      qs[cb][0] = __shfl_sync(0xffffffffu, down, 8 * t);
+      qs[cb][1] = __shfl_sync(0xffffffffu, down, 8 * t + 4);
     }
     const int score_lim = a.score_out ? (int)min((int64_t)min(a.score_len[b], seg.list.nA), a.score_stride) : 0;
     float* score_row = a.score_out ? a.score_out + ((size_t)kvh * a.B + b) * a.score_stride : nullptr;
@@ -465,7 +465,7 @@ decode_attn_kv8_kernel(const A8Args a, const __grid_constant__ CUtensorMap tm_k,
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
               float& z = x[i][cb][2 * u + e];
-              z = ok ? z * (ks * qs[cb][e]) : -INFINITY;  // (z * ks may leave fp32's range where the logit is in it)
+              z = ok ? z * (ks * qs[cb][e]) * factor : -INFINITY;  // (z * ks may leave fp32's range where the logit is in it)
             }
         }
       if (a.score_out) {
