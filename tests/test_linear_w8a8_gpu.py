@@ -244,3 +244,13 @@ def test_codes_and_scales_have_memory_of_their_own(tmp_path):
     torch.save((codes, scale), tmp_path / "w.pt")
     for a, b in zip(torch.load(tmp_path / "w.pt"), (codes, scale)):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("out_dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("n,N,K", [(1, 500, 512), (40, 1024, 8192), (24, 19000, 1040), (300, 300, 1040)])  # every kernel
+def test_activations_of_extreme_size(out_dtype, n, N, K):
+    """Results in the range of normal numbers (2^-33 2^-92 at least, as the scales are at least 10^-5) whose integer sum times
+    the token's scale leaves fp32 (about 2^17 to 2^20 times 2^112)."""
+    x8, sx, w8, sw = operands(n, N, K, seed=7)
+    for e in (122, -92):
+        check(ops().linear_w8a8(x8, sx * 2.0 ** e, w8, sw, out_dtype=out_dtype), x8, sx * 2.0 ** e, w8, sw)
