@@ -719,3 +719,69 @@ def test_the_most_pairs_of_sequence_and_head():
         check_attention(out[b:b + 1], q[b:b + 1], k, v, [list(range(b % 41))])
     with pytest.raises(OmniKVError, match="4096"):
         ops().kv8_decode_attn(q, *wide(4097), lens, block=16)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("B,KVH,G,rows,splits", [(1, 8, 4, 900, None), (3, 2, 5, 333, 3), (2, 1, 12, 2500, 40)])
+def test_codes_of_k_and_v_in_separate_buffers(fmt, B, KVH, G, rows, splits):
+    """Two code tensors with nothing between them but their layout: every entry point, and rows of both fetched apart."""
+    dtype, block = torch.float16, 32
+    k8, v8 = (torch.zeros(B, KVH, rows, D, dtype=torch.int8, device="cuda").view(CODES[fmt]) for _ in range(2))
+    ks, vs = (torch.zeros(B, KVH, -(-rows // block), device="cuda") for _ in range(2))
+    cache = (k8, v8, ks, vs)
+    xk, xv = draw((B, KVH, rows, D), dtype, 201), draw((B, KVH, rows, D), dtype, 202)
+    ops().kv8_store(xk, xv, *cache, block=block)
+    ops().kv8_append(xk[:, :, 7].contiguous(), xv[:, :, 9].contiguous(), *cache, i32([rows - 1 - b for b in range(B)]), block=block)
+    k, v = as_read(cache, block)
+    back = ops().kv8_load(*cache, block=block, dtype=dtype)
+    for got, want in zip(back, (k, v)):
+        assert ((got.double() - want).abs() <= (2.0 ** -24 + 2.0 ** -11) * want.abs() + 2.0 ** -25).all()
+    q = draw((B, KVH * G, D), dtype, 203, outliers=False)
+    lens = [rows - 11 * b for b in range(B)]
+    score = torch.full((KVH, B, rows), 123.0, device="cuda")
+    out = ops().kv8_decode_attn(q, *cache, i32(lens), block=block, n_splits=splits, score_out=score, score_len=i32(lens))
+    check_attention(out, q, k, v, [list(range(n)) for n in lens])
+    for b in range(B):
+        _, _, logits, size = ko.attention(q[b].double(), k[b], v[b], list(range(lens[b])))
+        assert ((score[:, b, :lens[b]].double() - logits.view(KVH, G, -1).amax(1)).abs() <= 2.0 ** -17 * size).all()
+    g = torch.Generator().manual_seed(5)
+    lists = [torch.randperm(rows - 40, generator=g)[:rows // 3 + b].tolist() for b in range(B)]
+    idx, counts = i32([r + [-1] * (rows // 3 + B - len(r)) for r in lists]), i32([len(r) for r in lists])
+    starts, tails = i32([rows - 40] * B), [40 - 13 * b for b in range(B)]
+    out = ops().kv8_decode_attn(q, *cache, counts, block=block, n_splits=splits, idx=idx, tail_start=starts, tail_len=i32(tails))
+    check_attention(out, q, k, v, [r + list(range(rows - 40, rows - 40 + t)) for r, t in zip(lists, tails)])
+    heads = [100 + b for b in range(B)]  # a tail behind the first rows
+    out = ops().kv8_decode_attn(q, *cache, i32(heads), block=block, n_splits=splits, tail_start=starts, tail_len=i32(tails))
+    check_attention(out, q, k, v, [list(range(n)) + list(range(rows - 40, rows - 40 + t)) for n, t in zip(heads, tails)])
+
+
+@pytest.mark.parametrize("tokens_first", [False, True])
+def test_all_rows_of_a_cache_past_32_bits(tokens_first):
+    """1.1 million rows of 8 heads (2.25 GB of codes), of which the last ones hold something.  The others have scales of
+    zero: a logit of 0 and a value of 0 each, so the definition is a sum over the rows that do.  Tolerance: as above, and
+    2^-13 for the sum of the weights of one (a thread adds 1240 of them up in fp32, 2^-24 each)."""
+    KVH, H, rows, block = 8, 32, 1_100_000, 64
+    cache = ops().kv8_alloc(1, KVH, rows, block=block, dtype=torch.int8, device="cuda", tokens_first=tokens_first)
+    last = rows // block * block - block
+    k, v = draw((1, KVH, 64, D), torch.bfloat16, 1), draw((1, KVH, 64, D), torch.bfloat16, 2)
+    ops().kv8_store(k, v, *cache, block=block, start=last)
+    ops().kv8_append(k[:, :, 3], v[:, :, 5], *cache, i32([rows - 1]), block=block)
+    q = draw((1, H, D), torch.bfloat16, 5, outliers=False) * 4
+    score = torch.zeros(KVH, 1, rows, device="cuda")
+    out = ops().kv8_decode_attn(q, *cache, i32([rows]), block=block, score_out=score, score_len=i32([rows]))[0].double()
+    at = list(range(last, last + 64)) + [rows - 1]
+    blocks = torch.tensor([r // block for r in at], device="cuda")
+    kk, vv = (c[0][:, at].double() * s[0][:, blocks].double()[..., None] for c, s in (cache[0::2], cache[1::2]))
+    logits = torch.einsum("hgd,hnd->hgn", q[0].double().view(KVH, H // KVH, D), kk) / math.sqrt(D)
+    size = (torch.einsum("hgd,hnd->hgn", q[0].double().view(KVH, H // KVH, D).abs(), kk.abs()) / math.sqrt(D)).max().item()
+    top = logits.amax(2, keepdim=True).clamp(min=0)
+    p = torch.exp(logits - top)
+    p = p / (p.sum(2, keepdim=True) + (rows - len(at)) * torch.exp(-top))
+    assert (p.sum(2) > 0.01).float().mean() > 0.5  # what was stored matters
+    want, mass = (torch.einsum("hgn,hnd->hgd", p, x).reshape(H, D) for x in (vv, vv.abs()))
+    tol = 2.0 ** -8 * want.abs() + (2.0 ** -11 + 2.0 ** -16 + 2 * 2.0 ** -17 * size + 2.0 ** -13) * mass + 1e-30
+    assert ((out - want).abs() <= tol).all(), ((out - want).abs() / tol).max().item()
+    best = logits.amax(1)
+    assert ((score[:, 0, at].double() - best).abs() <= 2.0 ** -17 * size).all()
+    score[:, 0, at] = 0
+    assert (score == 0).all()
