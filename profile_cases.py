@@ -11,7 +11,8 @@ Cases: tp_timeline (one graph-replayed decode step of the benchmark on N GPUs, o
 stamps of the profiling build, with the wait for the peers' flags separated from the streaming time), dense_attn (filter layer: K and V of 8 KV heads x ctx rows, fused scores), sparse_attn
 (8781 selected rows + tail), topk (ctx scores, 8 planes), score_window (16-slot window, exp),
 offload_gather (30150 tokens x 12 layers from pinned host memory), kv8 (8-bit KV cache: attention over ctx rows, selected rows and
-short caches, store and load), linear_w8a8 (the layer's projections in 8-bit integers).  Each prints the CUDA-event time per launch.
+short caches, store and load), linear_w8a8 (the layer's projections in 8-bit integers), decode_step (one graph-replayed step of the
+Llama-3-8B shape with the KV cache and the projections in 16 and in 8 bits).  Each prints the CUDA-event time per launch.
 """
 from __future__ import annotations
 
@@ -206,6 +207,41 @@ def linear_w8a8_cases(n_tokens: int):
     ops.check_status(dev)
 
 
+def decode_step_cases(ctx: int, batch: int, selector: str, steps: int = 50):
+    """ms per decode step of the Llama-3-8B shape (OmniKV 2,8,18 / wait 1) with synthetic KV: one sequence of ``ctx`` tokens
+    (0.067 of them selected), or ``batch`` of ctx / 2 to ctx tokens (2048 selected); in 16 bits, with an 8-bit KV cache, with
+    int8 projections, with both."""
+    from omnikv_b200.modeling import LlamaCompressorConfig, OmniKVMulLM
+    from omnikv_b200.modeling.omnikv import DecodeRunner
+    g = torch.Generator().manual_seed(0)
+    lens = [ctx] if batch == 1 else torch.randint(ctx // 2, ctx + 1, (batch,), generator=g).tolist()
+    for kv, linear in ((None, None), ("int8", None), ("fp8_e4m3", None), (None, "int8"), ("int8", "int8"), ("fp8_e4m3", "int8")):
+        cfg = LlamaCompressorConfig()
+        cfg.set_config_of_compressor(model_cls="multi", cache_cls="multi", do_select_layers="2,8,18", num_wait_load_layers=1,
+                                     real_offload=False, dense_more=True, num_of_selected_tokens=0.067 if batch == 1 else 2048,
+                                     selector_cls=selector, window_size=16, kv_cache_dtype=kv, linear_dtype=linear)
+        lm = OmniKVMulLM.from_config(cfg, dtype=torch.bfloat16, device="cuda", seed=0)
+        lm.prepare_synthetic_decode(batch)
+        cache = lm.new_cache().init_synthetic(batch, cfg.num_key_value_heads, cfg.head_dim, lens, torch.bfloat16, "cuda",
+                                              reserve=3 * steps + 64)
+        runner = DecodeRunner(lm, None, cache=cache, first_token=torch.ones(batch, 1, dtype=torch.int64, device="cuda"),
+                              max_new_tokens=3 * steps + 32)
+        runner.run(10)
+        times = []
+        for _ in range(2):
+            e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            e0.record()
+            runner.run(steps)
+            e1.record()
+            torch.cuda.synchronize()
+            times.append(e0.elapsed_time(e1) / steps)
+        print(f"batch {batch}, {min(lens)} to {max(lens)} tokens, {selector}: KV {kv or 'bf16'}, projections {linear or 'bf16'}: {min(times):.3f} ms per step, "
+              f"{runner.launches_per_step} launches of this library", flush=True)
+        ops.check_status("cuda")
+        del runner, cache, lm
+        torch.cuda.empty_cache()
+
+
 def tp_timeline(ctx: int, replays: int = 6):
     """One decode step of the benchmark (Llama-3-8B shape, batch 1, ``ctx`` tokens of synthetic KV, fused kernels,
     peer-memory exchange, CUDA graph) on the ranks of this torchrun job, with the profiling build of the library:
@@ -365,13 +401,14 @@ def prefill_case(ctx: int, reps: int, library: bool):
 def main():
     ap = argparse.ArgumentParser()
     ap.add_argument("case", choices=["dense_attn", "sparse_attn", "topk", "score_window", "offload_gather", "gemv", "operator",
-                                     "tp_timeline", "prefill_attn", "batched_linear", "kv8", "linear_w8a8"])
+                                     "tp_timeline", "prefill_attn", "batched_linear", "kv8", "linear_w8a8", "decode_step"])
     ap.add_argument("--tokens", type=int, default=16, help="batched_linear, linear_w8a8: sequences decoding together")
+    ap.add_argument("--selector", default="last", help="decode_step: last, uniform or exp")
     ap.add_argument("--reps", type=int, default=3)
     ap.add_argument("--ctx", type=int, default=131072)
     ap.add_argument("--splits", type=int, default=0)
     ap.add_argument("--contiguous-idx", action="store_true", help="sparse_attn: select rows 0..k-1 instead of random ones")
-    ap.add_argument("--batch", type=int, default=1, help="sparse_attn: sequences (2048 selected rows + 64 tail rows each)")
+    ap.add_argument("--batch", type=int, default=1, help="sparse_attn: sequences (2048 selected rows + 64 tail rows each); decode_step: sequences")
     ap.add_argument("--library", action="store_true", help="prefill_attn: also time PyTorch's fused attention")
     ap.add_argument("--kv-layout", default="interleaved", choices=["interleaved", "planes"],
                     help="dense_attn / score_window: K|V rows of a head interleaved, or in two separate runs of rows")
@@ -395,6 +432,8 @@ def main():
         return kv8_cases(args.ctx)
     if args.case == "linear_w8a8":
         return linear_w8a8_cases(args.tokens)
+    if args.case == "decode_step":
+        return decode_step_cases(args.ctx, args.batch, args.selector)
     if args.case == "prefill_attn":
         return prefill_case(args.ctx if args.ctx != 131072 else 16384, args.reps, args.library)
     if args.case == "operator":
