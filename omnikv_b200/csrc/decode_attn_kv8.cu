@@ -916,7 +916,7 @@ extern "C" int omnikv_kv8_decode_attn(const omnikv_kv8_attn_params* p, void* str
   if (p->score_out && (p->idx || p->tail_len || !p->score_len || p->score_stride <= 0)) return OMNIKV_E_BADARG;
   if (!is_16bit(p->dtype) || p->H / c.KVH > MAX_G) return OMNIKV_E_UNSUPPORTED;
   const int64_t most = (p->idx ? p->idx_cap : (int64_t)c.rows) + (p->tail_len ? c.rows : 0);
-  if ((most / TILE + 2) * c.B * c.KVH > 0x7fffffff) return OMNIKV_E_UNSUPPORTED;  // tiles are counted in 32 bits
+  if (most > 0x7fffffff - TILE || (most / TILE + 2) * c.B * c.KVH > 0x7fffffff) return OMNIKV_E_UNSUPPORTED;  // rows and tiles are counted in 32 bits
   if (p->n_ctas > kMaxCtas || (size_t)c.B * c.KVH * 4 > kAttnCntBytes) return OMNIKV_E_UNSUPPORTED;
   if (!p->workspace || p->workspace_bytes < omnikv_kv8_attn_workspace_bytes(c.B, p->H, c.KVH, p->n_ctas)) return OMNIKV_E_WORKSPACE;
   if (bad16(p->workspace)) return OMNIKV_E_BADARG;

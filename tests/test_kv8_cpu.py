@@ -177,3 +177,18 @@ def test_every_status_of_a_bounded_wait_is_named(monkeypatch):
         with pytest.raises(ops.abi.OmniKVError, match=f"status {code}") as e:
             ops.check_status("cuda")
         assert "unknown" not in str(e.value) and int(word) == 0
+
+
+def test_rows_that_32_bits_do_not_count_are_refused():
+    """Listed rows and the tail together pass 2^31: refused before anything is planned."""
+    from omnikv_b200 import abi
+    lib = abi.lib()
+    p = abi.Kv8AttnParams()
+    p.cache, p.dtype, p.H, p.scale = _cache(abi), abi.BF16, 32, 0.1
+    p.cache.KVH, p.H = 1, 4
+    p.q = p.out = p.len = p.workspace = p.idx = p.tail_start = p.tail_len = 256
+    p.q_stride_b, p.q_stride_h, p.out_stride_b, p.out_stride_h, p.n_ctas = 512, 128, 512, 128, 4
+    p.workspace_bytes = lib.omnikv_kv8_attn_workspace_bytes(1, 4, 1, 4)
+    for cap in (2 ** 31 - 1, 2 ** 31 - 1000):
+        p.idx_cap = p.idx_stride = cap
+        assert lib.omnikv_kv8_decode_attn(ctypes.byref(p), None) == -2, cap
