@@ -985,6 +985,7 @@ inline LinearPlan linear_plan(int n, int N, int K) {
   }
   return p;
 }
+constexpr int kMostRows = 0x7fffffff - 256;  // tokens or channels: rounded up to a tile they still fit 32 bits
 inline size_t linear_workspace(const LinearPlan& p) {
   return p.shared ? 1024 + (size_t)(p.sharers + p.shared) * p.tokens * TK_M * sizeof(int) : 0;
 }
@@ -1084,7 +1085,7 @@ extern "C" int omnikv_quant_rows(int dtype, const void* x, int64_t x_stride_row,
 
 extern "C" size_t omnikv_linear_w8a8_workspace_bytes(int n_tokens, int channels, int K) {
   using namespace omnikv;
-  if (n_tokens <= 0 || channels <= 0 || K <= 0) return 0;
+  if (n_tokens <= 0 || channels <= 0 || K <= 0 || n_tokens > kMostRows || channels > kMostRows) return 0;
   return linear_workspace(linear_plan(n_tokens, channels, K));
 }
 
@@ -1094,6 +1095,7 @@ extern "C" int omnikv_linear_w8a8(const omnikv_linear_w8a8_params* p, void* stre
   if (p->n_tokens <= 0 || p->channels <= 0 || p->K <= 0 || p->K % 16) return OMNIKV_E_BADARG;
   if (p->x_stride_row % 16 || p->w_stride_row % 16 || p->x_stride_row < p->K || p->w_stride_row < p->K) return OMNIKV_E_BADARG;
   if (p->out_stride_row < p->channels || (p->residual && p->residual_stride_row && p->residual_stride_row < p->channels)) return OMNIKV_E_BADARG;
+  if (p->n_tokens > kMostRows || p->channels > kMostRows) return OMNIKV_E_UNSUPPORTED;
   if (p->K > 32768 || (p->out_dtype != OMNIKV_F32 && !is_16bit(p->out_dtype))) return OMNIKV_E_UNSUPPORTED;
   LinArgs a{p->x, p->x_stride_row, p->x_scale, p->w, p->w_stride_row, p->w_scale, p->residual, p->residual_stride_row,
             p->out, p->out_stride_row, p->n_tokens, p->channels, p->K};

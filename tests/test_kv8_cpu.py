@@ -192,3 +192,13 @@ def test_rows_that_32_bits_do_not_count_are_refused():
     for cap in (2 ** 31 - 1, 2 ** 31 - 1000):
         p.idx_cap = p.idx_stride = cap
         assert lib.omnikv_kv8_decode_attn(ctypes.byref(p), None) == -2, cap
+
+
+def test_tokens_and_channels_that_32_bits_do_not_count_are_refused():
+    """Rounded up to a tile they pass 2^31: refused before anything is planned."""
+    from omnikv_b200 import abi
+    lib = abi.lib()
+    for n, channels in ((1, 2 ** 31 - 1), (1, 2 ** 31 - 100), (2 ** 31 - 1, 16), (2 ** 31 - 50, 300)):
+        assert lib.omnikv_linear_w8a8_workspace_bytes(n, channels, 16) == 0
+        q = abi.LinearW8A8Params(n, channels, 16, 256, 16, 256, 256, 16, 256, abi.BF16, None, 0, 256, channels, None, 0, None)
+        assert lib.omnikv_linear_w8a8(ctypes.byref(q), None) == -2, (n, channels)
