@@ -141,7 +141,8 @@ const Device& device(int dev) {
 }
 // A zero-filled workspace for calls that follow one another: one per stream, and one per captured graph (two graphs, or a
 // graph and eager calls, may run at the same time).  One that was outgrown is kept: a captured graph may still use it.  Those
-// of a captured graph go when the graph has been destroyed, of which a driver thread tells (graph_ended).
+// of a captured graph go when the graph has been destroyed, of which a driver thread tells (graph_ended).  Their fill is a node
+// of the graph and runs at every replay: in a memory pool that graphs share, another one's temporaries may have lain there.
 struct Ended {
   std::mutex lock;
   std::vector<unsigned long long> ids;

@@ -530,6 +530,38 @@ def test_a_destroyed_graph_gives_its_workspace_back():
     assert max(used[4:]) - used[3] < 8 * (1 << 20), used  # not one of 1 MiB and more for each graph
 
 
+def test_graphs_that_share_a_memory_pool():
+    """A graph's workspace lies in its pool, where another graph's temporaries may have been: it is zeroed by the graph itself,
+    whatever ran in between."""
+    cache, k, v = filled(2, 2, 9000, "int8", torch.bfloat16, 64, 179)
+    q, n = draw((2, 16, D), torch.bfloat16, 180, outliers=False), i32([9000, 5000])
+    w8, sw = ops().quant_rows(draw((19000, 1040), torch.bfloat16, 181))
+    x8, sx = ops().quant_rows(draw((40, 1040), torch.bfloat16, 182))
+
+    def call():
+        a, b = ops().kv8_decode_attn(q, *cache, n, block=64, n_splits=37), ops().linear_w8a8(x8, sx, w8, sw)
+        for size in (1 << 18, 1 << 20, 1 << 22, 1 << 24):  # temporaries, given back to the pool
+            torch.full((size,), -1, dtype=torch.int32, device="cuda")
+        return a, b
+
+    want = [t.clone() for t in call()]
+    check_attention(want[0], q, k, v, [list(range(9000)), list(range(5000))])
+    graphs, pool = [], None
+    for _ in range(3):
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=pool):
+            got = call()
+        pool = graph.pool()
+        graphs.append((graph, got))
+    for i in (0, 1, 2, 2, 0, 1, 0, 2, 1):
+        graphs[i][0].replay()
+        torch.cuda.synchronize()
+        for a, b in zip(graphs[i][1], want):
+            assert torch.equal(a, b), i
+        assert torch.equal(call()[0], want[0])
+
+
 def test_two_streams_at_once():
     B, H, KVH, rows, block = 1, 32, 8, 20000, 64
     cache, _, _ = filled(B, KVH, rows, "int8", torch.bfloat16, block, 81)
