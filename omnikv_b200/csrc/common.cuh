@@ -30,7 +30,8 @@ __host__ __device__ inline int ceil_div(int a, int b) { return (a + b - 1) / b; 
 // pdl_trigger(): this CTA allows the NEXT kernel's CTAs to be scheduled (they take SMs as CTAs of this grid
 // exit).  pdl_wait(): blocks until the PREVIOUS kernel has completed and its writes are visible; everything
 // that reads or overwrites data shared with earlier kernels must come after it.  Both are no-ops for a
-// kernel launched without the attribute.  Only grids that are fully resident may trigger early.
+// kernel launched without the attribute.  The next kernel is scheduled once every CTA of this grid has triggered or exited, so
+// its CTAs, which wait in pdl_wait(), never hold the place of one that has yet to start: a grid of any size may trigger.
 __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory"); }
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;\n" ::: "memory"); }
 

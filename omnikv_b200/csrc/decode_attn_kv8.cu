@@ -11,7 +11,8 @@
 // counts.
 //
 // The codes are fp16 numbers exactly (e4m3: the conversion instruction; int8: a byte permutation and a subtraction), the
-// queries too after a power of two per head.  Sums are fp32, in the MMA and outside.
+// queries too after a power of two per head, but for elements more than 2^27 below the head's largest, which fp16's subnormals
+// round to 2^-38 of it.  Sums are fp32, in the MMA and outside.
 //
 // Layout.  A warp works alone: its own ring of 32-row tiles, its own mbarriers, no CTA barrier until the end of a segment.
 // Rows are the M side of both products (S^T = K q^T and O^T = V^T P^T with m16n8k16), the query heads of a KV head the N
@@ -36,7 +37,8 @@ namespace omnikv {
 namespace {
 
 constexpr int MAX_G = 16;
-constexpr int kWarps[3] = {0, 12, 8};        // warps of a CTA by column blocks: 168 and 255 registers a thread
+// Warps of a CTA by column blocks: 168 and 255 registers a thread (of the 168, six instantiations of 32 spill one or two).
+constexpr int kWarps[3] = {0, 12, 8};
 constexpr int TILE = 32;                     // rows per tile: one lane per row when rows are fetched one by one
 constexpr int STAGES = 2;
 constexpr int BOX = TILE * kHeadDim;         // bytes of a K or V tile

@@ -110,7 +110,7 @@ __device__ __forceinline__ uint4 ld_stream(const int8_t* p) {  // weights: read 
   return v;
 }
 
-// NB: blocks of eight tokens of a CTA
+// NB: blocks of eight tokens of a CTA (four of them spill six registers of 128)
 template <typename T, int NB>
 __global__ void __launch_bounds__(SK_THREADS, NB == 1 ? 3 : 2) linear_stream_kernel(const LinArgs a) {
   constexpr int SK_DEPTH = NB == 2 ? 3 : 2;
