@@ -123,7 +123,19 @@ def rope_parameters(config, seq_len: Optional[int] = None) -> Tuple[torch.Tensor
     raise NotImplementedError(f"rope_scaling type {kind!r}")
 
 
-class OmniKVRotaryEmbedding(nn.Module):
+class _Fp32Buffers(nn.Module):
+    """A module whose fp32 buffers move to another device with the model but keep their 32 bits in ``.to(dtype)``, ``.half()``."""
+
+    def _apply(self, fn, recurse=True):
+        kept = {name: t for name, t in self._buffers.items() if t.dtype is torch.float32}
+        super()._apply(fn, recurse)
+        for name, t in kept.items():
+            if self._buffers[name].dtype != t.dtype:
+                self._buffers[name] = t.to(self._buffers[name].device)
+        return self
+
+
+class OmniKVRotaryEmbedding(_Fp32Buffers):
     """cos / sin generation of the Llama patch (modeling/patch_of_llama3_1.py:545-629).  One instance serves every
     layer of a model (the reference holds an identical copy per layer).  ``inv_freq`` is a device buffer that the
     fused decode kernels read directly; for dynamic-NTK scaling it is rewritten IN PLACE, on the device, whenever
@@ -285,18 +297,10 @@ def _project(x: torch.Tensor, owner: nn.Module, name: str, lo: int = 0, hi: Opti
     return y.view(*x.shape[:-1], -1)
 
 
-class _Projections(nn.Module):
+class _Projections(_Fp32Buffers):
     """A module whose fused matrices may be held as int8 codes with fp32 scales (``OmniKVMulLM.quantize_weights_``)."""
 
     holds_codes = False  # some matrix of the model is: its layers then decode through the modules
-
-    def _apply(self, fn, recurse=True):  # .to(), .half(): the scales move to another device but keep their 32 bits
-        scales = {name: t for name, t in self._buffers.items() if name.endswith("_scale")}
-        super()._apply(fn, recurse)
-        for name, t in scales.items():
-            if self._buffers[name].dtype != t.dtype:
-                self._buffers[name] = t.to(self._buffers[name].device)
-        return self
 
 
 class OmniKVAttention(_Projections):

@@ -158,3 +158,13 @@ def test_a_16_bit_projection_asks_for_no_missing_attribute():
     x = torch.randn(3, 4)
     Owner.missed = 0  # setting a parameter looks its name up once
     assert torch.equal(_project(x, owner, "qkv"), torch.nn.functional.linear(x, owner.qkv_weight)) and Owner.missed == 0
+
+
+@pytest.mark.parametrize("kind", [None, "int8"])
+def test_rotary_frequencies_stay_fp32_when_the_model_is_cast(kind):
+    lm = build(1, linear_dtype=kind)
+    before = lm.model.rotary_emb.inv_freq.clone()
+    for dtype in (torch.bfloat16, torch.float16, torch.float64):
+        lm.to(dtype)
+        for rotary in [lm.model.rotary_emb] + [layer.self_attn.rotary_emb for layer in lm.model.layers]:
+            assert rotary.inv_freq.dtype is torch.float32 and torch.equal(rotary.inv_freq, before), dtype
