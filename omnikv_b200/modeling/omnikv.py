@@ -885,7 +885,7 @@ class OmniKVMulLM(nn.Module):
         and multiply them with per-token int8 activations (``omnikv_linear_w8a8``); the 16-bit matrices are given up.
         Embedding, norms and lm_head stay.  Decoding then runs through the modules (the fused batch-1 kernels stream 16-bit
         weights).  ``state_dict`` holds codes and scales in the matrices' place; ``load_state_dict`` takes them into a model
-        that is quantised too."""
+        that is quantised too.  A decode step captured before reads the matrices that are given up: capture it anew."""
         for layer in self.model.layers:
             for owner, names in ((layer.self_attn, ("qkv", "o")), (layer.mlp, ("gate_up", "down"))):
                 for name in names:

@@ -267,3 +267,22 @@ def test_a_model_quantised_in_part_decodes_as_its_modules_do(part, monkeypatch):
         assert torch.equal(*got)
     else:  # nothing was changed: the fused kernels decode, whose sums run in another order
         assert torch.nn.functional.cosine_similarity(got[0].flatten().double(), got[1].flatten().double(), 0) > 0.99
+
+
+def test_a_saved_quantised_model_decodes_as_it_did(tmp_path):
+    """Through a file, into a model whose projections are others; then cast to the other 16-bit type, which leaves codes and scales."""
+    a = build(linear_dtype="int8")
+    ids = tokens(1, 150, 13)
+    want = a.generate_greedy(ids, 12)
+    torch.save(a.state_dict(), tmp_path / "model.pt")
+    c = build(linear_dtype="int8")
+    for layer in c.model.layers:
+        layer.mlp.down_codes.zero_()
+    c.load_state_dict(torch.load(tmp_path / "model.pt"))
+    assert torch.equal(c.generate_greedy(ids, 12), want)
+    half = c.to(torch.float16)
+    out = half(input_ids=ids)
+    logits, _ = half._decode_step(tokens(1, 1, 14), out.past_key_values)
+    assert torch.isfinite(logits).all()
+    for x, y in zip(half.model.layers, a.model.layers):
+        assert torch.equal(x.self_attn.qkv_scale, y.self_attn.qkv_scale) and torch.equal(x.mlp.gate_up_codes, y.mlp.gate_up_codes)
